@@ -9,9 +9,9 @@ probabilities by which a user sees what the 4 bits cost.
 * ``logprobs``: the log probability of a given token in every row of logits, the row's entropy and its likeliest tokens.
 
 The format: 16 neighbouring elements of a head are a group with one scale s, whose byte holds the upper bits of a half (5 of the
-exponent, 3 of the fraction, no sign); an element is a whole number c of [-7, 7] in 4 bits, held as c + 8, the even element of a
-pair in the low half of its byte; the value is c s.  s is the group's largest magnitude over 7, rounded to the nearest such number
-(at most 9216), c the nearest whole number to x / s.
+exponent, 3 of the fraction, no sign) that is s / 8; an element is a whole number c of [-7, 7] in 4 bits, held as c + 8, the even
+element of a pair in the low half of its byte; the value is c s.  s is the group's largest magnitude over 7, rounded to the nearest
+such number (at most 480), c the nearest whole number to x / s.
 """
 from __future__ import annotations
 
@@ -26,7 +26,8 @@ DEVICE = "cuda:0"
 DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 PAGE = 64
 GROUP = 16
-LARGEST_SCALE = 9216.0
+UNIT = 8.0                 # a scale over the half that its byte is the upper part of
+LARGEST_SCALE = 480.0
 
 
 def _append(name, dtype, nq, nkv, d, past, new, norms=True, rotary=None, theta=1e6):
@@ -138,8 +139,8 @@ def _numbers(text):
 # ---- the format ----------------------------------------------------------------------------------------------------
 
 def _rounded_scale(s):
-    """The nearest number of 4 significant bits (below 2^-14: the nearest multiple of 2^-17), ties to even."""
-    step = torch.exp2(torch.floor(torch.log2(s.clamp(min=2.0 ** -14))) - 3.0)
+    """The nearest number of 4 significant bits (below 2^-11: the nearest multiple of 2^-14), ties to even."""
+    step = torch.exp2(torch.floor(torch.log2(s.clamp(min=2.0 ** -11))) - 3.0)
     return torch.round(s / step) * step
 
 
@@ -154,13 +155,13 @@ def _quantised(x):
 def _packed(codes, scale):
     """The bytes of codes and scales."""
     u = (codes + 8).to(torch.uint8)
-    return u[..., 0::2] | (u[..., 1::2] << 4), (scale.to(torch.float16).view(torch.int16) >> 7).to(torch.uint8)
+    return u[..., 0::2] | (u[..., 1::2] << 4), ((scale / UNIT).to(torch.float16).view(torch.int16) >> 7).to(torch.uint8)
 
 
 def _unpacked(codes, scales):
     """The values of bytes, in 32 bits."""
     c = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).to(torch.float32) - 8.0
-    s = (scales.to(torch.int16) << 7).view(torch.float16).to(torch.float32)
+    s = (scales.to(torch.int16) << 7).view(torch.float16).to(torch.float32) * UNIT
     return (c.unflatten(-1, (-1, GROUP)) * s[..., None]).flatten(-2)
 
 
@@ -344,7 +345,7 @@ def run(state):
 
 def _exact_values(x):
     """What x (float64) is held as: by the table of all the scales there are."""
-    bits = torch.arange(0, 0x7081, 0x80, dtype=torch.int16).view(torch.float16).double().to(x.device)
+    bits = torch.arange(0, 0x5381, 0x80, dtype=torch.int16).view(torch.float16).double().to(x.device) * 8
     shape = x.shape
     x = x.reshape(-1, GROUP)
     wanted = torch.clamp(x.abs().max(dim=1).values / 7.0, max=LARGEST_SCALE)
@@ -366,7 +367,7 @@ def _exact_cached(state, i, sequence, keys):
     value[..., 1::2] = (code // 16 - 8).double()
     b = state["scales"][i][pages].to(torch.int64)
     e, f = b // 8, (b % 8).double()
-    s = torch.where(e == 0, f * 2.0 ** -17, (1 + f / 8) * torch.exp2(e.double() - 15))
+    s = torch.where(e == 0, f * 2.0 ** -14, (1 + f / 8) * torch.exp2(e.double() - 12))
     value *= s.repeat_interleave(GROUP, dim=-1)
     return value.transpose(0, 1).flatten(1, 2)[:, :keys]
 
