@@ -10,7 +10,7 @@ from .config import (QwenConfig, LanizenConfig, GidiraxConfig, SobunexConfig, Pi
                      unregister_architecture)
 from .weights import (SafetensorsFile, TensorSpec, WeightHandle, WeightLoader, write_random_model,
                       write_safetensors)
-from .cache import PAGE_SIZE, KVRequirement, SequenceCache, StateRequirement
+from .cache import PAGE_SIZE, KVRequirement, KVView, Packed4, SequenceCache, StateRequirement
 from .parts import BuildContext, StepBatch, build_part, register_part, registered_parts, unregister_part
 from .engine import (DecoderModel, GenerationOptions, GenerationResult, InferenceSession, StepEntry,
                      StopReason, expected_tensors, run_generation)

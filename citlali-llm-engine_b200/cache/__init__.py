@@ -1,2 +1,2 @@
 from .allocators import PageAllocator, SlotAllocator
-from .sequence_cache import (PAGE_SIZE, KVRequirement, KVView, SequenceCache, StateRequirement, StateView)
+from .sequence_cache import (PAGE_SIZE, KVRequirement, KVView, Packed4, SequenceCache, StateRequirement, StateView)

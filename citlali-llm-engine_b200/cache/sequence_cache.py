@@ -34,12 +34,31 @@ class KVRequirement:
     """What an attention-like mixer needs cached per token: keys and values of ``num_kv_heads``
     heads of ``head_dim``; ``window`` keys back at most (None: all of them).  ``value_dim``: the size of a value
     (None: ``head_dim``; 0: the mixer keeps one vector per token and no values, and the group holds no value pool).
-    ``keep_first``: so many first tokens of a sequence stay visible beside the window."""
+    ``keep_first``: so many first tokens of a sequence stay visible beside the window.  ``packed4``: keys and values are held in
+    4 bits (:class:`Packed4`)."""
     num_kv_heads: int
     head_dim: int
     window: Optional[int] = None
     value_dim: Optional[int] = None
     keep_first: int = 0        # with a window: the sequence's first tokens stay visible, so their pages are never given back
+    packed4: bool = False
+
+
+@dataclass(frozen=True)
+class Packed4:
+    """Keys (or values) in 4 bits, as csrc/cache4.cuh defines them: ``codes`` uint8 [..., pages, kv_heads, page_size, head_dim / 2]
+    and ``scales`` uint8 [..., pages, kv_heads, page_size, head_dim / 16].  16 neighbouring elements are a group with one scale s,
+    whose byte is the upper part of the half s / 8; an element is c s with a whole c of [-7, 7], held as c + 8, the even element of
+    a pair in the low half of its byte.  A scale of 0xff is a NaN: the group held a number that was not finite."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __getitem__(self, index) -> "Packed4":
+        return Packed4(self.codes[index], self.scales[index])
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
 
 
 @dataclass(frozen=True)
@@ -56,7 +75,7 @@ class KVGroup:
     pages: PageAllocator
     table_host: torch.Tensor          # [slots, max_pages] int32, the host's record
     table: torch.Tensor               # the same on the device
-    keys: torch.Tensor                # [layers, pages, kv_heads, page_size, head_dim]
+    keys: torch.Tensor                # [layers, pages, kv_heads, page_size, head_dim], or a Packed4 of as many
     values: torch.Tensor
     held: Dict[int, Dict[int, int]] = field(default_factory=dict)   # slot -> {page index -> page}
 
@@ -71,7 +90,7 @@ class StateGroup:
 @dataclass
 class KVView:
     """What a mixer sees of the cache: its layer's keys and values and the group's page table."""
-    keys: torch.Tensor                # [pages, kv_heads, page_size, head_dim]
+    keys: torch.Tensor                # [pages, kv_heads, page_size, head_dim], or a Packed4 of as many
     values: torch.Tensor
     page_table: torch.Tensor          # [slots, max_pages] int32
     page_size: int
@@ -136,8 +155,7 @@ class SequenceCache:
             table_host = torch.zeros((num_slots, self.max_pages_per_slot), dtype=torch.int32)
             group = KVGroup(req, steps, PageAllocator(self.num_pages), table_host,
                             torch.zeros_like(table_host, device=self.device),
-                            torch.zeros(shape, dtype=dtype, device=self.device),
-                            torch.zeros(shape[:-1] + (value_dim,), dtype=dtype, device=self.device))
+                            self._pool(req, shape, dtype), self._pool(req, shape[:-1] + (value_dim,), dtype))
             for j, s in enumerate(steps):
                 self._where[s] = ("kv", len(self.kv_groups), j)
             self.kv_groups.append(group)
@@ -146,6 +164,13 @@ class SequenceCache:
             for j, s in enumerate(steps):
                 self._where[s] = ("state", len(self.state_groups), j)
             self.state_groups.append(StateGroup(req, steps, storage))
+
+    def _pool(self, req: KVRequirement, shape, dtype):
+        if not req.packed4:
+            return torch.zeros(shape, dtype=dtype, device=self.device)
+        require(shape[-1] % 16 == 0 and 0 < shape[-1] <= 256,
+                f"a cache in 4 bits takes head sizes that are multiples of 16 up to 256, not {shape[-1]}")
+        return Packed4(*(torch.zeros(shape[:-1] + (shape[-1] // n,), dtype=torch.uint8, device=self.device) for n in (2, 16)))
 
     # ---- slots -----------------------------------------------------------------------
     def acquire(self) -> int:
@@ -266,7 +291,7 @@ class SequenceCache:
     def bytes(self) -> int:
         total = 0
         for g in self.kv_groups:
-            total += (g.keys.numel() + g.values.numel()) * g.keys.element_size()
+            total += g.keys.nbytes + g.values.nbytes
         for g in self.state_groups:
             total += g.storage.numel() * g.storage.element_size()
         return total

@@ -173,6 +173,37 @@ int citlali_latent_gather(const void* pool, const int32_t* page_table, int table
 int citlali_latent_queries(const float* q, int H, int P, const float* inv_freq, int rot_dims, int rot_halves, const int32_t* row_pos,
                            void* out, int rows, cudaStream_t stream);
 
+// ---- keys and values in 4 bits (cache4.cuh says what a byte stands for) -------------------------------------------
+// Pools: codes [pages, nkv, page_size, head_dim / 2] and scales [pages, nkv, page_size, head_dim / 16], bytes; head sizes are multiples of
+// 16 up to 256.  citlali_qk_norm_rope_cache for such a cache: the queries go to q_out (rows q_out_stride elements apart; it may be
+// qkv itself, whose rows are (nq + 2 nkv) head_dim apart), keys and values into pages.  Gains may be null (no head norm); rotary_dim
+// may be 0.  store 0: the queries only (the cache's arguments are not looked at).
+int citlali_cache4_append(const void* qkv, int dtype, void* q_out, size_t q_out_stride, const void* q_gain, const void* k_gain,
+                          int gain_dtype, const float* inv_freq, int rotary_dim, const int32_t* row_slot, const int32_t* row_pos,
+                          const int32_t* page_table, int page_table_stride, void* k_codes, void* k_scales, void* v_codes,
+                          void* v_scales, int page_size, int rows, int nq, int nkv, int head_dim, float eps, int store,
+                          cudaStream_t stream);
+// keys[r], values[r] [nkv, head_dim] (out_dtype) = what the cache holds for position positions[r] of slot slots[r].
+int citlali_cache4_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                        const int32_t* page_table, int page_table_stride, int page_size, const int32_t* slots,
+                        const int32_t* positions, void* keys, void* values, int out_dtype, int rows, int nkv, int head_dim,
+                        cudaStream_t stream);
+// citlali_attention_rows over such a cache, in 32-bit arithmetic; the launch depends on no length.
+int citlali_attention4_rows(const void* q, size_t q_stride, int dtype, const void* k_codes, const void* k_scales,
+                            const void* v_codes, const void* v_scales, const int32_t* page_table, int page_table_stride,
+                            const int32_t* row_slot, const int32_t* row_pos, void* out, size_t out_stride, int rows, int nq,
+                            int nkv, int head_dim, int page_size, int window, float scale, cudaStream_t stream);
+// The same on the tensor cores, bfloat16, for single tokens (seq_start null: a row a sequence, seq_slot and seq_past the rows' slots and
+// positions) and for runs of at most max_new tokens.  Lengths are read on the device only.  partial: as many floats as
+// citlali_attention4_scratch_floats says, of this call alone.
+int citlali_attention4_supports(int head_dim, int page_size);
+size_t citlali_attention4_scratch_floats(int nq, int nkv, int head_dim, int max_new);
+int citlali_attention4(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes,
+                       const void* v_scales, const int32_t* page_table, int page_table_stride, const int32_t* seq_start,
+                       const int32_t* seq_slot, const int32_t* seq_past, void* out, size_t out_stride, float* partial,
+                       size_t partial_floats, int sequences, int max_new, int nq, int nkv, int head_dim, int page_size,
+                       int window, float scale, cudaStream_t stream);
+
 // tokens[r] = argmax of logits[r, :] over finite values, lowest index on ties.
 int citlali_argmax_rows(const float* logits, int32_t* tokens, int rows, int vocab, cudaStream_t stream);
 // The same with 64 blocks per row; scratch holds rows * 128 floats.

@@ -1,0 +1,329 @@
+// The cache in 4 bits: appending a step's keys and values to it, with head norms and rotation on the way, and reading rows back.
+//
+// append does what qk_norm_rope_cache (attention_generic.cu) does for a cache of 16 or 32 bits: for every row of the projection
+// [q | k | v], y = x / sqrt(mean x^2 + eps) gain on the q and k heads, pairs (i, i + rotated / 2) turned by pos inv_freq[i], then the
+// queries back to memory and keys and values into the row's page, here as codes and scales (cache4.cuh).  Nothing is rounded between.
+//
+// The angle.  pos inv_freq[i] in 32 bits is off by up to 2^-24 of itself, 0.004 at position 65,536: as much as a bfloat16 query's own
+// rounding.  The product's rounding error e is one fma away, and cos(a + e) = cos a - e sin a to 32 bits, so it is put right.
+#include "api.h"
+#include "cache4.cuh"
+#include "common.cuh"
+
+namespace citlali {
+namespace c4 {
+
+constexpr int kThreads = 128;
+constexpr int kWarps = 8;          // of the form that takes any size
+
+__device__ __forceinline__ float2 turn_of(int pos, float f) {
+    const float p = (float)pos, a = p * f, e = fmaf(p, f, -a);       // positions are below 2^24
+    float sn, cs;
+    sincosf(a, &sn, &cs);
+    return make_float2(fmaf(-e, sn, cs), fmaf(e, cs, sn));
+}
+
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 v = __bfloat1622float2(h[i]); f[2 * i] = v.x; f[2 * i + 1] = v.y; }
+}
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
+    uint4 w;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = w;
+}
+
+struct Pools {
+    uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+};
+struct Rows {
+    const int32_t *row_slot, *row_pos, *page_table;
+    int page_table_stride, page_size;
+};
+
+// Eight elements of half a group (its other half is the neighbouring lane's): their word of codes and the group's byte.
+__device__ __forceinline__ void put8(uint8_t* codes, uint8_t* scales, size_t at, int d, int e, const float (&x)[8], bool on) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, magnitude(x[i]));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    if (!on) return;
+    float s;
+    const int byte = scale_byte(most, s);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= code(x[i], s) << (4 * i);
+    *reinterpret_cast<uint32_t*>(codes + at * (d / 2) + e / 2) = w;
+    if (e % kGroup == 0) scales[at * (d / kGroup) + e / kGroup] = (uint8_t)byte;
+}
+
+// `lanes` = d / 16 neighbouring lanes share a head.  Lane p < rotated / 16 has elements 8p .. 8p + 7 and their partners rotated / 2
+// further on; the lanes behind share the elements that are not rotated the same way.  Sizes are such that an even lane and the next
+// one always hold the two halves of one group (rotated and the rest multiples of 32).
+template <typename T, typename TG>
+__global__ void __launch_bounds__(kThreads)
+append_kernel(const T* __restrict__ qkv, T* q_out, size_t q_out_stride, const TG* __restrict__ q_gain, const TG* __restrict__ k_gain,
+              const float* __restrict__ inv_freq, int rotated, const __grid_constant__ Rows rows, const __grid_constant__ Pools pools,
+              int nq, int nkv, int d, float eps, int store, int heads_per_block, int lanes) {
+    extern __shared__ __align__(16) float2 turns[];                  // [rotated / 2]: the row's, shared by the block's heads
+    dependents_may_launch();
+    // positions, slots and page tables come from the host before the step: the turns and the row's place in the cache are worked
+    // out while the kernel ahead (the projection) is still running
+    const int row = blockIdx.x;
+    const int total = nq + 2 * nkv, used = store ? total : nq;
+    const int begin = blockIdx.y * heads_per_block, end = min(used, begin + heads_per_block);
+    const int half = rotated >> 1;
+    const int pos = rows.row_pos[row];
+    if (begin < nq + nkv)
+        for (int i = threadIdx.x; i < half; i += kThreads) turns[i] = turn_of(pos, inv_freq[i]);
+    int page = 0;
+    if (store) page = rows.page_table[(size_t)rows.row_slot[row] * rows.page_table_stride + pos / rows.page_size];
+    __syncthreads();
+    wait_for_predecessor();
+    const T* in = qkv + (size_t)row * total * d;
+    const int part = threadIdx.x % lanes, pairs = half >> 3;
+    const bool turned = part < pairs;
+    const int rest = d - rotated;
+    const int e0 = turned ? 8 * part : rotated + 8 * (part - pairs), e1 = e0 + (turned ? half : rest >> 1);
+    const int heads_per_pass = kThreads / lanes;
+    for (int h0 = begin; h0 < end; h0 += heads_per_pass) {           // the same trip count for every lane
+        const int head = h0 + threadIdx.x / lanes;
+        const bool on = head < end;
+        float x0[8], x1[8];
+        if (on) {
+            load8(in + (size_t)head * d + e0, x0);
+            load8(in + (size_t)head * d + e1, x1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0.0f;
+        }
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { ss = fmaf(x0[i], x0[i], ss); ss = fmaf(x1[i], x1[i], ss); }
+        for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const bool is_q = head < nq, is_v = head >= nq + nkv;
+        if (on && !is_v) {
+            const TG* gain = is_q ? q_gain : k_gain;
+            if (gain) {
+                const float inv = rsqrtf(ss / (float)d + eps);
+                float g0[8], g1[8];
+                load8(gain + e0, g0);
+                load8(gain + e1, g1);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { x0[i] = x0[i] * inv * g0[i]; x1[i] = x1[i] * inv * g1[i]; }
+            }
+            if (turned) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 t = turns[e0 + i];
+                    const float a = x0[i], b = x1[i];
+                    x0[i] = a * t.x - b * t.y;
+                    x1[i] = b * t.x + a * t.y;
+                }
+            }
+        }
+        if (on && is_q) {
+            T* out = q_out + (size_t)row * q_out_stride + (size_t)head * d;
+            store8(out + e0, x0);
+            store8(out + e1, x1);
+        }
+        const bool cached = on && !is_q;
+        const size_t at = cached ? place(page, nkv, (head - nq) % nkv, rows.page_size, pos % rows.page_size) : 0;
+        uint8_t* codes = is_v ? pools.v_codes : pools.k_codes;
+        uint8_t* scales = is_v ? pools.v_scales : pools.k_scales;
+        put8(codes, scales, at, d, e0, x0, cached);                  // (every lane: a group's two lanes exchange their maxima)
+        put8(codes, scales, at, d, e1, x1, cached);
+    }
+}
+
+// Any head size that groups divide and any even number of rotated elements: a warp a head, the head in shared memory.
+template <typename T, typename TG>
+__global__ void __launch_bounds__(kWarps * 32)
+append_any_kernel(const T* __restrict__ qkv, T* q_out, size_t q_out_stride, const TG* __restrict__ q_gain, const TG* __restrict__ k_gain,
+                  const float* __restrict__ inv_freq, int rotated, const __grid_constant__ Rows rows, const __grid_constant__ Pools pools,
+                  int nq, int nkv, int d, float eps, int store) {
+    extern __shared__ float shared[];                                // [kWarps][d], then the turns [rotated / 2]
+    float2* turns = reinterpret_cast<float2*>(shared + kWarps * d);
+    dependents_may_launch();
+    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int total = nq + 2 * nkv, used = store ? total : nq;
+    const int half = rotated >> 1;
+    const int pos = rows.row_pos[row];
+    for (int i = threadIdx.x; i < half; i += kWarps * 32) turns[i] = turn_of(pos, inv_freq[i]);
+    int page = 0;
+    if (store) page = rows.page_table[(size_t)rows.row_slot[row] * rows.page_table_stride + pos / rows.page_size];
+    __syncthreads();
+    wait_for_predecessor();
+    float* y = shared + warp * d;
+    for (int head = blockIdx.y * kWarps + warp; head < used; head += gridDim.y * kWarps) {
+        const T* in = qkv + ((size_t)row * total + head) * d;
+        const bool is_q = head < nq, is_v = head >= nq + nkv;
+        const TG* gain = is_v ? nullptr : (is_q ? q_gain : k_gain);
+        float ss = 0.0f;
+        for (int i = lane; i < d; i += 32) {
+            const float x = ldf(in, i);
+            y[i] = x;
+            ss = fmaf(x, x, ss);
+        }
+        ss = warp_sum(ss);
+        __syncwarp();
+        if (!is_v) {
+            const float inv = gain ? rsqrtf(ss / (float)d + eps) : 1.0f;
+            for (int i = lane; i < half; i += 32) {
+                const float a = gain ? y[i] * inv * ldf(gain, i) : y[i], b = gain ? y[i + half] * inv * ldf(gain, i + half) : y[i + half];
+                y[i] = a * turns[i].x - b * turns[i].y;
+                y[i + half] = b * turns[i].x + a * turns[i].y;
+            }
+            if (gain)
+                for (int i = rotated + lane; i < d; i += 32) y[i] = y[i] * inv * ldf(gain, i);
+            __syncwarp();
+        }
+        if (is_q) {
+            T* out = q_out + (size_t)row * q_out_stride + (size_t)head * d;
+            for (int i = lane; i < d; i += 32) stf(out, i, y[i]);
+        } else {
+            uint8_t* codes = is_v ? pools.v_codes : pools.k_codes;
+            uint8_t* scales = is_v ? pools.v_scales : pools.k_scales;
+            const size_t at = place(page, nkv, (head - nq) % nkv, rows.page_size, pos % rows.page_size);
+            for (int g = lane; g < d / kGroup; g += 32) {
+                uint32_t most = 0;
+                for (int i = 0; i < kGroup; ++i) most = max(most, magnitude(y[g * kGroup + i]));
+                float s;
+                scales[at * (d / kGroup) + g] = (uint8_t)scale_byte(most, s);
+                for (int i = 0; i < kGroup; i += 2)
+                    codes[at * (d / 2) + (g * kGroup + i) / 2] = (uint8_t)(code(y[g * kGroup + i], s) | code(y[g * kGroup + i + 1], s) << 4);
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// keys[r, h, :], values[r, h, :] = what the cache holds for position positions[r] of slot slots[r].  A thread a group.
+template <typename TO>
+__global__ void __launch_bounds__(kThreads)
+read_kernel(const __grid_constant__ Rows rows, const __grid_constant__ Pools pools, TO* __restrict__ keys, TO* __restrict__ values,
+            long long groups, int nkv, int d) {
+    dependents_may_launch();
+    wait_for_predecessor();
+    const int per_head = d / kGroup;
+    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= groups) return;
+    const bool is_v = blockIdx.y != 0;
+    const int g = (int)(i % per_head), head = (int)(i / per_head % nkv);
+    const long long row = i / ((long long)per_head * nkv);
+    const int pos = rows.row_pos[row];
+    const int page = rows.page_table[(size_t)rows.row_slot[row] * rows.page_table_stride + pos / rows.page_size];
+    const size_t at = place(page, nkv, head, rows.page_size, pos % rows.page_size);
+    const uint2 w = *reinterpret_cast<const uint2*>((is_v ? pools.v_codes : pools.k_codes) + at * (d / 2) + g * 8);
+    const float s = scale_of((is_v ? pools.v_scales : pools.k_scales)[at * per_head + g]);
+    TO* out = (is_v ? values : keys) + ((size_t)row * nkv + head) * d + g * kGroup;
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = value_of(w.x, e, s);
+    store8(out, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = value_of(w.y, e, s);
+    store8(out + 8, y);
+}
+
+static int check_sizes(const char* what, int nkv, int d, int page_size) {
+    if (d < kGroup || d % kGroup != 0 || d > 256) {
+        set_last_error("%s: a cache in 4 bits takes head sizes that are multiples of %d up to 256, not %d", what, kGroup, d);
+        return kBadShape;
+    }
+    if (nkv <= 0 || page_size <= 0) {
+        set_last_error("%s: bad number of key/value heads (%d) or page size (%d)", what, nkv, page_size);
+        return kBadShape;
+    }
+    return 0;
+}
+
+static bool aligned(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+template <typename T, typename TG>
+static int launch_append(const T* qkv, T* q_out, size_t q_out_stride, const TG* q_gain, const TG* k_gain, const float* inv_freq, int rotated,
+                         const Rows& where, const Pools& pools, int rows, int nq, int nkv, int d, float eps, int store, cudaStream_t stream) {
+    const int used = store ? nq + 2 * nkv : nq, lanes = d / 16;
+    const bool in_pairs = d >= 32 && (lanes & (lanes - 1)) == 0 && rotated % 32 == 0 && (d - rotated) % 32 == 0;
+    const bool wide = aligned(qkv, 16) && aligned(q_out, 16) && q_out_stride * sizeof(T) % 16 == 0 && aligned(q_gain, 16)
+                      && aligned(k_gain, 16) && aligned(pools.k_codes, 4) && aligned(pools.v_codes, 4);
+    if (in_pairs && wide) {
+        // few rows: a pass of heads a block, so that the heads spread over the SMs; many rows: a row a block, whose turns serve all heads
+        const int pass = kThreads / lanes, blocks = rows >= 4 * device_sm_count() ? 1 : (used + pass - 1) / pass;
+        const int each = blocks == 1 ? used : pass;
+        launch_kernel(append_kernel<T, TG>, dim3(rows, blocks), kThreads, (size_t)(rotated / 2) * sizeof(float2), stream, qkv, q_out,
+                      q_out_stride, q_gain, k_gain, inv_freq, rotated, where, pools, nq, nkv, d, eps, store, each, lanes);
+    } else {
+        const int blocks = rows >= 4 * device_sm_count() ? 1 : (used + kWarps - 1) / kWarps;
+        launch_kernel(append_any_kernel<T, TG>, dim3(rows, blocks), kWarps * 32, (size_t)(kWarps * d + rotated) * sizeof(float), stream, qkv,
+                      q_out, q_out_stride, q_gain, k_gain, inv_freq, rotated, where, pools, nq, nkv, d, eps, store);
+    }
+    return CITLALI_LAUNCH_CHECK();
+}
+
+}  // namespace c4
+}  // namespace citlali
+
+using namespace citlali;
+
+extern "C" int citlali_cache4_append(const void* qkv, int dtype, void* q_out, size_t q_out_stride, const void* q_gain, const void* k_gain,
+                                     int gain_dtype, const float* inv_freq, int rotary_dim, const int32_t* row_slot, const int32_t* row_pos,
+                                     const int32_t* page_table, int page_table_stride, void* k_codes, void* k_scales, void* v_codes,
+                                     void* v_scales, int page_size, int rows, int nq, int nkv, int head_dim, float eps, int store,
+                                     cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (int bad = c4::check_sizes("cache4_append", store ? nkv : 1, head_dim, page_size)) return bad;
+    if (nq < 0 || nkv < 0 || nq + 2 * nkv <= 0 || (!store && nq == 0) || rotary_dim < 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim) {
+        set_last_error("cache4_append: bad head counts (%d, %d), or a rotated part (%d) that is odd or larger than the head (%d)", nq, nkv,
+                       rotary_dim, head_dim);
+        return kBadShape;
+    }
+    if (nq + 2 * nkv > 65535) {
+        set_last_error("cache4_append: too many heads (%d)", nq + 2 * nkv);
+        return kTooLarge;
+    }
+    const c4::Rows where = {row_slot, row_pos, page_table, page_table_stride, page_size};
+    const c4::Pools pools = {(uint8_t*)k_codes, (uint8_t*)k_scales, (uint8_t*)v_codes, (uint8_t*)v_scales};
+    return CITLALI_DISPATCH_FLOAT(dtype, T, [&]() {
+        return CITLALI_DISPATCH_FLOAT(gain_dtype, TG, [&]() {
+            return c4::launch_append<T, TG>((const T*)qkv, (T*)q_out, q_out_stride, (const TG*)q_gain, (const TG*)k_gain, inv_freq, rotary_dim,
+                                            where, pools, rows, nq, nkv, head_dim, eps, store, stream);
+        });
+    });
+}
+
+extern "C" int citlali_cache4_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                                   const int32_t* page_table, int page_table_stride, int page_size, const int32_t* slots,
+                                   const int32_t* positions, void* keys, void* values, int out_dtype, int rows, int nkv, int head_dim,
+                                   cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (int bad = c4::check_sizes("cache4_read", nkv, head_dim, page_size)) return bad;
+    if (!c4::aligned(k_codes, 8) || !c4::aligned(v_codes, 8) || !c4::aligned(keys, 16) || !c4::aligned(values, 16)) {
+        set_last_error("cache4_read: codes must be 8-byte and rows 16-byte aligned");
+        return kBadAlignment;
+    }
+    const long long groups = (long long)rows * nkv * (head_dim / c4::kGroup), blocks = (groups + c4::kThreads - 1) / c4::kThreads;
+    if (blocks > 0x7fffffffLL) {
+        set_last_error("cache4_read: too many rows (%d)", rows);
+        return kTooLarge;
+    }
+    const c4::Rows where = {slots, positions, page_table, page_table_stride, page_size};
+    const c4::Pools pools = {(uint8_t*)k_codes, (uint8_t*)k_scales, (uint8_t*)v_codes, (uint8_t*)v_scales};
+    return CITLALI_DISPATCH_FLOAT(out_dtype, TO, [&]() {
+        launch_kernel(c4::read_kernel<TO>, dim3((unsigned)blocks, 2), c4::kThreads, 0, stream, where, pools, (TO*)keys, (TO*)values, groups,
+                      nkv, head_dim);
+        return CITLALI_LAUNCH_CHECK();
+    });
+}

@@ -1,0 +1,71 @@
+// Keys and values in 4 bits: what a byte stands for, and how numbers become bytes.
+//
+// 16 consecutive elements of a head of one token are a group.  A group has one scale s, held as a byte b that is the upper part of
+// the half s / 8: s = 8 half(b << 7), 5 bits of exponent and 3 of fraction, no sign (from 2^-11 on four significant bits, below that
+// the multiples of 2^-14).  An element is a whole number c of [-7, 7], held as c + 8 in 4 bits, element 2i in the low half of byte i.
+// The value is c s: 4.5 bits an element.
+//   s = the number nearest to min(max |x|, 3360) / 7 that a byte can be (at most 480), c = the whole number nearest to x / s, ties to even.
+// A group with an element that is not finite has b = 0xff, a NaN, and all its elements read as NaN: as with a cache of 16 bits, what
+// is wrong in a token reaches every row that sees the token, and no other.
+//
+// Why these numbers.  c s has at most 3 + 4 significant bits: it is exact in bfloat16, and c s / 8 in half, so the kernels that put
+// codes back into operands of the tensor cores round nothing.  s / 8 stays below 63.5 so that the constant 1032 (s / 8) of that
+// conversion is finite in half (see Words in attention4.cu).  A scale for 16 elements costs half a bit an element; per 32 elements
+// with 16 bits it would cost the same and leave a larger step (2.1 against 2.4 standard deviations to the largest of a group).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace citlali {
+namespace c4 {
+
+constexpr int kGroup = 16;
+constexpr float kUnit = 8.0f;
+constexpr float kLargestScale = 480.0f;
+constexpr int kNoNumber = 0xff;
+
+// |x| as a whole number: in the order of the magnitudes, infinities and then NaNs last (fmaxf would lose a NaN).
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// The scale's byte for a group whose largest magnitude is `most`, and the scale.  The division and the two roundings are exact
+// in the sense that the same numbers come out in any precision for elements of 16 bits (a tie is seen as one).
+__device__ __forceinline__ int scale_byte(uint32_t most, float& s) {
+    if (most >= 0x7f800000u) {
+        s = __int_as_float(0x7fc00000);
+        return kNoNumber;
+    }
+    const float wanted = fminf(__fdiv_rn(__uint_as_float(most), 7.0f), kLargestScale);
+    if (wanted < 0.00048828125f) {                                   // below 2^-11: multiples of 2^-14
+        const float n = rintf(wanted * 16384.0f);
+        s = n * 0.00006103515625f;
+        return (int)n;
+    }
+    uint32_t bits = __float_as_uint(wanted);
+    bits = (bits + 0x7ffffu + ((bits >> 20) & 1u)) & 0xfff00000u;    // three bits of fraction, ties to even
+    s = __uint_as_float(bits);
+    return (int)(((bits >> 23) - 127u + 12u) << 3 | ((bits >> 20) & 7u));
+}
+
+// c + 8 of an element.
+__device__ __forceinline__ uint32_t code(float x, float s) {
+    if (!(s > 0.0f)) return 8u;                                      // a group of zeros, or one that holds no number
+    const float c = fminf(fmaxf(rintf(__fdiv_rn(x, s)), -7.0f), 7.0f);
+    return (uint32_t)((int)c + 8);
+}
+
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+    return __half2float(__ushort_as_half((unsigned short)(byte << 7))) * kUnit;
+}
+// The value of nibble i of a word of eight codes.
+__device__ __forceinline__ float value_of(uint32_t word, int i, float s) { return (float)((int)((word >> (4 * i)) & 15u) - 8) * s; }
+
+// Where a token's key or value of a head lies: codes [page][head][token of the page][d / 2], scales [page][head][token][d / 16].
+__device__ __forceinline__ size_t place(int page, int nkv, int head, int page_size, int at) {
+    return ((size_t)page * nkv + head) * page_size + at;             // times d / 2 or d / 16
+}
+
+}  // namespace c4
+}  // namespace citlali

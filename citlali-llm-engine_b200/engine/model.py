@@ -13,6 +13,7 @@ from typing import Dict, List, Optional
 import torch
 
 from .. import ops
+from ..cache import KVRequirement
 from ..config.spec import ModelSpec
 from ..errors import require
 from ..parts.base import BuildContext, StepBatch, build_part, named_sources, part_class
@@ -25,6 +26,13 @@ def _numel(shape) -> int:
     for d in shape:
         n *= int(d)
     return n
+
+
+def _keeps_keys(requirement) -> bool:
+    """Whether a requirement, or one nested in it, asks for keys and values."""
+    if isinstance(requirement, (tuple, list)):
+        return any(_keeps_keys(r) for r in requirement)
+    return isinstance(requirement, KVRequirement)
 
 
 def _build_layers(spec: ModelSpec):
@@ -85,6 +93,12 @@ class DecoderModel:
         self.embedding: Optional[torch.Tensor] = None
         self.tied = None
         streams = spec.residual_streams
+        if ctx.packed4:
+            for i, block in enumerate(self.layers):
+                for part in block.parts():
+                    wanted = part.cache_requirement() if callable(getattr(part, "cache_requirement", None)) else None
+                    require(not _keeps_keys(wanted) or getattr(part, "takes_packed4", False),
+                            f"layer {i}'s mixer ({type(part).__name__}) does not cache its keys and values in 4 bits")
         for i, block in enumerate(self.layers):
             takes = getattr(block, "residual_streams", None)
             require(takes == streams, f"layer {i}'s block works on {takes or 'one'} residual stream(s), the model has "
@@ -127,6 +141,8 @@ class DecoderModel:
         out = {"elementwise", "gemm_simt" if dtype == torch.float32 else "gemm_tcgen05"}
         if self.spec.residual_streams is not None:
             out.add("hyper_connection")
+        if self.ctx.packed4:
+            out.update(("cache4", "attention4_rows") if dtype == torch.float32 else ("cache4", "attention4"))
         for owner in [self.final_norm, self.embedding_norm, self.embedding_addition] + [p for b in self.layers for p in [b] + list(b.parts())]:
             if owner is not None:
                 out.update(named_sources(owner, dtype))

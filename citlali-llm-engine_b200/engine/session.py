@@ -37,6 +37,15 @@ def parse_dtype(name) -> torch.dtype:
     return _DTYPES[str(name)]
 
 
+def parse_cache_dtype(name, dtype) -> bool:
+    """Whether keys and values are held in 4 bits: ``name`` is None, "int4", or the compute dtype."""
+    if name is None or name == "int4":
+        return name == "int4"
+    require(not isinstance(name, str) or name in _DTYPES, f"cache_dtype must be int4 or the compute dtype, not '{name}'")
+    require(parse_dtype(name) == dtype, f"cache_dtype must be int4 or the compute dtype ({dtype}), not {name}")
+    return False
+
+
 def _cuda_device(device) -> torch.device:
     dev = torch.device(device)
     require(dev.type == "cuda", f"models run on a CUDA device only, not on '{dev}'")
@@ -58,17 +67,18 @@ class InferenceSession:
 
     # ---- loading ---------------------------------------------------------------------
     def load_model(self, model_path: str, max_context: int = 2048, dtype="bfloat16", device="cuda:0",
-                   max_batch: int = 8, max_tokens: Optional[int] = None, progress=None) -> "InferenceSession":
+                   max_batch: int = 8, max_tokens: Optional[int] = None, progress=None, cache_dtype=None) -> "InferenceSession":
         """``max_context``: the most tokens one sequence may hold, capped by the model's own limit
         (src/model/qwen_model.cpp:51).  ``max_batch``: sequence slots.  ``max_tokens``: the most
         tokens all live sequences hold together, each rounded up to whole cache pages (default:
-        every slot full)."""
+        every slot full).  ``cache_dtype``: what keys and values are held in: None, ``dtype``; "int4", 4 bits with a scale
+        for 16 elements, 9/32 of bfloat16's bytes (models whose attention can: ``takes_packed4``)."""
         config = config_from_model_dir(model_path)
         dev = _cuda_device(device)
         loader = WeightLoader(model_path)
         try:
             spec = config.to_model_spec()
-            ctx = self._context(dev, dtype)
+            ctx = self._context(dev, dtype, cache_dtype)
             model = DecoderModel(spec, ctx)
             ops.prepare_kernels(model.kernel_sources())
             weights = loader.load_all(model.tensor_specs(), device="cpu", progress=progress)
@@ -79,7 +89,7 @@ class InferenceSession:
 
     def load_random(self, config, seed: int, max_context: int = 2048, dtype="bfloat16", device="cuda:0",
                     max_batch: int = 8, max_tokens: Optional[int] = None, gain_spread: float = 0.0,
-                    stored_dtype=None) -> "InferenceSession":
+                    stored_dtype=None, cache_dtype=None) -> "InferenceSession":
         """Random weights made on the device, tensor by tensor, for measurements and for tests at
         sizes a folder would be too large for: nothing is written.  ``stored_dtype`` (default:
         ``dtype``) is the precision the values are rounded to before the model takes them, as if
@@ -87,7 +97,7 @@ class InferenceSession:
         values whatever they compute in."""
         dev = _cuda_device(device)
         spec = config.to_model_spec()
-        ctx = self._context(dev, dtype)
+        ctx = self._context(dev, dtype, cache_dtype)
         model = DecoderModel(spec, ctx)
         ops.prepare_kernels(model.kernel_sources())
         stored = parse_dtype(stored_dtype if stored_dtype is not None else dtype)
@@ -102,9 +112,10 @@ class InferenceSession:
         model.bind(handles)
         return self._finish(config, model, max_context, max_batch, max_tokens)
 
-    def _context(self, dev, dtype) -> BuildContext:
+    def _context(self, dev, dtype, cache_dtype=None) -> BuildContext:
+        dtype, packed4 = parse_dtype(dtype), parse_cache_dtype(cache_dtype, dtype)
         flag = torch.zeros(4, dtype=torch.int32, device=dev)
-        return BuildContext(device=dev, dtype=parse_dtype(dtype), error_flag=flag)
+        return BuildContext(device=dev, dtype=dtype, error_flag=flag, packed4=packed4)
 
     def _finish(self, config, model, max_context, max_batch, max_tokens):
         require(max_context > 0 and max_batch > 0, "max_context and max_batch must be positive")

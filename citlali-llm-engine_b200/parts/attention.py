@@ -11,6 +11,9 @@ residual stream.
 Parameters: hidden_size, num_heads, num_kv_heads, head_dim, qk_norm_eps (None: no head norm),
 position ({"kind": ..., ...}), window (None: all keys), kv_projection (False: the layer has no
 k/v matrices and only reads another layer's cache).
+
+Bound in a context with ``packed4`` the layer caches its keys and values in 4 bits (csrc/cache4.cuh); what it does is otherwise
+the same.
 """
 from __future__ import annotations
 
@@ -27,6 +30,9 @@ from .linear import DenseLinear
 
 
 class GQAttention:
+    takes_packed4 = True       # it can cache in 4 bits
+    packed4 = False            # it does (set by bind)
+
     def __init__(self, params, prefix: str):
         self.hidden = int(params["hidden_size"])
         self.nq = int(params["num_heads"])
@@ -56,8 +62,8 @@ class GQAttention:
     def graph_safe(self) -> bool:
         """A step of single tokens reads slots and positions from device memory only: true once bound
         to a dtype and head size that the split-context kernel takes; the other attention kernels size
-        their launch from the host's lists."""
-        if getattr(self, "dtype", None) is None or not ops.attention_steps_from_device(self.dtype, self.d):
+        their launch from the host's lists (over a cache in 4 bits none does)."""
+        if getattr(self, "dtype", None) is None or not (self.packed4 or ops.attention_steps_from_device(self.dtype, self.d)):
             return False
         return self.position.inv_freq is not None or bool(getattr(self.position, "graph_safe", False))
 
@@ -78,7 +84,7 @@ class GQAttention:
     def cache_requirement(self):
         if not self.kv_projection:
             return None
-        return KVRequirement(self.nkv, self.d, None if self.window is None else int(self.window))
+        return KVRequirement(self.nkv, self.d, None if self.window is None else int(self.window), packed4=self.packed4)
 
     def bind(self, weights, ctx):
         self.qkv.bind(weights, ctx)
@@ -100,6 +106,9 @@ class GQAttention:
             self.rotary_dim = self.d
             self.inv_freq = torch.zeros(self.d // 2, dtype=torch.float32, device=ctx.device)   # no rotation by the kernel
         self.dtype = ctx.dtype
+        self.packed4 = ctx.packed4
+        require(not self.packed4 or self.d % 16 == 0 and self.d <= 256,
+                f"{self.prefix}: a cache in 4 bits takes head sizes that are multiples of 16 up to 256, not {self.d}")
 
     # ---- the norm in front of this part, done by its products ---------------------------------------------------
     def can_absorb_norm(self) -> bool:
@@ -124,6 +133,8 @@ class GQAttention:
         else:
             qkv = self.qkv.forward(h)
         store = write_cache and self.kv_projection
+        if req.packed4:
+            return self._forward_packed4(qkv, batch, cache_view, residual, store, emit)
         common = (batch.row_slot, batch.row_pos, cache_view.page_table, cache_view.keys, cache_view.values,
                   cache_view.page_size, self.nq, nkv_here, self.d, float(self.eps or 0.0))
         if self.fused_position:
@@ -139,6 +150,24 @@ class GQAttention:
         out = torch.empty((batch.rows, self.nq * self.d), dtype=self.dtype, device=qkv.device)
         ops.attention(qkv, qkv.shape[1], cache_view, batch, out, self.nq, self.nkv, self.d,
                       int(self.window or 0), self.scale)
+        self.o.forward(out, accumulate_into=residual, emit=emit)
+        return residual
+
+    def _forward_packed4(self, qkv, batch, cache_view, residual, store, emit):
+        nkv_here = self.nkv if self.kv_projection else 0
+        rows = (cache_view, batch.row_slot, batch.row_pos, self.nq, nkv_here, self.d)
+        if self.fused_position:
+            ops.cache4_append(qkv, *rows, self.inv_freq, self.rotary_dim, self.q_gain, self.k_gain, float(self.eps or 0.0), store=store)
+        else:
+            # as with a cache of 16 bits: head norm with the keys kept in the row, the encoding's own work, then the store
+            ops.qk_norm_rope_cache(qkv, self.q_gain, self.k_gain, self.inv_freq, self.rotary_dim, batch.row_slot, batch.row_pos,
+                                   cache_view.page_table, None, None, cache_view.page_size, self.nq, nkv_here, self.d,
+                                   float(self.eps or 0.0), write_cache="keys_in_place" if store else False)
+            self.position.apply(qkv, batch, self.nq, nkv_here, self.d)
+            if store:
+                ops.cache4_append(qkv, *rows, self.inv_freq[:0], 0)
+        out = torch.empty((batch.rows, self.nq * self.d), dtype=self.dtype, device=qkv.device)
+        ops.cache4_attention(qkv, qkv.shape[1], cache_view, batch, out, self.nq, self.nkv, self.d, int(self.window or 0), self.scale)
         self.o.forward(out, accumulate_into=residual, emit=emit)
         return residual
 

@@ -78,10 +78,12 @@ def named_sources(part, dtype) -> tuple:
 class BuildContext:
     """Where and how a model is built: device, compute dtype (bfloat16: the serving kernels and
     precisions; float32: everything in true 32-bit) and the device word kernels raise on a
-    fault they detect themselves."""
+    fault they detect themselves.  ``packed4``: keys and values are to be cached in 4 bits, by mixers that say they can
+    (``takes_packed4``)."""
     device: torch.device
     dtype: torch.dtype
     error_flag: Optional[torch.Tensor] = None
+    packed4: bool = False
 
     @property
     def is_float32(self) -> bool:

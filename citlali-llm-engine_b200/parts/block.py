@@ -87,7 +87,7 @@ class PreNormResidualBlock:
                 or not mixer.fused_position or cache_view is None or batch.is_decode or torch.cuda.is_current_stream_capturing()):
             return False
         req = cache_view.requirement
-        return (req.head_dim == mixer.d and req.num_kv_heads == mixer.nkv and cache_view.keys.dtype == torch.bfloat16
+        return (req.head_dim == mixer.d and req.num_kv_heads == mixer.nkv and not req.packed4 and cache_view.keys.dtype == torch.bfloat16
                 and ops.dense_layer_supports(mixer.nq, mixer.nkv, mixer.d, cache_view.page_size, batch.max_new))
 
     def forward(self, x, batch, cache_view, write_cache=True):
