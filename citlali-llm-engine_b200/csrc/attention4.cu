@@ -21,11 +21,12 @@
 // element above 2^-32 of that.  P is rounded to half (half a step is 2^-11 of it, an eighth of bfloat16's); all weights are 2^15 times
 // what the formula says, which the division takes out again, so that those below 2^-14 of the largest are not subnormal halves.
 //
-// Work.  16 keys are a unit.  The units of all (sequence, key/value head, tile) are laid end to end and dealt out evenly to the
-// blocks, whatever the sequences' lengths, which are read on the device: the launch depends on none and can be captured.  A block's
-// share is made of pieces of one or more (sequence, head, tile); its eight warps take the piece's units in turn, and are merged in
-// warp order.  A piece that is the whole goes to memory as the result, another as (m, l, O) in float, which a second kernel merges in
-// the order of the keys.  So every sum has an order that the step's lengths fix.
+// Work.  16 keys are a unit.  The units of all segments (sequence, key/value head, tile) lie end to end on a line, a little room
+// ahead of each segment for what it costs to begin one, and the line is dealt out evenly to the warps, eight neighbouring ones a
+// block, whatever the sequences' lengths, which are read on the device: the launch depends on none and can be captured.  A warp that
+// has a whole segment stores its result.  The parts of one that several warps share are merged by the block when its warps are done,
+// in the order of the keys, and the parts of one that several blocks share go to memory as (m, l, O) in float, for a second kernel
+// that merges them in the same order.  So every sum has an order that the step's lengths fix.
 #include "api.h"
 #include "cache4.cuh"
 #include "common.cuh"
@@ -37,7 +38,8 @@ namespace c4 {
 constexpr int kPage = 64, kUnitKeys = 16;
 constexpr int kWarps4 = 8, kThreads4 = 32 * kWarps4;
 constexpr float kWeightBits = 15.0f;
-constexpr int kLeastUnits = 8;          // of a block's share: a unit a warp
+constexpr float kNoScore = -3.402823466e+38f;
+constexpr int kRoom = 4;                // what beginning a segment costs, in units
 
 struct Attention4 {
     const __nv_bfloat16* q;
@@ -58,6 +60,7 @@ struct Attention4 {
 // What a sequence of the step asks for: `units` of 16 keys for each of `segments` (head tile of a key/value head, token tile).
 struct Sequence {
     int past, fresh, row, first_unit, units, tiles, segments;
+    __device__ __forceinline__ uint32_t length() const { return (uint32_t)segments * (units + kRoom); }      // on the line
 };
 __device__ __forceinline__ Sequence sequence_of(const Attention4& a, int b) {
     Sequence s;
@@ -71,76 +74,71 @@ __device__ __forceinline__ Sequence sequence_of(const Attention4& a, int b) {
     s.segments = s.tiles * a.nkv * a.head_tiles;
     return s;
 }
-
-// A place in the line of all units, and the piece of one segment from there to the share's end.
-struct Cursor {
-    long long x, base;                                   // the place, and where its sequence begins
-    int b, segment, from, to;                            // units [from, to) of the sequence's segment
-    Sequence s;
+// One segment: its tile's tokens and query heads.
+struct Tile {
+    int token0, tokens, head0, heads, kv;
+    __device__ __forceinline__ int used() const { return tokens * heads; }               // columns
 };
-__device__ __forceinline__ bool enter(const Attention4& a, Cursor& c, long long end) {
-    if (c.x >= end) return false;
-    while (c.x >= c.base + (long long)c.s.segments * c.s.units) {      // ends: c.x < end <= all units
-        c.base += (long long)c.s.segments * c.s.units;
-        ++c.b;
-        c.s = sequence_of(a, c.b);
-    }
-    const int off = (int)(c.x - c.base);
-    c.segment = off / c.s.units;
-    c.from = off - c.segment * c.s.units;
-    c.to = (int)min((long long)c.s.units, c.from + (end - c.x));
-    return true;
-}
-__device__ __forceinline__ bool next_piece(const Attention4& a, Cursor& c, long long end) {
-    c.x += c.to - c.from;
-    return enter(a, c, end);
+__device__ __forceinline__ Tile tile_of(const Attention4& a, const Sequence& s, int segment) {
+    Tile t;
+    const int part = segment / s.tiles, head_tile = part % a.head_tiles;
+    t.kv = part / a.head_tiles;
+    t.token0 = (segment - part * s.tiles) * a.tokens;
+    t.tokens = min(a.tokens, s.fresh - t.token0);
+    t.head0 = t.kv * a.group + head_tile * a.heads;
+    t.heads = min(a.heads, a.group - head_tile * a.heads);
+    return t;
 }
 
-// All lanes of a warp: the units of the step, and the share of a block of `blocks`.
-__device__ __forceinline__ long long share_of(const Attention4& a, int blocks) {
-    long long total = 0;
-    for (int b = threadIdx.x & 31; b < a.sequences; b += 32) {
-        const Sequence s = sequence_of(a, b);
-        total += (long long)s.segments * s.units;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const long long wanted = (total + kLeastUnits - 1) / kLeastUnits;
-    const long long used = wanted < blocks ? (wanted > 0 ? wanted : 1) : blocks;
-    return (total + used - 1) / used;
+// A place on the line: its sequence and where that begins.
+struct Place {
+    uint32_t base;
+    int b;
+};
+// All lanes of a warp: the line's length.
+__device__ __forceinline__ uint32_t line_length(const Attention4& a) {
+    uint32_t total = 0;
+    for (int b = threadIdx.x & 31; b < a.sequences; b += 32) total += sequence_of(a, b).length();
+    return __reduce_add_sync(0xffffffffu, total);
 }
-// All lanes of a warp: the cursor at place x (with the piece up to `end`), or false where the line ends before.  `end` is cut to the line.
-__device__ __forceinline__ bool find(const Attention4& a, Cursor& c, long long x, long long& end) {
+// All lanes of a warp: the sequence of place x, which is on the line.
+__device__ __forceinline__ Place place_of(const Attention4& a, uint32_t x) {
     const int lane = threadIdx.x & 31;
-    long long run = 0;
-    bool found = false;
+    uint32_t run = 0;
     for (int b0 = 0; b0 < a.sequences; b0 += 32) {
-        long long mine = 0;
-        if (b0 + lane < a.sequences) {
-            const Sequence s = sequence_of(a, b0 + lane);
-            mine = (long long)s.segments * s.units;
-        }
-        long long sum = mine;
+        const uint32_t mine = b0 + lane < a.sequences ? sequence_of(a, b0 + lane).length() : 0;
+        uint32_t sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+            const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += up;
         }
-        const unsigned past = __ballot_sync(0xffffffffu, run + sum > x);
-        if (!found && past) {
-            const int which = __ffs(past) - 1;
-            c.b = b0 + which;
-            c.base = run + __shfl_sync(0xffffffffu, sum - mine, which);
-            found = true;
+        const unsigned behind = __ballot_sync(0xffffffffu, run + sum > x);
+        if (behind) {
+            const int which = __ffs(behind) - 1;
+            return {run + __shfl_sync(0xffffffffu, sum - mine, which), b0 + which};
         }
         run += __shfl_sync(0xffffffffu, sum, 31);
-        if (found && run >= end) break;
     }
-    if (!found) return false;
-    end = min(end, run);
-    c.x = x;
-    c.s = sequence_of(a, c.b);
-    return enter(a, c, end);
+    return {run, a.sequences};
+}
+// Units of the segment from place x to `end` (one warp's share ends there): [from, to), none if the share ends ahead of them.
+struct Piece {
+    int segment, from, to;
+    uint32_t first;                                      // the place of the segment's unit 0
+};
+__device__ __forceinline__ Piece piece_of(const Sequence& s, uint32_t base, uint32_t x, uint32_t end) {
+    Piece p;
+    const uint32_t each = s.units + kRoom;
+    p.segment = (int)((x - base) / each);
+    p.first = base + p.segment * each + kRoom;
+    p.from = x > p.first ? (int)(x - p.first) : 0;
+    p.to = end > p.first ? min(s.units, (int)(end - p.first)) : 0;
+    return p;
+}
+// How the line is dealt out: places of a warp.
+__device__ __forceinline__ uint32_t places_of_a_warp(uint32_t length, int blocks) {
+    return (length + blocks * kWarps4 - 1) / (blocks * kWarps4);
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -189,15 +187,30 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
     }
 }
 
-// Sizes of a block's shared memory: the warps' rings, then where the warps are merged.
+template <int N>
+__device__ __forceinline__ uint32_t load_bytes(const uint8_t* p) {
+    if constexpr (N == 1) return *p;
+    else if constexpr (N == 2) return *reinterpret_cast<const uint16_t*>(p);
+    else return *reinterpret_cast<const uint32_t*>(p);
+}
+
+// A part of a segment that its warp does not have whole, as the block's merge finds it.
+struct Part {
+    uint32_t first;                                      // the segment's place; ~0: there is no such part
+    int units, row, head0, heads, used;
+};
+
+// Sizes of a block's shared memory: the warps' rings (each at least as large as what its warp parks there at the end), then what a warp
+// parks of a segment that began ahead of it, and the parts' descriptions.
 template <int D, int NT>
 struct Layout {
     static constexpr int columns = 8 * NT;
     static constexpr int codes = kUnitKeys * D / 2, scales = kUnitKeys * D / kGroup, unit = 2 * (codes + scales);
+    static constexpr int parked = columns * (D + 2) * 4;
     static constexpr int stages = D == 64 ? 8 : (NT == 1 ? 4 : 6);
-    static constexpr int ring = kWarps4 * stages * unit;
-    static constexpr int parked = kWarps4 * columns * (D + 2) * 4;
-    static constexpr int bytes = ring + parked + kWarps4 * columns * 4 + columns * 8;
+    static constexpr int ring = stages * unit;
+    static_assert(ring >= parked && ring % 16 == 0 && parked % 16 == 0, "a warp parks its last part in its ring");
+    static constexpr int bytes = kWarps4 * (ring + parked + 2 * (int)sizeof(Part)) + kWarps4 * 2 * columns * 4 + columns * 8;
     static constexpr int per_sm = D == 256 ? 1 : (NT == 1 ? 2 : 1);
 };
 
@@ -209,62 +222,83 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     constexpr int KW = D / 32, VW = D / 64;              // words of a key and of a value that a lane holds
     extern __shared__ __align__(16) uint8_t shared[];
     dependents_may_launch();
-    wait_for_predecessor();
+    // (positions and page tables come from the host before the step; what other kernels write is read behind the wait)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, t = lane & 3;
-    const long long share = share_of(a, gridDim.x);
-    const long long begin = share * blockIdx.x;
-    long long end = begin + share;
-    Cursor c;
-    if (!find(a, c, begin, end)) return;                 // (all warps alike)
+    uint8_t* ring = shared + warp * L::ring;
+    float* early = reinterpret_cast<float*>(shared + kWarps4 * L::ring + warp * L::parked);      // [column][m, l, O]
+    Part* parts = reinterpret_cast<Part*>(shared + kWarps4 * (L::ring + L::parked));             // [warp][early, late]
+    float* weight = reinterpret_cast<float*>(parts + 2 * kWarps4);                               // [part][column]
+    float* whole = weight + 2 * kWarps4 * C;                                                     // [column]: M, then the sum
 
-    uint8_t* ring = shared + warp * (S * L::unit);
-    float* parked = reinterpret_cast<float*>(shared + L::ring);                       // [warp][column][m, l, O]
-    float* weight = reinterpret_cast<float*>(shared + L::ring + L::parked);           // [warp][column]
-    float* whole = weight + kWarps4 * C;                                              // [column]: M, then the sum
+    const uint32_t length = line_length(a), each = places_of_a_warp(length, gridDim.x);
+    const uint32_t begin = min(length, (blockIdx.x * kWarps4 + warp) * each), end = min(length, begin + each);
+    if (blockIdx.x * kWarps4 * each >= length) {         // (all warps alike)
+        wait_for_predecessor();
+        return;
+    }
+    if (lane < 2) parts[2 * warp + lane].first = ~0u;
+    Place here = begin < end ? place_of(a, begin) : Place{0, 0};
 
-    // the ring's own cursor, ahead of the one that computes
-    Cursor f = c;
-    bool more = true;
-    int fetch = f.from + warp;
+    // ---- the ring's own way along the line, ahead of the one that computes
+    uint32_t fetch_x = begin;                            // the next piece's place
+    Place fetch = here;
+    int fetch_unit = 0, fetch_end = 0, fetch_head = 0, page = 0, next_page = 0;
+    const int32_t* fetch_pages = a.table;
     auto load_next = [&](int slot) {
-        while (more && fetch >= f.to) {
-            more = next_piece(a, f, end);
-            fetch = f.from + warp;
+        while (fetch_unit == fetch_end && fetch_x < end) {                       // the next piece with a unit
+            Sequence s = sequence_of(a, fetch.b);
+            while (fetch_x >= fetch.base + s.length()) {
+                fetch.base += s.length();
+                s = sequence_of(a, ++fetch.b);
+            }
+            const Piece p = piece_of(s, fetch.base, fetch_x, end);
+            fetch_x = p.first + s.units;
+            if (p.to <= p.from) continue;
+            fetch_head = tile_of(a, s, p.segment).kv;
+            fetch_pages = a.table + (size_t)a.seq_slot[fetch.b] * a.table_stride;
+            fetch_unit = s.first_unit + p.from;
+            fetch_end = s.first_unit + p.to;
+            page = fetch_pages[fetch_unit >> 2];
+            next_page = fetch_pages[(fetch_end - 1) >> 2 > fetch_unit >> 2 ? (fetch_unit >> 2) + 1 : fetch_unit >> 2];
         }
-        if (more) {
-            const int unit = f.s.first_unit + fetch;
-            const int head = f.segment / f.s.tiles / a.head_tiles;
-            const int page = a.table[(size_t)a.seq_slot[f.b] * a.table_stride + (unit >> 2)];
-            const size_t at = place(page, a.nkv, head, kPage, (unit & 3) * kUnitKeys);
-            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + slot * L::unit);
-            const uint8_t *kc = a.k_codes + at * (D / 2), *vc = a.v_codes + at * (D / 2);
-            const uint8_t *ks = a.k_scales + at * (D / kGroup), *vs = a.v_scales + at * (D / kGroup);
+        if (fetch_unit < fetch_end) {
+            const size_t at = place(page, a.nkv, fetch_head, kPage, (fetch_unit & 3) * kUnitKeys);
+            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + slot * L::unit) + lane * 16;
+            const uint8_t *kc = a.k_codes + at * (D / 2) + lane * 16, *vc = a.v_codes + at * (D / 2) + lane * 16;
 #pragma unroll
-            for (int i = 0; i < L::codes / 16; i += 32) {
-                const int o = (i + lane) * 16;
-                fa::cp_async16(dst + o, kc + o);
-                fa::cp_async16(dst + L::codes + o, vc + o);
+            for (int i = 0; i < L::codes; i += 512) {
+                fa::cp_async16(dst + i, kc + i);
+                fa::cp_async16(dst + L::codes + i, vc + i);
             }
-            constexpr int each = L::scales / 16;         // 16-byte pieces of the scales of a unit's keys
-            if (lane < 2 * each) {
-                const int o = (lane % each) * 16;
-                fa::cp_async16(dst + 2 * L::codes + lane * 16, (lane < each ? ks : vs) + o);
+            constexpr int pieces = L::scales / 16;       // 16-byte pieces of the scales of a unit's keys
+            if (lane < 2 * pieces)
+                fa::cp_async16(dst + 2 * L::codes, (lane < pieces ? a.k_scales : a.v_scales) + at * (D / kGroup) + (lane % pieces) * 16);
+            ++fetch_unit;
+            if ((fetch_unit & 3) == 0) {
+                page = next_page;
+                if (fetch_unit + 4 < fetch_end) next_page = fetch_pages[(fetch_unit >> 2) + 1];
             }
-            fetch += kWarps4;
         }
         fa::cp_async_commit();
     };
+    wait_for_predecessor();
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) load_next(i);
     int slot = 0;
 
-    do {
+    for (uint32_t x = begin; x < end;) {
         // ---- the piece: its tile's columns and their queries
-        const int tile = c.segment % c.s.tiles, part = c.segment / c.s.tiles, head_tile = part % a.head_tiles, kv = part / a.head_tiles;
-        const int token0 = tile * a.tokens, tokens = min(a.tokens, c.s.fresh - token0);
-        const int head0 = kv * a.group + head_tile * a.heads, heads = min(a.heads, a.group - head_tile * a.heads);
-        const int used = tokens * heads;                 // columns
-        const int pos0 = c.s.past + token0, last = pos0 + tokens - 1;        // of the first and the last token
+        Sequence s = sequence_of(a, here.b);
+        while (x >= here.base + s.length()) {
+            here.base += s.length();
+            s = sequence_of(a, ++here.b);
+        }
+        const Piece piece = piece_of(s, here.base, x, end);
+        x = piece.first + s.units;
+        if (piece.to <= piece.from) continue;
+        const Tile tile = tile_of(a, s, piece.segment);
+        const int used = tile.used(), heads = tile.heads;
+        const int pos0 = s.past + tile.token0, last = pos0 + tile.tokens - 1;         // of the first and the last token
         const int low0 = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, low1 = a.window > 0 ? max(0, last - a.window + 1) : 0;
 
         uint32_t qf[NT][2 * KW][2];                      // [columns' eight][contraction step][b0, b1]
@@ -274,8 +308,8 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
         for (int n = 0; n < NT; ++n) {
             const int column = n * 8 + r;
             const bool on = column < used;
-            const __nv_bfloat16* src = a.q + (size_t)(c.s.row + token0 + (on ? column / heads : 0)) * a.q_stride
-                                       + (size_t)(head0 + (on ? column % heads : 0)) * D + t * (D / 4);
+            const __nv_bfloat16* src = a.q + (size_t)(s.row + tile.token0 + (on ? column / heads : 0)) * a.q_stride
+                                       + (size_t)(tile.head0 + (on ? column % heads : 0)) * D + t * (D / 4);
             uint4 raw[KW];
             uint32_t most = 0;
 #pragma unroll
@@ -291,17 +325,17 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
             const float by = __int_as_float((127 + up) << 23);
 #pragma unroll
             for (int w = 0; w < KW; ++w) {
-                float x[8];
+                float y[8];
                 const uint32_t* p = &raw[w].x;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[2 * i] = __uint_as_float(p[i] << 16) * by;
-                    x[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u) * by;
+                    y[2 * i] = __uint_as_float(p[i] << 16) * by;
+                    y[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u) * by;
                 }
-                qf[n][2 * w][0] = as_word(__floats2half2_rn(x[0], x[4]));
-                qf[n][2 * w][1] = as_word(__floats2half2_rn(x[1], x[5]));
-                qf[n][2 * w + 1][0] = as_word(__floats2half2_rn(x[2], x[6]));
-                qf[n][2 * w + 1][1] = as_word(__floats2half2_rn(x[3], x[7]));
+                qf[n][2 * w][0] = as_word(__floats2half2_rn(y[0], y[4]));
+                qf[n][2 * w][1] = as_word(__floats2half2_rn(y[1], y[5]));
+                qf[n][2 * w + 1][0] = as_word(__floats2half2_rn(y[2], y[6]));
+                qf[n][2 * w + 1][1] = as_word(__floats2half2_rn(y[3], y[7]));
             }
             const float back = __int_as_float((127 - up) << 23) * (a.scale_log2 * kUnit);
 #pragma unroll
@@ -310,38 +344,39 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                 seen[n][j] = pos0 + min(n * 8 + 2 * t + j, used - 1) / heads;
             }
         }
+        // m: the running maximum less kWeightBits; the lowest number there is where there is none, which no sum with a score overflows to a NaN
         float m[NT][2], l[NT][2], o[NT][D / 16][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            m[n][0] = m[n][1] = -INFINITY;
+            m[n][0] = m[n][1] = kNoScore;
             l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
         }
 
         // ---- its units
-        for (int u = c.from + warp; u < c.to; u += kWarps4) {
+        for (int u = s.first_unit + piece.from; u < s.first_unit + piece.to; ++u) {
             fa::cp_async_wait<S - 2>();
             __syncwarp();                                // the unit is there for all lanes, and all are done with the one before
             load_next(slot == 0 ? S - 1 : slot - 1);
             uint8_t* at = ring + slot * L::unit;
             slot = slot + 1 == S ? 0 : slot + 1;
-            const int key0 = (c.s.first_unit + u) * kUnitKeys;
+            const int key0 = u * kUnitKeys;
             if (key0 > last || key0 + kUnitKeys <= low0) continue;        // none of the tile's tokens sees any of them
             const bool border = key0 + kUnitKeys - 1 > pos0 || key0 < low1;
 
-            float s[NT][4];
+            float e[NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            for (int n = 0; n < NT; ++n) e[n][0] = e[n][1] = e[n][2] = e[n][3] = 0.0f;
             {
                 uint32_t ka[KW], kb[KW];
                 load_words<KW>(ka, at + r * (D / 2) + t * (D / 8));
                 load_words<KW>(kb, at + (r + 8) * (D / 2) + t * (D / 8));
                 const uint8_t* sa = at + 2 * L::codes + r * (D / kGroup) + t * (D / 64);
-                const uint8_t* sb = sa + 8 * (D / kGroup);
+                const uint32_t ba = load_bytes<D / 64>(sa), bb = load_bytes<D / 64>(sa + 8 * (D / kGroup));
 #pragma unroll
                 for (int g = 0; g < D / 64; ++g) {
-                    const Scale ga(sa[g] * 0x10001u), gb(sb[g] * 0x10001u);
+                    const Scale ga(__byte_perm(ba, 0, 0x4040 + 0x101 * g)), gb(__byte_perm(bb, 0, 0x4040 + 0x101 * g));
 #pragma unroll
                     for (int w = 2 * g; w < 2 * g + 2; ++w) {
                         const uint32_t a0 = first_of(ka[w], ga), a2 = second_of(ka[w], ga), a1 = first_of(kb[w], gb), a3 = second_of(kb[w], gb);
@@ -349,36 +384,43 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                         const uint32_t c0 = first_of(ha, ga), c2 = second_of(ha, ga), c1 = first_of(hb, gb), c3 = second_of(hb, gb);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma_f16(s[n], a0, a1, a2, a3, qf[n][2 * w][0], qf[n][2 * w][1]);
-                            mma_f16(s[n], c0, c1, c2, c3, qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
+                            mma_f16(e[n], a0, a1, a2, a3, qf[n][2 * w][0], qf[n][2 * w][1]);
+                            mma_f16(e[n], c0, c1, c2, c3, qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
                         }
                     }
                 }
             }
+            if (border) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int key = key0 + r + (j >> 1) * 8, p = seen[n][j & 1];
+                        e[n][j] *= factor[n][j & 1];
+                        if (key > p || (a.window > 0 && key <= p - a.window)) e[n][j] = -INFINITY;
+                    }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) e[n][j] *= factor[n][j & 1];
+            }
+            // The maximum only has to keep the weights in range: it is looked for where a score exceeds it.
             bool grows = false;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[n][j] *= factor[n][j & 1];
-                    if (border) {
-                        const int key = key0 + r + (j >> 1) * 8, p = seen[n][j & 1];
-                        if (key > p || (a.window > 0 && key <= p - a.window)) s[n][j] = -INFINITY;
-                    }
-                    grows |= s[n][j] > m[n][j & 1];
-                }
-            }
-            // The maximum only has to keep the exponentials in range: it is looked for where a score exceeds it.
+                for (int j = 0; j < 4; ++j) grows |= e[n][j] - m[n][j & 1] > kWeightBits;
             if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float most = fmaxf(m[n][j], fmaxf(s[n][j], s[n][j + 2]));
+                        float most = fmaxf(e[n][j], e[n][j + 2]);
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
-                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-                        const float turn = most == -INFINITY ? 1.0f : fa::fast_exp2(m[n][j] - most);
+                        most = fmaxf(m[n][j], fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16)) - kWeightBits);
+                        const float turn = fa::fast_exp2(m[n][j] - most);
                         m[n][j] = most;
                         l[n][j] *= turn;
 #pragma unroll
@@ -388,15 +430,13 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
             uint32_t p0[NT], p1[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float e[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float to = m[n][j & 1];
-                    e[j] = fa::fast_exp2(s[n][j] - (to == -INFINITY ? 0.0f : to - kWeightBits));       // a score that is no number gives none
-                    l[n][j & 1] += e[j];
+                    e[n][j] = fa::fast_exp2(e[n][j] - m[n][j & 1]);
+                    l[n][j & 1] += e[n][j];
                 }
-                p0[n] = transposed(as_word(__floats2half2_rn(e[0], e[1])));
-                p1[n] = transposed(as_word(__floats2half2_rn(e[2], e[3])));
+                p0[n] = transposed(as_word(__floats2half2_rn(e[n][0], e[n][1])));
+                p1[n] = transposed(as_word(__floats2half2_rn(e[n][2], e[n][3])));
             }
             uint8_t* scales = at + 2 * L::codes + L::scales;
             if (border) {
@@ -412,7 +452,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                     if (at_word < words && key >= low0 && key <= last) w[i] = reinterpret_cast<const uint32_t*>(scales)[at_word];
                     none |= __vcmpgeu4(w[i], 0xf8f8f8f8u) != 0;
                 }
-                const bool by_hand = tokens > 1 && __any_sync(0xffffffffu, none);
+                const bool by_hand = tile.tokens > 1 && __any_sync(0xffffffffu, none);
                 if (by_hand) {
                     for (int k = 0; k < kUnitKeys; ++k)
 #pragma unroll
@@ -451,21 +491,27 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const uint32_t pick = half == 0 ? 0x5410u : 0x7632u;
-                        uint32_t x = __byte_perm(va[w], vb[w], pick), y = __byte_perm(vc[w], vd[w], pick);
+                        uint32_t y = __byte_perm(va[w], vb[w], pick), z = __byte_perm(vc[w], vd[w], pick);
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            const uint32_t a0 = first_of(x, ab), a1 = second_of(x, ab), a2 = first_of(y, cd), a3 = second_of(y, cd);
+                            const uint32_t a0 = first_of(y, ab), a1 = second_of(y, ab), a2 = first_of(z, cd), a3 = second_of(z, cd);
 #pragma unroll
                             for (int n = 0; n < NT; ++n) mma_f16(o[n][4 * w + 2 * half + k], a0, a1, a2, a3, p0[n], p1[n]);
-                            x >>= 8;
                             y >>= 8;
+                            z >>= 8;
                         }
                     }
                 }
             }
         }
 
-        // ---- the warps' (m, l, O), merged in warp order
+        // ---- the piece's end: the whole segment's result, or a part to merge
+        const bool all = piece.from == 0 && piece.to == s.units, late = !all && x >= end;      // a part is the warp's first or its last
+        if (late) {
+            fa::cp_async_wait<0>();
+            __syncwarp();                                // the ring is the warp's own and empty
+        }
+        float* parked = late ? reinterpret_cast<float*>(ring) : early;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -475,85 +521,102 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                 sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                 const int column = n * 8 + 2 * t + j;
-                if (column < used) {
-                    float* mine = parked + (size_t)(warp * C + column) * (D + 2);
-                    if (r == 0) { mine[0] = sum == sum ? m[n][j] : 0.0f; mine[1] = sum; }     // (a sum that is no number must count)
+                if (column >= used) continue;
+                if (all) {
+                    const float by = kUnit / sum;
+                    __nv_bfloat16* dst = a.out + (size_t)(s.row + tile.token0 + column / heads) * a.out_stride
+                                         + (size_t)(tile.head0 + column % heads) * D + r * (D / 8);
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+                        *reinterpret_cast<uint32_t*>(dst + 2 * i) = fa::pack_bf16(o[n][i][j] * by, o[n][i][j + 2] * by);
+                } else {
+                    float* mine = parked + column * (D + 2);
+                    if (r == 0) { mine[0] = m[n][j]; mine[1] = sum; }
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i)
                         *reinterpret_cast<float2*>(mine + 2 + r * (D / 8) + 2 * i) = make_float2(o[n][i][j], o[n][i][j + 2]);
                 }
             }
-        __syncthreads();
-        if (tid < used) {
-            float M = -INFINITY;
-            for (int w = 0; w < kWarps4; ++w) M = fmaxf(M, parked[(size_t)(w * C + tid) * (D + 2)]);
+        if (!all && lane == 0)
+            parts[2 * warp + (late ? 1 : 0)] = {piece.first, s.units, s.row + tile.token0, tile.head0, heads, used};
+    }
+
+    // ---- the block's parts, in the order of the line: those of one segment are neighbours
+    __syncthreads();
+    const uint32_t block_begin = blockIdx.x * kWarps4 * each, block_end = min(length, block_begin + kWarps4 * each);
+    for (int i = 0; i < 2 * kWarps4;) {
+        const Part part = parts[i];
+        if (part.first == ~0u) { ++i; continue; }
+        int stop = i + 1;
+        while (stop < 2 * kWarps4 && (parts[stop].first == part.first || parts[stop].first == ~0u)) ++stop;
+        auto its = [&](int k) {                          // of part k
+            return reinterpret_cast<const float*>((k & 1) ? shared + (k >> 1) * L::ring : shared + kWarps4 * L::ring + (k >> 1) * L::parked);
+        };
+        if (tid < part.used) {
+            float M = kNoScore;
+            for (int k = i; k < stop; ++k)
+                if (parts[k].first != ~0u) M = fmaxf(M, its(k)[tid * (D + 2)]);
             float sum = 0.0f;
-            for (int w = 0; w < kWarps4; ++w) {
-                const float* its = parked + (size_t)(w * C + tid) * (D + 2);
-                const float by = its[0] == -INFINITY ? 0.0f : fa::fast_exp2(its[0] - M);
-                weight[w * C + tid] = by;
-                sum = fmaf(its[1], by, sum);
+            for (int k = i; k < stop; ++k) {
+                if (parts[k].first == ~0u) continue;
+                const float by = fa::fast_exp2(its(k)[tid * (D + 2)] - M);
+                weight[k * C + tid] = by;
+                sum = fmaf(its(k)[tid * (D + 2) + 1], by, sum);
             }
             whole[2 * tid] = M;
             whole[2 * tid + 1] = sum;
         }
         __syncthreads();
-        const bool all = c.from == 0 && c.to == c.s.units;
-        float* part_out = a.partial + (size_t)(blockIdx.x * 2 + (c.from == 0 ? 1 : 0)) * C * (D + 2);
-        for (int i = tid; i < used * D; i += kThreads4) {
-            const int column = i / D, e = i % D;
+        const bool begins = part.first >= block_begin, all = begins && part.first + part.units <= block_end;
+        float* part_out = a.partial + (size_t)(blockIdx.x * 2 + (begins ? 1 : 0)) * C * (D + 2);
+        for (int k = tid; k < part.used * D; k += kThreads4) {
+            const int column = k / D, element = k % D;
             float sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps4; ++w) {
-                sum = fmaf(parked[(size_t)(w * C + column) * (D + 2) + 2 + e], weight[w * C + column], sum);
-            }
+            for (int n = i; n < stop; ++n)
+                if (parts[n].first != ~0u) sum = fmaf(its(n)[column * (D + 2) + 2 + element], weight[n * C + column], sum);
             if (all) {
-                const float value = sum * (kUnit / whole[2 * column + 1]);
-                a.out[(size_t)(c.s.row + token0 + column / heads) * a.out_stride + (size_t)(head0 + column % heads) * D + e] = __float2bfloat16_rn(value);
+                a.out[(size_t)(part.row + column / part.heads) * a.out_stride + (size_t)(part.head0 + column % part.heads) * D + element]
+                    = __float2bfloat16_rn(sum * (kUnit / whole[2 * column + 1]));
             } else {
-                part_out[(size_t)column * (D + 2) + 2 + e] = sum;
-                if (e < 2) part_out[(size_t)column * (D + 2) + e] = whole[2 * column + e];
+                part_out[column * (D + 2) + 2 + element] = sum;
+                if (element < 2) part_out[column * (D + 2) + element] = whole[2 * column + element];
             }
         }
-        __syncthreads();                                 // before the next piece's warps park theirs
-    } while (next_piece(a, c, end));
+        __syncthreads();
+        i = stop;
+    }
 }
 
-// Block i merges the segment that begins in share i and goes on behind it, if there is one: its first part is in slot 1 of block i,
-// the others in slot 0 of the blocks behind.
+// Block i merges the segment whose unit 0 is in the share of block i and that goes on behind it, if there is one: its first part is in
+// slot 1 of block i, the others in slot 0 of the blocks behind.
 template <int D>
 __global__ void __launch_bounds__(128)
 attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
     extern __shared__ float merge[];                     // [columns][parts]
     dependents_may_launch();
-    wait_for_predecessor();
-    const long long share = share_of(a, gridDim.x);
-    const long long begin = share * blockIdx.x;
-    long long end = begin + share;
-    Cursor c;
-    if (!find(a, c, begin, end)) return;
-    // the segment of the share's last unit
-    long long whole_end = end;
-    if (!find(a, c, end - 1, whole_end)) return;
-    const long long from = c.x - c.from, to = from + c.s.units;          // its place in the line
-    if (from < begin || to <= end) return;               // it began earlier, or ends here
-    const int parts = (int)((to - 1) / share - blockIdx.x) + 1;
-    const int tile = c.segment % c.s.tiles, part = c.segment / c.s.tiles, head_tile = part % a.head_tiles, kv = part / a.head_tiles;
-    const int token0 = tile * a.tokens, tokens = min(a.tokens, c.s.fresh - token0);
-    const int head0 = kv * a.group + head_tile * a.heads, heads = min(a.heads, a.group - head_tile * a.heads);
-    const int used = tokens * heads;
+    const uint32_t length = line_length(a), share = places_of_a_warp(length, gridDim.x) * kWarps4;
+    const uint32_t begin = blockIdx.x * share, end = begin + share;
+    Place here = {0, 0};
+    if (end < length) here = place_of(a, end);           // the segment that the next share begins in
+    wait_for_predecessor();                              // (every block: the kernel behind this one waits for this one alone)
+    if (end >= length) return;                           // nothing lies behind
+    const Sequence s = sequence_of(a, here.b);
+    const Piece piece = piece_of(s, here.base, end, end + 1);
+    if (piece.first < begin || piece.first >= end) return;               // it began earlier, or only its room is here
+    const Tile tile = tile_of(a, s, piece.segment);
+    const int parts = (int)((piece.first + s.units - 1) / share - blockIdx.x) + 1, used = tile.used();
     auto its = [&](int column, int p) {
         return a.partial + ((size_t)((blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * columns + column) * (D + 2);
     };
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int column = warp; column < used; column += 4) {
-        float M = -INFINITY;
+        float M = kNoScore;
         for (int p = lane; p < parts; p += 32) M = fmaxf(M, its(column, p)[0]);
         M = warp_max(M);
         float sum = 0.0f;
         for (int p = lane; p < parts; p += 32) {
             const float* one = its(column, p);
-            const float by = one[0] == -INFINITY ? 0.0f : fa::fast_exp2(one[0] - M);
+            const float by = fa::fast_exp2(one[0] - M);
             merge[column * parts + p] = by;
             sum = fmaf(one[1], by, sum);
         }
@@ -563,7 +626,7 @@ attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
         for (int e = lane; e < D; e += 32) {
             float value = 0.0f;
             for (int p = 0; p < parts; ++p) value = fmaf(its(column, p)[2 + e], merge[column * parts + p], value);
-            a.out[(size_t)(c.s.row + token0 + column / heads) * a.out_stride + (size_t)(head0 + column % heads) * D + e]
+            a.out[(size_t)(s.row + tile.token0 + column / tile.heads) * a.out_stride + (size_t)(tile.head0 + column % tile.heads) * D + e]
                 = __float2bfloat16_rn(value * back);
         }
     }
@@ -642,10 +705,11 @@ extern "C" int citlali_attention4(const void* q, size_t q_stride, const void* k_
         set_last_error("attention4: the scratch holds %zu floats, too few", partial_floats);
         return kTooLarge;
     }
-    const long long units = ((long long)page_table_stride * page_size + max_new) / c4::kUnitKeys + 2;
+    const long long units = ((long long)page_table_stride * page_size + max_new) / c4::kUnitKeys + 2 + c4::kRoom;
     const long long segments = ((long long)max_new + t.tokens - 1) / t.tokens * nkv * t.head_tiles;
-    if (units * segments > 0x7fffffffLL) {
-        set_last_error("attention4: %d new tokens of one sequence over %d pages are too many for one launch", max_new, page_table_stride);
+    if (units * segments > 0x3fffffffLL / sequences) {             // (places on the line are 32 bits)
+        set_last_error("attention4: %d sequences of up to %d new tokens over %d pages are too many for one launch", sequences, max_new,
+                       page_table_stride);
         return kTooLarge;
     }
     c4::Attention4 a = {};
