@@ -238,6 +238,90 @@ read_kernel(const __grid_constant__ Rows rows, const __grid_constant__ Pools poo
     store8(out + 8, y);
 }
 
+// The pages that a run's rows see, as bfloat16 pages of their own (exact), with a page table and slots for the attention kernels of a
+// cache of 16 bits: sequence b is slot b there.  A block a (page, key/value head).  Positions that no row of the run sees become
+// zeros.  A value that is no number becomes zero too, and its token's key none: a row that does not see the token gives it the
+// weight zero, and zero times a NaN would reach it; a row that does see it gets a NaN from the key.
+struct Runs {
+    const int32_t *seq_start, *seq_slot, *seq_past;
+    int sequences, window;
+};
+constexpr int kExpandThreads = 256, kRunPage = 64;
+__global__ void __launch_bounds__(kExpandThreads)
+expand_kernel(const __grid_constant__ Runs runs, const int32_t* __restrict__ page_table, int page_table_stride,
+              const __grid_constant__ Pools pools, __nv_bfloat16* __restrict__ keys, __nv_bfloat16* __restrict__ values,
+              int32_t* __restrict__ table_out, int table_out_stride, int32_t* __restrict__ slots_out, int nkv, int d) {
+    dependents_may_launch();
+    const int lane = threadIdx.x & 31, head = blockIdx.y;
+    // the sequence of this page: every warp finds it for itself (lists and page tables come from the host before the step)
+    auto tiles_of = [&](int b, int& first) {
+        const int past = runs.seq_past[b], fresh = runs.seq_start[b + 1] - runs.seq_start[b];
+        first = runs.window > 0 ? max(0, past - runs.window + 1) / kRunPage : 0;
+        return fresh > 0 ? (past + fresh - 1) / kRunPage - first + 1 : 0;
+    };
+    int b = -1, tile = 0, run = 0;
+    for (int b0 = 0; b0 < runs.sequences && b < 0; b0 += 32) {
+        int first, mine = b0 + lane < runs.sequences ? tiles_of(b0 + lane, first) : 0, sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+        }
+        const unsigned behind = __ballot_sync(0xffffffffu, run + sum > (int)blockIdx.x);
+        if (behind) {
+            const int which = __ffs(behind) - 1;
+            b = b0 + which;
+            tile = (int)blockIdx.x - run - __shfl_sync(0xffffffffu, sum - mine, which);
+        }
+        run += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    wait_for_predecessor();
+    if (b < 0) return;
+    int first;
+    tiles_of(b, first);
+    tile += first;
+    if (tile >= table_out_stride) return;
+    const int past = runs.seq_past[b], last = past + runs.seq_start[b + 1] - runs.seq_start[b] - 1;
+    const int low = runs.window > 0 ? max(0, past - runs.window + 1) : 0;
+    if (head == 0 && threadIdx.x == 0) {
+        table_out[(size_t)b * table_out_stride + tile] = blockIdx.x;
+        if (tile == first) slots_out[b] = b;
+    }
+    const int page = page_table[(size_t)runs.seq_slot[b] * page_table_stride + tile];
+    const int per_row = d / kGroup;
+    for (int i = threadIdx.x; i < 2 * kRunPage * per_row; i += kExpandThreads) {
+        const bool is_v = i >= kRunPage * per_row;
+        const int j = is_v ? i - kRunPage * per_row : i, row = j / per_row, g = j % per_row, pos = tile * kRunPage + row;
+        const size_t from = place(page, nkv, head, kRunPage, row), to = place(blockIdx.x, nkv, head, kRunPage, row);
+        float y[8];
+        __nv_bfloat16* out = (is_v ? values : keys) + to * d + g * kGroup;
+        if (pos < low || pos > last) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = 0.0f;
+            store8(out, y);
+            store8(out + 8, y);
+            continue;
+        }
+        const uint2 w = *reinterpret_cast<const uint2*>((is_v ? pools.v_codes : pools.k_codes) + from * (d / 2) + g * 8);
+        float s;
+        if (is_v) {
+            const uint8_t byte = pools.v_scales[from * per_row + g];
+            s = byte >= 0xf8 ? 0.0f : scale_of(byte);
+        } else {
+            s = scale_of(pools.k_scales[from * per_row + g]);
+            bool none = false;
+            for (int k = 0; k < per_row; ++k) none |= pools.v_scales[from * per_row + k] >= 0xf8;
+            if (none) s = __int_as_float(0x7fc00000);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = value_of(w.x, e, s);
+        store8(out, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = value_of(w.y, e, s);
+        store8(out + 8, y);
+    }
+}
+
 static int check_sizes(const char* what, int nkv, int d, int page_size) {
     if (d < kGroup || d % kGroup != 0 || d > 256) {
         set_last_error("%s: a cache in 4 bits takes head sizes that are multiples of %d up to 256, not %d", what, kGroup, d);
@@ -326,4 +410,26 @@ extern "C" int citlali_cache4_read(const void* k_codes, const void* k_scales, co
                       nkv, head_dim);
         return CITLALI_LAUNCH_CHECK();
     });
+}
+
+extern "C" int citlali_cache4_expand(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                                     const int32_t* page_table, int page_table_stride, const int32_t* seq_start, const int32_t* seq_slot,
+                                     const int32_t* seq_past, int sequences, int window, void* keys, void* values, int pages,
+                                     int32_t* table_out, int table_out_stride, int32_t* slots_out, int page_size, int nkv, int head_dim,
+                                     cudaStream_t stream) {
+    if (sequences <= 0 || pages <= 0) return 0;
+    if (int bad = c4::check_sizes("cache4_expand", nkv, head_dim, page_size)) return bad;
+    if (page_size != c4::kRunPage || nkv > 65535 || window < 0) {
+        set_last_error("cache4_expand: pages of %d (only of 64), %d heads, window %d", page_size, nkv, window);
+        return kBadShape;
+    }
+    if (!c4::aligned(k_codes, 8) || !c4::aligned(v_codes, 8) || !c4::aligned(keys, 16) || !c4::aligned(values, 16)) {
+        set_last_error("cache4_expand: codes must be 8-byte and pages 16-byte aligned");
+        return kBadAlignment;
+    }
+    const c4::Runs runs = {seq_start, seq_slot, seq_past, sequences, window};
+    const c4::Pools pools = {(uint8_t*)k_codes, (uint8_t*)k_scales, (uint8_t*)v_codes, (uint8_t*)v_scales};
+    launch_kernel(c4::expand_kernel, dim3(pages, nkv), c4::kExpandThreads, 0, stream, runs, page_table, page_table_stride, pools,
+                  (__nv_bfloat16*)keys, (__nv_bfloat16*)values, table_out, table_out_stride, slots_out, nkv, head_dim);
+    return CITLALI_LAUNCH_CHECK();
 }

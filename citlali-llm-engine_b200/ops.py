@@ -385,10 +385,50 @@ def _attention4_floats(nq: int, nkv: int, head_dim: int, page_size: int, max_new
     return l.citlali_attention4_scratch_floats(nq, nkv, head_dim, max_new)
 
 
+_EXPAND_FROM = 40                          # new tokens
+_EXPAND_BYTES = 1 << 30
+
+
+def _attention4_expands(q, q_stride, out, batch, nq, nkv, head_dim, page_size) -> bool:
+    """Whether runs go over pages that were made bfloat16 first, by the kernels of a cache of 16 bits."""
+    return (batch.max_new >= _EXPAND_FROM and q.dtype is torch.bfloat16 and page_size == 64 and nkv > 0 and nq % nkv == 0 and q_stride % 8 == 0
+            and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0 and lib().citlali_attention_run_form(q_stride, out.shape[1], head_dim, 64, batch.max_new) > 0)
+
+
+def _attention4_expanded(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
+    """The pages that the rows see as bfloat16 (the values are exact there), then prompt attention over them: as many sequences at a
+    time as a gigabyte holds, at least one."""
+    require(not torch.cuda.is_current_stream_capturing(), "cache4_attention: runs of tokens are sized from the host's lists of lengths, "
+            "which a captured step would freeze")
+    pools, l, page_bytes = _packed4(kv, nkv, head_dim, "cache4_attention"), lib(), 2 * nkv * 64 * head_dim * 2
+    kc, ks, vc, vs, table, table_width = pools
+    tiles, ends = [], []                      # pages of each sequence, and where its last one lies in its row of the table
+    for p, n in zip(batch.past, batch.n_new):
+        ends.append((p + n - 1) // 64 + 1)
+        tiles.append(ends[-1] - (max(0, p - window + 1) // 64 if window else 0))
+    b0 = 0
+    while b0 < len(tiles):
+        b1, pages = b0 + 1, tiles[b0]
+        while b1 < len(tiles) and (pages + tiles[b1]) * page_bytes <= _EXPAND_BYTES:
+            pages += tiles[b1]
+            b1 += 1
+        count, width, max_new = b1 - b0, max(ends[b0:b1]), max(batch.n_new[b0:b1])
+        held = torch.empty((2, pages, nkv, 64, head_dim), dtype=torch.bfloat16, device=q.device)
+        found = torch.empty((count + 1, max(width, count)), dtype=torch.int32, device=q.device)        # the table's rows, then the slots
+        seq_start, seq_slot, seq_past = batch.seq_start[b0:b1 + 1], batch.seq_slot[b0:b1], batch.seq_past[b0:b1]
+        _check(l.citlali_cache4_expand(kc, ks, vc, vs, table, table_width, seq_start.data_ptr(), seq_slot.data_ptr(), seq_past.data_ptr(), count,
+                                       window, held[0].data_ptr(), held[1].data_ptr(), pages, found.data_ptr(), found.shape[1],
+                                       found[count].data_ptr(), 64, nkv, head_dim, _stream()), "cache4_expand")
+        run = attention_prefill_tc if l.citlali_attention_run_form(q_stride, out.shape[1], head_dim, 64, max_new) == 2 else attention_prefill
+        run(q, q_stride, held[0], held[1], found[:count], seq_start, found[count, :count], seq_past, out, count, max_new, nq, nkv, head_dim, 64,
+            window, scale)
+        b0 = b1
+
+
 def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
     """:func:`attention` over a cache in 4 bits: every row of the step over its slot's keys up to its own position (the last
     ``window`` of them; 0 or None: all).  bfloat16 with head size 64, 128 or 256 and pages of 64 runs on the tensor cores, anything
-    else in 32-bit arithmetic.  A step of single tokens launches nothing that depends on the host's lists of lengths."""
+    else in 32-bit arithmetic; longer runs of tokens go over pages that were made bfloat16 first.  A step of single tokens launches nothing that depends on the host's lists of lengths."""
     kc, ks, vc, vs, table, table_width = _packed4(kv, nkv, head_dim, "cache4_attention")
     row_slot, row_pos, seq_start = batch.row_slot, batch.row_pos, batch.seq_start
     rows, wide = row_slot.shape[0], nq * head_dim
@@ -401,6 +441,9 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
     if rows == 0:
         return
     q_ptr, window = q.data_ptr(), _i(window or 0)
+    if not batch.is_decode and _attention4_expands(q, q_stride, out, batch, nq, nkv, head_dim, kv.page_size):
+        _attention4_expanded(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale)
+        return
     if q.dtype is torch.bfloat16 and q_stride % 8 == 0 and (q_ptr | kc | ks | vc | vs) % 16 == 0 and nkv > 0 and nq % nkv == 0:
         single = batch.is_decode
         max_new = 1 if single else batch.max_new

@@ -267,13 +267,13 @@ def test_single_tokens(nq, nkv, d, lengths, window):
 RUNS = [
     # nq, nkv, d, past, new, window
     (16, 8, 128, [0], [1 + 16], 0),
-    (16, 8, 128, [0, 5, 100], [7, 1, 40], 0),
+    (16, 8, 128, [0, 5, 100], [7, 1, 39], 0),
     (40, 8, 128, [61, 200], [24, 5], 50),
-    (4, 4, 128, [0], [150], 0),
+    (4, 4, 128, [0], [39], 0),
     (8, 1, 64, [33, 0], [20, 3], 16),
     (6, 2, 256, [10], [9], 0),
     (40, 2, 128, [17], [4], 0),
-    (3, 1, 128, [1000, 3], [2, 70], 7),
+    (3, 1, 128, [1000, 3], [2, 37], 7),
 ]
 
 
@@ -461,3 +461,67 @@ def test_refusals():
         ops.cache4_read(kv, batch.row_slot, batch.row_pos, dtype=torch.float16)
     with pytest.raises(cb.CitlaliError, match="float32 or bfloat16"):
         ops.cache4_append(q.half(), kv, batch.row_slot, batch.row_pos, 4, 2, 64, f, 64)
+
+
+LONG_RUNS = [
+    # nq, nkv, d, past, new, window
+    (16, 8, 128, [0], [300], 0),
+    (4, 2, 128, [65, 0, 500], [50, 130, 1], 0),
+    (5, 1, 128, [200, 10], [64, 47], 100),
+    (8, 2, 64, [0, 31], [129, 60], 0),
+    (2, 1, 96, [0, 70], [70, 41], 33),
+    (2, 2, 256, [3], [90], 0),
+]
+
+
+def check_long_run(st, nq, window, seed, expect_nan=None):
+    """As check_attention, with the weights rounded to bfloat16 by the kernels for runs: half a step is 2^-8 of a weight."""
+    g = torch.Generator().manual_seed(seed)
+    nkv, d = st.nkv, st.d
+    rows, pitch, scale = len(st.row_slot), (nq + 2 * nkv) * d, 1.0 / math.sqrt(d)
+    q = (1.5 * torch.randn(rows, pitch, generator=g)).bfloat16()
+    out = torch.full((rows + 1, nq * d), 5.0, dtype=torch.bfloat16, device=DEV)
+    before = ops.launch_count()
+    ops.cache4_attention(q.to(DEV), pitch, st.view(), st.batch(), out, nq, nkv, d, window, scale)
+    got = out.cpu().double()
+    assert (got[rows:] == 5.0).all()
+    row = 0
+    for s, past, n in zip(st.slots, st.past, st.new):
+        k, v = (plain.gathered(part, st.table, s, past + n, st.page) for part in (st.keys, st.values))
+        for i in range(n):
+            o, weight, reach = plain.attention(q[row, :nq * d].view(nq, d), k, v, past + i, window, scale, nq // nkv)
+            off = 4 * (d / 8 + 8) * 2.0 ** -23 * reach[:, None] + 2.0 ** -8 + (past + n + 64) / 32 * 2.0 ** -23
+            have = got[row].view(nq, d)
+            if expect_nan is not None and expect_nan(s, past + i):
+                assert have.isnan().all()
+            else:
+                assert ((have - o).abs() <= 2.0 ** -8 * o.abs() + off * weight).all(), (s, past + i)
+            row += 1
+    return ops.launch_count() - before
+
+
+@pytest.mark.parametrize("nq,nkv,d,past,new,window", LONG_RUNS)
+def test_longer_runs(nq, nkv, d, past, new, window):
+    st = Step(past, new, nkv, d, seed=nq + d)
+    st.fill(sum(new))
+    check_long_run(st, nq, window, nq)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("which", ["keys", "values"])
+@pytest.mark.parametrize("window", [0, 20])
+def test_a_token_that_is_not_finite_in_a_longer_run(d, which, window):
+    st = Step([30, 10], [90, 50], 1, d, seed=5)
+    st.fill(5)
+    slot, at = st.slots[0], 75
+    part = getattr(st, which)
+    part.scales[int(st.table[slot, at // 64]), :, at % 64] = 255
+    check_long_run(st, 2, window, 2, expect_nan=lambda s, p: s == slot and p >= at and (not window or p < at + window))
+
+
+def test_longer_runs_a_few_sequences_at_a_time(monkeypatch):
+    st = Step([0, 100, 5], [70, 60, 45], 2, 128, seed=8)
+    st.fill(8)
+    assert check_long_run(st, 4, 0, 1) == 2                              # one expansion, one attention
+    monkeypatch.setattr(ops, "_EXPAND_BYTES", 1)
+    assert check_long_run(st, 4, 0, 1) == 6
