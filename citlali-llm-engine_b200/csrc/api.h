@@ -223,6 +223,13 @@ int citlali_argmax_rows_wide(const float* logits, int32_t* tokens, float* scratc
 int citlali_sample_rows(const float* logits, const float* temperature, const float* uniform,
                         int32_t* tokens, int rows, int vocab, cudaStream_t stream);
 
+// Over the finite entries of each row of logits [rows, vocab] (dtype 0 or 1): logprobs[r] = log probability of tokens[r] (tokens null:
+// none are asked for; NaN for an id outside the vocabulary, minus infinity for an entry that is not finite), entropy[r] of the row's
+// distribution, and its `top` (0 to 32) likeliest tokens, likeliest first, the lowest id first among equals: top_ids, top_logprobs
+// [rows, top] (-1 and minus infinity where the row has no more finite entries).
+int citlali_token_logprobs(const void* logits, int dtype, const int32_t* tokens, float* logprobs, float* entropy, int32_t* top_ids,
+                           float* top_logprobs, int rows, int vocab, int top, cudaStream_t stream);
+
 // The tensor-core product (bfloat16 operands, float accumulation).  citlali_gemm_tc_plan_for tells how a shape runs: whether the
 // weights are the 128-row operand (*swapped), the narrow tile (*bn), the K split (*splits) and in how many float sums K is added
 // up before these are added (*sums: a block may keep several).  gated: a gate epilogue (SiLU or GELU); normed: a norm's

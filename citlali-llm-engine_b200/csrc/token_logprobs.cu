@@ -1,0 +1,314 @@
+// Log probabilities of given tokens, the entropy of a row's distribution and its likeliest tokens, from logits in one pass.
+//
+//   over the finite entries of a row:  m = max x,  S = sum e^(x - m),  T = sum (x - m) e^(x - m)
+//   log p(token) = x_token - m - log S      entropy = log S - T / S      the `top` largest entries, the lowest index first among equals
+//
+// Entries that are not finite have no probability, as in sampling.cu; a row without a finite entry has none at all (log
+// probabilities of minus infinity, entropy 0, ids -1).  Logits are float32 or bfloat16; all sums are float32.
+//
+// What bounds it: reading the logits once.  A cluster of 1 to 8 blocks takes a row, a block an even share of it; a thread has 16
+// entries in registers and the next 16 on their way.  m, S and T are the thread's own until the end (the running maximum is looked
+// at once for 16 entries).  The likeliest 32 are the warp's: lane i holds the i-th.  An entry is looked at one by one only if it
+// exceeds the last one that still counts, which for 512 entries at a time hardly happens once a row has begun; for the first 512 that
+// bound is the top-th of the lanes' own maxima, which sorting gives.  Warps and then blocks (through distributed shared memory)
+// merge their lists pairwise: the larger of a[i] and b[31 - i] are the 32 largest, and five exchanges sort them.
+#include "api.h"
+#include "common.cuh"
+#include "mma_common.cuh"
+
+namespace citlali {
+namespace lp {
+
+constexpr int kThreads = 256, kWarps = 8, kEach = 16, kMost = 32;
+constexpr int kMaxCluster = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kNone = 0x7fffffff;                        // no entry: behind every index
+
+struct Summary { float m, s, t; };
+
+__device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+
+// The summary over both.
+__device__ __forceinline__ Summary joined(Summary a, Summary b) {
+    const float m = fmaxf(a.m, b.m);
+    if (m == -INFINITY) return a;
+    // (x - m) e^(x - m) from (x - a.m) e^(x - a.m): the exponent shifts by a.m - m, and every term by as much
+    const float da = fmaxf(a.m - m, -104.0f), db = fmaxf(b.m - m, -104.0f);
+    const float ea = expf(da), eb = expf(db);
+    return {m, a.s * ea + b.s * eb, (a.t + a.s * da) * ea + (b.t + b.s * db) * eb};
+}
+
+// A warp's list: lane i holds its i-th entry.
+__device__ __forceinline__ void exchange(float& v, int& i, int distance, bool larger_first) {
+    const float w = __shfl_xor_sync(0xffffffffu, v, distance);
+    const int j = __shfl_xor_sync(0xffffffffu, i, distance);
+    const bool low = (threadIdx.x & distance) == 0;
+    if (before(w, j, v, i) == (low == larger_first)) { v = w; i = j; }
+}
+__device__ __forceinline__ void sort(float& v, int& i) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int distance = size >> 1; distance > 0; distance >>= 1) exchange(v, i, distance, (threadIdx.x & size & 31) == 0);
+}
+// (w, j): another list, lane i given its entry 31 - i.
+__device__ __forceinline__ void merge(float& v, int& i, float w, int j) {
+    if (before(w, j, v, i)) { v = w; i = j; }
+#pragma unroll
+    for (int distance = 16; distance > 0; distance >>= 1) exchange(v, i, distance, true);
+}
+
+__device__ __forceinline__ void load(const float* p, float (&x)[kEach]) {
+#pragma unroll
+    for (int k = 0; k < kEach / 4; ++k) {
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(p) + k * kThreads);
+        x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+    }
+}
+__device__ __forceinline__ void load(const __nv_bfloat16* p, float (&x)[kEach]) {
+#pragma unroll
+    for (int k = 0; k < kEach / 8; ++k) {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + k * kThreads);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { x[8 * k + 2 * e] = __uint_as_float(w[e] << 16); x[8 * k + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+    }
+}
+
+struct Block {                                           // what a block tells the first of its cluster
+    Summary sum;
+    float v[kMost];
+    int i[kMost];
+};
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads)
+token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ tokens, float* __restrict__ logprobs,
+                      float* __restrict__ entropy, int32_t* __restrict__ top_ids, float* __restrict__ top_logprobs, int vocab, int top,
+                      int cluster) {
+    constexpr int kVec = 16 / sizeof(T);                 // entries of a 16-byte load
+    __shared__ Summary sums[kWarps];
+    __shared__ float list_v[kWarps][32];
+    __shared__ int list_i[kWarps][32];
+    __shared__ Block blocks[kMaxCluster];
+    dependents_may_launch();
+    wait_for_predecessor();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long row = blockIdx.x / cluster;
+    const int rank = blockIdx.x % cluster;
+    const T* x = logits + row * vocab;
+
+    // the row from its first 16-byte boundary on, in tiles of kThreads * kEach entries, dealt out to the cluster's blocks evenly;
+    // the first block also takes the entries ahead of the boundary, the last one those behind the last whole vector
+    const int lead = min(vocab, (int)((16 - ((uintptr_t)x & 15)) % 16 / sizeof(T)));
+    const int vectors = (vocab - lead) / kVec, share = (vectors + cluster - 1) / cluster;
+    const int first = min(vectors, rank * share), stop = min(vectors, first + share);      // this block's vectors
+
+    Summary mine = {-INFINITY, 0.0f, 0.0f};
+    float best = -INFINITY;                              // lane i: the warp's i-th largest entry
+    int at = kNone;
+    float bound = -INFINITY;                             // the top-th
+    int bound_at = kNone;
+
+    // 16 entries a lane, `where(e)` their indices; entries that are none or not finite come as minus infinity
+    auto take = [&](float (&y)[kEach], auto where) {
+        float most = y[0];
+#pragma unroll
+        for (int e = 1; e < kEach; ++e) most = fmaxf(most, y[e]);
+        if (most > mine.m) {
+            const float d = fmaxf(mine.m - most, -104.0f), by = fa::fast_exp2(d * kLog2e);
+            mine.t = (mine.t + mine.s * d) * by;
+            mine.s *= by;
+            mine.m = most;
+        }
+        const float m = mine.m == -INFINITY ? 0.0f : mine.m;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const float u = fmaxf(y[e] - m, -104.0f), p = fa::fast_exp2(u * kLog2e);       // 2^-150 is zero here
+            mine.s += p;
+            mine.t = fmaf(p, u, mine.t);
+        }
+        if constexpr (TOP) {
+            if (!__any_sync(0xffffffffu, most >= bound && most > -INFINITY)) return;
+            if (__all_sync(0xffffffffu, at == kNone)) {  // the first entries: no more than `top` lanes' maxima are above the bound
+                float v = most;
+                int i = lane;
+                sort(v, i);
+                bound = __shfl_sync(0xffffffffu, v, top - 1);
+            }
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int index = where(e);
+                unsigned who = __ballot_sync(0xffffffffu, y[e] > -INFINITY && (y[e] > bound || (y[e] == bound && index < bound_at)));
+                while (who) {
+                    const int from = __ffs(who) - 1;
+                    who &= who - 1;
+                    const float v = __shfl_sync(0xffffffffu, y[e], from);
+                    const int i = __shfl_sync(0xffffffffu, index, from);
+                    const int rank_of = __popc(__ballot_sync(0xffffffffu, before(best, at, v, i)));
+                    const float up = __shfl_up_sync(0xffffffffu, best, 1);
+                    const int up_at = __shfl_up_sync(0xffffffffu, at, 1);
+                    if (lane > rank_of) { best = up; at = up_at; }
+                    if (lane == rank_of) { best = v; at = i; }
+                }
+                const float last = __shfl_sync(0xffffffffu, best, top - 1);
+                if (last >= bound) {
+                    bound = last;
+                    bound_at = __shfl_sync(0xffffffffu, at, top - 1);
+                }
+            }
+        }
+    };
+    auto finite = [](float (&y)[kEach]) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) y[e] = fabsf(y[e]) <= 3.402823466e+38f ? y[e] : -INFINITY;
+    };
+
+    constexpr int kTile = kThreads * kEach / kVec;       // vectors of a tile
+    const int tiles = (stop - first) / kTile;            // whole ones
+    const T* base = x + lead + ((long long)first + tid) * kVec;
+    float y[kEach], next[kEach];
+    if (tiles > 0) load(base, next);
+    for (int k = 0; k < tiles; ++k) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) y[e] = next[e];
+        if (k + 1 < tiles) load(base + (long long)(k + 1) * kTile * kVec, next);
+        finite(y);
+        const int index0 = lead + (first + k * kTile + tid) * kVec;
+        take(y, [&](int e) { return index0 + e / kVec * (kThreads * kVec) + e % kVec; });
+    }
+    {   // the rest of this block's vectors, less than a tile, and the row's ends: the lead with the first block, the tail with the last
+        const int rest = first + tiles * kTile;
+        const int index0 = lead + (rest + tid) * kVec;
+        bool any = rest < stop;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) y[e] = -INFINITY;
+        if (any) {
+#pragma unroll
+            for (int k = 0; k < kEach / kVec; ++k)
+                if (rest + k * kThreads + tid < stop) {
+                    const T* p = x + lead + ((long long)rest + k * kThreads + tid) * kVec;
+                    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+                    const T* in = reinterpret_cast<const T*>(&v);
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) y[k * kVec + e] = ldf(in, e);
+                }
+            finite(y);
+            take(y, [&](int e) { return index0 + e / kVec * (kThreads * kVec) + e % kVec; });
+        }
+        const int tail = lead + vectors * kVec;          // entries from here on: fewer than kVec
+        int odd = -1;
+        if (rank == 0 && tid < lead) odd = tid;
+        if (rank == cluster - 1 && tid >= 32 && tail + tid - 32 < vocab) odd = tail + tid - 32;
+        if (warp < 2) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) y[e] = -INFINITY;
+            if (odd >= 0) y[0] = ldf(x, odd);
+            finite(y);
+            take(y, [&](int) { return odd; });
+        }
+    }
+
+    // ---- the warp's, the block's, the cluster's
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        mine = joined(mine, {__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o), __shfl_xor_sync(0xffffffffu, mine.t, o)});
+    if (lane == 0) sums[warp] = mine;
+    if constexpr (TOP) { list_v[warp][lane] = best; list_i[warp][lane] = at; }
+    __syncthreads();
+    if constexpr (TOP) {
+#pragma unroll
+        for (int half = kWarps / 2; half > 0; half >>= 1) {
+            if (warp < half) {
+                merge(best, at, list_v[warp + half][31 - lane], list_i[warp + half][31 - lane]);
+                list_v[warp][lane] = best;
+                list_i[warp][lane] = at;
+            }
+            __syncthreads();
+        }
+    }
+    if (warp == 0) {
+        Summary all = sums[0];
+        for (int w = 1; w < kWarps; ++w) all = joined(all, sums[w]);
+        mine = all;
+    }
+    if (cluster > 1) {
+        if (warp == 0) {                                 // to the cluster's first block
+            auto put = [&](void* here, uint32_t bits) {
+                uint32_t remote;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(here)), "r"(0));
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(bits) : "memory");
+            };
+            if (lane == 0) {
+                put(&blocks[rank].sum.m, __float_as_uint(mine.m));
+                put(&blocks[rank].sum.s, __float_as_uint(mine.s));
+                put(&blocks[rank].sum.t, __float_as_uint(mine.t));
+            }
+            if constexpr (TOP) {
+                put(&blocks[rank].v[lane], __float_as_uint(best));
+                put(&blocks[rank].i[lane], (uint32_t)at);
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (rank != 0 || warp != 0) return;
+        mine = blocks[0].sum;
+        for (int b = 1; b < cluster; ++b) {
+            mine = joined(mine, blocks[b].sum);
+            if constexpr (TOP) merge(best, at, blocks[b].v[31 - lane], blocks[b].i[31 - lane]);
+        }
+    }
+    if (warp != 0) return;
+    const float log_s = logf(mine.s);                    // (no finite entry: log 0, and m is minus infinity)
+    const bool some = mine.m > -INFINITY;
+    if (lane == 0) {
+        entropy[row] = some ? log_s - mine.t / mine.s : 0.0f;
+        if (tokens) {
+            const int token = tokens[row];
+            float lp = __int_as_float(0x7fc00000);       // no such token
+            if (token >= 0 && token < vocab) {
+                const float v = ldf(x, token);
+                lp = fabsf(v) <= 3.402823466e+38f ? v - mine.m - log_s : -INFINITY;
+            }
+            logprobs[row] = lp;
+        }
+    }
+    if constexpr (TOP) {
+        if (lane < top) {
+            top_ids[row * top + lane] = at == kNone ? -1 : at;
+            top_logprobs[row * top + lane] = at == kNone ? -INFINITY : best - mine.m - log_s;
+        }
+    }
+}
+
+template <typename T, bool TOP>
+static int launch(const void* logits, const int32_t* tokens, float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, int rows,
+                  int vocab, int top, int cluster, cudaStream_t stream) {
+    launch_kernel_clustered(token_logprobs_kernel<T, TOP>, dim3((unsigned)(rows * cluster)), kThreads, 0, cluster, stream, (const T*)logits, tokens,
+                            logprobs, entropy, top_ids, top_logprobs, vocab, top, cluster);
+    return CITLALI_LAUNCH_CHECK();
+}
+
+}  // namespace lp
+}  // namespace citlali
+
+using namespace citlali;
+
+extern "C" int citlali_token_logprobs(const void* logits, int dtype, const int32_t* tokens, float* logprobs, float* entropy, int32_t* top_ids,
+                                      float* top_logprobs, int rows, int vocab, int top, cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (vocab <= 0 || vocab > 0x7fffffff - 65536 || top < 0 || top > lp::kMost || top > vocab || rows > 0x7fffffff / lp::kMaxCluster) {
+        set_last_error("token_logprobs: %d rows of %d entries, %d alternatives (at most %d, and no more than entries)", rows, vocab, top, lp::kMost);
+        return kBadShape;
+    }
+    if ((uintptr_t)logits % (dtype == kF32 ? 4 : 2) != 0) {
+        set_last_error("token_logprobs: logits are not aligned");
+        return kBadAlignment;
+    }
+    int cluster = 1;
+    while (cluster < lp::kMaxCluster && rows * cluster < 4 * device_sm_count() && vocab >= 2 * cluster * lp::kThreads * lp::kEach) cluster *= 2;
+    return CITLALI_DISPATCH_FLOAT(dtype, T, [&]() {
+        return top > 0 ? lp::launch<T, true>(logits, tokens, logprobs, entropy, top_ids, top_logprobs, rows, vocab, top, cluster, stream)
+                       : lp::launch<T, false>(logits, tokens, logprobs, entropy, top_ids, top_logprobs, rows, vocab, top, cluster, stream);
+    });
+}

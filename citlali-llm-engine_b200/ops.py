@@ -488,6 +488,36 @@ def sample_rows(logits, temperature, uniform, tokens):
                                      _i(vocab), _stream()), "sample_rows")
 
 
+def token_logprobs(logits, tokens=None, top: int = 0) -> dict:
+    """What a model says about the tokens of its rows.  Over the finite entries of each row of ``logits`` (float32 or bfloat16
+    [rows, vocab]): ``"logprobs"`` [rows], the log probability of ``tokens[r]`` (int32; None: not asked for), ``"entropy"`` [rows], and with
+    ``top`` > 0 (at most 32) the likeliest tokens, ``"top_ids"`` (int32) and ``"top_logprobs"`` [rows, top], likeliest first, the lowest
+    id first among equals, -1 and minus infinity where a row has no more.  A token outside the vocabulary has the log probability NaN, one
+    whose entry is not finite minus infinity."""
+    if logits.dim() != 2 or not _are_here(logits, tokens):
+        require(logits.dim() == 2, "token_logprobs: logits are [rows, vocabulary]")
+        _here("token_logprobs", logits, tokens)
+    rows, vocab = logits.shape
+    top = _i(top)
+    if not (0 <= top <= 32 and top <= max(vocab, 0)):
+        require(False, f"token_logprobs: {top} alternatives of {vocab} entries (at most 32)")
+    if tokens is not None and not (tokens.dtype is torch.int32 and tokens.numel() == rows):
+        require(False, "token_logprobs: tokens are int32, one a row")
+    floats = torch.empty((2 + top) * rows, dtype=torch.float32, device=logits.device)
+    found = {"logprobs": floats[:rows], "entropy": floats[rows:2 * rows]}
+    if tokens is None:
+        del found["logprobs"]
+    ids = None
+    if top:
+        ids = found["top_ids"] = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+        found["top_logprobs"] = floats[2 * rows:].view(rows, top)
+    if rows:
+        at = floats.data_ptr()
+        _check(lib().citlali_token_logprobs(logits.data_ptr(), _dtype_code(logits), _ptr(tokens), at, at + 4 * rows, _ptr(ids), at + 8 * rows, rows,
+                                            vocab, top, _stream()), "token_logprobs")
+    return found
+
+
 # ---- choices between kernels ---------------------------------------------------------------
 
 def attention_steps_from_device(dtype, head_dim: int) -> bool:
