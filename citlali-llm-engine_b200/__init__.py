@@ -13,7 +13,7 @@ from .weights import (SafetensorsFile, TensorSpec, WeightHandle, WeightLoader, w
 from .cache import PAGE_SIZE, KVRequirement, KVView, Packed4, SequenceCache, StateRequirement
 from .parts import BuildContext, StepBatch, build_part, register_part, registered_parts, unregister_part
 from .engine import (DecoderModel, GenerationOptions, GenerationResult, InferenceSession, StepEntry,
-                     StopReason, expected_tensors, run_generation)
+                     StopReason, TokenDetails, expected_tensors, run_generation)
 from .sampling import Sampler, uniform
 
 __all__ = [n for n in dir() if not n.startswith("_")]

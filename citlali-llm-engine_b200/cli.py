@@ -8,7 +8,7 @@ Kept from the reference with their names, defaults and meaning (main.cpp:203-247
 prompts are token ids: ``--prompt-ids 1,2,3`` (repeat it for a batch) or ``--prompt-file``
 (a JSON list of lists).  Text modes, quantized residency and remote offload have no
 counterpart: their options are refused with the reason.  Added: ``--temperature``, ``--seed``, ``--stop-ids``, ``--dtype``, ``--slots``,
-``--json``, ``--random-weights SEED``.
+``--json``, ``--random-weights SEED``, ``--cache-dtype int4``, ``--logprobs N``.
 """
 from __future__ import annotations
 
@@ -30,6 +30,8 @@ USAGE = """usage: citlali_cli --model <dir> (--prompt-ids 1,2,3 [--prompt-ids ..
   --seed N                 seed of temperature sampling (default 0)
   --stop-ids a,b           stop tokens (default: eos_token_id of config.json)
   --dtype bfloat16|float32 compute precision (default bfloat16)
+  --cache-dtype int4       keys and values in 4 bits (default: the compute precision)
+  --logprobs N             log probabilities and entropies of the generated tokens, and the N likeliest beside each (0 to 32)
   --slots N                sequences run together (default 8)
   --random-weights SEED    ignore model.safetensors: random weights from this seed
   --info                   print the configuration and sizes; load no weights
@@ -60,6 +62,8 @@ class CliArgs:
     stop_ids: Optional[List[int]] = None
     dtype: str = "bfloat16"
     slots: int = 8
+    cache_dtype: Optional[str] = None
+    logprobs: Optional[int] = None
     random_weights: Optional[int] = None
     info: bool = False
     json: bool = False
@@ -108,6 +112,10 @@ def parse_args(argv: List[str]) -> CliArgs:
             args.stop_ids = _ids(need_value(arg), arg)
         elif arg == "--dtype":
             args.dtype = need_value(arg)
+        elif arg == "--cache-dtype":
+            args.cache_dtype = need_value(arg)
+        elif arg == "--logprobs":
+            args.logprobs = int(need_value(arg))
         elif arg == "--slots":
             args.slots = int(need_value(arg))
         elif arg == "--random-weights":
@@ -197,11 +205,12 @@ def run_cli(argv: List[str]) -> int:
     if args.random_weights is not None:
         session.load_random(config_from_model_dir(args.model_path), args.random_weights,
                             max_context=args.max_context, dtype=args.dtype, max_batch=args.slots,
-                            gain_spread=0.1)
+                            gain_spread=0.1, cache_dtype=args.cache_dtype)
     else:
-        session.load_model(args.model_path, max_context=args.max_context, dtype=args.dtype, max_batch=args.slots)
+        session.load_model(args.model_path, max_context=args.max_context, dtype=args.dtype, max_batch=args.slots,
+                           cache_dtype=args.cache_dtype)
     options = GenerationOptions(max_new_tokens=args.max_new_tokens, max_context=args.max_context,
-                                temperature=args.temperature, seed=args.seed, stop_ids=args.stop_ids)
+                                temperature=args.temperature, seed=args.seed, stop_ids=args.stop_ids, logprobs=args.logprobs)
     started = time.perf_counter()
     results = session.generate(args.prompts, options)
     seconds = time.perf_counter() - started
@@ -210,11 +219,15 @@ def run_cli(argv: List[str]) -> int:
     if args.json:
         print(json.dumps({
             "results": [{"tokens": r.tokens, "generated_tokens": r.generated_tokens,
-                         "stop_reason": r.stop_reason.value} for r in results],
+                         "stop_reason": r.stop_reason.value,
+                         **({} if args.logprobs is None else {"logprobs": r.logprobs, "entropies": r.entropies,
+                                                              "alternatives": r.alternatives})} for r in results],
             "stats": {"tokens": generated, "time_s": seconds, **st}}))
     else:
         for i, r in enumerate(results):
             print(f"[{i}] " + ",".join(str(t) for t in r.tokens))
+            if args.logprobs is not None:
+                print(f"[{i}] logprobs " + ",".join(f"{v:.4f}" for v in r.logprobs))
     speed = generated / seconds if seconds > 0 else 0.0
     stops = ",".join(r.stop_reason.value for r in results)
     pre_s, dec_s = st.get("prefill_s", 0.0), st.get("decode_s", 0.0)

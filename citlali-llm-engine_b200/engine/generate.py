@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import enum
 from dataclasses import dataclass, field
-from typing import Callable, List, Optional, Sequence
+from typing import Callable, List, Optional, Sequence, Tuple
 
 from ..errors import require
 from ..sampling.rng import uniform
@@ -33,6 +33,7 @@ class GenerationOptions:           # include/citlali/runtime/session.h:16-20, pl
     seed: int = 0
     stop_ids: Optional[Sequence[int]] = None    # None: the model's eos ids from config.json
     max_batch: Optional[int] = None             # None: as many as the session has slots
+    logprobs: Optional[int] = None              # so many likeliest tokens beside each token's log probability (0: none beside; None: neither)
 
 
 @dataclass
@@ -40,6 +41,26 @@ class GenerationResult:            # include/citlali/runtime/session.h:30-34, to
     tokens: List[int] = field(default_factory=list)
     generated_tokens: int = 0
     stop_reason: StopReason = StopReason.MAX_NEW_TOKENS
+    # With ``GenerationOptions.logprobs``, for every token of ``tokens``: its log probability and the entropy of the distribution it
+    # came from (of the logits themselves, whatever the temperature), and the likeliest tokens as (id, log probability).
+    logprobs: Optional[List[float]] = None
+    entropies: Optional[List[float]] = None
+    alternatives: Optional[List[List[Tuple[int, float]]]] = None
+
+
+@dataclass
+class TokenDetails:
+    """What the model says of the tokens of some rows, on the host (``ops.token_logprobs``)."""
+    logprobs: List[float]
+    entropies: List[float]
+    alternatives: List[List[Tuple[int, float]]]
+
+    @staticmethod
+    def of(found: dict) -> "TokenDetails":
+        ids, logs = ((found[k].tolist() if k in found else None) for k in ("top_ids", "top_logprobs"))
+        rows = found["entropy"].tolist()
+        beside = [[(i, v) for i, v in zip(a, b) if i >= 0] for a, b in zip(ids, logs)] if ids is not None else [[] for _ in rows]
+        return TokenDetails(found["logprobs"].tolist(), rows, beside)
 
 
 def run_generation(stepper, prompts: Sequence[Sequence[int]], options: GenerationOptions,
@@ -47,7 +68,8 @@ def run_generation(stepper, prompts: Sequence[Sequence[int]], options: Generatio
                    on_token: Optional[Callable[[int, int], None]] = None) -> List[GenerationResult]:
     """``stepper`` provides ``acquire() -> slot``, ``release(slot)``,
     ``prefill(slots, prompts, temperature, uniforms) -> tokens`` and
-    ``decode(slots, tokens, temperature, uniforms) -> tokens`` (one sampled token per sequence)."""
+    ``decode(slots, tokens, temperature, uniforms) -> tokens`` (one sampled token per sequence); with ``options.logprobs`` also
+    ``details``, the :class:`TokenDetails` of the tokens it sampled last."""
     require(len(prompts) > 0, "no prompts were given")
     require(max_batch > 0, "max_batch must be positive")
     require(options.max_new_tokens >= 0, "max_new_tokens must not be negative")
@@ -56,7 +78,11 @@ def run_generation(stepper, prompts: Sequence[Sequence[int]], options: Generatio
         require(len(p) < options.max_context,
                 f"prompt {i} has {len(p)} tokens, which leaves no room in a context of {options.max_context}")
     stops = set(int(s) for s in stop_ids)
+    require(options.logprobs is None or 0 <= options.logprobs <= 32, "logprobs must be None or a number of alternatives from 0 to 32")
     results = [GenerationResult() for _ in prompts]
+    if options.logprobs is not None:
+        for res in results:
+            res.logprobs, res.entropies, res.alternatives = [], [], []
     for first in range(0, len(prompts), max_batch):
         _run_batch(stepper, prompts, list(range(first, min(first + max_batch, len(prompts)))),
                    options, stops, results, on_token)
@@ -89,7 +115,8 @@ def _run_batch(stepper, prompts, requests, options, stops, results, on_token):
                                   temperature, draws(active))
         while True:
             survivors, feed = [], []
-            for (r, slot), token in zip(active, sampled):
+            details = stepper.details if options.logprobs is not None else None
+            for row, ((r, slot), token) in enumerate(zip(active, sampled)):
                 res = results[r]
                 done = None
                 if token in stops:
@@ -97,6 +124,10 @@ def _run_batch(stepper, prompts, requests, options, stops, results, on_token):
                 else:
                     res.tokens.append(int(token))
                     res.generated_tokens += 1
+                    if details is not None:
+                        res.logprobs.append(details.logprobs[row])
+                        res.entropies.append(details.entropies[row])
+                        res.alternatives.append(details.alternatives[row])
                     if on_token is not None:
                         on_token(r, int(token))
                     if res.generated_tokens >= options.max_new_tokens:

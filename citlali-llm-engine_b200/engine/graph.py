@@ -172,6 +172,10 @@ class DecodeGraphRunner:
         """Make the tokens just sampled the next step's input, on the device."""
         self._piece(self.ints, 0, n).copy_(self.out_tokens[:n], non_blocking=True)
 
+    def last_logits(self, n: int, temperature: float) -> torch.Tensor:
+        """The logits of the step launched last, which had ``n`` sequences (the next step of as many overwrites them)."""
+        return self.logits[(n, temperature <= 0.0)]
+
     def read_tokens(self, n: int) -> List[int]:
         self.out_host[:n].copy_(self.out_tokens[:n], non_blocking=True)
         torch.cuda.current_stream().synchronize()

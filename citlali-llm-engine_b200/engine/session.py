@@ -22,7 +22,7 @@ from ..sampling.sampler import Sampler
 from ..weights.loader import WeightHandle, WeightLoader
 from ..weights.random_init import random_tensor
 from .graph import DecodeGraphRunner, model_is_graph_safe
-from .generate import GenerationOptions, GenerationResult, run_generation
+from .generate import GenerationOptions, GenerationResult, TokenDetails, run_generation
 from .model import DecoderModel
 from .step import StepEntry, pack_step
 
@@ -54,6 +54,8 @@ def _cuda_device(device) -> torch.device:
 
 
 class InferenceSession:
+    SCORE_ROWS = 1024          # tokens that :meth:`score` makes logits of at a time
+
     def __init__(self):
         self.model: Optional[DecoderModel] = None
         self.cache: Optional[SequenceCache] = None
@@ -62,6 +64,8 @@ class InferenceSession:
         self.max_context = 0
         self.stats: Dict[str, float] = {}
         self.runner = None
+        self.details: Optional[TokenDetails] = None    # of the tokens sampled last, while a generation asks for them
+        self._alternatives: Optional[int] = None
         self.use_graphs = True     # set False before loading to step without CUDA graphs
         self.page_size = PAGE_SIZE  # tokens a cache page holds; set before loading (the tensor-core attention kernels take 64)
 
@@ -191,6 +195,7 @@ class InferenceSession:
         t0 = time.perf_counter()
         logits = self.step([StepEntry(s, p, [len(p) - 1]) for s, p in zip(slots, prompts)])
         tokens = self.sampler.sample(logits, temperature, uniforms)
+        self._keep_details(logits, self.sampler.last_tokens(len(tokens)))
         self.stats["prefill_s"] = self.stats.get("prefill_s", 0.0) + time.perf_counter() - t0
         self.stats["prefill_tokens"] = self.stats.get("prefill_tokens", 0) + sum(len(p) for p in prompts)
         return tokens
@@ -206,12 +211,65 @@ class InferenceSession:
                         f"slot {s}: one more token exceeds max_context {self.max_context}")
             self.runner.launch(slots, tokens, temperature, uniforms)
             out = self.runner.read_tokens(len(slots))
+            if self._alternatives is not None:
+                self._keep_details(self.runner.last_logits(len(slots), temperature), self.runner.out_tokens[:len(slots)])
         else:
             logits = self.step([StepEntry(s, [t], [0]) for s, t in zip(slots, tokens)])
             out = self.sampler.sample(logits, temperature, uniforms)
+            self._keep_details(logits, self.sampler.last_tokens(len(out)))
         self.stats["decode_s"] = self.stats.get("decode_s", 0.0) + time.perf_counter() - t0
         self.stats["decode_tokens"] = self.stats.get("decode_tokens", 0) + len(slots)
         return out
+
+    def _keep_details(self, logits, tokens) -> None:
+        """What the model says of the tokens just sampled, if a generation asks for it (on the device ``tokens``, int32)."""
+        if self._alternatives is not None:
+            top = min(self._alternatives, logits.shape[1])
+            self.details = TokenDetails.of(ops.token_logprobs(logits, tokens, top))
+
+    def score(self, texts: Sequence[Sequence[int]], top: int = 0) -> List[TokenDetails]:
+        """How likely the model finds each text (a list of token ids): for every token but the first its log probability given
+        the ones before it, the entropy of the distribution it is drawn from, and the ``top`` (at most 32) likeliest tokens there as
+        (id, log probability).  As many texts at a time as there are slots; logits are made for up to ``SCORE_ROWS`` tokens at a time."""
+        require(self.model is not None, "no model is loaded")
+        require(0 <= top <= 32, "top must be a number of alternatives from 0 to 32")
+        texts = [list(t) for t in texts]
+        vocab = self.model.spec.vocab_size
+        for i, t in enumerate(texts):
+            require(len(t) > 0, f"text {i} has no tokens")
+            require(len(t) - 1 <= self.max_context, f"text {i} has {len(t)} tokens, more than a context of {self.max_context} and the one behind it")
+            require(0 <= int(t[-1]) < vocab, f"token id {t[-1]} out of vocab range [0, {vocab})")       # (the step checks those it reads)
+        found = [TokenDetails([], [], []) for _ in texts]
+        for first in range(0, len(texts), self.max_batch):
+            active = [i for i in range(first, min(first + self.max_batch, len(texts))) if len(texts[i]) > 1]
+            slots, done = {}, {i: 0 for i in active}
+            try:
+                for i in active:
+                    slots[i] = self.acquire()
+                while active:
+                    room, entries, wanted = self.SCORE_ROWS, [], []
+                    for i in active:
+                        n = min(room, len(texts[i]) - 1 - done[i])
+                        if n > 0:
+                            entries.append(StepEntry(slots[i], texts[i][done[i]:done[i] + n], range(n)))
+                            wanted.append((i, n))
+                            room -= n
+                    logits = self.step(entries)
+                    given = torch.tensor([t for i, n in wanted for t in texts[i][done[i] + 1:done[i] + n + 1]], dtype=torch.int32).to(logits.device)
+                    details = TokenDetails.of(ops.token_logprobs(logits, given, min(top, vocab)))
+                    at = 0
+                    for i, n in wanted:
+                        found[i].logprobs += details.logprobs[at:at + n]
+                        found[i].entropies += details.entropies[at:at + n]
+                        found[i].alternatives += details.alternatives[at:at + n]
+                        at += n
+                        done[i] += n
+                    active = [i for i in active if done[i] < len(texts[i]) - 1]
+            finally:
+                for slot in slots.values():
+                    self.release(slot)
+        self.check_device_errors()
+        return found
 
     def generate(self, prompts: Sequence[Sequence[int]], options: Optional[GenerationOptions] = None,
                  on_token: Optional[Callable[[int, int], None]] = None) -> List[GenerationResult]:
@@ -223,11 +281,15 @@ class InferenceSession:
         options = options or GenerationOptions()
         context = min(options.max_context, self.max_context)
         opts = GenerationOptions(options.max_new_tokens, context, options.temperature, options.seed,
-                                 options.stop_ids, options.max_batch)
+                                 options.stop_ids, options.max_batch, options.logprobs)
         stops = options.stop_ids if options.stop_ids is not None else self.model.spec.stop_token_ids
         batch = min(options.max_batch or self.max_batch, self.max_batch)
         self.stats = {}
-        results = run_generation(self, prompts, opts, stops, batch, on_token)
+        self._alternatives = options.logprobs
+        try:
+            results = run_generation(self, prompts, opts, stops, batch, on_token)
+        finally:
+            self._alternatives = self.details = None
         self.check_device_errors()
         return results
 

@@ -258,213 +258,6 @@ def attention_rows(q, q_stride, k_pool, v_pool, page_table, row_slot, row_pos, o
         _stream()), "attention_rows")
 
 
-# ---- keys and values in 4 bits --------------------------------------------------------------
-
-def _here(what: str, *tensors):
-    """Says what is wrong with tensors that are not all contiguous and on the device whose stream the kernels are launched on."""
-    _need_cuda(*tensors)
-    for t in tensors:
-        require(t is None or t.device.index == _current_device(), f"{what}: a tensor is on {None if t is None else t.device}, kernels are launched "
-                f"on the current device, cuda:{_current_device()}")
-
-
-def _are_here(*tensors) -> bool:
-    """Whether all of them are contiguous and on the device whose stream the kernels are launched on."""
-    here = _current_device()
-    for t in tensors:
-        if t is not None and not (t.get_device() == here and t.is_contiguous()):
-            return False
-    return True
-
-
-def _check_packed4(kv, nkv: int, head_dim: int, what: str):
-    """Says what is wrong with a view of a cache in 4 bits (a step has many calls: the callers look quickly, and come here for the words)."""
-    require(head_dim % 16 == 0 and 16 <= head_dim <= 256,
-            f"{what}: a cache in 4 bits takes head sizes that are multiples of 16 up to 256, not {head_dim}")
-    pages = None
-    for part in (kv.keys, kv.values):
-        require(isinstance(part, Packed4), f"{what}: the cache does not hold its keys and values in 4 bits")
-        for t, width in ((part.codes, head_dim // 2), (part.scales, head_dim // 16)):
-            pages = t.shape[0] if pages is None else pages
-            require(t.dtype == torch.uint8 and tuple(t.shape) == (pages, nkv, kv.page_size, width),
-                    f"{what}: the cache's pools are bytes of [pages, {nkv} heads, {kv.page_size} tokens, {head_dim} / 2 or / 16], "
-                    f"not {t.dtype} {list(t.shape)}")
-    require(kv.page_table.dtype == torch.int32 and kv.page_table.dim() == 2, f"{what}: the page table is int32 [slots, pages]")
-    _here(what, kv.keys.codes, kv.keys.scales, kv.values.codes, kv.values.scales, kv.page_table)
-
-
-def _packed4(kv, nkv: int, head_dim: int, what: str):
-    """Addresses of the four pools and of the page table, and the table's width."""
-    keys, values, table = kv.keys, kv.values, kv.page_table
-    if type(keys) is Packed4 and type(values) is Packed4 and head_dim % 16 == 0 and 16 <= head_dim <= 256:
-        kc, ks, vc, vs = keys.codes, keys.scales, values.codes, values.scales
-        codes, scales, shape = kc.shape, ks.shape, (nkv, kv.page_size)
-        if (codes[1:3] == shape and codes[3] * 2 == head_dim and scales[0] == codes[0] and scales[1:3] == shape and scales[3] * 16 == head_dim
-                and vc.shape == codes and vs.shape == scales and len(codes) == len(scales) == 4
-                and kc.dtype is torch.uint8 and ks.dtype is torch.uint8 and vc.dtype is torch.uint8 and vs.dtype is torch.uint8
-                and table.dtype is torch.int32 and table.dim() == 2 and _are_here(kc, ks, vc, vs, table)):
-            return kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), table.data_ptr(), table.shape[1]
-    _check_packed4(kv, nkv, head_dim, what)
-    raise CitlaliError(f"{what}: the cache's view does not fit")
-
-
-def cache4_append(qkv, kv, row_slot, row_pos, nq: int, nkv: int, head_dim: int, inv_freq, rotary_dim: int, q_gain=None, k_gain=None,
-                  eps: float = 0.0, q_out=None, store: bool = True):
-    """:func:`qk_norm_rope_cache` for a cache in 4 bits (``kv``: its view, keys and values :class:`~.cache.Packed4`).  Of the rows
-    ``qkv`` [rows, (nq + 2 nkv) head_dim] = [q | k | v], q and k heads get their norm (gains None: none) and the rotation of their
-    first ``rotary_dim`` elements in pairs (i, i + rotary_dim / 2); queries go to ``q_out`` [rows, nq head_dim] (None: back into the
-    rows), keys and values into the page of each row's slot and position.  ``store`` False: the queries only.  The angles are the
-    products of position and frequency to more than 32 bits."""
-    rows, width = qkv.shape
-    wide = nq * head_dim
-    if not (nq >= 0 and nkv >= 0 and width == wide + 2 * nkv * head_dim and rotary_dim % 2 == 0 and 0 <= rotary_dim <= head_dim
-            and inv_freq.dtype is torch.float32 and inv_freq.numel() * 2 == rotary_dim and row_slot.dtype is torch.int32
-            and row_pos.dtype is torch.int32 and row_slot.numel() == rows and row_pos.numel() == rows
-            and (q_gain is None or q_gain.numel() == head_dim) and (k_gain is None or k_gain.numel() == head_dim)
-            and (q_gain is None or k_gain is None or q_gain.dtype is k_gain.dtype)
-            and _are_here(qkv, q_gain, k_gain, inv_freq, row_slot, row_pos)):
-        require(nq >= 0 and nkv >= 0 and width == wide + 2 * nkv * head_dim, "cache4_append: the projection's width does not fit")
-        require(rotary_dim % 2 == 0 and 0 <= rotary_dim <= head_dim, f"cache4_append: the rotated part of a head ({rotary_dim} elements) "
-                f"must be even and at most the head size {head_dim}")
-        require(inv_freq.dtype == torch.float32 and inv_freq.numel() == rotary_dim // 2, "cache4_append: bad frequency table")
-        require(row_slot.dtype == torch.int32 and row_pos.dtype == torch.int32 and row_slot.numel() == rows and row_pos.numel() == rows,
-                "cache4_append: slots and positions are int32, one a row")
-        for gain in (q_gain, k_gain):
-            require(gain is None or gain.numel() == head_dim, "cache4_append: a head norm's gain has the head's size")
-        require(q_gain is None or k_gain is None or q_gain.dtype == k_gain.dtype, "cache4_append: q and k gains differ in dtype")
-        _here("cache4_append", qkv, q_gain, k_gain, inv_freq, row_slot, row_pos)
-    store = 1 if store and nkv > 0 else 0
-    pools, page_size = (None, None, None, None, None, 0), 1
-    if store:
-        pools, page_size = _packed4(kv, nkv, head_dim, "cache4_append"), kv.page_size
-    q_ptr, q_stride = qkv.data_ptr(), width
-    if q_out is not None:
-        q_ptr, q_stride = q_out.data_ptr(), q_out.stride(0)
-        if not (q_out.shape == (rows, wide) and q_out.dtype is qkv.dtype and q_out.get_device() == qkv.get_device()
-                and (q_out.stride(1) == 1 or wide <= 1) and (rows <= 1 or q_stride >= wide)):
-            require(False, "cache4_append: q_out is [rows, query heads * head size] of the rows' dtype and device, its rows apart")
-        if rows <= 1:
-            q_stride = wide
-    if rows == 0 or (nq == 0 and not store):
-        return
-    gain = q_gain if q_gain is not None else k_gain
-    kc, ks, vc, vs, table, table_width = pools
-    _check(lib().citlali_cache4_append(
-        qkv.data_ptr(), _dtype_code(qkv), q_ptr, q_stride, _ptr(q_gain), _ptr(k_gain), _F32 if gain is None else _dtype_code(gain),
-        inv_freq.data_ptr(), _i(rotary_dim), row_slot.data_ptr(), row_pos.data_ptr(), table, table_width, kc, ks, vc, vs, _i(page_size), rows,
-        _i(nq), _i(nkv), _i(head_dim), _f(eps), store, _stream()), "cache4_append")
-
-
-def cache4_read(kv, slots, positions, dtype=torch.bfloat16):
-    """What a cache in 4 bits holds: (keys, values) [rows, kv heads, head size] in ``dtype`` (bfloat16 holds the values exactly) for
-    ``positions[r]`` (int32) of slot ``slots[r]``."""
-    require(isinstance(kv.keys, Packed4), "cache4_read: the cache does not hold its keys and values in 4 bits")
-    _, nkv, _, width = kv.keys.codes.shape
-    pools = _packed4(kv, nkv, 2 * width, "cache4_read")
-    rows = slots.numel()
-    if not (slots.dtype is torch.int32 and positions.dtype is torch.int32 and positions.numel() == rows and _are_here(slots, positions)):
-        _here("cache4_read", slots, positions)
-        require(False, "cache4_read: slots and positions are int32, one a row")
-    if dtype is not torch.bfloat16 and dtype is not torch.float32:
-        require(False, f"cache4_read: values come in bfloat16 or float32, not {dtype}")
-    held = torch.empty((2, rows, nkv, 2 * width), dtype=dtype, device=slots.device)
-    keys, values = held[0], held[1]
-    if rows:
-        kc, ks, vc, vs, table, table_width = pools
-        _check(lib().citlali_cache4_read(kc, ks, vc, vs, table, table_width, _i(kv.page_size), slots.data_ptr(), positions.data_ptr(),
-                                         keys.data_ptr(), values.data_ptr(), _dtype_code(held), rows, nkv, 2 * width, _stream()), "cache4_read")
-    return keys, values
-
-
-@functools.lru_cache(maxsize=None)
-def _attention4_floats(nq: int, nkv: int, head_dim: int, page_size: int, max_new: int, device: int) -> int:
-    """The scratch that the tensor-core kernel asks for on this device; -1: it does not take these sizes."""
-    l = lib()
-    if not l.citlali_attention4_supports(head_dim, page_size):
-        return -1
-    return l.citlali_attention4_scratch_floats(nq, nkv, head_dim, max_new)
-
-
-_EXPAND_FROM = 40                          # new tokens
-_EXPAND_BYTES = 1 << 30
-
-
-def _attention4_expands(q, q_stride, out, batch, nq, nkv, head_dim, page_size) -> bool:
-    """Whether runs go over pages that were made bfloat16 first, by the kernels of a cache of 16 bits."""
-    return (batch.max_new >= _EXPAND_FROM and q.dtype is torch.bfloat16 and page_size == 64 and nkv > 0 and nq % nkv == 0 and q_stride % 8 == 0
-            and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0 and lib().citlali_attention_run_form(q_stride, out.shape[1], head_dim, 64, batch.max_new) > 0)
-
-
-def _attention4_expanded(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
-    """The pages that the rows see as bfloat16 (the values are exact there), then prompt attention over them: as many sequences at a
-    time as a gigabyte holds, at least one."""
-    require(not torch.cuda.is_current_stream_capturing(), "cache4_attention: runs of tokens are sized from the host's lists of lengths, "
-            "which a captured step would freeze")
-    pools, l, page_bytes = _packed4(kv, nkv, head_dim, "cache4_attention"), lib(), 2 * nkv * 64 * head_dim * 2
-    kc, ks, vc, vs, table, table_width = pools
-    tiles, ends = [], []                      # pages of each sequence, and where its last one lies in its row of the table
-    for p, n in zip(batch.past, batch.n_new):
-        ends.append((p + n - 1) // 64 + 1)
-        tiles.append(ends[-1] - (max(0, p - window + 1) // 64 if window else 0))
-    b0 = 0
-    while b0 < len(tiles):
-        b1, pages = b0 + 1, tiles[b0]
-        while b1 < len(tiles) and (pages + tiles[b1]) * page_bytes <= _EXPAND_BYTES:
-            pages += tiles[b1]
-            b1 += 1
-        count, width, max_new = b1 - b0, max(ends[b0:b1]), max(batch.n_new[b0:b1])
-        held = torch.empty((2, pages, nkv, 64, head_dim), dtype=torch.bfloat16, device=q.device)
-        found = torch.empty((count + 1, max(width, count)), dtype=torch.int32, device=q.device)        # the table's rows, then the slots
-        seq_start, seq_slot, seq_past = batch.seq_start[b0:b1 + 1], batch.seq_slot[b0:b1], batch.seq_past[b0:b1]
-        _check(l.citlali_cache4_expand(kc, ks, vc, vs, table, table_width, seq_start.data_ptr(), seq_slot.data_ptr(), seq_past.data_ptr(), count,
-                                       window, held[0].data_ptr(), held[1].data_ptr(), pages, found.data_ptr(), found.shape[1],
-                                       found[count].data_ptr(), 64, nkv, head_dim, _stream()), "cache4_expand")
-        run = attention_prefill_tc if l.citlali_attention_run_form(q_stride, out.shape[1], head_dim, 64, max_new) == 2 else attention_prefill
-        run(q, q_stride, held[0], held[1], found[:count], seq_start, found[count, :count], seq_past, out, count, max_new, nq, nkv, head_dim, 64,
-            window, scale)
-        b0 = b1
-
-
-def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
-    """:func:`attention` over a cache in 4 bits: every row of the step over its slot's keys up to its own position (the last
-    ``window`` of them; 0 or None: all).  bfloat16 with head size 64, 128 or 256 and pages of 64 runs on the tensor cores, anything
-    else in 32-bit arithmetic; longer runs of tokens go over pages that were made bfloat16 first.  A step of single tokens launches nothing that depends on the host's lists of lengths."""
-    kc, ks, vc, vs, table, table_width = _packed4(kv, nkv, head_dim, "cache4_attention")
-    row_slot, row_pos, seq_start = batch.row_slot, batch.row_pos, batch.seq_start
-    rows, wide = row_slot.shape[0], nq * head_dim
-    if not (q.dtype is out.dtype and out.dim() == 2 and out.shape[0] >= rows and out.shape[1] == wide and q_stride >= wide
-            and q.numel() >= (rows - 1) * q_stride + wide and _are_here(q, out, row_slot, row_pos, seq_start, batch.seq_slot, batch.seq_past)):
-        _here("cache4_attention", q, out, row_slot, row_pos, seq_start, batch.seq_slot, batch.seq_past)
-        require(q.dtype == out.dtype and out.dim() == 2 and out.shape[0] >= rows and out.shape[1] == wide,
-                "cache4_attention: the result is [rows, query heads * head size] of the queries' dtype")
-        require(False, "cache4_attention: the queries' rows do not fit")
-    if rows == 0:
-        return
-    q_ptr, window = q.data_ptr(), _i(window or 0)
-    if not batch.is_decode and _attention4_expands(q, q_stride, out, batch, nq, nkv, head_dim, kv.page_size):
-        _attention4_expanded(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale)
-        return
-    if q.dtype is torch.bfloat16 and q_stride % 8 == 0 and (q_ptr | kc | ks | vc | vs) % 16 == 0 and nkv > 0 and nq % nkv == 0:
-        single = batch.is_decode
-        max_new = 1 if single else batch.max_new
-        floats = _attention4_floats(nq, nkv, head_dim, kv.page_size, max_new, _current_device())
-        if floats >= 0:
-            # of this call alone, and given back in stream order: two graphs, or two streams, share nothing
-            partial = torch.empty(floats, dtype=torch.float32, device=q.device)
-            start, slot, past = (None, row_slot, row_pos) if single else (seq_start.data_ptr(), batch.seq_slot, batch.seq_past)
-            _check(lib().citlali_attention4(
-                q_ptr, _sz(q_stride), kc, ks, vc, vs, table, table_width, start, slot.data_ptr(), past.data_ptr(), out.data_ptr(), wide,
-                partial.data_ptr(), floats, len(batch.slots), max_new, nq, nkv, head_dim, kv.page_size, window, _f(scale), _stream()),
-                "cache4_attention")
-            return
-    _check(lib().citlali_attention4_rows(
-        q_ptr, _sz(q_stride), _dtype_code(q), kc, ks, vc, vs, table, table_width, row_slot.data_ptr(), row_pos.data_ptr(), out.data_ptr(), wide, rows,
-        _i(nq), _i(nkv), _i(head_dim), _i(kv.page_size), window, _f(scale), _stream()), "cache4_attention_rows")
-
-
-_KERNELS_PER_CALL["cache4_attention"] = 2
-
-
 def argmax_rows(logits: torch.Tensor, tokens: torch.Tensor):
     _need_cuda(logits, tokens)
     require(logits.dtype == torch.float32 and tokens.dtype == torch.int32, "argmax_rows: float32 in, int32 out")
@@ -656,6 +449,219 @@ def attention_decode_with(q, kv, batch, out, nq, nkv, d, vd, window, scale, soft
         _sz(counters.numel() // 4), _i(rows), _i(nq), _i(nkv), _i(d), _i(vd), _i(kv.page_size), _i(int(window or 0)), _f(scale),
         _f(float(softcap or 0.0)), _ptr(gate), _sz(gate.stride(0) if gate is not None else 0), _ptr(sink), _ptr(turns),
         _i(1 if turn_pairs else 0), _ptr(out if out.dtype == torch.float32 else None), _stream()), "attention_decode_with")
+
+
+# ---- keys and values in 4 bits --------------------------------------------------------------
+
+def _here(what: str, *tensors):
+    """Says what is wrong with tensors that are not all contiguous and on the device whose stream the kernels are launched on."""
+    _need_cuda(*tensors)
+    for t in tensors:
+        require(t is None or t.device.index == _current_device(), f"{what}: a tensor is on {None if t is None else t.device}, kernels are launched "
+                f"on the current device, cuda:{_current_device()}")
+
+
+def _are_here(*tensors) -> bool:
+    """Whether all of them are contiguous and on the device whose stream the kernels are launched on."""
+    here = -1
+    for t in tensors:
+        if t is not None:
+            device = t.get_device()
+            if device < 0 or (device != here and here >= 0) or not t.is_contiguous():
+                return False
+            here = device
+    return here < 0 or here == _current_device()
+
+
+def _check_packed4(kv, nkv: int, head_dim: int, what: str):
+    """Says what is wrong with a view of a cache in 4 bits (a step has many calls: the callers look quickly, and come here for the words)."""
+    require(head_dim % 16 == 0 and 16 <= head_dim <= 256,
+            f"{what}: a cache in 4 bits takes head sizes that are multiples of 16 up to 256, not {head_dim}")
+    pages = None
+    for part in (kv.keys, kv.values):
+        require(isinstance(part, Packed4), f"{what}: the cache does not hold its keys and values in 4 bits")
+        for t, width in ((part.codes, head_dim // 2), (part.scales, head_dim // 16)):
+            pages = t.shape[0] if pages is None else pages
+            require(t.dtype == torch.uint8 and tuple(t.shape) == (pages, nkv, kv.page_size, width),
+                    f"{what}: the cache's pools are bytes of [pages, {nkv} heads, {kv.page_size} tokens, {head_dim} / 2 or / 16], "
+                    f"not {t.dtype} {list(t.shape)}")
+    require(kv.page_table.dtype == torch.int32 and kv.page_table.dim() == 2, f"{what}: the page table is int32 [slots, pages]")
+    _here(what, kv.keys.codes, kv.keys.scales, kv.values.codes, kv.values.scales, kv.page_table)
+
+
+def _packed4(kv, nkv: int, head_dim: int, what: str):
+    """Addresses of the four pools and of the page table, and the table's width."""
+    keys, values, table = kv.keys, kv.values, kv.page_table
+    if type(keys) is Packed4 and type(values) is Packed4 and head_dim % 16 == 0 and 16 <= head_dim <= 256:
+        kc, ks, vc, vs = keys.codes, keys.scales, values.codes, values.scales
+        codes, scales, shape = kc.shape, ks.shape, (nkv, kv.page_size)
+        if (codes[1:3] == shape and codes[3] * 2 == head_dim and scales[0] == codes[0] and scales[1:3] == shape and scales[3] * 16 == head_dim
+                and vc.shape == codes and vs.shape == scales and len(codes) == len(scales) == 4
+                and kc.dtype is torch.uint8 and ks.dtype is torch.uint8 and vc.dtype is torch.uint8 and vs.dtype is torch.uint8
+                and table.dtype is torch.int32 and table.dim() == 2 and _are_here(kc, ks, vc, vs, table)):
+            return kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), table.data_ptr(), table.shape[1]
+    _check_packed4(kv, nkv, head_dim, what)
+    raise CitlaliError(f"{what}: the cache's view does not fit")
+
+
+def cache4_append(qkv, kv, row_slot, row_pos, nq: int, nkv: int, head_dim: int, inv_freq, rotary_dim: int, q_gain=None, k_gain=None,
+                  eps: float = 0.0, q_out=None, store: bool = True):
+    """:func:`qk_norm_rope_cache` for a cache in 4 bits (``kv``: its view, keys and values :class:`~.cache.Packed4`).  Of the rows
+    ``qkv`` [rows, (nq + 2 nkv) head_dim] = [q | k | v], q and k heads get their norm (gains None: none) and the rotation of their
+    first ``rotary_dim`` elements in pairs (i, i + rotary_dim / 2); queries go to ``q_out`` [rows, nq head_dim] (None: back into the
+    rows), keys and values into the page of each row's slot and position.  ``store`` False: the queries only.  The angles are the
+    products of position and frequency to more than 32 bits."""
+    rows, width = qkv.shape
+    wide = nq * head_dim
+    if not (nq >= 0 and nkv >= 0 and width == wide + 2 * nkv * head_dim and rotary_dim % 2 == 0 and 0 <= rotary_dim <= head_dim
+            and inv_freq.dtype is torch.float32 and inv_freq.numel() * 2 == rotary_dim and row_slot.dtype is torch.int32
+            and row_pos.dtype is torch.int32 and row_slot.numel() == rows and row_pos.numel() == rows
+            and (q_gain is None or q_gain.numel() == head_dim) and (k_gain is None or k_gain.numel() == head_dim)
+            and (q_gain is None or k_gain is None or q_gain.dtype is k_gain.dtype)
+            and _are_here(qkv, q_gain, k_gain, inv_freq, row_slot, row_pos)):
+        require(nq >= 0 and nkv >= 0 and width == wide + 2 * nkv * head_dim, "cache4_append: the projection's width does not fit")
+        require(rotary_dim % 2 == 0 and 0 <= rotary_dim <= head_dim, f"cache4_append: the rotated part of a head ({rotary_dim} elements) "
+                f"must be even and at most the head size {head_dim}")
+        require(inv_freq.dtype == torch.float32 and inv_freq.numel() == rotary_dim // 2, "cache4_append: bad frequency table")
+        require(row_slot.dtype == torch.int32 and row_pos.dtype == torch.int32 and row_slot.numel() == rows and row_pos.numel() == rows,
+                "cache4_append: slots and positions are int32, one a row")
+        for gain in (q_gain, k_gain):
+            require(gain is None or gain.numel() == head_dim, "cache4_append: a head norm's gain has the head's size")
+        require(q_gain is None or k_gain is None or q_gain.dtype == k_gain.dtype, "cache4_append: q and k gains differ in dtype")
+        _here("cache4_append", qkv, q_gain, k_gain, inv_freq, row_slot, row_pos)
+    store = 1 if store and nkv > 0 else 0
+    pools, page_size = (None, None, None, None, None, 0), 1
+    if store:
+        pools, page_size = _packed4(kv, nkv, head_dim, "cache4_append"), kv.page_size
+    q_ptr, q_stride = qkv.data_ptr(), width
+    if q_out is not None:
+        q_ptr, q_stride = q_out.data_ptr(), q_out.stride(0)
+        if not (q_out.shape == (rows, wide) and q_out.dtype is qkv.dtype and q_out.get_device() == qkv.get_device()
+                and (q_out.stride(1) == 1 or wide <= 1) and (rows <= 1 or q_stride >= wide)):
+            require(False, "cache4_append: q_out is [rows, query heads * head size] of the rows' dtype and device, its rows apart")
+        if rows <= 1:
+            q_stride = wide
+    if rows == 0 or (nq == 0 and not store):
+        return
+    gain = q_gain if q_gain is not None else k_gain
+    kc, ks, vc, vs, table, table_width = pools
+    _check(lib().citlali_cache4_append(
+        qkv.data_ptr(), _dtype_code(qkv), q_ptr, q_stride, _ptr(q_gain), _ptr(k_gain), _F32 if gain is None else _dtype_code(gain),
+        inv_freq.data_ptr(), _i(rotary_dim), row_slot.data_ptr(), row_pos.data_ptr(), table, table_width, kc, ks, vc, vs, _i(page_size), rows,
+        _i(nq), _i(nkv), _i(head_dim), _f(eps), store, _stream()), "cache4_append")
+
+
+def cache4_read(kv, slots, positions, dtype=torch.bfloat16):
+    """What a cache in 4 bits holds: (keys, values) [rows, kv heads, head size] in ``dtype`` (bfloat16 holds the values exactly) for
+    ``positions[r]`` (int32) of slot ``slots[r]``."""
+    require(isinstance(kv.keys, Packed4), "cache4_read: the cache does not hold its keys and values in 4 bits")
+    _, nkv, _, width = kv.keys.codes.shape
+    pools = _packed4(kv, nkv, 2 * width, "cache4_read")
+    rows = slots.numel()
+    if not (slots.dtype is torch.int32 and positions.dtype is torch.int32 and positions.numel() == rows and _are_here(slots, positions)):
+        _here("cache4_read", slots, positions)
+        require(False, "cache4_read: slots and positions are int32, one a row")
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        require(False, f"cache4_read: values come in bfloat16 or float32, not {dtype}")
+    held = torch.empty((2, rows, nkv, 2 * width), dtype=dtype, device=slots.device)
+    keys, values = held[0], held[1]
+    if rows:
+        kc, ks, vc, vs, table, table_width = pools
+        _check(lib().citlali_cache4_read(kc, ks, vc, vs, table, table_width, _i(kv.page_size), slots.data_ptr(), positions.data_ptr(),
+                                         keys.data_ptr(), values.data_ptr(), _dtype_code(held), rows, nkv, 2 * width, _stream()), "cache4_read")
+    return keys, values
+
+
+@functools.lru_cache(maxsize=None)
+def _attention4_floats(nq: int, nkv: int, head_dim: int, page_size: int, max_new: int, device: int) -> int:
+    """The scratch that the tensor-core kernel asks for on this device; -1: it does not take these sizes."""
+    l = lib()
+    if not l.citlali_attention4_supports(head_dim, page_size):
+        return -1
+    return l.citlali_attention4_scratch_floats(nq, nkv, head_dim, max_new)
+
+
+_EXPAND_FROM = 40                          # new tokens
+_EXPAND_BYTES = 1 << 30
+
+
+def _attention4_expands(q, q_stride, out, batch, nq, nkv, head_dim, page_size) -> bool:
+    """Whether runs go over pages that were made bfloat16 first, by the kernels of a cache of 16 bits."""
+    return (batch.max_new >= _EXPAND_FROM and q.dtype is torch.bfloat16 and page_size == 64 and nkv > 0 and nq % nkv == 0 and q_stride % 8 == 0
+            and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0 and lib().citlali_attention_run_form(q_stride, out.shape[1], head_dim, 64, batch.max_new) > 0)
+
+
+def _attention4_expanded(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
+    """The pages that the rows see as bfloat16 (the values are exact there), then prompt attention over them: as many sequences at a
+    time as a gigabyte holds, at least one."""
+    require(not torch.cuda.is_current_stream_capturing(), "cache4_attention: runs of tokens are sized from the host's lists of lengths, "
+            "which a captured step would freeze")
+    pools, l, page_bytes = _packed4(kv, nkv, head_dim, "cache4_attention"), lib(), 2 * nkv * 64 * head_dim * 2
+    kc, ks, vc, vs, table, table_width = pools
+    tiles, ends = [], []                      # pages of each sequence, and where its last one lies in its row of the table
+    for p, n in zip(batch.past, batch.n_new):
+        ends.append((p + n - 1) // 64 + 1)
+        tiles.append(ends[-1] - (max(0, p - window + 1) // 64 if window else 0))
+    b0 = 0
+    while b0 < len(tiles):
+        b1, pages = b0 + 1, tiles[b0]
+        while b1 < len(tiles) and (pages + tiles[b1]) * page_bytes <= _EXPAND_BYTES:
+            pages += tiles[b1]
+            b1 += 1
+        count, width, max_new = b1 - b0, max(ends[b0:b1]), max(batch.n_new[b0:b1])
+        held = torch.empty((2, pages, nkv, 64, head_dim), dtype=torch.bfloat16, device=q.device)
+        found = torch.empty((count + 1, max(width, count)), dtype=torch.int32, device=q.device)        # the table's rows, then the slots
+        seq_start, seq_slot, seq_past = batch.seq_start[b0:b1 + 1], batch.seq_slot[b0:b1], batch.seq_past[b0:b1]
+        _check(l.citlali_cache4_expand(kc, ks, vc, vs, table, table_width, seq_start.data_ptr(), seq_slot.data_ptr(), seq_past.data_ptr(), count,
+                                       window, held[0].data_ptr(), held[1].data_ptr(), pages, found.data_ptr(), found.shape[1],
+                                       found[count].data_ptr(), 64, nkv, head_dim, _stream()), "cache4_expand")
+        run = _run_kernels[l.citlali_attention_run_form(q_stride, out.shape[1], head_dim, 64, max_new) == 2]
+        run(q, q_stride, held[0], held[1], found[:count], seq_start, found[count, :count], seq_past, out, count, max_new, nq, nkv, head_dim, 64,
+            window, scale)
+        b0 = b1
+
+
+_run_kernels = (attention_prefill, attention_prefill_tc)        # (as they are here: one who times the calls of this module times the whole)
+
+
+def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
+    """:func:`attention` over a cache in 4 bits: every row of the step over its slot's keys up to its own position (the last
+    ``window`` of them; 0 or None: all).  bfloat16 with head size 64, 128 or 256 and pages of 64 runs on the tensor cores, anything
+    else in 32-bit arithmetic; longer runs of tokens go over pages that were made bfloat16 first.  A step of single tokens launches nothing that depends on the host's lists of lengths."""
+    kc, ks, vc, vs, table, table_width = _packed4(kv, nkv, head_dim, "cache4_attention")
+    row_slot, row_pos, seq_start = batch.row_slot, batch.row_pos, batch.seq_start
+    rows, wide = row_slot.shape[0], nq * head_dim
+    if not (q.dtype is out.dtype and out.dim() == 2 and out.shape[0] >= rows and out.shape[1] == wide and q_stride >= wide
+            and q.numel() >= (rows - 1) * q_stride + wide and _are_here(q, out, row_slot, row_pos, seq_start, batch.seq_slot, batch.seq_past)):
+        _here("cache4_attention", q, out, row_slot, row_pos, seq_start, batch.seq_slot, batch.seq_past)
+        require(q.dtype == out.dtype and out.dim() == 2 and out.shape[0] >= rows and out.shape[1] == wide,
+                "cache4_attention: the result is [rows, query heads * head size] of the queries' dtype")
+        require(False, "cache4_attention: the queries' rows do not fit")
+    if rows == 0:
+        return
+    q_ptr, window = q.data_ptr(), _i(window or 0)
+    if not batch.is_decode and _attention4_expands(q, q_stride, out, batch, nq, nkv, head_dim, kv.page_size):
+        _attention4_expanded(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale)
+        return
+    if q.dtype is torch.bfloat16 and q_stride % 8 == 0 and (q_ptr | kc | ks | vc | vs) % 16 == 0 and nkv > 0 and nq % nkv == 0:
+        single = batch.is_decode
+        max_new = 1 if single else batch.max_new
+        floats = _attention4_floats(nq, nkv, head_dim, kv.page_size, max_new, _current_device())
+        if floats >= 0:
+            # of this call alone, and given back in stream order: two graphs, or two streams, share nothing
+            partial = torch.empty(floats, dtype=torch.float32, device=q.device)
+            start, slot, past = (None, row_slot, row_pos) if single else (seq_start.data_ptr(), batch.seq_slot, batch.seq_past)
+            _check(lib().citlali_attention4(
+                q_ptr, _sz(q_stride), kc, ks, vc, vs, table, table_width, start, slot.data_ptr(), past.data_ptr(), out.data_ptr(), wide,
+                partial.data_ptr(), floats, len(batch.slots), max_new, nq, nkv, head_dim, kv.page_size, window, _f(scale), _stream()),
+                "cache4_attention")
+            return
+    _check(lib().citlali_attention4_rows(
+        q_ptr, _sz(q_stride), _dtype_code(q), kc, ks, vc, vs, table, table_width, row_slot.data_ptr(), row_pos.data_ptr(), out.data_ptr(), wide, rows,
+        _i(nq), _i(nkv), _i(head_dim), _i(kv.page_size), window, _f(scale), _stream()), "cache4_attention_rows")
+
+
+_KERNELS_PER_CALL["cache4_attention"] = 2
 
 
 _sm_count = {}

@@ -49,6 +49,10 @@ class Sampler:
         ops.sample_rows(logits, self._params[0], self._params[1], tokens)
         return tokens
 
+    def last_tokens(self, rows: int) -> torch.Tensor:
+        """The ids chosen last (int32, on the device), until the next call."""
+        return self._tokens[:rows]
+
     def sample(self, logits: torch.Tensor, temperature: float, uniforms: Sequence[float]) -> List[int]:
         """Token ids on the host (one device-to-host copy and one synchronisation)."""
         rows = logits.shape[0]
