@@ -81,8 +81,8 @@ struct Tile {
 };
 __device__ __forceinline__ Tile tile_of(const Attention4& a, const Sequence& s, int segment) {
     Tile t;
-    const int part = segment / s.tiles, head_tile = part % a.head_tiles;
-    t.kv = part / a.head_tiles;
+    const int part = s.tiles == 1 ? segment : segment / s.tiles, head_tile = a.head_tiles == 1 ? 0 : part % a.head_tiles;
+    t.kv = a.head_tiles == 1 ? part : part / a.head_tiles;
     t.token0 = (segment - part * s.tiles) * a.tokens;
     t.tokens = min(a.tokens, s.fresh - t.token0);
     t.head0 = t.kv * a.group + head_tile * a.heads;
@@ -135,6 +135,11 @@ __device__ __forceinline__ Piece piece_of(const Sequence& s, uint32_t base, uint
     p.from = x > p.first ? (int)(x - p.first) : 0;
     p.to = end > p.first ? min(s.units, (int)(end - p.first)) : 0;
     return p;
+}
+// Of a column: the token of the tile and the head of the group.
+__device__ __forceinline__ void split_column(int column, int tokens, int heads, int& token, int& head) {
+    token = tokens == 1 ? 0 : column / heads;
+    head = column - token * heads;
 }
 // How the line is dealt out: places of a warp.
 __device__ __forceinline__ uint32_t places_of_a_warp(uint32_t length, int blocks) {
@@ -201,16 +206,16 @@ struct Part {
 };
 
 // Sizes of a block's shared memory: the warps' rings (each at least as large as what its warp parks there at the end), then what a warp
-// parks of a segment that began ahead of it, and the parts' descriptions.
+// parks of a segment that began ahead of it, and the parts' descriptions.  A stage of a ring holds up to two units of one page.
 template <int D, int NT>
 struct Layout {
     static constexpr int columns = 8 * NT;
-    static constexpr int codes = kUnitKeys * D / 2, scales = kUnitKeys * D / kGroup, unit = 2 * (codes + scales);
+    static constexpr int codes = kUnitKeys * D / 2, scales = kUnitKeys * D / kGroup, stage = 4 * (codes + scales);
     static constexpr int parked = columns * (D + 2) * 4;
-    static constexpr int stages = D == 64 ? 8 : (NT == 1 ? 4 : 6);
-    static constexpr int ring = stages * unit;
+    static constexpr int stages = D == 64 ? 4 : (D == 128 && NT == 2 ? 3 : 2);
+    static constexpr int ring = stages * stage;
     static_assert(ring >= parked && ring % 16 == 0 && parked % 16 == 0, "a warp parks its last part in its ring");
-    static constexpr int bytes = kWarps4 * (ring + parked + 2 * (int)sizeof(Part)) + kWarps4 * 2 * columns * 4 + columns * 8;
+    static constexpr int bytes = kWarps4 * (ring + parked + 2 * (int)sizeof(Part));
     static constexpr int per_sm = D == 256 ? 1 : (NT == 1 ? 2 : 1);
 };
 
@@ -220,6 +225,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     using L = Layout<D, NT>;
     constexpr int C = L::columns, S = L::stages;
     constexpr int KW = D / 32, VW = D / 64;              // words of a key and of a value that a lane holds
+    constexpr int KSC = 4 * L::codes, VSC = KSC + 2 * L::scales;          // in a stage: keys' codes, values' codes, keys' scales, values' scales
     extern __shared__ __align__(16) uint8_t shared[];
     dependents_may_launch();
     // (positions and page tables come from the host before the step; what other kernels write is read behind the wait)
@@ -227,8 +233,6 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     uint8_t* ring = shared + warp * L::ring;
     float* early = reinterpret_cast<float*>(shared + kWarps4 * L::ring + warp * L::parked);      // [column][m, l, O]
     Part* parts = reinterpret_cast<Part*>(shared + kWarps4 * (L::ring + L::parked));             // [warp][early, late]
-    float* weight = reinterpret_cast<float*>(parts + 2 * kWarps4);                               // [part][column]
-    float* whole = weight + 2 * kWarps4 * C;                                                     // [column]: M, then the sum
 
     const uint32_t length = line_length(a), each = places_of_a_warp(length, gridDim.x);
     const uint32_t begin = min(length, (blockIdx.x * kWarps4 + warp) * each), end = min(length, begin + each);
@@ -239,13 +243,13 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     if (lane < 2) parts[2 * warp + lane].first = ~0u;
     Place here = begin < end ? place_of(a, begin) : Place{0, 0};
 
-    // ---- the ring's own way along the line, ahead of the one that computes
+    // ---- the ring's own way along the line, ahead of the one that computes: a piece's units in stages of one or two
     uint32_t fetch_x = begin;                            // the next piece's place
     Place fetch = here;
     int fetch_unit = 0, fetch_end = 0, fetch_head = 0, page = 0, next_page = 0;
     const int32_t* fetch_pages = a.table;
-    auto load_next = [&](int slot) {
-        while (fetch_unit == fetch_end && fetch_x < end) {                       // the next piece with a unit
+    auto next_piece = [&]() {                            // the next piece with a unit
+        while (fetch_unit == fetch_end && fetch_x < end) {
             Sequence s = sequence_of(a, fetch.b);
             while (fetch_x >= fetch.base + s.length()) {
                 fetch.base += s.length();
@@ -261,19 +265,29 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
             page = fetch_pages[fetch_unit >> 2];
             next_page = fetch_pages[(fetch_end - 1) >> 2 > fetch_unit >> 2 ? (fetch_unit >> 2) + 1 : fetch_unit >> 2];
         }
+    };
+    auto load_next = [&](uint8_t* to) {
+        if (fetch_unit == fetch_end) next_piece();
         if (fetch_unit < fetch_end) {
+            const int units = min(2 - (fetch_unit & 1), fetch_end - fetch_unit);
             const size_t at = place(page, a.nkv, fetch_head, kPage, (fetch_unit & 3) * kUnitKeys);
-            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + slot * L::unit) + lane * 16;
+            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to) + lane * 16;
             const uint8_t *kc = a.k_codes + at * (D / 2) + lane * 16, *vc = a.v_codes + at * (D / 2) + lane * 16;
+            constexpr int rounds = L::codes / 512;       // of 32 pieces of 16 bytes, a unit's codes
 #pragma unroll
-            for (int i = 0; i < L::codes; i += 512) {
-                fa::cp_async16(dst + i, kc + i);
-                fa::cp_async16(dst + L::codes + i, vc + i);
-            }
+            for (int i = 0; i < 2 * rounds; ++i)
+                if (i < rounds || units == 2) {
+                    fa::cp_async16(dst + i * 512, kc + i * 512);
+                    fa::cp_async16(dst + 2 * L::codes + i * 512, vc + i * 512);
+                }
             constexpr int pieces = L::scales / 16;       // 16-byte pieces of the scales of a unit's keys
-            if (lane < 2 * pieces)
-                fa::cp_async16(dst + 2 * L::codes, (lane < pieces ? a.k_scales : a.v_scales) + at * (D / kGroup) + (lane % pieces) * 16);
-            ++fetch_unit;
+#pragma unroll
+            for (int i = 0; i < (4 * pieces + 31) / 32; ++i) {
+                const int k = i * 32 + lane, o = k % (2 * pieces);
+                if (k < 4 * pieces && o < units * pieces)
+                    fa::cp_async16(dst + KSC + i * 512, (k < 2 * pieces ? a.k_scales : a.v_scales) + at * (D / kGroup) + o * 16);
+            }
+            fetch_unit += units;
             if ((fetch_unit & 3) == 0) {
                 page = next_page;
                 if (fetch_unit + 4 < fetch_end) next_page = fetch_pages[(fetch_unit >> 2) + 1];
@@ -281,10 +295,11 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
         }
         fa::cp_async_commit();
     };
+    next_piece();
     wait_for_predecessor();
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) load_next(i);
-    int slot = 0;
+    for (int i = 0; i < S - 1; ++i) load_next(ring + i * L::stage);
+    uint8_t *at = ring, *free_stage = ring + (S - 1) * L::stage;
 
     for (uint32_t x = begin; x < end;) {
         // ---- the piece: its tile's columns and their queries
@@ -297,19 +312,19 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
         x = piece.first + s.units;
         if (piece.to <= piece.from) continue;
         const Tile tile = tile_of(a, s, piece.segment);
-        const int used = tile.used(), heads = tile.heads;
+        const int used = tile.used();
         const int pos0 = s.past + tile.token0, last = pos0 + tile.tokens - 1;         // of the first and the last token
         const int low0 = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, low1 = a.window > 0 ? max(0, last - a.window + 1) : 0;
 
         uint32_t qf[NT][2 * KW][2];                      // [columns' eight][contraction step][b0, b1]
         float factor[NT][2];                             // of the columns 2t, 2t + 1
-        int seen[NT][2];                                 // their tokens' positions
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int column = n * 8 + r;
             const bool on = column < used;
-            const __nv_bfloat16* src = a.q + (size_t)(s.row + tile.token0 + (on ? column / heads : 0)) * a.q_stride
-                                       + (size_t)(tile.head0 + (on ? column % heads : 0)) * D + t * (D / 4);
+            int token, head;
+            split_column(on ? column : 0, tile.tokens, tile.heads, token, head);
+            const __nv_bfloat16* src = a.q + (size_t)(s.row + tile.token0 + token) * a.q_stride + (size_t)(tile.head0 + head) * D + t * (D / 4);
             uint4 raw[KW];
             uint32_t most = 0;
 #pragma unroll
@@ -339,10 +354,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
             }
             const float back = __int_as_float((127 - up) << 23) * (a.scale_log2 * kUnit);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                factor[n][j] = __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
-                seen[n][j] = pos0 + min(n * 8 + 2 * t + j, used - 1) / heads;
-            }
+            for (int j = 0; j < 2; ++j) factor[n][j] = __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
         }
         // m: the running maximum less kWeightBits; the lowest number there is where there is none, which no sum with a score overflows to a NaN
         float m[NT][2], l[NT][2], o[NT][D / 16][4];
@@ -353,27 +365,40 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
         }
+        auto position = [&](int column) {                // of the column's token
+            int token, head;
+            split_column(min(column, used - 1), tile.tokens, tile.heads, token, head);
+            return pos0 + token;
+        };
 
         // ---- its units
-        for (int u = s.first_unit + piece.from; u < s.first_unit + piece.to; ++u) {
+        const int stop = s.first_unit + piece.to;
+        for (int u = s.first_unit + piece.from; u < stop;) {
             fa::cp_async_wait<S - 2>();
-            __syncwarp();                                // the unit is there for all lanes, and all are done with the one before
-            load_next(slot == 0 ? S - 1 : slot - 1);
-            uint8_t* at = ring + slot * L::unit;
-            slot = slot + 1 == S ? 0 : slot + 1;
+            __syncwarp();                                // the stage is there for all lanes, and all are done with the one before
+            load_next(free_stage);
+            const uint8_t* const stage = at;
+            free_stage = at;
+            at = at + L::stage == ring + L::ring ? ring : at + L::stage;
             const int key0 = u * kUnitKeys;
-            if (key0 > last || key0 + kUnitKeys <= low0) continue;        // none of the tile's tokens sees any of them
-            const bool border = key0 + kUnitKeys - 1 > pos0 || key0 < low1;
+            const bool two = (u & 1) == 0 && u + 1 < stop;
+            u += two ? 2 : 1;
+            const int key1 = key0 + (two ? 2 : 1) * kUnitKeys;
+            if (key0 > last || key1 <= low0) continue;   // none of the tile's tokens sees any of them
+            const bool border = key1 - 1 > pos0 || key0 < low1;
 
-            float e[NT][4];
+            float e[2][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) e[n][0] = e[n][1] = e[n][2] = e[n][3] = 0.0f;
-            {
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) e[h][n][0] = e[h][n][1] = e[h][n][2] = e[h][n][3] = 0.0f;
+                if (h == 1 && !two) break;
                 uint32_t ka[KW], kb[KW];
-                load_words<KW>(ka, at + r * (D / 2) + t * (D / 8));
-                load_words<KW>(kb, at + (r + 8) * (D / 2) + t * (D / 8));
-                const uint8_t* sa = at + 2 * L::codes + r * (D / kGroup) + t * (D / 64);
-                const uint32_t ba = load_bytes<D / 64>(sa), bb = load_bytes<D / 64>(sa + 8 * (D / kGroup));
+                const uint8_t* codes = stage + h * L::codes + r * (D / 2) + t * (D / 8);
+                load_words<KW>(ka, codes);
+                load_words<KW>(kb, codes + 8 * (D / 2));
+                const uint8_t* scales = stage + KSC + h * L::scales + r * (D / kGroup) + t * (D / 64);
+                const uint32_t ba = load_bytes<D / 64>(scales), bb = load_bytes<D / 64>(scales + 8 * (D / kGroup));
 #pragma unroll
                 for (int g = 0; g < D / 64; ++g) {
                     const Scale ga(__byte_perm(ba, 0, 0x4040 + 0x101 * g)), gb(__byte_perm(bb, 0, 0x4040 + 0x101 * g));
@@ -384,39 +409,33 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                         const uint32_t c0 = first_of(ha, ga), c2 = second_of(ha, ga), c1 = first_of(hb, gb), c3 = second_of(hb, gb);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma_f16(e[n], a0, a1, a2, a3, qf[n][2 * w][0], qf[n][2 * w][1]);
-                            mma_f16(e[n], c0, c1, c2, c3, qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
+                            mma_f16(e[h][n], a0, a1, a2, a3, qf[n][2 * w][0], qf[n][2 * w][1]);
+                            mma_f16(e[h][n], c0, c1, c2, c3, qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
                         }
                     }
                 }
-            }
-            if (border) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int key = key0 + r + (j >> 1) * 8, p = seen[n][j & 1];
-                        e[n][j] *= factor[n][j & 1];
-                        if (key > p || (a.window > 0 && key <= p - a.window)) e[n][j] = -INFINITY;
-                    }
-            } else {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) e[n][j] *= factor[n][j & 1];
             }
             // The maximum only has to keep the weights in range: it is looked for where a score exceeds it.
             bool grows = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) grows |= e[n][j] - m[n][j & 1] > kWeightBits;
+                for (int j = 0; j < 4; ++j) {
+                    e[0][n][j] *= factor[n][j & 1];
+                    e[1][n][j] = two ? e[1][n][j] * factor[n][j & 1] : -INFINITY;
+                    if (border) {
+                        const int p = position(n * 8 + 2 * t + (j & 1)), key = key0 + r + (j >> 1) * 8;
+                        if (key > p || (a.window > 0 && key <= p - a.window)) e[0][n][j] = -INFINITY;
+                        if (key + kUnitKeys > p || (a.window > 0 && key + kUnitKeys <= p - a.window)) e[1][n][j] = -INFINITY;
+                    }
+                    grows |= fmaxf(e[0][n][j], e[1][n][j]) - m[n][j & 1] > kWeightBits;
+                }
             if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float most = fmaxf(e[n][j], e[n][j + 2]);
+                        float most = fmaxf(fmaxf(e[0][n][j], e[0][n][j + 2]), fmaxf(e[1][n][j], e[1][n][j + 2]));
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
                         most = fmaxf(m[n][j], fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16)) - kWeightBits);
@@ -427,34 +446,36 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                         for (int i = 0; i < D / 16; ++i) { o[n][i][j] *= turn; o[n][i][j + 2] *= turn; }
                     }
             }
-            uint32_t p0[NT], p1[NT];
+            uint32_t p[2][NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    e[n][j] = fa::fast_exp2(e[n][j] - m[n][j & 1]);
-                    l[n][j & 1] += e[n][j];
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        e[h][n][j] = fa::fast_exp2(e[h][n][j] - m[n][j & 1]);
+                        l[n][j & 1] += e[h][n][j];
+                    }
+                    p[h][n][0] = transposed(as_word(__floats2half2_rn(e[h][n][0], e[h][n][1])));
+                    p[h][n][1] = transposed(as_word(__floats2half2_rn(e[h][n][2], e[h][n][3])));
                 }
-                p0[n] = transposed(as_word(__floats2half2_rn(e[n][0], e[n][1])));
-                p1[n] = transposed(as_word(__floats2half2_rn(e[n][2], e[n][3])));
-            }
-            uint8_t* scales = at + 2 * L::codes + L::scales;
             if (border) {
                 // What a key that no token of the tile sees holds must not count: even zero times a NaN is one.  Its scales are put to zero
                 // here, where they lie.  A key that is no number and that only some of the tokens see makes their results none by hand.
-                constexpr int words = L::scales / 4, per_key = D / kGroup / 4;
+                uint8_t* const scales = const_cast<uint8_t*>(stage) + VSC;
+                constexpr int words = 2 * L::scales / 4, per_key = D / kGroup / 4;
                 uint32_t w[(words + 31) / 32];
                 bool none = false;
 #pragma unroll
                 for (int i = 0; i < (words + 31) / 32; ++i) {
                     const int at_word = i * 32 + lane, key = key0 + at_word / per_key;
                     w[i] = 0;
-                    if (at_word < words && key >= low0 && key <= last) w[i] = reinterpret_cast<const uint32_t*>(scales)[at_word];
+                    if (at_word < words && key >= low0 && key <= last && key < key1) w[i] = reinterpret_cast<const uint32_t*>(scales)[at_word];
                     none |= __vcmpgeu4(w[i], 0xf8f8f8f8u) != 0;
                 }
                 const bool by_hand = tile.tokens > 1 && __any_sync(0xffffffffu, none);
                 if (by_hand) {
-                    for (int k = 0; k < kUnitKeys; ++k)
+                    for (int k = 0; key0 + k < key1; ++k)
 #pragma unroll
                         for (int h = 0; h < (VW + 1) / 2; ++h) {
                             if (scales[k * (D / kGroup) + (r * (D / 8)) / kGroup + h] < 0xf8) continue;
@@ -462,8 +483,8 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
                                 for (int j = 0; j < 2; ++j) {
-                                    const int key = key0 + k, p = seen[n][j];
-                                    if (key > p || (a.window > 0 && key <= p - a.window)) continue;
+                                    const int key = key0 + k, q = position(n * 8 + 2 * t + j);
+                                    if (key > q || (a.window > 0 && key <= q - a.window)) continue;
 #pragma unroll
                                     for (int i = 8 * h; i < min(8 * h + 8, D / 16); ++i) o[n][i][j] = o[n][i][j + 2] = __int_as_float(0x7fc00000);
                                 }
@@ -476,29 +497,34 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                         reinterpret_cast<uint32_t*>(scales)[i * 32 + lane] = by_hand ? w[i] & ~__vcmpgeu4(w[i], 0xf8f8f8f8u) : w[i];
                 __syncwarp();
             }
-            uint32_t va[VW], vb[VW], vc[VW], vd[VW];
-            const uint8_t* codes = at + L::codes + r * (D / 16);
-            load_words<VW>(va, codes + (2 * t) * (D / 2));
-            load_words<VW>(vb, codes + (2 * t + 1) * (D / 2));
-            load_words<VW>(vc, codes + (2 * t + 8) * (D / 2));
-            load_words<VW>(vd, codes + (2 * t + 9) * (D / 2));
 #pragma unroll
-            for (int h = 0; h < (VW + 1) / 2; ++h) {
-                auto byte = [&](int k) { return (uint32_t)scales[k * (D / kGroup) + (r * (D / 8)) / kGroup + h]; };
-                const Scale ab(byte(2 * t) | byte(2 * t + 1) << 16), cd(byte(2 * t + 8) | byte(2 * t + 9) << 16);
+            for (int half = 0; half < 2; ++half) {
+                if (half == 1 && !two) break;
+                uint32_t va[VW], vb[VW], vc[VW], vd[VW];
+                const uint8_t* codes = stage + 2 * L::codes + half * L::codes + r * (D / 16);
+                load_words<VW>(va, codes + (2 * t) * (D / 2));
+                load_words<VW>(vb, codes + (2 * t + 1) * (D / 2));
+                load_words<VW>(vc, codes + (2 * t + 8) * (D / 2));
+                load_words<VW>(vd, codes + (2 * t + 9) * (D / 2));
+                const uint8_t* scales = stage + VSC + half * L::scales + (r * (D / 8)) / kGroup;
 #pragma unroll
-                for (int w = 2 * h; w < min(2 * h + 2, VW); ++w) {
+                for (int h = 0; h < (VW + 1) / 2; ++h) {
+                    auto byte = [&](int k) { return (uint32_t)scales[k * (D / kGroup) + h]; };
+                    const Scale ab(byte(2 * t) | byte(2 * t + 1) << 16), cd(byte(2 * t + 8) | byte(2 * t + 9) << 16);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t pick = half == 0 ? 0x5410u : 0x7632u;
-                        uint32_t y = __byte_perm(va[w], vb[w], pick), z = __byte_perm(vc[w], vd[w], pick);
+                    for (int w = 2 * h; w < min(2 * h + 2, VW); ++w) {
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const uint32_t a0 = first_of(y, ab), a1 = second_of(y, ab), a2 = first_of(z, cd), a3 = second_of(z, cd);
+                        for (int part = 0; part < 2; ++part) {
+                            const uint32_t pick = part == 0 ? 0x5410u : 0x7632u;
+                            uint32_t y = __byte_perm(va[w], vb[w], pick), z = __byte_perm(vc[w], vd[w], pick);
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) mma_f16(o[n][4 * w + 2 * half + k], a0, a1, a2, a3, p0[n], p1[n]);
-                            y >>= 8;
-                            z >>= 8;
+                            for (int k = 0; k < 2; ++k) {
+                                const uint32_t a0 = first_of(y, ab), a1 = second_of(y, ab), a2 = first_of(z, cd), a3 = second_of(z, cd);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) mma_f16(o[n][4 * w + 2 * part + k], a0, a1, a2, a3, p[half][n][0], p[half][n][1]);
+                                y >>= 8;
+                                z >>= 8;
+                            }
                         }
                     }
                 }
@@ -524,8 +550,9 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                 if (column >= used) continue;
                 if (all) {
                     const float by = kUnit / sum;
-                    __nv_bfloat16* dst = a.out + (size_t)(s.row + tile.token0 + column / heads) * a.out_stride
-                                         + (size_t)(tile.head0 + column % heads) * D + r * (D / 8);
+                    int token, head;
+                    split_column(column, tile.tokens, tile.heads, token, head);
+                    __nv_bfloat16* dst = a.out + (size_t)(s.row + tile.token0 + token) * a.out_stride + (size_t)(tile.head0 + head) * D + r * (D / 8);
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i)
                         *reinterpret_cast<uint32_t*>(dst + 2 * i) = fa::pack_bf16(o[n][i][j] * by, o[n][i][j + 2] * by);
@@ -538,61 +565,56 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                 }
             }
         if (!all && lane == 0)
-            parts[2 * warp + (late ? 1 : 0)] = {piece.first, s.units, s.row + tile.token0, tile.head0, heads, used};
+            parts[2 * warp + (late ? 1 : 0)] = {piece.first, s.units, s.row + tile.token0, tile.head0, tile.heads, used};
     }
 
-    // ---- the block's parts, in the order of the line: those of one segment are neighbours
+    // ---- the block's parts, in the order of the line: those of one segment are neighbours.  Nothing is written to shared memory any more.
     __syncthreads();
     const uint32_t block_begin = blockIdx.x * kWarps4 * each, block_end = min(length, block_begin + kWarps4 * each);
-    for (int i = 0; i < 2 * kWarps4;) {
-        const Part part = parts[i];
-        if (part.first == ~0u) { ++i; continue; }
-        int stop = i + 1;
-        while (stop < 2 * kWarps4 && (parts[stop].first == part.first || parts[stop].first == ~0u)) ++stop;
-        auto its = [&](int k) {                          // of part k
-            return reinterpret_cast<const float*>((k & 1) ? shared + (k >> 1) * L::ring : shared + kWarps4 * L::ring + (k >> 1) * L::parked);
-        };
-        if (tid < part.used) {
-            float M = kNoScore;
-            for (int k = i; k < stop; ++k)
-                if (parts[k].first != ~0u) M = fmaxf(M, its(k)[tid * (D + 2)]);
-            float sum = 0.0f;
-            for (int k = i; k < stop; ++k) {
-                if (parts[k].first == ~0u) continue;
-                const float by = fa::fast_exp2(its(k)[tid * (D + 2)] - M);
-                weight[k * C + tid] = by;
-                sum = fmaf(its(k)[tid * (D + 2) + 1], by, sum);
-            }
-            whole[2 * tid] = M;
-            whole[2 * tid + 1] = sum;
-        }
-        __syncthreads();
+    const uint32_t mine = lane < 2 * kWarps4 ? parts[lane].first : ~0u;
+    for (unsigned left = __ballot_sync(0xffffffffu, mine != ~0u); left;) {
+        const int k0 = __ffs(left) - 1;
+        const unsigned run = __ballot_sync(0xffffffffu, mine == __shfl_sync(0xffffffffu, mine, k0)) & left;
+        left &= ~run;
+        const Part part = parts[k0];
         const bool begins = part.first >= block_begin, all = begins && part.first + part.units <= block_end;
         float* part_out = a.partial + (size_t)(blockIdx.x * 2 + (begins ? 1 : 0)) * C * (D + 2);
-        for (int k = tid; k < part.used * D; k += kThreads4) {
-            const int column = k / D, element = k % D;
-            float sum = 0.0f;
-            for (int n = i; n < stop; ++n)
-                if (parts[n].first != ~0u) sum = fmaf(its(n)[column * (D + 2) + 2 + element], weight[n * C + column], sum);
+        for (int i = tid; i < part.used * D; i += kThreads4) {
+            const int column = i / D, element = i % D;
+            auto its = [&](int k) {                      // of part k
+                return reinterpret_cast<const float*>(shared + (k >> 1) * ((k & 1) ? L::ring : L::parked) + ((k & 1) ? 0 : kWarps4 * L::ring))
+                       + column * (D + 2);
+            };
+            float M = kNoScore, sum = 0.0f, value = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2 * kWarps4; ++k)
+                if (run >> k & 1) M = fmaxf(M, its(k)[0]);
+#pragma unroll
+            for (int k = 0; k < 2 * kWarps4; ++k)
+                if (run >> k & 1) {
+                    const float* one = its(k);
+                    const float by = fa::fast_exp2(one[0] - M);
+                    sum = fmaf(one[1], by, sum);
+                    value = fmaf(one[2 + element], by, value);
+                }
             if (all) {
-                a.out[(size_t)(part.row + column / part.heads) * a.out_stride + (size_t)(part.head0 + column % part.heads) * D + element]
-                    = __float2bfloat16_rn(sum * (kUnit / whole[2 * column + 1]));
+                const int tokens = part.used / part.heads;
+                int token, head;
+                split_column(column, tokens, part.heads, token, head);
+                a.out[(size_t)(part.row + token) * a.out_stride + (size_t)(part.head0 + head) * D + element] = __float2bfloat16_rn(value * (kUnit / sum));
             } else {
-                part_out[column * (D + 2) + 2 + element] = sum;
-                if (element < 2) part_out[column * (D + 2) + element] = whole[2 * column + element];
+                part_out[column * (D + 2) + 2 + element] = value;
+                if (element == 0) *reinterpret_cast<float2*>(part_out + column * (D + 2)) = make_float2(M, sum);
             }
         }
-        __syncthreads();
-        i = stop;
     }
 }
 
 // Block i merges the segment whose unit 0 is in the share of block i and that goes on behind it, if there is one: its first part is in
 // slot 1 of block i, the others in slot 0 of the blocks behind.
 template <int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(256)
 attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
-    extern __shared__ float merge[];                     // [columns][parts]
     dependents_may_launch();
     const uint32_t length = line_length(a), share = places_of_a_warp(length, gridDim.x) * kWarps4;
     const uint32_t begin = blockIdx.x * share, end = begin + share;
@@ -605,30 +627,25 @@ attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
     if (piece.first < begin || piece.first >= end) return;               // it began earlier, or only its room is here
     const Tile tile = tile_of(a, s, piece.segment);
     const int parts = (int)((piece.first + s.units - 1) / share - blockIdx.x) + 1, used = tile.used();
-    auto its = [&](int column, int p) {
-        return a.partial + ((size_t)((blockIdx.x + p) * 2 + (p == 0 ? 1 : 0)) * columns + column) * (D + 2);
-    };
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int column = warp; column < used; column += 4) {
-        float M = kNoScore;
-        for (int p = lane; p < parts; p += 32) M = fmaxf(M, its(column, p)[0]);
-        M = warp_max(M);
-        float sum = 0.0f;
-        for (int p = lane; p < parts; p += 32) {
-            const float* one = its(column, p);
-            const float by = fa::fast_exp2(one[0] - M);
-            merge[column * parts + p] = by;
-            sum = fmaf(one[1], by, sum);
+    for (int i = threadIdx.x; i < used * D; i += 256) {
+        const int column = i / D, e = i % D;
+        // part 0 is in slot 1 of this block, part p in slot 0 of block i + p
+        const float* one = a.partial + ((size_t)(blockIdx.x * 2 + 1) * columns + column) * (D + 2);
+        const size_t block = (size_t)2 * columns * (D + 2), slot = (size_t)columns * (D + 2);
+        auto its = [&](int p) { return one + p * block - (p ? slot : 0); };
+        float M = kNoScore, sum = 0.0f, value = 0.0f;
+#pragma unroll 8
+        for (int p = 0; p < parts; ++p) M = fmaxf(M, its(p)[0]);
+#pragma unroll 8
+        for (int p = 0; p < parts; ++p) {
+            const float2 ml = *reinterpret_cast<const float2*>(its(p));
+            const float by = fa::fast_exp2(ml.x - M);
+            sum = fmaf(ml.y, by, sum);
+            value = fmaf(its(p)[2 + e], by, value);
         }
-        sum = warp_sum(sum);
-        __syncwarp();
-        const float back = kUnit / sum;
-        for (int e = lane; e < D; e += 32) {
-            float value = 0.0f;
-            for (int p = 0; p < parts; ++p) value = fmaf(its(column, p)[2 + e], merge[column * parts + p], value);
-            a.out[(size_t)(s.row + tile.token0 + column / tile.heads) * a.out_stride + (size_t)(tile.head0 + column % tile.heads) * D + e]
-                = __float2bfloat16_rn(value * back);
-        }
+        int token, head;
+        split_column(column, tile.tokens, tile.heads, token, head);
+        a.out[(size_t)(s.row + tile.token0 + token) * a.out_stride + (size_t)(tile.head0 + head) * D + e] = __float2bfloat16_rn(value * (kUnit / sum));
     }
 }
 
@@ -661,10 +678,7 @@ static int launch(const Attention4& a, int blocks, cudaStream_t stream) {
     if (int e = raise_shared_limit(kernel, bytes, bytes)) return e;
     launch_kernel(kernel, dim3(blocks), kThreads4, bytes, stream, a);
     if (int e = CITLALI_LAUNCH_CHECK()) return e;
-    constexpr int columns = Layout<D, NT>::columns;
-    const size_t weights = (size_t)columns * blocks * sizeof(float);
-    if (int e = raise_shared_limit(attention4_merge_kernel<D>, weights, kRowShared)) return e;
-    launch_kernel(attention4_merge_kernel<D>, dim3(blocks), 128, weights, stream, a, columns);
+    launch_kernel(attention4_merge_kernel<D>, dim3(blocks), 256, 0, stream, a, Layout<D, NT>::columns);
     return CITLALI_LAUNCH_CHECK();
 }
 

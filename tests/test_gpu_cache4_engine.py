@@ -20,10 +20,11 @@ def load(path, dtype, max_context=256, **more):
     return cb.InferenceSession().load_model(path, max_context=max_context, dtype=dtype, max_batch=4, cache_dtype="int4", **more)
 
 
-@pytest.mark.parametrize("name,length", [("A", 40), ("B", 70), ("C", 20)])
-def test_logits_follow_the_plain_model_with_rounded_keys_and_values(model_dirs, monkeypatch, name, length):
+# (tokens whose keys and values all have codes that 32-bit arithmetic settles: see below)
+@pytest.mark.parametrize("name,length,seed", [("A", 40, 4), ("B", 70, 4), ("C", 20, 3)])
+def test_logits_follow_the_plain_model_with_rounded_keys_and_values(model_dirs, monkeypatch, name, length, seed):
     cfg, w = plain.load_folder(model_dirs[(name, "float32")])
-    tokens = random_tokens(cfg["vocab_size"], length, 3)
+    tokens = random_tokens(cfg["vocab_size"], length, seed)
     nearest = [1.0]
 
     def rounded(x):
@@ -41,8 +42,7 @@ def test_logits_follow_the_plain_model_with_rounded_keys_and_values(model_dirs, 
     want = plain.model_logits(cfg, w, tokens)
     # A code is settled where the element is further from the middle between two than 32-bit arithmetic can move it: keys and values
     # are within 2^-18 of their size here, 7 codes' worth of that in steps.
-    if min(nearest) < 7 * 2.0 ** -18:
-        pytest.skip("an element of this model lies next to the middle between two codes")
+    assert min(nearest) > 7 * 2.0 ** -18
     session = load(model_dirs[(name, "float32")], "float32")
     slot = session.acquire()
     got = session.step([cb.StepEntry(slot, tokens, range(length))]).cpu().double()
