@@ -18,15 +18,16 @@
 // c s = (1032 + c) s - 1032 s is one fma whose operands and result are exact (cache4.cuh): four lop3, a shift and four fmas for
 // eight elements.  s here is the byte's half, an eighth of the scale; the 8 comes back in f and in the last division.
 // Queries are made halves after they were multiplied by a power of two that puts the row's largest into [2^14, 2^15): exact for every
-// element above 2^-32 of that.  P is rounded to half (half a step is 2^-11 of it, an eighth of bfloat16's); all weights are 2^15 times
-// what the formula says, which the division takes out again, so that those below 2^-14 of the largest are not subnormal halves.
+// element above 2^-32 of that.  P is rounded to half (half a step is 2^-11 of it, an eighth of bfloat16's); the weights are kept near
+// 2^11 times what the formula says, which the division takes out again, so that only those below 2^-25 of the largest are subnormal halves.
+// l, the sum of the weights, is one more product, with ones.
 //
 // Work.  16 keys are a unit.  The units of all segments (sequence, key/value head, tile) lie end to end on a line, a little room
 // ahead of each segment for what it costs to begin one, and the line is dealt out evenly to the warps, eight neighbouring ones a
 // block, whatever the sequences' lengths, which are read on the device: the launch depends on none and can be captured.  A warp that
 // has a whole segment stores its result.  The parts of one that several warps share are merged by the block when its warps are done,
 // in the order of the keys, and the parts of one that several blocks share go to memory as (m, l, O) in float, for a second kernel
-// that merges them in the same order.  So every sum has an order that the step's lengths fix.
+// that merges them in the same order, or, where the caller gives counters, for the block that comes last.  So every sum has an order that the step's lengths fix.
 #include "api.h"
 #include "cache4.cuh"
 #include "common.cuh"
@@ -35,11 +36,12 @@
 namespace citlali {
 namespace c4 {
 
-constexpr int kPage = 64, kUnitKeys = 16;
+constexpr int kPage = 64, kUnitKeys = 32, kUnitsOfAPage = kPage / kUnitKeys;
 constexpr int kWarps4 = 8, kThreads4 = 32 * kWarps4;
-constexpr float kWeightBits = 15.0f;
+constexpr float kWeightBits = 11.0f, kMostBits = 15.0f;         // of the largest weight when the maximum is looked for, and before it is again
+constexpr uint32_t kOnes = 0x3c003c00u;
 constexpr float kNoScore = -3.402823466e+38f;
-constexpr int kRoom = 4;                // what beginning a segment costs, in units
+constexpr int kRoom = 2;                // what beginning a segment costs, in units
 
 struct Attention4 {
     const __nv_bfloat16* q;
@@ -55,9 +57,10 @@ struct Attention4 {
     int window;
     float scale_log2;
     float* partial;                                      // [blocks][2][columns][D + 2]
+    int32_t* arrived;                                    // [blocks], zero before and after: parts in memory of the segment that begins in a block
 };
 
-// What a sequence of the step asks for: `units` of 16 keys for each of `segments` (head tile of a key/value head, token tile).
+// What a sequence of the step asks for: `units` of 32 keys for each of `segments` (head tile of a key/value head, token tile).
 struct Sequence {
     int past, fresh, row, first_unit, units, tiles, segments;
     __device__ __forceinline__ uint32_t length() const { return (uint32_t)segments * (units + kRoom); }      // on the line
@@ -168,13 +171,23 @@ struct Scale {
         high = __hmul2(s, __float2half2_rn(-72.0f));
     }
 };
-// Nibbles 0 and 4 (first), 1 and 5 (second) of w times the scale.
-__device__ __forceinline__ uint32_t first_of(uint32_t w, const Scale& k) {
-    return as_word(__hfma2(as_half2((w & 0x000f000fu) | 0x64006400u), k.s, k.low));
+// (w & mask) | bits in one instruction: written in C it becomes two, since only one of two constants fits an instruction.
+template <uint32_t kMask>
+__device__ __forceinline__ __half2 picked(uint32_t w, uint32_t bits) {
+    uint32_t x;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "n"(kMask), "r"(bits));
+    return as_half2(x);
 }
-__device__ __forceinline__ uint32_t second_of(uint32_t w, const Scale& k) {
-    return as_word(__hfma2(as_half2((w & 0x00f000f0u) | 0x54005400u), k.s, k.high));
-}
+// Nibbles 0 and 4 (first), 1 and 5 (second) of a word times the scale.  The two constants stay in registers.
+struct Words {
+    uint32_t low, high;
+    __device__ __forceinline__ Words() {
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(low));
+        asm volatile("mov.b32 %0, 0x54005400;" : "=r"(high));
+    }
+    __device__ __forceinline__ uint32_t first_of(uint32_t w, const Scale& k) const { return as_word(__hfma2(picked<0x000f000fu>(w, low), k.s, k.low)); }
+    __device__ __forceinline__ uint32_t second_of(uint32_t w, const Scale& k) const { return as_word(__hfma2(picked<0x00f000f0u>(w, high), k.s, k.high)); }
+};
 
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
@@ -206,11 +219,11 @@ struct Part {
 };
 
 // Sizes of a block's shared memory: the warps' rings (each at least as large as what its warp parks there at the end), then what a warp
-// parks of a segment that began ahead of it, and the parts' descriptions.  A stage of a ring holds up to two units of one page.
+// parks of a segment that began ahead of it, and the parts' descriptions.
 template <int D, int NT>
 struct Layout {
     static constexpr int columns = 8 * NT;
-    static constexpr int codes = kUnitKeys * D / 2, scales = kUnitKeys * D / kGroup, stage = 4 * (codes + scales);
+    static constexpr int codes = kUnitKeys * D / 2, scales = kUnitKeys * D / kGroup, stage = 2 * (codes + scales);
     static constexpr int parked = columns * (D + 2) * 4;
     static constexpr int stages = D == 64 ? 4 : (D == 128 && NT == 2 ? 3 : 2);
     static constexpr int ring = stages * stage;
@@ -219,20 +232,68 @@ struct Layout {
     static constexpr int per_sm = D == 256 ? 1 : (NT == 1 ? 2 : 1);
 };
 
+// The result of a segment from its parts in memory, part 0 in slot 1 of block `first`, part p in slot 0 of block first + p, in the order
+// of the keys.  A warp has 32 elements of one column (D is a multiple of 32); lane p holds the weight of part p.
+template <int D>
+__device__ __forceinline__ void merge_parts(const Attention4& a, int columns, int first, int parts, int row, int tokens, int head0, int heads,
+                                            int threads) {
+    constexpr int kAhead = 16;
+    const int lane = threadIdx.x & 31;
+    const float* part0 = a.partial + (size_t)(first * 2 + 1) * columns * (D + 2);
+    const int block = 2 * columns * (D + 2), slot = columns * (D + 2);
+    for (int i = threadIdx.x; i < tokens * heads * D; i += threads) {
+        const int column = i / D, e = i % D;
+        auto its = [&](int p) { return part0 + (size_t)p * block - (p ? slot : 0) + column * (D + 2); };
+        float ahead[kAhead];                             // the first values are on their way while the weights are worked out
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p) ahead[p] = p < parts ? __ldcg(its(p) + 2 + e) : 0.0f;
+        float M = kNoScore;
+        float2 ml = make_float2(kNoScore, 0.0f);
+        for (int p = lane; p < parts; p += 32) {
+            ml = __ldcg(reinterpret_cast<const float2*>(its(p)));
+            M = fmaxf(M, ml.x);
+        }
+        M = warp_max(M);
+        float sum = 0.0f, value = 0.0f;
+        for (int p0 = 0; p0 < parts; p0 += 32) {
+            if (parts > 32) ml = p0 + lane < parts ? __ldcg(reinterpret_cast<const float2*>(its(p0 + lane))) : make_float2(kNoScore, 0.0f);
+            const float by = fa::fast_exp2(ml.x - M);
+            sum = fmaf(ml.y, by, sum);
+            const int stop = min(32, parts - p0);
+#pragma unroll
+            for (int p = 0; p < kAhead; ++p)
+                if (p < stop) value = fmaf(p0 == 0 ? ahead[p] : __ldcg(its(p0 + p) + 2 + e), __shfl_sync(0xffffffffu, by, p), value);
+            if (stop > kAhead) {
+#pragma unroll
+                for (int p = kAhead; p < 32; ++p)
+                    if (p < stop) value = fmaf(__ldcg(its(p0 + p) + 2 + e), __shfl_sync(0xffffffffu, by, p), value);
+            }
+        }
+        sum = warp_sum(sum);
+        int token, head;
+        split_column(column, tokens, heads, token, head);
+        a.out[(size_t)(row + token) * a.out_stride + (size_t)(head0 + head) * D + e] = __float2bfloat16_rn(value * (kUnit / sum));
+    }
+}
+
 template <int D, int NT>
 __global__ void __launch_bounds__(kThreads4, Layout<D, NT>::per_sm)
 attention4_kernel(const __grid_constant__ Attention4 a) {
     using L = Layout<D, NT>;
     constexpr int C = L::columns, S = L::stages;
     constexpr int KW = D / 32, VW = D / 64;              // words of a key and of a value that a lane holds
-    constexpr int KSC = 4 * L::codes, VSC = KSC + 2 * L::scales;          // in a stage: keys' codes, values' codes, keys' scales, values' scales
+    constexpr int KSC = 2 * L::codes, VSC = KSC + L::scales;              // in a stage: keys' codes, values' codes, keys' scales, values' scales
     extern __shared__ __align__(16) uint8_t shared[];
     dependents_may_launch();
     // (positions and page tables come from the host before the step; what other kernels write is read behind the wait)
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, t = lane & 3;
+    // (the warp's number by way of a shuffle: so the compiler knows that all lanes go the same way wherever it decides)
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), r = lane >> 2, t = lane & 3;
+    const Words words;
     uint8_t* ring = shared + warp * L::ring;
     float* early = reinterpret_cast<float*>(shared + kWarps4 * L::ring + warp * L::parked);      // [column][m, l, O]
     Part* parts = reinterpret_cast<Part*>(shared + kWarps4 * (L::ring + L::parked));             // [warp][early, late]
+    __shared__ Part pending[2];                          // what goes to memory: of a segment that began earlier, and of one that goes on
+    __shared__ int2 merged[2];                           // of those: the first block and the number of parts, where this block merges them
 
     const uint32_t length = line_length(a), each = places_of_a_warp(length, gridDim.x);
     const uint32_t begin = min(length, (blockIdx.x * kWarps4 + warp) * each), end = min(length, begin + each);
@@ -241,9 +302,10 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
         return;
     }
     if (lane < 2) parts[2 * warp + lane].first = ~0u;
+    if (tid < 2) pending[tid].used = 0;
     Place here = begin < end ? place_of(a, begin) : Place{0, 0};
 
-    // ---- the ring's own way along the line, ahead of the one that computes: a piece's units in stages of one or two
+    // ---- the ring's own way along the line, ahead of the one that computes
     uint32_t fetch_x = begin;                            // the next piece's place
     Place fetch = here;
     int fetch_unit = 0, fetch_end = 0, fetch_head = 0, page = 0, next_page = 0;
@@ -262,35 +324,32 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
             fetch_pages = a.table + (size_t)a.seq_slot[fetch.b] * a.table_stride;
             fetch_unit = s.first_unit + p.from;
             fetch_end = s.first_unit + p.to;
-            page = fetch_pages[fetch_unit >> 2];
-            next_page = fetch_pages[(fetch_end - 1) >> 2 > fetch_unit >> 2 ? (fetch_unit >> 2) + 1 : fetch_unit >> 2];
+            page = fetch_pages[fetch_unit / kUnitsOfAPage];
+            next_page = fetch_pages[min(fetch_unit / kUnitsOfAPage + 1, (fetch_end - 1) / kUnitsOfAPage)];
         }
     };
     auto load_next = [&](uint8_t* to) {
         if (fetch_unit == fetch_end) next_piece();
         if (fetch_unit < fetch_end) {
-            const int units = min(2 - (fetch_unit & 1), fetch_end - fetch_unit);
-            const size_t at = place(page, a.nkv, fetch_head, kPage, (fetch_unit & 3) * kUnitKeys);
+            const size_t at = place(page, a.nkv, fetch_head, kPage, fetch_unit % kUnitsOfAPage * kUnitKeys);
             const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to) + lane * 16;
             const uint8_t *kc = a.k_codes + at * (D / 2) + lane * 16, *vc = a.v_codes + at * (D / 2) + lane * 16;
-            constexpr int rounds = L::codes / 512;       // of 32 pieces of 16 bytes, a unit's codes
 #pragma unroll
-            for (int i = 0; i < 2 * rounds; ++i)
-                if (i < rounds || units == 2) {
-                    fa::cp_async16(dst + i * 512, kc + i * 512);
-                    fa::cp_async16(dst + 2 * L::codes + i * 512, vc + i * 512);
-                }
+            for (int i = 0; i < L::codes; i += 512) {
+                fa::cp_async16(dst + i, kc + i);
+                fa::cp_async16(dst + L::codes + i, vc + i);
+            }
             constexpr int pieces = L::scales / 16;       // 16-byte pieces of the scales of a unit's keys
 #pragma unroll
-            for (int i = 0; i < (4 * pieces + 31) / 32; ++i) {
-                const int k = i * 32 + lane, o = k % (2 * pieces);
-                if (k < 4 * pieces && o < units * pieces)
-                    fa::cp_async16(dst + KSC + i * 512, (k < 2 * pieces ? a.k_scales : a.v_scales) + at * (D / kGroup) + o * 16);
+            for (int i = 0; i < (2 * pieces + 31) / 32; ++i) {
+                const int k = i * 32 + lane;
+                if (k < 2 * pieces)
+                    fa::cp_async16(dst + KSC + i * 512, (k < pieces ? a.k_scales : a.v_scales) + at * (D / kGroup) + k % pieces * 16);
             }
-            fetch_unit += units;
-            if ((fetch_unit & 3) == 0) {
+            ++fetch_unit;
+            if (fetch_unit % kUnitsOfAPage == 0) {
                 page = next_page;
-                if (fetch_unit + 4 < fetch_end) next_page = fetch_pages[(fetch_unit >> 2) + 1];
+                if (fetch_unit + kUnitsOfAPage < fetch_end) next_page = fetch_pages[fetch_unit / kUnitsOfAPage + 1];
             }
         }
         fa::cp_async_commit();
@@ -356,12 +415,12 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) factor[n][j] = __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
         }
-        // m: the running maximum less kWeightBits; the lowest number there is where there is none, which no sum with a score overflows to a NaN
-        float m[NT][2], l[NT][2], o[NT][D / 16][4];
+        // m: a running maximum less kWeightBits; the lowest number there is where there is none, which no sum with a score overflows to a NaN
+        float m[NT][2], l[NT][4], o[NT][D / 16][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             m[n][0] = m[n][1] = kNoScore;
-            l[n][0] = l[n][1] = 0.0f;
+            l[n][0] = l[n][1] = l[n][2] = l[n][3] = 0.0f;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
         }
@@ -373,17 +432,14 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
 
         // ---- its units
         const int stop = s.first_unit + piece.to;
-        for (int u = s.first_unit + piece.from; u < stop;) {
+        for (int u = s.first_unit + piece.from; u < stop; ++u) {
             fa::cp_async_wait<S - 2>();
             __syncwarp();                                // the stage is there for all lanes, and all are done with the one before
             load_next(free_stage);
             const uint8_t* const stage = at;
             free_stage = at;
             at = at + L::stage == ring + L::ring ? ring : at + L::stage;
-            const int key0 = u * kUnitKeys;
-            const bool two = (u & 1) == 0 && u + 1 < stop;
-            u += two ? 2 : 1;
-            const int key1 = key0 + (two ? 2 : 1) * kUnitKeys;
+            const int key0 = u * kUnitKeys, key1 = key0 + kUnitKeys;
             if (key0 > last || key1 <= low0) continue;   // none of the tile's tokens sees any of them
             const bool border = key1 - 1 > pos0 || key0 < low1;
 
@@ -392,21 +448,20 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) e[h][n][0] = e[h][n][1] = e[h][n][2] = e[h][n][3] = 0.0f;
-                if (h == 1 && !two) break;
                 uint32_t ka[KW], kb[KW];
-                const uint8_t* codes = stage + h * L::codes + r * (D / 2) + t * (D / 8);
+                const uint8_t* codes = stage + h * (L::codes / 2) + r * (D / 2) + t * (D / 8);
                 load_words<KW>(ka, codes);
                 load_words<KW>(kb, codes + 8 * (D / 2));
-                const uint8_t* scales = stage + KSC + h * L::scales + r * (D / kGroup) + t * (D / 64);
+                const uint8_t* scales = stage + KSC + h * (L::scales / 2) + r * (D / kGroup) + t * (D / 64);
                 const uint32_t ba = load_bytes<D / 64>(scales), bb = load_bytes<D / 64>(scales + 8 * (D / kGroup));
 #pragma unroll
                 for (int g = 0; g < D / 64; ++g) {
                     const Scale ga(__byte_perm(ba, 0, 0x4040 + 0x101 * g)), gb(__byte_perm(bb, 0, 0x4040 + 0x101 * g));
 #pragma unroll
                     for (int w = 2 * g; w < 2 * g + 2; ++w) {
-                        const uint32_t a0 = first_of(ka[w], ga), a2 = second_of(ka[w], ga), a1 = first_of(kb[w], gb), a3 = second_of(kb[w], gb);
+                        const uint32_t a0 = words.first_of(ka[w], ga), a2 = words.second_of(ka[w], ga), a1 = words.first_of(kb[w], gb), a3 = words.second_of(kb[w], gb);
                         const uint32_t ha = ka[w] >> 8, hb = kb[w] >> 8;
-                        const uint32_t c0 = first_of(ha, ga), c2 = second_of(ha, ga), c1 = first_of(hb, gb), c3 = second_of(hb, gb);
+                        const uint32_t c0 = words.first_of(ha, ga), c2 = words.second_of(ha, ga), c1 = words.first_of(hb, gb), c3 = words.second_of(hb, gb);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             mma_f16(e[h][n], a0, a1, a2, a3, qf[n][2 * w][0], qf[n][2 * w][1]);
@@ -415,35 +470,46 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                     }
                 }
             }
-            // The maximum only has to keep the weights in range: it is looked for where a score exceeds it.
-            bool grows = false;
+            // w = 2^(score - m).  m only has to keep the weights in range: it is looked for where one exceeds 2^kMostBits.
+            float w[2][NT][4];
+            float most = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    e[0][n][j] *= factor[n][j & 1];
-                    e[1][n][j] = two ? e[1][n][j] * factor[n][j & 1] : -INFINITY;
+                    w[0][n][j] = fmaf(e[0][n][j], factor[n][j & 1], -m[n][j & 1]);
+                    w[1][n][j] = fmaf(e[1][n][j], factor[n][j & 1], -m[n][j & 1]);
                     if (border) {
                         const int p = position(n * 8 + 2 * t + (j & 1)), key = key0 + r + (j >> 1) * 8;
-                        if (key > p || (a.window > 0 && key <= p - a.window)) e[0][n][j] = -INFINITY;
-                        if (key + kUnitKeys > p || (a.window > 0 && key + kUnitKeys <= p - a.window)) e[1][n][j] = -INFINITY;
+                        if (key > p || (a.window > 0 && key <= p - a.window)) w[0][n][j] = -INFINITY;
+                        if (key + 16 > p || (a.window > 0 && key + 16 <= p - a.window)) w[1][n][j] = -INFINITY;
                     }
-                    grows |= fmaxf(e[0][n][j], e[1][n][j]) - m[n][j & 1] > kWeightBits;
+                    most = fmaxf(most, fmaxf(w[0][n][j], w[1][n][j]));
                 }
-            if (__any_sync(0xffffffffu, grows)) {
+            if (__any_sync(0xffffffffu, most > kMostBits)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float most = fmaxf(fmaxf(e[0][n][j], e[0][n][j + 2]), fmaxf(e[1][n][j], e[1][n][j + 2]));
-                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
-                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
-                        most = fmaxf(m[n][j], fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16)) - kWeightBits);
-                        const float turn = fa::fast_exp2(m[n][j] - most);
-                        m[n][j] = most;
+                        float top = kNoScore;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int i = j; i < 4; i += 2)
+                                if (w[h][n][i] != -INFINITY) top = fmaxf(top, e[h][n][i] * factor[n][j]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(m[n][j], fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - kWeightBits);
+                        const float turn = fa::fast_exp2(m[n][j] - top);
+                        m[n][j] = top;
                         l[n][j] *= turn;
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i) { o[n][i][j] *= turn; o[n][i][j + 2] *= turn; }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int i = j; i < 4; i += 2)
+                                if (w[h][n][i] != -INFINITY) w[h][n][i] = fmaf(e[h][n][i], factor[n][j], -top);
                     }
             }
             uint32_t p[2][NT][2];
@@ -451,26 +517,22 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        e[h][n][j] = fa::fast_exp2(e[h][n][j] - m[n][j & 1]);
-                        l[n][j & 1] += e[h][n][j];
-                    }
-                    p[h][n][0] = transposed(as_word(__floats2half2_rn(e[h][n][0], e[h][n][1])));
-                    p[h][n][1] = transposed(as_word(__floats2half2_rn(e[h][n][2], e[h][n][3])));
+                    p[h][n][0] = transposed(as_word(__floats2half2_rn(fa::fast_exp2(w[h][n][0]), fa::fast_exp2(w[h][n][1]))));
+                    p[h][n][1] = transposed(as_word(__floats2half2_rn(fa::fast_exp2(w[h][n][2]), fa::fast_exp2(w[h][n][3]))));
+                    mma_f16(l[n], kOnes, kOnes, kOnes, kOnes, p[h][n][0], p[h][n][1]);        // every row of the product is the columns' sums
                 }
             if (border) {
                 // What a key that no token of the tile sees holds must not count: even zero times a NaN is one.  Its scales are put to zero
                 // here, where they lie.  A key that is no number and that only some of the tokens see makes their results none by hand.
                 uint8_t* const scales = const_cast<uint8_t*>(stage) + VSC;
-                constexpr int words = 2 * L::scales / 4, per_key = D / kGroup / 4;
-                uint32_t w[(words + 31) / 32];
+                constexpr int count = L::scales / 4, per_key = D / kGroup / 4;
+                uint32_t w[(count + 31) / 32];
                 bool none = false;
 #pragma unroll
-                for (int i = 0; i < (words + 31) / 32; ++i) {
+                for (int i = 0; i < (count + 31) / 32; ++i) {
                     const int at_word = i * 32 + lane, key = key0 + at_word / per_key;
                     w[i] = 0;
-                    if (at_word < words && key >= low0 && key <= last && key < key1) w[i] = reinterpret_cast<const uint32_t*>(scales)[at_word];
+                    if (at_word < count && key >= low0 && key <= last) w[i] = reinterpret_cast<const uint32_t*>(scales)[at_word];
                     none |= __vcmpgeu4(w[i], 0xf8f8f8f8u) != 0;
                 }
                 const bool by_hand = tile.tokens > 1 && __any_sync(0xffffffffu, none);
@@ -492,21 +554,20 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                 }
                 __syncwarp();
 #pragma unroll
-                for (int i = 0; i < (words + 31) / 32; ++i)
-                    if (i * 32 + lane < words)
+                for (int i = 0; i < (count + 31) / 32; ++i)
+                    if (i * 32 + lane < count)
                         reinterpret_cast<uint32_t*>(scales)[i * 32 + lane] = by_hand ? w[i] & ~__vcmpgeu4(w[i], 0xf8f8f8f8u) : w[i];
                 __syncwarp();
             }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                if (half == 1 && !two) break;
                 uint32_t va[VW], vb[VW], vc[VW], vd[VW];
-                const uint8_t* codes = stage + 2 * L::codes + half * L::codes + r * (D / 16);
+                const uint8_t* codes = stage + L::codes + half * (L::codes / 2) + r * (D / 16);
                 load_words<VW>(va, codes + (2 * t) * (D / 2));
                 load_words<VW>(vb, codes + (2 * t + 1) * (D / 2));
                 load_words<VW>(vc, codes + (2 * t + 8) * (D / 2));
                 load_words<VW>(vd, codes + (2 * t + 9) * (D / 2));
-                const uint8_t* scales = stage + VSC + half * L::scales + (r * (D / 8)) / kGroup;
+                const uint8_t* scales = stage + VSC + half * (L::scales / 2) + (r * (D / 8)) / kGroup;
 #pragma unroll
                 for (int h = 0; h < (VW + 1) / 2; ++h) {
                     auto byte = [&](int k) { return (uint32_t)scales[k * (D / kGroup) + h]; };
@@ -519,7 +580,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                             uint32_t y = __byte_perm(va[w], vb[w], pick), z = __byte_perm(vc[w], vd[w], pick);
 #pragma unroll
                             for (int k = 0; k < 2; ++k) {
-                                const uint32_t a0 = first_of(y, ab), a1 = second_of(y, ab), a2 = first_of(z, cd), a3 = second_of(z, cd);
+                                const uint32_t a0 = words.first_of(y, ab), a1 = words.second_of(y, ab), a2 = words.first_of(z, cd), a3 = words.second_of(z, cd);
 #pragma unroll
                                 for (int n = 0; n < NT; ++n) mma_f16(o[n][4 * w + 2 * part + k], a0, a1, a2, a3, p[half][n][0], p[half][n][1]);
                                 y >>= 8;
@@ -542,10 +603,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float sum = l[n][j];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const float sum = l[n][j];
                 const int column = n * 8 + 2 * t + j;
                 if (column >= used) continue;
                 if (all) {
@@ -607,13 +665,35 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                 if (element == 0) *reinterpret_cast<float2*>(part_out + column * (D + 2)) = make_float2(M, sum);
             }
         }
+        if (!all && tid == 0) pending[begins ? 1 : 0] = part;
+    }
+    if (a.arrived == nullptr) return;
+    // The block whose part of a segment comes to memory last merges them all; nobody waits for anybody.
+    const uint32_t share = kWarps4 * each;
+    __syncthreads();
+    if (lane == 0 && warp < 2 && pending[warp].used) {
+        const uint32_t begins = pending[warp].first;
+        const int first = (int)(begins / share), count = (int)((begins + pending[warp].units - 1) / share) - first + 1;
+        __threadfence();                                 // (the block's writes, which the barrier has put ahead)
+        const bool last_one = atomicAdd(a.arrived + first, 1) == count - 1;
+        __threadfence();
+        if (last_one) a.arrived[first] = 0;              // as the next call wants it
+        merged[warp] = last_one ? make_int2(first, count) : make_int2(0, 0);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {
+        const Part part = pending[k];
+        if (part.used && merged[k].y)
+            merge_parts<D>(a, C, merged[k].x, merged[k].y, part.row, part.used / part.heads, part.head0, part.heads, kThreads4);
     }
 }
 
-// Block i merges the segment whose unit 0 is in the share of block i and that goes on behind it, if there is one: its first part is in
-// slot 1 of block i, the others in slot 0 of the blocks behind.
+// The same as a kernel of its own, where there is nothing to count arrivals in: block i merges the segment whose unit 0 is in the share
+// of block i and that goes on behind it, if there is one.
+constexpr int kMergeThreads = 256;
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kMergeThreads)
 attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
     dependents_may_launch();
     const uint32_t length = line_length(a), share = places_of_a_warp(length, gridDim.x) * kWarps4;
@@ -626,27 +706,8 @@ attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
     const Piece piece = piece_of(s, here.base, end, end + 1);
     if (piece.first < begin || piece.first >= end) return;               // it began earlier, or only its room is here
     const Tile tile = tile_of(a, s, piece.segment);
-    const int parts = (int)((piece.first + s.units - 1) / share - blockIdx.x) + 1, used = tile.used();
-    for (int i = threadIdx.x; i < used * D; i += 256) {
-        const int column = i / D, e = i % D;
-        // part 0 is in slot 1 of this block, part p in slot 0 of block i + p
-        const float* one = a.partial + ((size_t)(blockIdx.x * 2 + 1) * columns + column) * (D + 2);
-        const size_t block = (size_t)2 * columns * (D + 2), slot = (size_t)columns * (D + 2);
-        auto its = [&](int p) { return one + p * block - (p ? slot : 0); };
-        float M = kNoScore, sum = 0.0f, value = 0.0f;
-#pragma unroll 8
-        for (int p = 0; p < parts; ++p) M = fmaxf(M, its(p)[0]);
-#pragma unroll 8
-        for (int p = 0; p < parts; ++p) {
-            const float2 ml = *reinterpret_cast<const float2*>(its(p));
-            const float by = fa::fast_exp2(ml.x - M);
-            sum = fmaf(ml.y, by, sum);
-            value = fmaf(its(p)[2 + e], by, value);
-        }
-        int token, head;
-        split_column(column, tile.tokens, tile.heads, token, head);
-        a.out[(size_t)(s.row + tile.token0 + token) * a.out_stride + (size_t)(tile.head0 + head) * D + e] = __float2bfloat16_rn(value * (kUnit / sum));
-    }
+    merge_parts<D>(a, columns, blockIdx.x, (int)((piece.first + s.units - 1) / share - blockIdx.x) + 1, s.row + tile.token0, tile.tokens,
+                   tile.head0, tile.heads, kMergeThreads);
 }
 
 // How a step's columns are tiled.
@@ -674,11 +735,12 @@ template <int D, int NT>
 static int launch(const Attention4& a, int blocks, cudaStream_t stream) {
     auto kernel = attention4_kernel<D, NT>;
     constexpr int bytes = Layout<D, NT>::bytes;
-    static_assert(bytes * Layout<D, NT>::per_sm <= 227 * 1024, "the rings and the merge fit an SM");
+    static_assert((bytes + 1024) * Layout<D, NT>::per_sm <= 228 * 1024, "the blocks of an SM fit it");
     if (int e = raise_shared_limit(kernel, bytes, bytes)) return e;
     launch_kernel(kernel, dim3(blocks), kThreads4, bytes, stream, a);
     if (int e = CITLALI_LAUNCH_CHECK()) return e;
-    launch_kernel(attention4_merge_kernel<D>, dim3(blocks), 256, 0, stream, a, Layout<D, NT>::columns);
+    if (a.arrived) return 0;
+    launch_kernel(attention4_merge_kernel<D>, dim3(blocks), kMergeThreads, 0, stream, a, Layout<D, NT>::columns);
     return CITLALI_LAUNCH_CHECK();
 }
 
@@ -701,7 +763,7 @@ extern "C" size_t citlali_attention4_scratch_floats(int nq, int nkv, int head_di
 extern "C" int citlali_attention4(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes,
                                   const void* v_scales, const int32_t* page_table, int page_table_stride, const int32_t* seq_start,
                                   const int32_t* seq_slot, const int32_t* seq_past, void* out, size_t out_stride, float* partial,
-                                  size_t partial_floats, int sequences, int max_new, int nq, int nkv, int head_dim, int page_size,
+                                  size_t partial_floats, int32_t* arrived, size_t arrived_ints, int sequences, int max_new, int nq, int nkv, int head_dim, int page_size,
                                   int window, float scale, cudaStream_t stream) {
     if (sequences <= 0 || max_new <= 0) return 0;
     if (!citlali_attention4_supports(head_dim, page_size) || nq <= 0 || nkv <= 0 || nq % nkv != 0 || window < 0) {
@@ -717,6 +779,10 @@ extern "C" int citlali_attention4(const void* q, size_t q_stride, const void* k_
     const int blocks = c4::blocks_of(t, head_dim);
     if (partial == nullptr || partial_floats < citlali_attention4_scratch_floats(nq, nkv, head_dim, max_new)) {
         set_last_error("attention4: the scratch holds %zu floats, too few", partial_floats);
+        return kTooLarge;
+    }
+    if (arrived != nullptr && arrived_ints < (size_t)blocks) {
+        set_last_error("attention4: room for %zu counters, %d blocks", arrived_ints, blocks);
         return kTooLarge;
     }
     const long long units = ((long long)page_table_stride * page_size + max_new) / c4::kUnitKeys + 2 + c4::kRoom;
@@ -735,7 +801,7 @@ extern "C" int citlali_attention4(const void* q, size_t q_stride, const void* k_
     a.out = (__nv_bfloat16*)out; a.out_stride = out_stride;
     a.sequences = sequences; a.nq = nq; a.nkv = nkv; a.group = nq / nkv;
     a.tokens = t.tokens; a.heads = t.heads; a.head_tiles = t.head_tiles;
-    a.window = window; a.scale_log2 = scale * 1.4426950408889634f; a.partial = partial;
+    a.window = window; a.scale_log2 = scale * 1.4426950408889634f; a.partial = partial; a.arrived = arrived;
     if (head_dim == 64) return t.wide == 1 ? c4::launch<64, 1>(a, blocks, stream) : c4::launch<64, 2>(a, blocks, stream);
     if (head_dim == 128) return t.wide == 1 ? c4::launch<128, 1>(a, blocks, stream) : c4::launch<128, 2>(a, blocks, stream);
     return c4::launch<256, 1>(a, blocks, stream);

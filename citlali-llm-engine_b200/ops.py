@@ -11,6 +11,7 @@ import ctypes
 import functools
 import operator
 import struct
+import threading
 from typing import Optional
 
 import torch
@@ -624,6 +625,34 @@ def _attention4_expanded(q, q_stride, kv, batch, out, nq, nkv, head_dim, window,
 _run_kernels = (attention_prefill, attention_prefill_tc)        # (as they are here: one who times the calls of this module times the whole)
 
 
+# Counters of the blocks that share a segment, zero between calls.  Calls on one stream follow one another and use the same ones; a call
+# that is being captured gets counters that no other call ever gets, since its graph may be replayed beside anything.  They are cut from a
+# piece that a plain call zeroed; where none is left, the kernel does without.
+_arrivals = {}                              # (device, stream) -> counters
+_arrivals_spare = {}                        # device -> (zeroed counters, how many are given away)
+_arrivals_kept = []
+_arrivals_lock = threading.Lock()
+_ARRIVALS_SPARE = 1 << 18
+
+
+def _arrivals_of(device, stream):
+    """Counters for one call of ``citlali_attention4`` on this device and stream, or None."""
+    each = -(-2 * sm_count(device) // 64) * 64
+    with _arrivals_lock:
+        spare, used = _arrivals_spare.get(device.index, (None, 0))
+        if torch._C._cuda_isCurrentStreamCapturing():
+            if spare is None or used + each > spare.numel():
+                return None
+            _arrivals_spare[device.index] = (spare, used + each)
+            return spare[used:used + each]
+        if spare is None or used + each * 64 > spare.numel():
+            _arrivals_kept.append(spare)                     # (a graph may hold addresses in it)
+            _arrivals_spare[device.index] = (torch.zeros(_ARRIVALS_SPARE, dtype=torch.int32, device=device), 0)
+            torch.cuda.current_stream().synchronize()        # (a graph that is replayed on another stream finds them zeroed)
+        counters = _arrivals[device.index, stream] = torch.zeros(each, dtype=torch.int32, device=device)
+    return counters
+
+
 def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
     """:func:`attention` over a cache in 4 bits: every row of the step over its slot's keys up to its own position (the last
     ``window`` of them; 0 or None: all).  bfloat16 with head size 64, 128 or 256 and pages of 64 runs on the tensor cores, anything
@@ -649,19 +678,23 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
         floats = _attention4_floats(nq, nkv, head_dim, kv.page_size, max_new, _current_device())
         if floats >= 0:
             # of this call alone, and given back in stream order: two graphs, or two streams, share nothing
-            partial = torch.empty(floats, dtype=torch.float32, device=q.device)
+            device, stream = q.device, _stream()
+            partial = torch.empty(floats, dtype=torch.float32, device=device)
+            arrived = None if torch._C._cuda_isCurrentStreamCapturing() else _arrivals.get((device.index, stream))
+            if arrived is None:
+                arrived = _arrivals_of(device, stream)
             start, slot, past = (None, row_slot, row_pos) if single else (seq_start.data_ptr(), batch.seq_slot, batch.seq_past)
             _check(lib().citlali_attention4(
                 q_ptr, _sz(q_stride), kc, ks, vc, vs, table, table_width, start, slot.data_ptr(), past.data_ptr(), out.data_ptr(), wide,
-                partial.data_ptr(), floats, len(batch.slots), max_new, nq, nkv, head_dim, kv.page_size, window, _f(scale), _stream()),
-                "cache4_attention")
+                partial.data_ptr(), floats, _ptr(arrived), 0 if arrived is None else arrived.numel(), len(batch.slots), max_new, nq, nkv, head_dim,
+                kv.page_size, window, _f(scale), stream), "cache4_attention" if arrived is not None else "cache4_attention_merged")
             return
     _check(lib().citlali_attention4_rows(
         q_ptr, _sz(q_stride), _dtype_code(q), kc, ks, vc, vs, table, table_width, row_slot.data_ptr(), row_pos.data_ptr(), out.data_ptr(), wide, rows,
         _i(nq), _i(nkv), _i(head_dim), _i(kv.page_size), window, _f(scale), _stream()), "cache4_attention_rows")
 
 
-_KERNELS_PER_CALL["cache4_attention"] = 2
+_KERNELS_PER_CALL["cache4_attention_merged"] = 2
 
 
 _sm_count = {}
