@@ -56,7 +56,7 @@ struct Attention4 {
     int tokens, heads, head_tiles;                       // of a tile; the tiles a group's heads are cut into
     int window;
     float scale_log2;
-    float* partial;                                      // [blocks][2][columns][D + 2]
+    float* partial;                                      // [blocks][2][columns][m, l, two unused, D values]
     int32_t* arrived;                                    // [blocks], zero before and after: parts in memory of the segment that begins in a block
 };
 
@@ -233,46 +233,54 @@ struct Layout {
 };
 
 // The result of a segment from its parts in memory, part 0 in slot 1 of block `first`, part p in slot 0 of block first + p, in the order
-// of the keys.  A warp has 32 elements of one column (D is a multiple of 32); lane p holds the weight of part p.
+// of the keys.  All parts are brought to shared memory at once (`room` bytes there), as many columns at a time as fit.  This runs once
+// in a block, when its instructions have yet to be fetched: short loops are worth more here than unrolled ones.
 template <int D>
 __device__ __forceinline__ void merge_parts(const Attention4& a, int columns, int first, int parts, int row, int tokens, int head0, int heads,
-                                            int threads) {
-    constexpr int kAhead = 16;
-    const int lane = threadIdx.x & 31;
-    const float* part0 = a.partial + (size_t)(first * 2 + 1) * columns * (D + 2);
-    const int block = 2 * columns * (D + 2), slot = columns * (D + 2);
-    for (int i = threadIdx.x; i < tokens * heads * D; i += threads) {
-        const int column = i / D, e = i % D;
-        auto its = [&](int p) { return part0 + (size_t)p * block - (p ? slot : 0) + column * (D + 2); };
-        float ahead[kAhead];                             // the first values are on their way while the weights are worked out
-#pragma unroll
-        for (int p = 0; p < kAhead; ++p) ahead[p] = p < parts ? __ldcg(its(p) + 2 + e) : 0.0f;
-        float M = kNoScore;
-        float2 ml = make_float2(kNoScore, 0.0f);
-        for (int p = lane; p < parts; p += 32) {
-            ml = __ldcg(reinterpret_cast<const float2*>(its(p)));
-            M = fmaxf(M, ml.x);
-        }
-        M = warp_max(M);
-        float sum = 0.0f, value = 0.0f;
-        for (int p0 = 0; p0 < parts; p0 += 32) {
-            if (parts > 32) ml = p0 + lane < parts ? __ldcg(reinterpret_cast<const float2*>(its(p0 + lane))) : make_float2(kNoScore, 0.0f);
-            const float by = fa::fast_exp2(ml.x - M);
-            sum = fmaf(ml.y, by, sum);
-            const int stop = min(32, parts - p0);
-#pragma unroll
-            for (int p = 0; p < kAhead; ++p)
-                if (p < stop) value = fmaf(p0 == 0 ? ahead[p] : __ldcg(its(p0 + p) + 2 + e), __shfl_sync(0xffffffffu, by, p), value);
-            if (stop > kAhead) {
-#pragma unroll
-                for (int p = kAhead; p < 32; ++p)
-                    if (p < stop) value = fmaf(__ldcg(its(p0 + p) + 2 + e), __shfl_sync(0xffffffffu, by, p), value);
+                                            uint8_t* shared, int room, int threads) {
+    constexpr int kRow = (D + 4) * 4;                    // bytes of a part's column
+    const int used = tokens * heads, slot = columns * kRow, fit = min(used, room / (parts * kRow));
+    const uint8_t* part0 = reinterpret_cast<const uint8_t*>(a.partial) + (size_t)(first * 2 + 1) * slot;
+    auto its = [&](int p) { return part0 + (size_t)p * (2 * slot) - (p ? slot : 0); };
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(shared);
+    for (int column0 = 0; column0 < used; column0 += max(fit, 1)) {
+        const int here = min(max(fit, 1), used - column0), pieces = here * (kRow / 16);
+        __syncthreads();                                 // the room is free
+        if (fit > 0) {
+            for (int i = threadIdx.x; i < parts * pieces; i += threads) {
+                const int p = i / pieces, k = i - p * pieces;
+                fa::cp_async16(dst + i * 16, its(p) + column0 * kRow + k * 16);
             }
+            fa::cp_async_commit();
+            fa::cp_async_wait<0>();
+            __syncthreads();
         }
-        sum = warp_sum(sum);
-        int token, head;
-        split_column(column, tokens, heads, token, head);
-        a.out[(size_t)(row + token) * a.out_stride + (size_t)(head0 + head) * D + e] = __float2bfloat16_rn(value * (kUnit / sum));
+        for (int i = threadIdx.x; i < here * D; i += threads) {
+            const int column = i / D, e = i % D;
+            float M = kNoScore, sum = 0.0f, value = 0.0f;
+            if (fit > 0) {
+                const float* one = reinterpret_cast<const float*>(shared) + column * (D + 4);
+#pragma unroll 4
+                for (int p = 0; p < parts; ++p) M = fmaxf(M, one[p * here * (D + 4)]);
+#pragma unroll 4
+                for (int p = 0; p < parts; ++p) {
+                    const float by = fa::fast_exp2(one[p * here * (D + 4)] - M);
+                    sum = fmaf(one[p * here * (D + 4) + 1], by, sum);
+                    value = fmaf(one[p * here * (D + 4) + 4 + e], by, value);
+                }
+            } else {                                     // more parts than the room holds of one column
+                for (int p = 0; p < parts; ++p) M = fmaxf(M, __ldcg(reinterpret_cast<const float*>(its(p) + (column0 + column) * kRow)));
+                for (int p = 0; p < parts; ++p) {
+                    const float* one = reinterpret_cast<const float*>(its(p) + (column0 + column) * kRow);
+                    const float by = fa::fast_exp2(__ldcg(one) - M);
+                    sum = fmaf(__ldcg(one + 1), by, sum);
+                    value = fmaf(__ldcg(one + 4 + e), by, value);
+                }
+            }
+            int token, head;
+            split_column(column0 + column, tokens, heads, token, head);
+            a.out[(size_t)(row + token) * a.out_stride + (size_t)(head0 + head) * D + e] = __float2bfloat16_rn(value * (kUnit / sum));
+        }
     }
 }
 
@@ -329,7 +337,6 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
         }
     };
     auto load_next = [&](uint8_t* to) {
-        if (fetch_unit == fetch_end) next_piece();
         if (fetch_unit < fetch_end) {
             const size_t at = place(page, a.nkv, fetch_head, kPage, fetch_unit % kUnitsOfAPage * kUnitKeys);
             const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to) + lane * 16;
@@ -351,6 +358,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                 page = next_page;
                 if (fetch_unit + kUnitsOfAPage < fetch_end) next_page = fetch_pages[fetch_unit / kUnitsOfAPage + 1];
             }
+            if (fetch_unit == fetch_end) next_piece();   // what it reads is there when the next unit is asked for
         }
         fa::cp_async_commit();
     };
@@ -636,7 +644,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
         left &= ~run;
         const Part part = parts[k0];
         const bool begins = part.first >= block_begin, all = begins && part.first + part.units <= block_end;
-        float* part_out = a.partial + (size_t)(blockIdx.x * 2 + (begins ? 1 : 0)) * C * (D + 2);
+        float* part_out = a.partial + (size_t)(blockIdx.x * 2 + (begins ? 1 : 0)) * C * (D + 4);
         for (int i = tid; i < part.used * D; i += kThreads4) {
             const int column = i / D, element = i % D;
             auto its = [&](int k) {                      // of part k
@@ -644,25 +652,21 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                        + column * (D + 2);
             };
             float M = kNoScore, sum = 0.0f, value = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 2 * kWarps4; ++k)
-                if (run >> k & 1) M = fmaxf(M, its(k)[0]);
-#pragma unroll
-            for (int k = 0; k < 2 * kWarps4; ++k)
-                if (run >> k & 1) {
-                    const float* one = its(k);
-                    const float by = fa::fast_exp2(one[0] - M);
-                    sum = fmaf(one[1], by, sum);
-                    value = fmaf(one[2 + element], by, value);
-                }
+            for (unsigned rest = run; rest; rest &= rest - 1) M = fmaxf(M, its(__ffs(rest) - 1)[0]);
+            for (unsigned rest = run; rest; rest &= rest - 1) {
+                const float* one = its(__ffs(rest) - 1);
+                const float by = fa::fast_exp2(one[0] - M);
+                sum = fmaf(one[1], by, sum);
+                value = fmaf(one[2 + element], by, value);
+            }
             if (all) {
                 const int tokens = part.used / part.heads;
                 int token, head;
                 split_column(column, tokens, part.heads, token, head);
                 a.out[(size_t)(part.row + token) * a.out_stride + (size_t)(part.head0 + head) * D + element] = __float2bfloat16_rn(value * (kUnit / sum));
             } else {
-                part_out[column * (D + 2) + 2 + element] = value;
-                if (element == 0) *reinterpret_cast<float2*>(part_out + column * (D + 2)) = make_float2(M, sum);
+                part_out[column * (D + 4) + 4 + element] = value;
+                if (element == 0) *reinterpret_cast<float2*>(part_out + column * (D + 4)) = make_float2(M, sum);
             }
         }
         if (!all && tid == 0) pending[begins ? 1 : 0] = part;
@@ -685,16 +689,18 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     for (int k = 0; k < 2; ++k) {
         const Part part = pending[k];
         if (part.used && merged[k].y)
-            merge_parts<D>(a, C, merged[k].x, merged[k].y, part.row, part.used / part.heads, part.head0, part.heads, kThreads4);
+            merge_parts<D>(a, C, merged[k].x, merged[k].y, part.row, part.used / part.heads, part.head0, part.heads, shared,
+                           kWarps4 * (L::ring + L::parked), kThreads4);
     }
 }
 
 // The same as a kernel of its own, where there is nothing to count arrivals in: block i merges the segment whose unit 0 is in the share
 // of block i and that goes on behind it, if there is one.
-constexpr int kMergeThreads = 256;
+constexpr int kMergeThreads = 256, kMergeRoom = 40 * 1024;
 template <int D>
 __global__ void __launch_bounds__(kMergeThreads)
 attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
+    extern __shared__ __align__(16) uint8_t shared[];
     dependents_may_launch();
     const uint32_t length = line_length(a), share = places_of_a_warp(length, gridDim.x) * kWarps4;
     const uint32_t begin = blockIdx.x * share, end = begin + share;
@@ -707,7 +713,7 @@ attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
     if (piece.first < begin || piece.first >= end) return;               // it began earlier, or only its room is here
     const Tile tile = tile_of(a, s, piece.segment);
     merge_parts<D>(a, columns, blockIdx.x, (int)((piece.first + s.units - 1) / share - blockIdx.x) + 1, s.row + tile.token0, tile.tokens,
-                   tile.head0, tile.heads, kMergeThreads);
+                   tile.head0, tile.heads, shared, kMergeRoom, kMergeThreads);
 }
 
 // How a step's columns are tiled.
@@ -740,7 +746,7 @@ static int launch(const Attention4& a, int blocks, cudaStream_t stream) {
     launch_kernel(kernel, dim3(blocks), kThreads4, bytes, stream, a);
     if (int e = CITLALI_LAUNCH_CHECK()) return e;
     if (a.arrived) return 0;
-    launch_kernel(attention4_merge_kernel<D>, dim3(blocks), kMergeThreads, 0, stream, a, Layout<D, NT>::columns);
+    launch_kernel(attention4_merge_kernel<D>, dim3(blocks), kMergeThreads, kMergeRoom, stream, a, Layout<D, NT>::columns);
     return CITLALI_LAUNCH_CHECK();
 }
 
@@ -757,7 +763,7 @@ extern "C" int citlali_attention4_supports(int head_dim, int page_size) {
 extern "C" size_t citlali_attention4_scratch_floats(int nq, int nkv, int head_dim, int max_new) {
     if (nkv <= 0 || nq <= 0 || nq % nkv != 0 || max_new <= 0) return 0;
     const c4::Tiling t = c4::tiling(nq / nkv, head_dim, max_new);
-    return (size_t)c4::blocks_of(t, head_dim) * 2 * (8 * t.wide) * (head_dim + 2);
+    return (size_t)c4::blocks_of(t, head_dim) * 2 * (8 * t.wide) * (head_dim + 4);
 }
 
 extern "C" int citlali_attention4(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes,
