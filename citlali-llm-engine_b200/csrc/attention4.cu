@@ -101,6 +101,7 @@ struct Place {
 // All lanes of a warp: the line's length.
 __device__ __forceinline__ uint32_t line_length(const Attention4& a) {
     uint32_t total = 0;
+#pragma unroll 1
     for (int b = threadIdx.x & 31; b < a.sequences; b += 32) total += sequence_of(a, b).length();
     return __reduce_add_sync(0xffffffffu, total);
 }
@@ -108,6 +109,7 @@ __device__ __forceinline__ uint32_t line_length(const Attention4& a) {
 __device__ __forceinline__ Place place_of(const Attention4& a, uint32_t x) {
     const int lane = threadIdx.x & 31;
     uint32_t run = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < a.sequences; b0 += 32) {
         const uint32_t mine = b0 + lane < a.sequences ? sequence_of(a, b0 + lane).length() : 0;
         uint32_t sum = mine;
@@ -139,11 +141,9 @@ __device__ __forceinline__ Piece piece_of(const Sequence& s, uint32_t base, uint
     p.to = end > p.first ? min(s.units, (int)(end - p.first)) : 0;
     return p;
 }
-// Of a column: the token of the tile and the head of the group.
-__device__ __forceinline__ void split_column(int column, int tokens, int heads, int& token, int& head) {
-    token = tokens == 1 ? 0 : column / heads;
-    head = column - token * heads;
-}
+// Of a column (below 16): the token of the tile, and with it the head of the group.  Exact: column / 256 is less than 1 / heads.
+__device__ __forceinline__ int token_of(int column, int heads, int inverse) { return column * inverse >> 8; }
+__device__ __forceinline__ int inverse_of(int heads) { return (255 + heads) / heads; }
 // How the line is dealt out: places of a warp.
 __device__ __forceinline__ uint32_t places_of_a_warp(uint32_t length, int blocks) {
     return (length + blocks * kWarps4 - 1) / (blocks * kWarps4);
@@ -217,18 +217,26 @@ struct Part {
     uint32_t first;                                      // the segment's place; ~0: there is no such part
     int units, row, head0, heads, used;
 };
+// A piece that a warp works on: units [from, to) of a sequence (none: the end) for a tile.
+struct Job {
+    Part part;
+    int from, to, whole;                                 // whole: the segment has no others
+    int pos0, tokens, inverse;
+};
 
 // Sizes of a block's shared memory: the warps' rings (each at least as large as what its warp parks there at the end), then what a warp
-// parks of a segment that began ahead of it, and the parts' descriptions.
+// parks of a segment that began ahead of it, the parts' descriptions, and the warps' pieces: those that are being fetched or are there.
 template <int D, int NT>
 struct Layout {
     static constexpr int columns = 8 * NT;
     static constexpr int codes = kUnitKeys * D / 2, scales = kUnitKeys * D / kGroup, stage = 2 * (codes + scales);
     static constexpr int parked = columns * (D + 2) * 4;
     static constexpr int stages = D == 64 ? 4 : (D == 128 && NT == 2 ? 3 : 2);
+    static constexpr int jobs = 8;                       // at most one a stage, one that ends, one that was looked up, and the end
+    static_assert(stages + 3 <= jobs && (jobs & (jobs - 1)) == 0, "a piece's description is read before it is written over");
     static constexpr int ring = stages * stage;
     static_assert(ring >= parked && ring % 16 == 0 && parked % 16 == 0, "a warp parks its last part in its ring");
-    static constexpr int bytes = kWarps4 * (ring + parked + 2 * (int)sizeof(Part));
+    static constexpr int bytes = kWarps4 * (ring + parked + 2 * (int)sizeof(Part) + jobs * (int)sizeof(Job));
     static constexpr int per_sm = D == 256 ? 1 : (NT == 1 ? 2 : 1);
 };
 
@@ -236,25 +244,27 @@ struct Layout {
 // of the keys.  All parts are brought to shared memory at once (`room` bytes there), as many columns at a time as fit.  This runs once
 // in a block, when its instructions have yet to be fetched: short loops are worth more here than unrolled ones.
 template <int D>
-__device__ __forceinline__ void merge_parts(const Attention4& a, int columns, int first, int parts, int row, int tokens, int head0, int heads,
+__device__ __forceinline__ void merge_parts(const Attention4& a, int columns, int first, int parts, int row, int used, int head0, int heads,
                                             uint8_t* shared, int room, int threads) {
     constexpr int kRow = (D + 4) * 4;                    // bytes of a part's column
-    const int used = tokens * heads, slot = columns * kRow, fit = min(used, room / (parts * kRow));
+    const int inverse = inverse_of(heads), slot = columns * kRow, fit = parts * used * kRow <= room ? used : min(used, room / (parts * kRow));
     const uint8_t* part0 = reinterpret_cast<const uint8_t*>(a.partial) + (size_t)(first * 2 + 1) * slot;
     auto its = [&](int p) { return part0 + (size_t)p * (2 * slot) - (p ? slot : 0); };
     const uint32_t dst = (uint32_t)__cvta_generic_to_shared(shared);
+#pragma unroll 1
     for (int column0 = 0; column0 < used; column0 += max(fit, 1)) {
         const int here = min(max(fit, 1), used - column0), pieces = here * (kRow / 16);
         __syncthreads();                                 // the room is free
         if (fit > 0) {
-            for (int i = threadIdx.x; i < parts * pieces; i += threads) {
-                const int p = i / pieces, k = i - p * pieces;
-                fa::cp_async16(dst + i * 16, its(p) + column0 * kRow + k * 16);
-            }
+#pragma unroll 1
+            for (int p = threadIdx.x >> 5; p < parts; p += threads >> 5)
+#pragma unroll 1
+                for (int k = threadIdx.x & 31; k < pieces; k += 32) fa::cp_async16(dst + (p * pieces + k) * 16, its(p) + column0 * kRow + k * 16);
             fa::cp_async_commit();
             fa::cp_async_wait<0>();
             __syncthreads();
         }
+#pragma unroll 1
         for (int i = threadIdx.x; i < here * D; i += threads) {
             const int column = i / D, e = i % D;
             float M = kNoScore, sum = 0.0f, value = 0.0f;
@@ -269,7 +279,9 @@ __device__ __forceinline__ void merge_parts(const Attention4& a, int columns, in
                     value = fmaf(one[p * here * (D + 4) + 4 + e], by, value);
                 }
             } else {                                     // more parts than the room holds of one column
+#pragma unroll 1
                 for (int p = 0; p < parts; ++p) M = fmaxf(M, __ldcg(reinterpret_cast<const float*>(its(p) + (column0 + column) * kRow)));
+#pragma unroll 1
                 for (int p = 0; p < parts; ++p) {
                     const float* one = reinterpret_cast<const float*>(its(p) + (column0 + column) * kRow);
                     const float by = fa::fast_exp2(__ldcg(one) - M);
@@ -277,13 +289,13 @@ __device__ __forceinline__ void merge_parts(const Attention4& a, int columns, in
                     value = fmaf(__ldcg(one + 4 + e), by, value);
                 }
             }
-            int token, head;
-            split_column(column0 + column, tokens, heads, token, head);
+            const int token = token_of(column0 + column, heads, inverse), head = column0 + column - token * heads;
             a.out[(size_t)(row + token) * a.out_stride + (size_t)(head0 + head) * D + e] = __float2bfloat16_rn(value * (kUnit / sum));
         }
     }
 }
 
+// (What runs once in a piece or a block is kept short: it waits for its instructions more than for anything else.)
 template <int D, int NT>
 __global__ void __launch_bounds__(kThreads4, Layout<D, NT>::per_sm)
 attention4_kernel(const __grid_constant__ Attention4 a) {
@@ -292,6 +304,8 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     constexpr int KW = D / 32, VW = D / 64;              // words of a key and of a value that a lane holds
     constexpr int KSC = 2 * L::codes, VSC = KSC + L::scales;              // in a stage: keys' codes, values' codes, keys' scales, values' scales
     extern __shared__ __align__(16) uint8_t shared[];
+    __shared__ Part pending[2];                          // what goes to memory: of a segment that began earlier, and of one that goes on
+    __shared__ int2 merged[2];                           // of those: the first block and the number of parts, where this block merges them
     dependents_may_launch();
     // (positions and page tables come from the host before the step; what other kernels write is read behind the wait)
     // (the warp's number by way of a shuffle: so the compiler knows that all lanes go the same way wherever it decides)
@@ -300,8 +314,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     uint8_t* ring = shared + warp * L::ring;
     float* early = reinterpret_cast<float*>(shared + kWarps4 * L::ring + warp * L::parked);      // [column][m, l, O]
     Part* parts = reinterpret_cast<Part*>(shared + kWarps4 * (L::ring + L::parked));             // [warp][early, late]
-    __shared__ Part pending[2];                          // what goes to memory: of a segment that began earlier, and of one that goes on
-    __shared__ int2 merged[2];                           // of those: the first block and the number of parts, where this block merges them
+    Job* jobs = reinterpret_cast<Job*>(parts + 2 * kWarps4) + warp * L::jobs;
 
     const uint32_t length = line_length(a), each = places_of_a_warp(length, gridDim.x);
     const uint32_t begin = min(length, (blockIdx.x * kWarps4 + warp) * each), end = min(length, begin + each);
@@ -311,31 +324,12 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     }
     if (lane < 2) parts[2 * warp + lane].first = ~0u;
     if (tid < 2) pending[tid].used = 0;
-    Place here = begin < end ? place_of(a, begin) : Place{0, 0};
+    Place fetch = begin < end ? place_of(a, begin) : Place{0, 0};
 
-    // ---- the ring's own way along the line, ahead of the one that computes
+    // ---- the ring's way along the line, ahead of the work: a unit a call, then, where a piece ends, the next one is looked up
     uint32_t fetch_x = begin;                            // the next piece's place
-    Place fetch = here;
-    int fetch_unit = 0, fetch_end = 0, fetch_head = 0, page = 0, next_page = 0;
+    int fetch_unit = 0, fetch_end = 0, fetch_head = 0, page = 0, next_page = 0, job = 0;
     const int32_t* fetch_pages = a.table;
-    auto next_piece = [&]() {                            // the next piece with a unit
-        while (fetch_unit == fetch_end && fetch_x < end) {
-            Sequence s = sequence_of(a, fetch.b);
-            while (fetch_x >= fetch.base + s.length()) {
-                fetch.base += s.length();
-                s = sequence_of(a, ++fetch.b);
-            }
-            const Piece p = piece_of(s, fetch.base, fetch_x, end);
-            fetch_x = p.first + s.units;
-            if (p.to <= p.from) continue;
-            fetch_head = tile_of(a, s, p.segment).kv;
-            fetch_pages = a.table + (size_t)a.seq_slot[fetch.b] * a.table_stride;
-            fetch_unit = s.first_unit + p.from;
-            fetch_end = s.first_unit + p.to;
-            page = fetch_pages[fetch_unit / kUnitsOfAPage];
-            next_page = fetch_pages[min(fetch_unit / kUnitsOfAPage + 1, (fetch_end - 1) / kUnitsOfAPage)];
-        }
-    };
     auto load_next = [&](uint8_t* to) {
         if (fetch_unit < fetch_end) {
             const size_t at = place(page, a.nkv, fetch_head, kPage, fetch_unit % kUnitsOfAPage * kUnitKeys);
@@ -358,98 +352,147 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                 page = next_page;
                 if (fetch_unit + kUnitsOfAPage < fetch_end) next_page = fetch_pages[fetch_unit / kUnitsOfAPage + 1];
             }
-            if (fetch_unit == fetch_end) next_piece();   // what it reads is there when the next unit is asked for
         }
         fa::cp_async_commit();
-    };
-    next_piece();
-    wait_for_predecessor();
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i) load_next(ring + i * L::stage);
-    uint8_t *at = ring, *free_stage = ring + (S - 1) * L::stage;
-
-    for (uint32_t x = begin; x < end;) {
-        // ---- the piece: its tile's columns and their queries
-        Sequence s = sequence_of(a, here.b);
-        while (x >= here.base + s.length()) {
-            here.base += s.length();
-            s = sequence_of(a, ++here.b);
-        }
-        const Piece piece = piece_of(s, here.base, x, end);
-        x = piece.first + s.units;
-        if (piece.to <= piece.from) continue;
-        const Tile tile = tile_of(a, s, piece.segment);
-        const int used = tile.used();
-        const int pos0 = s.past + tile.token0, last = pos0 + tile.tokens - 1;         // of the first and the last token
-        const int low0 = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, low1 = a.window > 0 ? max(0, last - a.window + 1) : 0;
-
-        uint32_t qf[NT][2 * KW][2];                      // [columns' eight][contraction step][b0, b1]
-        float factor[NT][2];                             // of the columns 2t, 2t + 1
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int column = n * 8 + r;
-            const bool on = column < used;
-            int token, head;
-            split_column(on ? column : 0, tile.tokens, tile.heads, token, head);
-            const __nv_bfloat16* src = a.q + (size_t)(s.row + tile.token0 + token) * a.q_stride + (size_t)(tile.head0 + head) * D + t * (D / 4);
-            uint4 raw[KW];
-            uint32_t most = 0;
-#pragma unroll
-            for (int w = 0; w < KW; ++w) {
-                raw[w] = on ? *reinterpret_cast<const uint4*>(src + 8 * w) : make_uint4(0, 0, 0, 0);
-                const uint32_t* p = &raw[w].x;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) most = max(most, max((p[i] & 0x7fffu) << 16, p[i] & 0x7fff0000u));
-            }
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int up = min(100, max(-113, 14 + 127 - (int)(most >> 23)));
-            const float by = __int_as_float((127 + up) << 23);
-#pragma unroll
-            for (int w = 0; w < KW; ++w) {
-                float y[8];
-                const uint32_t* p = &raw[w].x;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    y[2 * i] = __uint_as_float(p[i] << 16) * by;
-                    y[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u) * by;
+        if (fetch_unit == fetch_end && fetch_end >= 0) { // (what it reads is there when the next unit is asked for)
+            Sequence s = {};
+            Piece p = {0, 0, 0, 0};
+#pragma unroll 1
+            while (fetch_x < end && p.to <= p.from) {
+                s = sequence_of(a, fetch.b);
+                if (fetch_x >= fetch.base + s.length()) {
+                    fetch.base += s.length();
+                    ++fetch.b;
+                } else {
+                    p = piece_of(s, fetch.base, fetch_x, end);
+                    fetch_x = p.first + s.units;
                 }
-                qf[n][2 * w][0] = as_word(__floats2half2_rn(y[0], y[4]));
-                qf[n][2 * w][1] = as_word(__floats2half2_rn(y[1], y[5]));
-                qf[n][2 * w + 1][0] = as_word(__floats2half2_rn(y[2], y[6]));
-                qf[n][2 * w + 1][1] = as_word(__floats2half2_rn(y[3], y[7]));
             }
-            const float back = __int_as_float((127 - up) << 23) * (a.scale_log2 * kUnit);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) factor[n][j] = __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
+            Job j = {};
+            fetch_end = fetch_unit = -1;                 // the end
+            if (p.to > p.from) {
+                const Tile tile = tile_of(a, s, p.segment);
+                fetch_head = tile.kv;
+                fetch_pages = a.table + (size_t)a.seq_slot[fetch.b] * a.table_stride;
+                fetch_unit = s.first_unit + p.from;
+                fetch_end = s.first_unit + p.to;
+                page = fetch_pages[fetch_unit / kUnitsOfAPage];
+                next_page = fetch_pages[min(fetch_unit / kUnitsOfAPage + 1, (fetch_end - 1) / kUnitsOfAPage)];
+                j.part = {p.first, s.units, s.row + tile.token0, tile.head0, tile.heads, tile.used()};
+                j.from = fetch_unit;
+                j.to = fetch_end;
+                j.whole = p.from == 0 && p.to == s.units;
+                j.pos0 = s.past + tile.token0;
+                j.tokens = tile.tokens;
+                j.inverse = inverse_of(tile.heads);
+            }
+            if (lane == 0) jobs[job & (L::jobs - 1)] = j;
+            ++job;
         }
-        // m: a running maximum less kWeightBits; the lowest number there is where there is none, which no sum with a score overflows to a NaN
-        float m[NT][2], l[NT][4], o[NT][D / 16][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            m[n][0] = m[n][1] = kNoScore;
-            l[n][0] = l[n][1] = l[n][2] = l[n][3] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+    };
+    auto fetch_queries = [&](const Job& j) {             // into L1, a line a lane
+        constexpr int lines = D * 2 / 128;
+        const int column = lane / lines;
+        if (column < j.part.used) {
+            const int token = token_of(column, j.part.heads, j.inverse), head = column - token * j.part.heads;
+            const __nv_bfloat16* p = a.q + (size_t)(j.part.row + token) * a.q_stride + (size_t)(j.part.head0 + head) * D + lane % lines * 64;
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
         }
-        auto position = [&](int column) {                // of the column's token
-            int token, head;
-            split_column(min(column, used - 1), tile.tokens, tile.heads, token, head);
-            return pos0 + token;
-        };
+    };
 
-        // ---- its units
-        const int stop = s.first_unit + piece.to;
-        for (int u = s.first_unit + piece.from; u < stop; ++u) {
+    uint32_t qf[NT][2 * KW][2];                          // [columns' eight][contraction step][b0, b1]
+    float factor[NT][2];                                 // of the columns 2t, 2t + 1
+    // m: a running maximum less kWeightBits; the lowest number there is where there is none, which no sum with a score overflows to a NaN
+    float m[NT][2], l[NT][4], o[NT][D / 16][4];
+    int u = 0, stop = 0, done = 0, pos0 = 0, last = 0, heads = 1, inverse = 256, used = 1;
+    uint8_t *at = ring, *free_stage = ring;
+#pragma unroll 1
+    for (int turn = 0;; ++turn) {
+        // the first S turns only look ahead: the first piece is looked up, then S - 1 units are asked for
+        if (turn == 1) wait_for_predecessor();
+        if (turn >= S) {
             fa::cp_async_wait<S - 2>();
             __syncwarp();                                // the stage is there for all lanes, and all are done with the one before
-            load_next(free_stage);
-            const uint8_t* const stage = at;
-            free_stage = at;
-            at = at + L::stage == ring + L::ring ? ring : at + L::stage;
-            const int key0 = u * kUnitKeys, key1 = key0 + kUnitKeys;
-            if (key0 > last || key1 <= low0) continue;   // none of the tile's tokens sees any of them
-            const bool border = key1 - 1 > pos0 || key0 < low1;
+        }
+        const int known = job;
+        load_next(free_stage);
+        if (turn > 0 && (turn == 1 || job > known)) {
+            __syncwarp();
+            if (turn == 1) fetch_queries(jobs[0]);
+            if (job > known) fetch_queries(jobs[known & (L::jobs - 1)]);
+        }
+        free_stage = free_stage + L::stage == ring + L::ring ? ring : free_stage + L::stage;
+        if (turn < S) {
+            if (turn == 0) free_stage = ring;            // (nothing was asked for)
+            continue;
+        }
+        if (u == stop) {
+            // ---- the next piece: its tile's columns and their queries
+            __syncwarp();
+            const Job& j = jobs[done++ & (L::jobs - 1)];
+            u = j.from;
+            stop = j.to;
+            if (u == stop) break;
+            used = j.part.used;
+            heads = j.part.heads;
+            inverse = j.inverse;
+            pos0 = j.pos0;
+            last = pos0 + j.tokens - 1;                  // positions of the first and the last token
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int column = n * 8 + r;
+                const bool on = column < used;
+                const int token = on ? token_of(column, heads, inverse) : 0, head = on ? column - token * heads : 0;
+                const __nv_bfloat16* src = a.q + (size_t)(j.part.row + token) * a.q_stride + (size_t)(j.part.head0 + head) * D + t * (D / 4);
+                uint4 raw[KW];
+                uint32_t most = 0;
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    raw[w] = on ? *reinterpret_cast<const uint4*>(src + 8 * w) : make_uint4(0, 0, 0, 0);
+                    const uint32_t* p = &raw[w].x;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) most = max(most, max((p[i] & 0x7fffu) << 16, p[i] & 0x7fff0000u));
+                }
+                most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                const int up = min(100, max(-113, 14 + 127 - (int)(most >> 23)));
+                const float by = __int_as_float((127 + up) << 23);
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    float y[8];
+                    const uint32_t* p = &raw[w].x;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        y[2 * i] = __uint_as_float(p[i] << 16) * by;
+                        y[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u) * by;
+                    }
+                    qf[n][2 * w][0] = as_word(__floats2half2_rn(y[0], y[4]));
+                    qf[n][2 * w][1] = as_word(__floats2half2_rn(y[1], y[5]));
+                    qf[n][2 * w + 1][0] = as_word(__floats2half2_rn(y[2], y[6]));
+                    qf[n][2 * w + 1][1] = as_word(__floats2half2_rn(y[3], y[7]));
+                }
+                const float back = __int_as_float((127 - up) << 23) * (a.scale_log2 * kUnit);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) factor[n][k] = __shfl_sync(0xffffffffu, back, (2 * t + k) * 4);
+                m[n][0] = m[n][1] = kNoScore;
+                l[n][0] = l[n][1] = l[n][2] = l[n][3] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+            }
+        }
+
+        // ---- a unit
+        const uint8_t* const stage = at;
+        at = at + L::stage == ring + L::ring ? ring : at + L::stage;
+        const int key0 = u * kUnitKeys, key1 = key0 + kUnitKeys;
+        const int low0 = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+        ++u;
+        if (key0 <= last && key1 > low0) {               // (some of the tile's tokens see some of them)
+            const bool border = key1 - 1 > pos0 || (a.window > 0 && key0 <= last - a.window);
+            auto sees = [&](int column, int key) {       // whether the column's token does
+                const int p = pos0 + token_of(min(column, used - 1), heads, inverse);
+                return key <= p && (a.window == 0 || key > p - a.window);
+            };
 
             float e[2][NT][4];
 #pragma unroll
@@ -488,9 +531,9 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                     w[0][n][j] = fmaf(e[0][n][j], factor[n][j & 1], -m[n][j & 1]);
                     w[1][n][j] = fmaf(e[1][n][j], factor[n][j & 1], -m[n][j & 1]);
                     if (border) {
-                        const int p = position(n * 8 + 2 * t + (j & 1)), key = key0 + r + (j >> 1) * 8;
-                        if (key > p || (a.window > 0 && key <= p - a.window)) w[0][n][j] = -INFINITY;
-                        if (key + 16 > p || (a.window > 0 && key + 16 <= p - a.window)) w[1][n][j] = -INFINITY;
+                        const int column = n * 8 + 2 * t + (j & 1), key = key0 + r + (j >> 1) * 8;
+                        if (!sees(column, key)) w[0][n][j] = -INFINITY;
+                        if (!sees(column, key + 16)) w[1][n][j] = -INFINITY;
                     }
                     most = fmaxf(most, fmaxf(w[0][n][j], w[1][n][j]));
                 }
@@ -531,40 +574,28 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                 }
             if (border) {
                 // What a key that no token of the tile sees holds must not count: even zero times a NaN is one.  Its scales are put to zero
-                // here, where they lie.  A key that is no number and that only some of the tokens see makes their results none by hand.
-                uint8_t* const scales = const_cast<uint8_t*>(stage) + VSC;
-                constexpr int count = L::scales / 4, per_key = D / kGroup / 4;
-                uint32_t w[(count + 31) / 32];
-                bool none = false;
+                // here, where they lie.  A value that is no number and that only some of the tokens see becomes zero as well, and spoils
+                // the sums of those that do see it.
+                uint32_t* const scales = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(stage) + VSC);
+                constexpr int per_key = D / kGroup / 4;
+#pragma unroll 1
+                for (int i = lane; i < L::scales / 4; i += 32) {
+                    const int key = key0 + i / per_key;
+                    uint32_t w = key >= low0 && key <= last ? scales[i] : 0;
+                    const uint32_t none = __vcmpgeu4(w, 0xf8f8f8f8u);
+                    const unsigned found = __ballot_sync(0xffffffffu, none != 0 && last > pos0);
+                    if (last > pos0) w &= ~none;
+                    scales[i] = w;
+#pragma unroll 1
+                    for (unsigned rest = found; rest; rest &= rest - 1) {
+                        const int spoilt = key0 + (i - lane + __ffs(rest) - 1) / per_key;
 #pragma unroll
-                for (int i = 0; i < (count + 31) / 32; ++i) {
-                    const int at_word = i * 32 + lane, key = key0 + at_word / per_key;
-                    w[i] = 0;
-                    if (at_word < count && key >= low0 && key <= last) w[i] = reinterpret_cast<const uint32_t*>(scales)[at_word];
-                    none |= __vcmpgeu4(w[i], 0xf8f8f8f8u) != 0;
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                if (sees(n * 8 + 2 * t + j, spoilt)) l[n][j] = __int_as_float(0x7fc00000);
+                    }
                 }
-                const bool by_hand = tile.tokens > 1 && __any_sync(0xffffffffu, none);
-                if (by_hand) {
-                    for (int k = 0; key0 + k < key1; ++k)
-#pragma unroll
-                        for (int h = 0; h < (VW + 1) / 2; ++h) {
-                            if (scales[k * (D / kGroup) + (r * (D / 8)) / kGroup + h] < 0xf8) continue;
-#pragma unroll
-                            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                for (int j = 0; j < 2; ++j) {
-                                    const int key = key0 + k, q = position(n * 8 + 2 * t + j);
-                                    if (key > q || (a.window > 0 && key <= q - a.window)) continue;
-#pragma unroll
-                                    for (int i = 8 * h; i < min(8 * h + 8, D / 16); ++i) o[n][i][j] = o[n][i][j + 2] = __int_as_float(0x7fc00000);
-                                }
-                        }
-                }
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < (count + 31) / 32; ++i)
-                    if (i * 32 + lane < count)
-                        reinterpret_cast<uint32_t*>(scales)[i * 32 + lane] = by_hand ? w[i] & ~__vcmpgeu4(w[i], 0xf8f8f8f8u) : w[i];
                 __syncwarp();
             }
 #pragma unroll
@@ -600,8 +631,12 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
             }
         }
 
+        if (u < stop) continue;
+
         // ---- the piece's end: the whole segment's result, or a part to merge
-        const bool all = piece.from == 0 && piece.to == s.units, late = !all && x >= end;      // a part is the warp's first or its last
+        __syncwarp();
+        const Job& j = jobs[(done - 1) & (L::jobs - 1)];
+        const bool late = !j.whole && j.part.first + j.part.units >= end;       // a part is the warp's first or its last
         if (late) {
             fa::cp_async_wait<0>();
             __syncwarp();                                // the ring is the warp's own and empty
@@ -610,59 +645,61 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float sum = l[n][j];
-                const int column = n * 8 + 2 * t + j;
+            for (int k = 0; k < 2; ++k) {
+                const int column = n * 8 + 2 * t + k;
                 if (column >= used) continue;
-                if (all) {
-                    const float by = kUnit / sum;
-                    int token, head;
-                    split_column(column, tile.tokens, tile.heads, token, head);
-                    __nv_bfloat16* dst = a.out + (size_t)(s.row + tile.token0 + token) * a.out_stride + (size_t)(tile.head0 + head) * D + r * (D / 8);
+                if (j.whole) {
+                    const float by = kUnit / l[n][k];
+                    const int token = token_of(column, heads, inverse);
+                    __nv_bfloat16* dst = a.out + (size_t)(j.part.row + token) * a.out_stride + (size_t)(j.part.head0 + column - token * heads) * D + r * (D / 8);
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i)
-                        *reinterpret_cast<uint32_t*>(dst + 2 * i) = fa::pack_bf16(o[n][i][j] * by, o[n][i][j + 2] * by);
+                        *reinterpret_cast<uint32_t*>(dst + 2 * i) = fa::pack_bf16(o[n][i][k] * by, o[n][i][k + 2] * by);
                 } else {
                     float* mine = parked + column * (D + 2);
-                    if (r == 0) { mine[0] = m[n][j]; mine[1] = sum; }
+                    if (r == 0) { mine[0] = m[n][k]; mine[1] = l[n][k]; }
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i)
-                        *reinterpret_cast<float2*>(mine + 2 + r * (D / 8) + 2 * i) = make_float2(o[n][i][j], o[n][i][j + 2]);
+                        *reinterpret_cast<float2*>(mine + 2 + r * (D / 8) + 2 * i) = make_float2(o[n][i][k], o[n][i][k + 2]);
                 }
             }
-        if (!all && lane == 0)
-            parts[2 * warp + (late ? 1 : 0)] = {piece.first, s.units, s.row + tile.token0, tile.head0, tile.heads, used};
+        if (!j.whole && lane == 0) parts[2 * warp + (late ? 1 : 0)] = j.part;
     }
 
     // ---- the block's parts, in the order of the line: those of one segment are neighbours.  Nothing is written to shared memory any more.
     __syncthreads();
     const uint32_t block_begin = blockIdx.x * kWarps4 * each, block_end = min(length, block_begin + kWarps4 * each);
     const uint32_t mine = lane < 2 * kWarps4 ? parts[lane].first : ~0u;
+#pragma unroll 1
     for (unsigned left = __ballot_sync(0xffffffffu, mine != ~0u); left;) {
         const int k0 = __ffs(left) - 1;
         const unsigned run = __ballot_sync(0xffffffffu, mine == __shfl_sync(0xffffffffu, mine, k0)) & left;
         left &= ~run;
+        // one part of each of the warps w0 .. w1: their last, but for w1's, which may be its first
+        const int w0 = k0 >> 1, k1 = 31 - __clz(run), count = (k1 >> 1) - w0;
         const Part part = parts[k0];
         const bool begins = part.first >= block_begin, all = begins && part.first + part.units <= block_end;
         float* part_out = a.partial + (size_t)(blockIdx.x * 2 + (begins ? 1 : 0)) * C * (D + 4);
+        const float* lates = reinterpret_cast<const float*>(shared + w0 * L::ring);
+        const float* final_one = reinterpret_cast<const float*>(shared + (k1 & 1 ? (k1 >> 1) * L::ring : kWarps4 * L::ring + (k1 >> 1) * L::parked));
+#pragma unroll 1
         for (int i = tid; i < part.used * D; i += kThreads4) {
-            const int column = i / D, element = i % D;
-            auto its = [&](int k) {                      // of part k
-                return reinterpret_cast<const float*>(shared + (k >> 1) * ((k & 1) ? L::ring : L::parked) + ((k & 1) ? 0 : kWarps4 * L::ring))
-                       + column * (D + 2);
-            };
-            float M = kNoScore, sum = 0.0f, value = 0.0f;
-            for (unsigned rest = run; rest; rest &= rest - 1) M = fmaxf(M, its(__ffs(rest) - 1)[0]);
-            for (unsigned rest = run; rest; rest &= rest - 1) {
-                const float* one = its(__ffs(rest) - 1);
+            const int column = i / D, element = i % D, at = column * (D + 2);
+            float M = final_one[at], sum = 0.0f, value = 0.0f;
+#pragma unroll 4
+            for (int w = 0; w < count; ++w) M = fmaxf(M, lates[w * (L::ring / 4) + at]);
+#pragma unroll 4
+            for (int w = 0; w < count; ++w) {
+                const float* one = lates + w * (L::ring / 4) + at;
                 const float by = fa::fast_exp2(one[0] - M);
                 sum = fmaf(one[1], by, sum);
                 value = fmaf(one[2 + element], by, value);
             }
+            const float by = fa::fast_exp2(final_one[at] - M);
+            sum = fmaf(final_one[at + 1], by, sum);
+            value = fmaf(final_one[at + 2 + element], by, value);
             if (all) {
-                const int tokens = part.used / part.heads;
-                int token, head;
-                split_column(column, tokens, part.heads, token, head);
+                const int token = token_of(column, part.heads, inverse_of(part.heads)), head = column - token * part.heads;
                 a.out[(size_t)(part.row + token) * a.out_stride + (size_t)(part.head0 + head) * D + element] = __float2bfloat16_rn(value * (kUnit / sum));
             } else {
                 part_out[column * (D + 4) + 4 + element] = value;
@@ -678,9 +715,9 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     if (lane == 0 && warp < 2 && pending[warp].used) {
         const uint32_t begins = pending[warp].first;
         const int first = (int)(begins / share), count = (int)((begins + pending[warp].units - 1) / share) - first + 1;
-        __threadfence();                                 // (the block's writes, which the barrier has put ahead)
-        const bool last_one = atomicAdd(a.arrived + first, 1) == count - 1;
-        __threadfence();
+        int before;                                      // (ordered behind the block's writes, which the barrier has put ahead, and ahead of what is read)
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.arrived + first) : "memory");
+        const bool last_one = before == count - 1;
         if (last_one) a.arrived[first] = 0;              // as the next call wants it
         merged[warp] = last_one ? make_int2(first, count) : make_int2(0, 0);
     }
@@ -689,7 +726,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     for (int k = 0; k < 2; ++k) {
         const Part part = pending[k];
         if (part.used && merged[k].y)
-            merge_parts<D>(a, C, merged[k].x, merged[k].y, part.row, part.used / part.heads, part.head0, part.heads, shared,
+            merge_parts<D>(a, C, merged[k].x, merged[k].y, part.row, part.used, part.head0, part.heads, shared,
                            kWarps4 * (L::ring + L::parked), kThreads4);
     }
 }
@@ -712,7 +749,7 @@ attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
     const Piece piece = piece_of(s, here.base, end, end + 1);
     if (piece.first < begin || piece.first >= end) return;               // it began earlier, or only its room is here
     const Tile tile = tile_of(a, s, piece.segment);
-    merge_parts<D>(a, columns, blockIdx.x, (int)((piece.first + s.units - 1) / share - blockIdx.x) + 1, s.row + tile.token0, tile.tokens,
+    merge_parts<D>(a, columns, blockIdx.x, (int)((piece.first + s.units - 1) / share - blockIdx.x) + 1, s.row + tile.token0, tile.used(),
                    tile.head0, tile.heads, shared, kMergeRoom, kMergeThreads);
 }
 
