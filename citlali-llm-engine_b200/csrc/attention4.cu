@@ -330,15 +330,20 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     uint32_t fetch_x = begin;                            // the next piece's place
     int fetch_unit = 0, fetch_end = 0, fetch_head = 0, page = 0, next_page = 0, job = 0;
     const int32_t* fetch_pages = a.table;
+    // Heads of 128: a value's 64 bytes of codes fill half of the banks.  A lane reads those of the keys 2t and 2t + 1: odd t take the second
+    // first, and keys whose number has bit 2 have the halves of their codes swapped, so that a half-warp's reads are of different banks.
+    const uint32_t swap_to = D == 128 ? (lane >> 4 & 1) * 32 : 0;         // (16 bytes a lane, four lanes a key)
+    const int odd = D == 128 ? t & 1 : 0, swap_from = D == 128 ? (t >> 1) * 32 : 0;
+    const uint32_t low_pick = odd ? 0x1054u : 0x5410u, high_pick = odd ? 0x3276u : 0x7632u;
     auto load_next = [&](uint8_t* to) {
         if (fetch_unit < fetch_end) {
             const size_t at = place(page, a.nkv, fetch_head, kPage, fetch_unit % kUnitsOfAPage * kUnitKeys);
-            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to) + lane * 16;
+            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to) + lane * 16, dst_v = dst ^ swap_to;
             const uint8_t *kc = a.k_codes + at * (D / 2) + lane * 16, *vc = a.v_codes + at * (D / 2) + lane * 16;
 #pragma unroll
             for (int i = 0; i < L::codes; i += 512) {
                 fa::cp_async16(dst + i, kc + i);
-                fa::cp_async16(dst + L::codes + i, vc + i);
+                fa::cp_async16(dst_v + L::codes + i, vc + i);
             }
             constexpr int pieces = L::scales / 16;       // 16-byte pieces of the scales of a unit's keys
 #pragma unroll
@@ -601,11 +606,11 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 uint32_t va[VW], vb[VW], vc[VW], vd[VW];
-                const uint8_t* codes = stage + L::codes + half * (L::codes / 2) + r * (D / 16);
-                load_words<VW>(va, codes + (2 * t) * (D / 2));
-                load_words<VW>(vb, codes + (2 * t + 1) * (D / 2));
-                load_words<VW>(vc, codes + (2 * t + 8) * (D / 2));
-                load_words<VW>(vd, codes + (2 * t + 9) * (D / 2));
+                const uint8_t* codes = stage + L::codes + half * (L::codes / 2) + ((r * (D / 16)) ^ swap_from);
+                load_words<VW>(va, codes + (2 * t + odd) * (D / 2));
+                load_words<VW>(vb, codes + (2 * t + 1 - odd) * (D / 2));
+                load_words<VW>(vc, codes + (2 * t + 8 + odd) * (D / 2));
+                load_words<VW>(vd, codes + (2 * t + 9 - odd) * (D / 2));
                 const uint8_t* scales = stage + VSC + half * (L::scales / 2) + (r * (D / 8)) / kGroup;
 #pragma unroll
                 for (int h = 0; h < (VW + 1) / 2; ++h) {
@@ -615,7 +620,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                     for (int w = 2 * h; w < min(2 * h + 2, VW); ++w) {
 #pragma unroll
                         for (int part = 0; part < 2; ++part) {
-                            const uint32_t pick = part == 0 ? 0x5410u : 0x7632u;
+                            const uint32_t pick = part == 0 ? low_pick : high_pick;
                             uint32_t y = __byte_perm(va[w], vb[w], pick), z = __byte_perm(vc[w], vd[w], pick);
 #pragma unroll
                             for (int k = 0; k < 2; ++k) {
