@@ -8,10 +8,15 @@
 //
 // What bounds it: reading the logits once.  A cluster of 1 to 8 blocks takes a row, a block an even share of it; a thread has 16
 // entries in registers and the next 16 on their way.  m, S and T are the thread's own until the end (the running maximum is looked
-// at once for 16 entries).  The likeliest 32 are the warp's: lane i holds the i-th.  An entry is looked at one by one only if it
-// exceeds the last one that still counts, which for 512 entries at a time hardly happens once a row has begun; for the first 512 that
-// bound is the top-th of the lanes' own maxima, which sorting gives.  Warps and then blocks (through distributed shared memory)
-// merge their lists pairwise: the larger of a[i] and b[31 - i] are the 32 largest, and five exchanges sort them.
+// at once for 16 entries).
+//
+// The likeliest tokens.  A share of a few tiles (few rows) is read a second time, out of the caches, once a bound is known: a warp's
+// ceil(top / 8)-th largest of its lanes' own maxima, the least of the eight warps', has at least `top` entries above or at it, and hardly
+// more lanes that hold any; those lanes alone look through their entries again, and what they find is sorted.  Of a longer share each
+// warp keeps a list as it goes, lane i the i-th largest entry so far: an entry is looked at only if it exceeds the last one that
+// still counts in any warp of the block, which for 512 entries at a time hardly happens once a row has begun; for a warp's first 512 the
+// bound is the top-th of the lanes' own maxima.  Warps and then blocks (through distributed shared memory) merge their lists
+// pairwise: the larger of a[i] and b[31 - i] are the 32 largest, and five exchanges sort them.
 #include "api.h"
 #include "common.cuh"
 #include "mma_common.cuh"
@@ -24,7 +29,17 @@ constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNone = 0x7fffffff;                        // no entry: behind every index
 
+constexpr int kTwice = 8;                                // a share of fewer tiles is read a second time
+constexpr int kFound = 512;
+
 struct Summary { float m, s, t; };
+
+// A float as a whole number in the same order, and back.
+__device__ __forceinline__ int ordered(float v) {
+    const int i = __float_as_int(v);
+    return i < 0 ? i ^ 0x7fffffff : i;
+}
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i < 0 ? i ^ 0x7fffffff : i); }
 
 __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
@@ -61,14 +76,14 @@ __device__ __forceinline__ void merge(float& v, int& i, float w, int j) {
 __device__ __forceinline__ void load(const float* p, float (&x)[kEach]) {
 #pragma unroll
     for (int k = 0; k < kEach / 4; ++k) {
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(p) + k * kThreads);
+        const float4 v = *(reinterpret_cast<const float4*>(p) + k * kThreads);
         x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
     }
 }
 __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&x)[kEach]) {
 #pragma unroll
     for (int k = 0; k < kEach / 8; ++k) {
-        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + k * kThreads);
+        const uint4 v = *(reinterpret_cast<const uint4*>(p) + k * kThreads);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) { x[8 * k + 2 * e] = __uint_as_float(w[e] << 16); x[8 * k + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
@@ -91,6 +106,8 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
     __shared__ float list_v[kWarps][32];
     __shared__ int list_i[kWarps][32];
     __shared__ Block blocks[kMaxCluster];
+    __shared__ float found_v[TOP ? kFound : 1];
+    __shared__ int found_i[TOP ? kFound : 1], found, shared_bound;
     dependents_may_launch();
     wait_for_predecessor();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -109,35 +126,56 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
     int at = kNone;
     float bound = -INFINITY;                             // the top-th
     int bound_at = kNone;
+    if (TOP && tid == 0) { found = 0; shared_bound = ordered(-INFINITY); }
+    if (TOP) __syncthreads();
 
-    // 16 entries a lane, `where(e)` their indices; entries that are none or not finite come as minus infinity
-    auto take = [&](float (&y)[kEach], auto where) {
-        float most = y[0];
+    // The largest of a thread's 16 entries, quarter by quarter.  Plus infinity is no entry (nor is a NaN, which no maximum takes).
+    auto largest = [&](float (&y)[kEach], float (&quarter)[4]) {
+        float most;
+        auto look = [&] {
 #pragma unroll
-        for (int e = 1; e < kEach; ++e) most = fmaxf(most, y[e]);
+            for (int k = 0; k < 4; ++k) quarter[k] = fmaxf(fmaxf(y[4 * k], y[4 * k + 1]), fmaxf(y[4 * k + 2], y[4 * k + 3]));
+            most = fmaxf(fmaxf(quarter[0], quarter[1]), fmaxf(quarter[2], quarter[3]));
+        };
+        look();
+        if (most == INFINITY) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) y[e] = y[e] == INFINITY ? -INFINITY : y[e];
+            look();
+        }
+        return most;
+    };
+    auto add = [&](const float (&y)[kEach], float most) {
         if (most > mine.m) {
             const float d = fmaxf(mine.m - most, -104.0f), by = fa::fast_exp2(d * kLog2e);
             mine.t = (mine.t + mine.s * d) * by;
             mine.s *= by;
             mine.m = most;
         }
-        const float m = mine.m == -INFINITY ? 0.0f : mine.m;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const float u = fmaxf(y[e] - m, -104.0f), p = fa::fast_exp2(u * kLog2e);       // 2^-150 is zero here
+            // 2^-150 is zero here; where the difference is no number (an entry that is none, or a thread without any yet) it is that, too
+            const float u = fmaxf(y[e] - mine.m, -104.0f), p = fa::fast_exp2(u * kLog2e);
             mine.s += p;
             mine.t = fmaf(p, u, mine.t);
         }
-        if constexpr (TOP) {
-            if (!__any_sync(0xffffffffu, most >= bound && most > -INFINITY)) return;
-            if (__all_sync(0xffffffffu, at == kNone)) {  // the first entries: no more than `top` lanes' maxima are above the bound
-                float v = most;
-                int i = lane;
-                sort(v, i);
-                bound = __shfl_sync(0xffffffffu, v, top - 1);
-            }
+    };
+    // 16 entries a lane, `where(e)` their indices
+    auto keep = [&](const float (&y)[kEach], const float (&quarter)[4], float most, auto where) {
+        const float others = unordered(*(volatile int*)&shared_bound);   // (at least `top` entries of the row are at or above it)
+        if (!__any_sync(0xffffffffu, most >= fmaxf(bound, others) && most > -INFINITY)) return;
+        if (__all_sync(0xffffffffu, at == kNone)) {      // the first entries: at least `top` lanes' maxima are at or above the bound
+            float v = most;
+            int i = lane;
+            sort(v, i);
+            bound = __shfl_sync(0xffffffffu, v, top - 1);
+        }
+        if (others > bound) { bound = others; bound_at = kNone; }
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
+        for (int k = 0; k < 4; ++k) {
+            if (!__any_sync(0xffffffffu, quarter[k] >= bound && quarter[k] > -INFINITY)) continue;
+#pragma unroll
+            for (int e = 4 * k; e < 4 * k + 4; ++e) {
                 const int index = where(e);
                 unsigned who = __ballot_sync(0xffffffffu, y[e] > -INFINITY && (y[e] > bound || (y[e] == bound && index < bound_at)));
                 while (who) {
@@ -151,61 +189,121 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
                     if (lane > rank_of) { best = up; at = up_at; }
                     if (lane == rank_of) { best = v; at = i; }
                 }
-                const float last = __shfl_sync(0xffffffffu, best, top - 1);
-                if (last >= bound) {
-                    bound = last;
-                    bound_at = __shfl_sync(0xffffffffu, at, top - 1);
-                }
+            }
+            const float last = __shfl_sync(0xffffffffu, best, top - 1);
+            if (last >= bound) {
+                bound = last;
+                bound_at = __shfl_sync(0xffffffffu, at, top - 1);
+                if (lane == 0) atomicMax(&shared_bound, ordered(bound));
             }
         }
     };
-    auto finite = [](float (&y)[kEach]) {
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) y[e] = fabsf(y[e]) <= 3.402823466e+38f ? y[e] : -INFINITY;
-    };
 
+    // The share tile by tile: whole ones, then the rest, less than a tile, then the row's ends (the lead with the first block, the tail
+    // with the last).  `use(y, where)` gets 16 entries a lane, minus infinity where there is none.
     constexpr int kTile = kThreads * kEach / kVec;       // vectors of a tile
     const int tiles = (stop - first) / kTile;            // whole ones
     const T* base = x + lead + ((long long)first + tid) * kVec;
-    float y[kEach], next[kEach];
-    if (tiles > 0) load(base, next);
-    for (int k = 0; k < tiles; ++k) {
+    auto walk = [&](auto use) {
+        float y[kEach], next[kEach];
+        if (tiles > 0) load(base, next);
+#pragma unroll 1
+        for (int k = 0; k < tiles; ++k) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) y[e] = next[e];
-        if (k + 1 < tiles) load(base + (long long)(k + 1) * kTile * kVec, next);
-        finite(y);
-        const int index0 = lead + (first + k * kTile + tid) * kVec;
-        take(y, [&](int e) { return index0 + e / kVec * (kThreads * kVec) + e % kVec; });
-    }
-    {   // the rest of this block's vectors, less than a tile, and the row's ends: the lead with the first block, the tail with the last
-        const int rest = first + tiles * kTile;
-        const int index0 = lead + (rest + tid) * kVec;
-        bool any = rest < stop;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) y[e] = -INFINITY;
-        if (any) {
-#pragma unroll
-            for (int k = 0; k < kEach / kVec; ++k)
-                if (rest + k * kThreads + tid < stop) {
-                    const T* p = x + lead + ((long long)rest + k * kThreads + tid) * kVec;
-                    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
-                    const T* in = reinterpret_cast<const T*>(&v);
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) y[k * kVec + e] = ldf(in, e);
-                }
-            finite(y);
-            take(y, [&](int e) { return index0 + e / kVec * (kThreads * kVec) + e % kVec; });
+            for (int e = 0; e < kEach; ++e) y[e] = next[e];
+            if (k + 1 < tiles) load(base + (long long)(k + 1) * kTile * kVec, next);
+            const int index0 = lead + (first + k * kTile + tid) * kVec;
+            use(y, [&](int e) { return index0 + e / kVec * (kThreads * kVec) + e % kVec; });
         }
-        const int tail = lead + vectors * kVec;          // entries from here on: fewer than kVec
-        int odd = -1;
+        const int rest = first + tiles * kTile, tail = lead + vectors * kVec;
+        int odd = -1;                                    // the ends: fewer than kVec entries each, a thread an entry
         if (rank == 0 && tid < lead) odd = tid;
         if (rank == cluster - 1 && tid >= 32 && tail + tid - 32 < vocab) odd = tail + tid - 32;
-        if (warp < 2) {
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+            if (part == 0 ? rest >= stop : warp >= 2) continue;
 #pragma unroll
             for (int e = 0; e < kEach; ++e) y[e] = -INFINITY;
-            if (odd >= 0) y[0] = ldf(x, odd);
-            finite(y);
-            take(y, [&](int) { return odd; });
+            if (part == 0) {
+#pragma unroll
+                for (int k = 0; k < kEach / kVec; ++k)
+                    if (rest + k * kThreads + tid < stop) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(x + lead + ((long long)rest + k * kThreads + tid) * kVec);
+                        const T* in = reinterpret_cast<const T*>(&v);
+#pragma unroll
+                        for (int e = 0; e < kVec; ++e) y[k * kVec + e] = ldf(in, e);
+                    }
+            } else if (odd >= 0) {
+                y[0] = ldf(x, odd);
+            }
+            const int index0 = part == 0 ? lead + (rest + tid) * kVec : odd;
+            use(y, [&](int e) { return index0 + e / kVec * (kThreads * kVec) + e % kVec; });
+        }
+    };
+
+    const bool twice = TOP && tiles < kTwice;            // (alike for all threads)
+    float top_of_mine = -INFINITY;
+    walk([&](float (&y)[kEach], auto where) {
+        float quarter[4];
+        const float most = largest(y, quarter);
+        add(y, most);
+        if constexpr (TOP) {
+            if (twice) top_of_mine = fmaxf(top_of_mine, most);
+            else keep(y, quarter, most, where);
+        }
+    });
+    if constexpr (TOP) {
+        if (twice) {
+            int rest = ordered(top_of_mine), nth = ordered(-INFINITY);
+#pragma unroll 1
+            for (int k = 0; k < (top + kWarps - 1) / kWarps; ++k) {
+                nth = __reduce_max_sync(0xffffffffu, rest);
+                const unsigned who = __ballot_sync(0xffffffffu, rest == nth);
+                if (lane == __ffs(who) - 1) rest = ordered(-INFINITY);
+            }
+            if (lane == 0) list_i[0][warp] = nth;
+            __syncthreads();
+            int least = list_i[0][0];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) least = min(least, list_i[0][w]);
+            const float at_least = unordered(least);
+            auto look = [&](float v, int index) {
+                if (v >= at_least && fabsf(v) <= 3.402823466e+38f) {
+                    const int k = atomicAdd(&found, 1);
+                    if (k < kFound) { found_v[k] = v; found_i[k] = index; }
+                }
+            };
+            if (top_of_mine >= at_least && top_of_mine > -INFINITY) {
+#pragma unroll 2
+                for (int k = first + tid; k < stop; k += kThreads) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(x + lead + (long long)k * kVec);
+                    const T* in = reinterpret_cast<const T*>(&v);
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) look(ldf(in, e), lead + k * kVec + e);
+                }
+                const int tail = lead + vectors * kVec;
+                if (rank == 0 && tid < lead) look(ldf(x, tid), tid);
+                if (rank == cluster - 1 && tid >= 32 && tail + tid - 32 < vocab) look(ldf(x, tail + tid - 32), tail + tid - 32);
+            }
+            __syncthreads();
+            if (found <= kFound) {
+                if (warp == 0) {
+#pragma unroll 1
+                    for (int k = 0; k < found; k += 32) {
+                        float v = k + lane < found ? found_v[k + lane] : -INFINITY;
+                        int i = k + lane < found ? found_i[k + lane] : kNone;
+                        sort(v, i);
+                        merge(best, at, __shfl_sync(0xffffffffu, v, 31 - lane), __shfl_sync(0xffffffffu, i, 31 - lane));
+                    }
+                }
+            } else {                                     // many entries alike: lists as for a long share
+                walk([&](float (&y)[kEach], auto where) {
+                    float quarter[4];
+                    const float most = largest(y, quarter);
+                    keep(y, quarter, most, where);
+                });
+            }
+            __syncthreads();                             // (the room of the lists is used again)
         }
     }
 
@@ -218,7 +316,7 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
     __syncthreads();
     if constexpr (TOP) {
 #pragma unroll
-        for (int half = kWarps / 2; half > 0; half >>= 1) {
+        for (int half = kWarps / 2; half > 0 && !(twice && found <= kFound); half >>= 1) {
             if (warp < half) {
                 merge(best, at, list_v[warp + half][31 - lane], list_i[warp + half][31 - lane]);
                 list_v[warp][lane] = best;
@@ -253,6 +351,7 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (rank != 0 || warp != 0) return;
         mine = blocks[0].sum;
+#pragma unroll 1
         for (int b = 1; b < cluster; ++b) {
             mine = joined(mine, blocks[b].sum);
             if constexpr (TOP) merge(best, at, blocks[b].v[31 - lane], blocks[b].i[31 - lane]);
