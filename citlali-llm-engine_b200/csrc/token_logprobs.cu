@@ -10,13 +10,14 @@
 // entries in registers and the next 16 on their way.  m, S and T are the thread's own until the end (the running maximum is looked
 // at once for 16 entries).
 //
-// The likeliest tokens.  A share of a few tiles (few rows) is read a second time, out of the caches, once a bound is known: a warp's
-// ceil(top / 8)-th largest of its lanes' own maxima, the least of the eight warps', has at least `top` entries above or at it, and hardly
-// more lanes that hold any; those lanes alone look through their entries again, and what they find is sorted.  Of a longer share each
-// warp keeps a list as it goes, lane i the i-th largest entry so far: an entry is looked at only if it exceeds the last one that
-// still counts in any warp of the block, which for 512 entries at a time hardly happens once a row has begun; for a warp's first 512 the
-// bound is the top-th of the lanes' own maxima.  Warps and then blocks (through distributed shared memory) merge their lists
-// pairwise: the larger of a[i] and b[31 - i] are the 32 largest, and five exchanges sort them.
+// The likeliest tokens.  A share's first tiles (all of a short share) are looked at a second time, out of the caches, once a bound is
+// known.  A thread remembers the largest of its tiles' maxima, which tile it was, and the second largest.  A warp's ceil(top / 8)-th
+// largest of its lanes' maxima, the least of the eight warps', has at least `top` entries at or above it, and hardly more threads that
+// hold any: of those threads alone the warp looks through the tile again (through all of the thread's tiles where the second maximum
+// reaches the bound too), and what it finds is sorted.  From then on a tile's entries are looked at only if one exceeds the last entry
+// that still counts in any warp of the block; a warp keeps a list of what it finds, lane i the i-th largest.  (So it does from the
+// start where more than 512 entries reached the first bound: many alike.)  Warps and then blocks, through distributed shared memory,
+// merge their lists pairwise: the larger of a[i] and b[31 - i] are the 32 largest of both, and five exchanges sort them.
 #include "api.h"
 #include "common.cuh"
 #include "mma_common.cuh"
@@ -29,8 +30,7 @@ constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNone = 0x7fffffff;                        // no entry: behind every index
 
-constexpr int kTwice = 8;                                // a share of fewer tiles is read a second time
-constexpr int kFound = 512;
+constexpr int kWindow = 8, kFound = 512;
 
 struct Summary { float m, s, t; };
 
@@ -97,7 +97,7 @@ struct Block {                                           // what a block tells t
 };
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ tokens, float* __restrict__ logprobs,
                       float* __restrict__ entropy, int32_t* __restrict__ top_ids, float* __restrict__ top_logprobs, int vocab, int top,
                       int cluster) {
@@ -164,12 +164,6 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
     auto keep = [&](const float (&y)[kEach], const float (&quarter)[4], float most, auto where) {
         const float others = unordered(*(volatile int*)&shared_bound);   // (at least `top` entries of the row are at or above it)
         if (!__any_sync(0xffffffffu, most >= fmaxf(bound, others) && most > -INFINITY)) return;
-        if (__all_sync(0xffffffffu, at == kNone)) {      // the first entries: at least `top` lanes' maxima are at or above the bound
-            float v = most;
-            int i = lane;
-            sort(v, i);
-            bound = __shfl_sync(0xffffffffu, v, top - 1);
-        }
         if (others > bound) { bound = others; bound_at = kNone; }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -200,111 +194,131 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
     };
 
     // The share tile by tile: whole ones, then the rest, less than a tile, then the row's ends (the lead with the first block, the tail
-    // with the last).  `use(y, where)` gets 16 entries a lane, minus infinity where there is none.
+    // with the last; a thread an entry).  `use(y, tile)` gets 16 entries a lane, minus infinity where there is none.
     constexpr int kTile = kThreads * kEach / kVec;       // vectors of a tile
     const int tiles = (stop - first) / kTile;            // whole ones
+    const int tail = lead + vectors * kVec;
     const T* base = x + lead + ((long long)first + tid) * kVec;
-    auto walk = [&](auto use) {
+    auto index_of = [&](int tile, int thread, int e) {   // the entry's, or -1: there is none
+        if (tile <= tiles) {
+            const int vector = first + tile * kTile + e / kVec * kThreads + thread;
+            return vector < stop ? lead + vector * kVec + e % kVec : -1;
+        }
+        if (e == 0 && rank == 0 && thread < lead) return thread;
+        return e == 0 && rank == cluster - 1 && thread >= 32 && tail + thread - 32 < vocab ? tail + thread - 32 : -1;
+    };
+    auto walk = [&](int from, int to, auto use) {        // tiles from .. to - 1; to = tiles + 2: the rest and the ends too
         float y[kEach], next[kEach];
-        if (tiles > 0) load(base, next);
+        const int whole = min(to, tiles);
+        if (from < whole) load(base + (long long)from * kTile * kVec, next);
 #pragma unroll 1
-        for (int k = 0; k < tiles; ++k) {
+        for (int k = from; k < whole; ++k) {
 #pragma unroll
             for (int e = 0; e < kEach; ++e) y[e] = next[e];
-            if (k + 1 < tiles) load(base + (long long)(k + 1) * kTile * kVec, next);
-            const int index0 = lead + (first + k * kTile + tid) * kVec;
-            use(y, [&](int e) { return index0 + e / kVec * (kThreads * kVec) + e % kVec; });
+            if (k + 1 < whole) load(base + (long long)(k + 1) * kTile * kVec, next);
+            use(y, k);
         }
-        const int rest = first + tiles * kTile, tail = lead + vectors * kVec;
-        int odd = -1;                                    // the ends: fewer than kVec entries each, a thread an entry
-        if (rank == 0 && tid < lead) odd = tid;
-        if (rank == cluster - 1 && tid >= 32 && tail + tid - 32 < vocab) odd = tail + tid - 32;
-#pragma unroll 1
-        for (int part = 0; part < 2; ++part) {
-            if (part == 0 ? rest >= stop : warp >= 2) continue;
+        const int rest = first + tiles * kTile;
+        if (to > tiles && rest < stop) {
+#pragma unroll
+            for (int k = 0; k < kEach / kVec; ++k) {
+                const int vector = rest + k * kThreads + tid;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (vector < stop) v = *reinterpret_cast<const uint4*>(x + lead + (long long)vector * kVec);
+                const T* in = reinterpret_cast<const T*>(&v);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) y[k * kVec + e] = vector < stop ? ldf(in, e) : -INFINITY;
+            }
+            use(y, tiles);
+        }
+        if (to > tiles && warp < 2) {
+            const int odd = index_of(tiles + 1, tid, 0);
 #pragma unroll
             for (int e = 0; e < kEach; ++e) y[e] = -INFINITY;
-            if (part == 0) {
-#pragma unroll
-                for (int k = 0; k < kEach / kVec; ++k)
-                    if (rest + k * kThreads + tid < stop) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(x + lead + ((long long)rest + k * kThreads + tid) * kVec);
-                        const T* in = reinterpret_cast<const T*>(&v);
-#pragma unroll
-                        for (int e = 0; e < kVec; ++e) y[k * kVec + e] = ldf(in, e);
-                    }
-            } else if (odd >= 0) {
-                y[0] = ldf(x, odd);
-            }
-            const int index0 = part == 0 ? lead + (rest + tid) * kVec : odd;
-            use(y, [&](int e) { return index0 + e / kVec * (kThreads * kVec) + e % kVec; });
+            if (odd >= 0) y[0] = ldf(x, odd);
+            use(y, tiles + 1);
         }
     };
 
-    const bool twice = TOP && tiles < kTwice;            // (alike for all threads)
-    float top_of_mine = -INFINITY;
-    walk([&](float (&y)[kEach], auto where) {
+    const int window = !TOP || tiles < 2 * kWindow ? tiles + 2 : kWindow;          // tiles ahead of the first bound
+    float largest_tile = -INFINITY, second_tile = -INFINITY;
+    int which_tile = 0;
+    walk(0, window, [&](float (&y)[kEach], int tile) {
         float quarter[4];
         const float most = largest(y, quarter);
         add(y, most);
-        if constexpr (TOP) {
-            if (twice) top_of_mine = fmaxf(top_of_mine, most);
-            else keep(y, quarter, most, where);
+        if (TOP && most > largest_tile) {
+            second_tile = largest_tile;
+            largest_tile = most;
+            which_tile = tile;
+        } else if (TOP) {
+            second_tile = fmaxf(second_tile, most);
         }
     });
+    bool listed = false;
     if constexpr (TOP) {
-        if (twice) {
-            int rest = ordered(top_of_mine), nth = ordered(-INFINITY);
+        int rest = ordered(largest_tile), nth = ordered(-INFINITY);
 #pragma unroll 1
-            for (int k = 0; k < (top + kWarps - 1) / kWarps; ++k) {
-                nth = __reduce_max_sync(0xffffffffu, rest);
-                const unsigned who = __ballot_sync(0xffffffffu, rest == nth);
-                if (lane == __ffs(who) - 1) rest = ordered(-INFINITY);
-            }
-            if (lane == 0) list_i[0][warp] = nth;
-            __syncthreads();
-            int least = list_i[0][0];
-#pragma unroll
-            for (int w = 1; w < kWarps; ++w) least = min(least, list_i[0][w]);
-            const float at_least = unordered(least);
-            auto look = [&](float v, int index) {
-                if (v >= at_least && fabsf(v) <= 3.402823466e+38f) {
-                    const int k = atomicAdd(&found, 1);
-                    if (k < kFound) { found_v[k] = v; found_i[k] = index; }
-                }
-            };
-            if (top_of_mine >= at_least && top_of_mine > -INFINITY) {
-#pragma unroll 2
-                for (int k = first + tid; k < stop; k += kThreads) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(x + lead + (long long)k * kVec);
-                    const T* in = reinterpret_cast<const T*>(&v);
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) look(ldf(in, e), lead + k * kVec + e);
-                }
-                const int tail = lead + vectors * kVec;
-                if (rank == 0 && tid < lead) look(ldf(x, tid), tid);
-                if (rank == cluster - 1 && tid >= 32 && tail + tid - 32 < vocab) look(ldf(x, tail + tid - 32), tail + tid - 32);
-            }
-            __syncthreads();
-            if (found <= kFound) {
-                if (warp == 0) {
-#pragma unroll 1
-                    for (int k = 0; k < found; k += 32) {
-                        float v = k + lane < found ? found_v[k + lane] : -INFINITY;
-                        int i = k + lane < found ? found_i[k + lane] : kNone;
-                        sort(v, i);
-                        merge(best, at, __shfl_sync(0xffffffffu, v, 31 - lane), __shfl_sync(0xffffffffu, i, 31 - lane));
-                    }
-                }
-            } else {                                     // many entries alike: lists as for a long share
-                walk([&](float (&y)[kEach], auto where) {
-                    float quarter[4];
-                    const float most = largest(y, quarter);
-                    keep(y, quarter, most, where);
-                });
-            }
-            __syncthreads();                             // (the room of the lists is used again)
+        for (int k = 0; k < (top + kWarps - 1) / kWarps; ++k) {
+            nth = __reduce_max_sync(0xffffffffu, rest);
+            const unsigned who = __ballot_sync(0xffffffffu, rest == nth);
+            if (lane == __ffs(who) - 1) rest = ordered(-INFINITY);
         }
+        if (lane == 0) list_i[0][warp] = nth;
+        __syncthreads();
+        const float at_least = unordered(__reduce_min_sync(0xffffffffu, list_i[0][lane % kWarps]));
+        auto look = [&](int i) {
+            if (i < 0) return;
+            const float v = ldf(x, i);
+            if (!(v >= at_least && fabsf(v) <= 3.402823466e+38f)) return;
+            const int k = atomicAdd(&found, 1);
+            if (k < kFound) { found_v[k] = v; found_i[k] = i; }
+        };
+#pragma unroll 1
+        for (unsigned who = __ballot_sync(0xffffffffu, largest_tile >= at_least && largest_tile > -INFINITY); who;) {
+            // two threads at a time, half a warp each
+            const int one = __ffs(who) - 1;
+            who &= who - 1;
+            const int two = who ? __ffs(who) - 1 : -1;
+            who &= who - 1;
+            const int from = lane < kEach ? one : two, tile = __shfl_sync(0xffffffffu, which_tile, from & 31);
+            const float second = __shfl_sync(0xffffffffu, second_tile, from & 31);           // (all lanes, also where there is no second thread)
+            const bool more = from >= 0 && second >= at_least;
+            if (from >= 0 && !more) look(index_of(tile, warp * 32 + from, lane % kEach));
+            if (more)
+#pragma unroll 4
+                for (int k = 0; k < window; ++k) look(index_of(k, warp * 32 + from, lane % kEach));
+        }
+        __syncthreads();
+        listed = found > kFound || window < tiles + 2;
+        if (found <= kFound) {
+            if (warp == 0) {
+#pragma unroll 1
+                for (int k = 0; k < found; k += 32) {
+                    float v = k + lane < found ? found_v[k + lane] : -INFINITY;
+                    int i = k + lane < found ? found_i[k + lane] : kNone;
+                    sort(v, i);
+                    merge(best, at, __shfl_sync(0xffffffffu, v, 31 - lane), __shfl_sync(0xffffffffu, i, 31 - lane));
+                }
+                if (lane == top - 1) shared_bound = ordered(best);
+                bound = __shfl_sync(0xffffffffu, best, top - 1);
+                bound_at = __shfl_sync(0xffffffffu, at, top - 1);
+            }
+        } else {
+            walk(0, window, [&](float (&y)[kEach], int tile) {
+                float quarter[4];
+                const float most = largest(y, quarter);
+                keep(y, quarter, most, [&](int e) { return index_of(tile, tid, e); });
+            });
+        }
+        __syncthreads();                                 // (the bound is there; the room of the lists is used again)
+        if (window < tiles + 2)
+            walk(window, tiles + 2, [&](float (&y)[kEach], int tile) {
+                float quarter[4];
+                const float most = largest(y, quarter);
+                add(y, most);
+                keep(y, quarter, most, [&](int e) { return index_of(tile, tid, e); });
+            });
     }
 
     // ---- the warp's, the block's, the cluster's
@@ -315,8 +329,8 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
     if constexpr (TOP) { list_v[warp][lane] = best; list_i[warp][lane] = at; }
     __syncthreads();
     if constexpr (TOP) {
-#pragma unroll
-        for (int half = kWarps / 2; half > 0 && !(twice && found <= kFound); half >>= 1) {
+#pragma unroll 1
+        for (int half = kWarps / 2; half > 0 && listed; half >>= 1) {
             if (warp < half) {
                 merge(best, at, list_v[warp + half][31 - lane], list_i[warp + half][31 - lane]);
                 list_v[warp][lane] = best;
@@ -325,11 +339,13 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
             __syncthreads();
         }
     }
-    if (warp == 0) {
-        Summary all = sums[0];
-        for (int w = 1; w < kWarps; ++w) all = joined(all, sums[w]);
-        mine = all;
-    }
+    auto all_of = [&](Summary one, int count) {          // over the first `count` lanes (a power of two), for all lanes
+#pragma unroll 1
+        for (int o = count >> 1; o > 0; o >>= 1)
+            one = joined(one, {__shfl_xor_sync(0xffffffffu, one.m, o), __shfl_xor_sync(0xffffffffu, one.s, o), __shfl_xor_sync(0xffffffffu, one.t, o)});
+        return one;
+    };
+    if (warp == 0) mine = all_of(sums[lane % kWarps], kWarps);
     if (cluster > 1) {
         if (warp == 0) {                                 // to the cluster's first block
             auto put = [&](void* here, uint32_t bits) {
@@ -349,12 +365,20 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
         }
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (rank != 0 || warp != 0) return;
-        mine = blocks[0].sum;
+        if (rank != 0) return;
+        if (warp == 0) mine = all_of(blocks[lane % cluster].sum, cluster);
+        if constexpr (TOP) {
 #pragma unroll 1
-        for (int b = 1; b < cluster; ++b) {
-            mine = joined(mine, blocks[b].sum);
-            if constexpr (TOP) merge(best, at, blocks[b].v[31 - lane], blocks[b].i[31 - lane]);
+            for (int half = cluster / 2; half > 0; half >>= 1) {
+                if (warp < half) {
+                    best = blocks[warp].v[lane];
+                    at = blocks[warp].i[lane];
+                    merge(best, at, blocks[warp + half].v[31 - lane], blocks[warp + half].i[31 - lane]);
+                    blocks[warp].v[lane] = best;
+                    blocks[warp].i[lane] = at;
+                }
+                __syncthreads();
+            }
         }
     }
     if (warp != 0) return;
