@@ -11,9 +11,10 @@
 // at once for 16 entries).
 //
 // The likeliest tokens.  A share's first tiles (all of a short share) are looked at a second time, out of the caches, once a bound is
-// known.  A thread remembers the largest of its tiles' maxima, which tile it was, and the second largest.  A warp's ceil(top / 8)-th
-// largest of its lanes' maxima, the least of the eight warps', has at least `top` entries at or above it, and hardly more threads that
-// hold any: of those threads alone the warp looks through the tile again (through all of the thread's tiles where the second maximum
+// known.  A thread remembers the largest of its tiles' maxima, which tile it was, and the second largest.  Every warp of the cluster
+// names as many of its lanes' largest as there have to be for `top` numbers; the top-th of them has at least `top` entries at or above
+// it, and hardly more threads that hold any: of those threads alone the warp looks through the tile again (through all of the thread's
+// tiles where the second maximum
 // reaches the bound too), and what it finds is sorted.  From then on a tile's entries are looked at only if one exceeds the last entry
 // that still counts in any warp of the block; a warp keeps a list of what it finds, lane i the i-th largest.  (So it does from the
 // start where more than 512 entries reached the first bound: many alike.)  Warps and then blocks, through distributed shared memory,
@@ -107,7 +108,7 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
     __shared__ int list_i[kWarps][32];
     __shared__ Block blocks[kMaxCluster];
     __shared__ float found_v[TOP ? kFound : 1];
-    __shared__ int found_i[TOP ? kFound : 1], found, shared_bound;
+    __shared__ int found_i[TOP ? kFound : 1], found, shared_bound, named[64];
     dependents_may_launch();
     wait_for_predecessor();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -126,8 +127,9 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
     int at = kNone;
     float bound = -INFINITY;                             // the top-th
     int bound_at = kNone;
-    if (TOP && tid == 0) { found = 0; shared_bound = ordered(-INFINITY); }
-    if (TOP) __syncthreads();
+    if (TOP && tid == 0) found = 0;
+    __syncwarp();
+    if (cluster > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");       // (waited for ahead of the first write to another block)
 
     // The largest of a thread's 16 entries, quarter by quarter.  Plus infinity is no entry (nor is a NaN, which no maximum takes).
     auto largest = [&](float (&y)[kEach], float (&quarter)[4]) {
@@ -255,24 +257,65 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
             second_tile = fmaxf(second_tile, most);
         }
     });
-    bool listed = false;
+    // Into the shared memory of the cluster's block `to`, where `here` lies in this one's; all blocks meet.
+    auto there = [&](const void* here, int to) {
+        uint32_t remote;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(here)), "r"(to));
+        return remote;
+    };
+    auto put = [&](const void* here, int to, uint32_t bits) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there(here, to)), "r"(bits) : "memory"); };
+    auto meet = [&] {
+        if (cluster == 1) {
+            __syncthreads();
+            return;
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    };
+    if (cluster > 1) {                                   // all of the cluster's blocks are there: their memory may be written to
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    bool listed = false;                                 // whether warps have lists
     if constexpr (TOP) {
-        int rest = ordered(largest_tile), nth = ordered(-INFINITY);
+        // the bound: every warp's `each` largest lanes, and the top-th of all of them
+        const int each = (top + kWarps * cluster - 1) / (kWarps * cluster), count = kWarps * cluster * each;        // 64 at most
+        int rest = ordered(largest_tile), mine_to_tell = 0;
 #pragma unroll 1
-        for (int k = 0; k < (top + kWarps - 1) / kWarps; ++k) {
-            nth = __reduce_max_sync(0xffffffffu, rest);
+        for (int k = 0; k < each; ++k) {
+            const int nth = __reduce_max_sync(0xffffffffu, rest);
             const unsigned who = __ballot_sync(0xffffffffu, rest == nth);
             if (lane == __ffs(who) - 1) rest = ordered(-INFINITY);
+            if (lane % each == k) mine_to_tell = nth;
         }
-        if (lane == 0) list_i[0][warp] = nth;
-        __syncthreads();
-        const float at_least = unordered(__reduce_min_sync(0xffffffffu, list_i[0][lane % kWarps]));
+        if (lane < cluster * each) put(&named[(rank * kWarps + warp) * each + lane % each], lane / each, (uint32_t)mine_to_tell);
+        meet();
+        int least = ordered(-INFINITY);
+        {
+            const int a = lane < count ? named[lane] : ordered(-INFINITY), b = lane + 32 < count ? named[lane + 32] : ordered(-INFINITY);
+            int before_a = 0, before_b = 0;
+#pragma unroll 4
+            for (int k = 0; k < count; ++k) {
+                const int v = named[k];
+                before_a += v > a || (v == a && k < lane);
+                before_b += v > b || (v == b && k < lane + 32);
+            }
+            if (lane < count && before_a == top - 1) least = a;
+            if (lane + 32 < count && before_b == top - 1) least = b;
+            least = __reduce_max_sync(0xffffffffu, least);
+        }
+        const float at_least = unordered(least);
         auto look = [&](int i) {
             if (i < 0) return;
             const float v = ldf(x, i);
             if (!(v >= at_least && fabsf(v) <= 3.402823466e+38f)) return;
-            const int k = atomicAdd(&found, 1);
-            if (k < kFound) { found_v[k] = v; found_i[k] = i; }
+            int k;
+            asm volatile("atom.shared::cluster.add.s32 %0, [%1], 1;" : "=r"(k) : "r"(there(&found, 0)) : "memory");
+            if (k < kFound) {
+                put(&found_v[k], 0, __float_as_uint(v));
+                put(&found_i[k], 0, (uint32_t)i);
+            }
         };
 #pragma unroll 1
         for (unsigned who = __ballot_sync(0xffffffffu, largest_tile >= at_least && largest_tile > -INFINITY); who;) {
@@ -289,36 +332,40 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
 #pragma unroll 4
                 for (int k = 0; k < window; ++k) look(index_of(k, warp * 32 + from, lane % kEach));
         }
-        __syncthreads();
-        listed = found > kFound || window < tiles + 2;
-        if (found <= kFound) {
-            if (warp == 0) {
-#pragma unroll 1
-                for (int k = 0; k < found; k += 32) {
-                    float v = k + lane < found ? found_v[k + lane] : -INFINITY;
-                    int i = k + lane < found ? found_i[k + lane] : kNone;
-                    sort(v, i);
-                    merge(best, at, __shfl_sync(0xffffffffu, v, 31 - lane), __shfl_sync(0xffffffffu, i, 31 - lane));
-                }
-                if (lane == top - 1) shared_bound = ordered(best);
-                bound = __shfl_sync(0xffffffffu, best, top - 1);
-                bound_at = __shfl_sync(0xffffffffu, at, top - 1);
-            }
-        } else {
+        meet();
+        int all_found;
+        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(all_found) : "r"(there(&found, 0)) : "memory");
+        listed = all_found > kFound || window < tiles + 2;
+        if (tid == 0) shared_bound = least;
+        if (all_found > kFound) {                        // (many alike)
+            __syncthreads();
             walk(0, window, [&](float (&y)[kEach], int tile) {
                 float quarter[4];
                 const float most = largest(y, quarter);
                 keep(y, quarter, most, [&](int e) { return index_of(tile, tid, e); });
             });
+        } else if (rank == 0 && warp == 0) {
+#pragma unroll 1
+            for (int k = 0; k < all_found; k += 32) {
+                float v = k + lane < all_found ? found_v[k + lane] : -INFINITY;
+                int i = k + lane < all_found ? found_i[k + lane] : kNone;
+                sort(v, i);
+                merge(best, at, __shfl_sync(0xffffffffu, v, 31 - lane), __shfl_sync(0xffffffffu, i, 31 - lane));
+            }
+            bound = __shfl_sync(0xffffffffu, best, top - 1);
+            bound_at = __shfl_sync(0xffffffffu, at, top - 1);
+            if (lane == 0) shared_bound = ordered(bound);
         }
-        __syncthreads();                                 // (the bound is there; the room of the lists is used again)
-        if (window < tiles + 2)
-            walk(window, tiles + 2, [&](float (&y)[kEach], int tile) {
-                float quarter[4];
-                const float most = largest(y, quarter);
-                add(y, most);
-                keep(y, quarter, most, [&](int e) { return index_of(tile, tid, e); });
-            });
+        if (listed) {
+            __syncthreads();                             // (the bound is there)
+            if (window < tiles + 2)
+                walk(window, tiles + 2, [&](float (&y)[kEach], int tile) {
+                    float quarter[4];
+                    const float most = largest(y, quarter);
+                    add(y, most);
+                    keep(y, quarter, most, [&](int e) { return index_of(tile, tid, e); });
+                });
+        }
     }
 
     // ---- the warp's, the block's, the cluster's
@@ -348,26 +395,20 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
     if (warp == 0) mine = all_of(sums[lane % kWarps], kWarps);
     if (cluster > 1) {
         if (warp == 0) {                                 // to the cluster's first block
-            auto put = [&](void* here, uint32_t bits) {
-                uint32_t remote;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(here)), "r"(0));
-                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(bits) : "memory");
-            };
             if (lane == 0) {
-                put(&blocks[rank].sum.m, __float_as_uint(mine.m));
-                put(&blocks[rank].sum.s, __float_as_uint(mine.s));
-                put(&blocks[rank].sum.t, __float_as_uint(mine.t));
+                put(&blocks[rank].sum.m, 0, __float_as_uint(mine.m));
+                put(&blocks[rank].sum.s, 0, __float_as_uint(mine.s));
+                put(&blocks[rank].sum.t, 0, __float_as_uint(mine.t));
             }
-            if constexpr (TOP) {
-                put(&blocks[rank].v[lane], __float_as_uint(best));
-                put(&blocks[rank].i[lane], (uint32_t)at);
+            if (listed) {
+                put(&blocks[rank].v[lane], 0, __float_as_uint(best));
+                put(&blocks[rank].i[lane], 0, (uint32_t)at);
             }
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        meet();                                          // (and no block is gone while another looks into its memory)
         if (rank != 0) return;
         if (warp == 0) mine = all_of(blocks[lane % cluster].sum, cluster);
-        if constexpr (TOP) {
+        if (listed) {
 #pragma unroll 1
             for (int half = cluster / 2; half > 0; half >>= 1) {
                 if (warp < half) {
