@@ -45,6 +45,20 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
     *reinterpret_cast<uint4*>(p) = w;
 }
 
+// The eight values of a word of codes.
+__device__ __forceinline__ void store_values(__nv_bfloat16* p, uint32_t w, float s) {
+    uint32_t v[4];
+    values_of(w, s, v);
+    *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store_values(float* p, uint32_t w, float s) {
+    uint32_t v[4];
+    values_of(w, s, v);
+    uint4* out = reinterpret_cast<uint4*>(p);
+    out[0] = make_uint4(v[0] << 16, v[0] & 0xffff0000u, v[1] << 16, v[1] & 0xffff0000u);
+    out[1] = make_uint4(v[2] << 16, v[2] & 0xffff0000u, v[3] << 16, v[3] & 0xffff0000u);
+}
+
 struct Pools {
     uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
 };
@@ -62,10 +76,7 @@ __device__ __forceinline__ void put8(uint8_t* codes, uint8_t* scales, size_t at,
     if (!on) return;
     float s;
     const int byte = scale_byte(most, s);
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w |= code(x[i], s) << (4 * i);
-    *reinterpret_cast<uint32_t*>(codes + at * (d / 2) + e / 2) = w;
+    *reinterpret_cast<uint32_t*>(codes + at * (d / 2) + e / 2) = codes_of(x, s);
     if (e % kGroup == 0) scales[at * (d / kGroup) + e / kGroup] = (uint8_t)byte;
 }
 
@@ -202,8 +213,15 @@ append_any_kernel(const T* __restrict__ qkv, T* q_out, size_t q_out_stride, cons
                 for (int i = 0; i < kGroup; ++i) most = max(most, magnitude(y[g * kGroup + i]));
                 float s;
                 scales[at * (d / kGroup) + g] = (uint8_t)scale_byte(most, s);
-                for (int i = 0; i < kGroup; i += 2)
-                    codes[at * (d / 2) + (g * kGroup + i) / 2] = (uint8_t)(code(y[g * kGroup + i], s) | code(y[g * kGroup + i + 1], s) << 4);
+                for (int half = 0; half < 2; ++half) {
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = y[g * kGroup + 8 * half + i];
+                    const uint32_t w = codes_of(x, s);
+                    uint8_t* out = codes + at * (d / 2) + (g * kGroup) / 2 + 4 * half;       // (any alignment)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out[i] = (uint8_t)(w >> (8 * i));
+                }
             }
         }
         __syncwarp();
@@ -229,13 +247,8 @@ read_kernel(const __grid_constant__ Rows rows, const __grid_constant__ Pools poo
     const uint2 w = *reinterpret_cast<const uint2*>((is_v ? pools.v_codes : pools.k_codes) + at * (d / 2) + g * 8);
     const float s = scale_of((is_v ? pools.v_scales : pools.k_scales)[at * per_head + g]);
     TO* out = (is_v ? values : keys) + ((size_t)row * nkv + head) * d + g * kGroup;
-    float y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = value_of(w.x, e, s);
-    store8(out, y);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = value_of(w.y, e, s);
-    store8(out + 8, y);
+    store_values(out, w.x, s);
+    store_values(out + 8, w.y, s);
 }
 
 // The pages that a run's rows see, as bfloat16 pages of their own (exact), with a page table and slots for the attention kernels of a
@@ -293,13 +306,9 @@ expand_kernel(const __grid_constant__ Runs runs, const int32_t* __restrict__ pag
         const bool is_v = i >= kRunPage * per_row;
         const int j = is_v ? i - kRunPage * per_row : i, row = j / per_row, g = j % per_row, pos = tile * kRunPage + row;
         const size_t from = place(page, nkv, head, kRunPage, row), to = place(blockIdx.x, nkv, head, kRunPage, row);
-        float y[8];
         __nv_bfloat16* out = (is_v ? values : keys) + to * d + g * kGroup;
         if (pos < low || pos > last) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = 0.0f;
-            store8(out, y);
-            store8(out + 8, y);
+            reinterpret_cast<uint4*>(out)[0] = reinterpret_cast<uint4*>(out)[1] = make_uint4(0, 0, 0, 0);
             continue;
         }
         const uint2 w = *reinterpret_cast<const uint2*>((is_v ? pools.v_codes : pools.k_codes) + from * (d / 2) + g * 8);
@@ -313,12 +322,8 @@ expand_kernel(const __grid_constant__ Runs runs, const int32_t* __restrict__ pag
             for (int k = 0; k < per_row; ++k) none |= pools.v_scales[from * per_row + k] >= 0xf8;
             if (none) s = __int_as_float(0x7fc00000);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = value_of(w.x, e, s);
-        store8(out, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = value_of(w.y, e, s);
-        store8(out + 8, y);
+        store_values(out, w.x, s);
+        store_values(out + 8, w.y, s);
     }
 }
 

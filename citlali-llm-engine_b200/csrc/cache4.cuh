@@ -30,14 +30,21 @@ constexpr int kNoNumber = 0xff;
 // |x| as a whole number: in the order of the magnitudes, infinities and then NaNs last (fmaxf would lose a NaN).
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// The scale's byte for a group whose largest magnitude is `most`, and the scale.  The division and the two roundings are exact
-// in the sense that the same numbers come out in any precision for elements of 16 bits (a tie is seen as one).
+// x / d, rounded to nearest: a product with the reciprocal, off by a last place or two, and one step from the exact remainder.  (Half
+// of what the division of all floats takes; the quotients here are far from the ends of the range.)  In particular a quotient that is
+// a float comes out as that: a tie between two codes is one.
+__device__ __forceinline__ float quotient(float x, float d, float reciprocal) {
+    const float q = x * reciprocal;
+    return fmaf(fmaf(-q, d, x), reciprocal, q);
+}
+
+// The scale's byte for a group whose largest magnitude is `most`, and the scale.
 __device__ __forceinline__ int scale_byte(uint32_t most, float& s) {
     if (most >= 0x7f800000u) {
         s = __int_as_float(0x7fc00000);
         return kNoNumber;
     }
-    const float wanted = fminf(__fdiv_rn(__uint_as_float(most), 7.0f), kLargestScale);
+    const float wanted = fminf(quotient(fminf(__uint_as_float(most), 7.0f * kLargestScale), 7.0f, 1.0f / 7.0f), kLargestScale);
     if (wanted < 0.00048828125f) {                                   // below 2^-11: multiples of 2^-14
         const float n = rintf(wanted * 16384.0f);
         s = n * 0.00006103515625f;
@@ -49,11 +56,20 @@ __device__ __forceinline__ int scale_byte(uint32_t most, float& s) {
     return (int)(((bits >> 23) - 127u + 12u) << 3 | ((bits >> 20) & 7u));
 }
 
-// c + 8 of an element.
-__device__ __forceinline__ uint32_t code(float x, float s) {
-    if (!(s > 0.0f)) return 8u;                                      // a group of zeros, or one that holds no number
-    const float c = fminf(fmaxf(rintf(__fdiv_rn(x, s)), -7.0f), 7.0f);
-    return (uint32_t)((int)c + 8);
+// Eight elements' codes c + 8 as a word, the first element's in the lowest bits.  1.5 2^23 + 8 + c, added up in a float, rounds to the
+// nearest c, ties to even, and has c + 8 in its lowest bits: so one multiply-add a code puts the word together.  A group that holds no
+// number, or zeros alone, gets codes that mean nothing, or zeros.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
+    const bool some = s > 0.0f;
+    const float d = some ? s : 0.0f, reciprocal = some ? __frcp_rn(s) : 0.0f;
+    constexpr uint32_t kOne = 0x4b400000u;                           // the bits of 1.5 2^23
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+        const float c = fminf(fmaxf(quotient(x[i], d, reciprocal), -7.0f), 7.0f);
+        w = w * 16u + (__float_as_uint(c + 12582920.0f) - kOne);
+    }
+    return w;
 }
 
 __device__ __forceinline__ float scale_of(uint32_t byte) {
@@ -61,6 +77,23 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
 }
 // The value of nibble i of a word of eight codes.
 __device__ __forceinline__ float value_of(uint32_t word, int i, float s) { return (float)((int)((word >> (4 * i)) & 15u) - 8) * s; }
+
+// A word's eight values in bfloat16, two a word, in order.  (w & 0x000f000f) | 0x4300 is 136 + c there, and (136 + c) s - 136 s is
+// exact: s has four significant bits, 136 s eight at most.
+__device__ __forceinline__ void values_of(uint32_t w, float s, uint32_t (&out)[4]) {
+    const __nv_bfloat162 s2 = __float2bfloat162_rn(s), low = __float2bfloat162_rn(-136.0f * s);
+    uint32_t pair[4];                                                // elements (i, i + 4)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t x = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+        const __nv_bfloat162 v = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&x), s2, low);
+        pair[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    out[0] = __byte_perm(pair[0], pair[1], 0x5410);
+    out[1] = __byte_perm(pair[2], pair[3], 0x5410);
+    out[2] = __byte_perm(pair[0], pair[1], 0x7632);
+    out[3] = __byte_perm(pair[2], pair[3], 0x7632);
+}
 
 // Where a token's key or value of a head lies: codes [page][head][token of the page][d / 2], scales [page][head][token][d / 16].
 __device__ __forceinline__ size_t place(int page, int nkv, int head, int page_size, int at) {
