@@ -297,14 +297,15 @@ def token_logprobs(logits, tokens=None, top: int = 0) -> dict:
         require(False, f"token_logprobs: {top} alternatives of {vocab} entries (at most 32)")
     if tokens is not None and not (tokens.dtype is torch.int32 and tokens.numel() == rows):
         require(False, "token_logprobs: tokens are int32, one a row")
-    floats = torch.empty((2 + top) * rows, dtype=torch.float32, device=logits.device)
-    found = {"logprobs": floats[:rows], "entropy": floats[rows:2 * rows]}
-    if tokens is None:
-        del found["logprobs"]
+    floats = logits.new_empty((2 + top) * rows, dtype=torch.float32)
+    logprobs, entropy, top_logprobs = floats.split((rows, rows, top * rows))
+    found = {"entropy": entropy}
+    if tokens is not None:
+        found["logprobs"] = logprobs
     ids = None
     if top:
-        ids = found["top_ids"] = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-        found["top_logprobs"] = floats[2 * rows:].view(rows, top)
+        ids = found["top_ids"] = logits.new_empty((rows, top), dtype=torch.int32)
+        found["top_logprobs"] = top_logprobs.view(rows, top)
     if rows:
         at = floats.data_ptr()
         _check(lib().citlali_token_logprobs(logits.data_ptr(), _dtype_code(logits), _ptr(tokens), at, at + 4 * rows, _ptr(ids), at + 8 * rows, rows,
@@ -495,12 +496,11 @@ def _packed4(kv, nkv: int, head_dim: int, what: str):
     keys, values, table = kv.keys, kv.values, kv.page_table
     if type(keys) is Packed4 and type(values) is Packed4 and head_dim % 16 == 0 and 16 <= head_dim <= 256:
         kc, ks, vc, vs = keys.codes, keys.scales, values.codes, values.scales
-        codes, scales, shape = kc.shape, ks.shape, (nkv, kv.page_size)
-        if (codes[1:3] == shape and codes[3] * 2 == head_dim and scales[0] == codes[0] and scales[1:3] == shape and scales[3] * 16 == head_dim
-                and vc.shape == codes and vs.shape == scales and len(codes) == len(scales) == 4
-                and kc.dtype is torch.uint8 and ks.dtype is torch.uint8 and vc.dtype is torch.uint8 and vs.dtype is torch.uint8
-                and table.dtype is torch.int32 and table.dim() == 2 and _are_here(kc, ks, vc, vs, table)):
-            return kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), table.data_ptr(), table.shape[1]
+        codes, scales, row, u8 = kc.shape, ks.shape, table.shape, torch.uint8
+        if (len(row) == 2 and codes[1:] == (nkv, kv.page_size, head_dim // 2) and scales == (codes[0], nkv, kv.page_size, head_dim // 16)
+                and vc.shape == codes and vs.shape == scales and kc.dtype is u8 and ks.dtype is u8 and vc.dtype is u8 and vs.dtype is u8
+                and table.dtype is torch.int32 and _are_here(kc, ks, vc, vs, table)):
+            return kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), table.data_ptr(), row[1]
     _check_packed4(kv, nkv, head_dim, what)
     raise CitlaliError(f"{what}: the cache's view does not fit")
 
@@ -564,8 +564,8 @@ def cache4_read(kv, slots, positions, dtype=torch.bfloat16):
         require(False, "cache4_read: slots and positions are int32, one a row")
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         require(False, f"cache4_read: values come in bfloat16 or float32, not {dtype}")
-    held = torch.empty((2, rows, nkv, 2 * width), dtype=dtype, device=slots.device)
-    keys, values = held[0], held[1]
+    held = slots.new_empty((2, rows, nkv, 2 * width), dtype=dtype)
+    keys, values = held.unbind(0)
     if rows:
         kc, ks, vc, vs, table, table_width = pools
         _check(lib().citlali_cache4_read(kc, ks, vc, vs, table, table_width, _i(kv.page_size), slots.data_ptr(), positions.data_ptr(),
@@ -679,7 +679,7 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
         if floats >= 0:
             # of this call alone, and given back in stream order: two graphs, or two streams, share nothing
             device, stream = q.device, _stream()
-            partial = torch.empty(floats, dtype=torch.float32, device=device)
+            partial = q.new_empty(floats, dtype=torch.float32)
             arrived = None if torch._C._cuda_isCurrentStreamCapturing() else _arrivals.get((device.index, stream))
             if arrived is None:
                 arrived = _arrivals_of(device, stream)
