@@ -252,7 +252,7 @@ read_kernel(const __grid_constant__ Rows rows, const __grid_constant__ Pools poo
 }
 
 // The pages that a run's rows see, as bfloat16 pages of their own (exact), with a page table and slots for the attention kernels of a
-// cache of 16 bits: sequence b is slot b there.  A block a (page, key/value head).  Positions that no row of the run sees become
+// cache of 16 bits: sequence b is slot b there.  A block a (page, key/value head, keys or values).  Positions that no row of the run sees become
 // zeros.  A value that is no number becomes zero too, and its token's key none: a row that does not see the token gives it the
 // weight zero, and zero times a NaN would reach it; a row that does see it gets a NaN from the key.
 struct Runs {
@@ -269,7 +269,7 @@ expand_kernel(const __grid_constant__ Runs runs, const int32_t* __restrict__ pag
     // the sequence of this page: every warp finds it for itself (lists and page tables come from the host before the step)
     auto tiles_of = [&](int b, int& first) {
         const int past = runs.seq_past[b], fresh = runs.seq_start[b + 1] - runs.seq_start[b];
-        first = runs.window > 0 ? max(0, past - runs.window + 1) / kRunPage : 0;
+        first = runs.window > 0 ? max(0, past - runs.window + 1) / kRunPage & ~1 : 0;        // (the kernels read pairs of pages)
         return fresh > 0 ? (past + fresh - 1) / kRunPage - first + 1 : 0;
     };
     int b = -1, tile = 0, run = 0;
@@ -296,34 +296,38 @@ expand_kernel(const __grid_constant__ Runs runs, const int32_t* __restrict__ pag
     if (tile >= table_out_stride) return;
     const int past = runs.seq_past[b], last = past + runs.seq_start[b + 1] - runs.seq_start[b] - 1;
     const int low = runs.window > 0 ? max(0, past - runs.window + 1) : 0;
-    if (head == 0 && threadIdx.x == 0) {
+    if (head == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
         table_out[(size_t)b * table_out_stride + tile] = blockIdx.x;
         if (tile == first) slots_out[b] = b;
     }
     const int page = page_table[(size_t)runs.seq_slot[b] * page_table_stride + tile];
     const int per_row = d / kGroup;
-    for (int i = threadIdx.x; i < 2 * kRunPage * per_row; i += kExpandThreads) {
-        const bool is_v = i >= kRunPage * per_row;
-        const int j = is_v ? i - kRunPage * per_row : i, row = j / per_row, g = j % per_row, pos = tile * kRunPage + row;
-        const size_t from = place(page, nkv, head, kRunPage, row), to = place(blockIdx.x, nkv, head, kRunPage, row);
-        __nv_bfloat16* out = (is_v ? values : keys) + to * d + g * kGroup;
+    const bool is_v = blockIdx.z != 0;
+    const size_t from0 = place(page, nkv, head, kRunPage, 0), to0 = place(blockIdx.x, nkv, head, kRunPage, 0);
+    const uint8_t* codes = (is_v ? pools.v_codes : pools.k_codes) + from0 * (d / 2);
+    const uint8_t *own = (is_v ? pools.v_scales : pools.k_scales) + from0 * per_row, *others = pools.v_scales + from0 * per_row;
+    __nv_bfloat16* out = (is_v ? values : keys) + to0 * d;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < kRunPage * per_row; i += kExpandThreads) {     // (a group's row and place follow from i alone)
+        const int row = i / per_row, pos = tile * kRunPage + row;
+        const uint2 w = *reinterpret_cast<const uint2*>(codes + i * 8);
+        const uint8_t byte = own[i];
+        bool none = false;                               // of the token's values
+        if (is_v) {
+            none = byte >= 0xf8;
+        } else if (per_row % 4 == 0) {
+            for (int k = 0; k < per_row; k += 4) none |= __vcmpgeu4(*reinterpret_cast<const uint32_t*>(others + row * per_row + k), 0xf8f8f8f8u) != 0;
+        } else {
+            for (int k = 0; k < per_row; ++k) none |= others[row * per_row + k] >= 0xf8;
+        }
+        __nv_bfloat16* to = out + (size_t)i * kGroup;
         if (pos < low || pos > last) {
-            reinterpret_cast<uint4*>(out)[0] = reinterpret_cast<uint4*>(out)[1] = make_uint4(0, 0, 0, 0);
+            reinterpret_cast<uint4*>(to)[0] = reinterpret_cast<uint4*>(to)[1] = make_uint4(0, 0, 0, 0);
             continue;
         }
-        const uint2 w = *reinterpret_cast<const uint2*>((is_v ? pools.v_codes : pools.k_codes) + from * (d / 2) + g * 8);
-        float s;
-        if (is_v) {
-            const uint8_t byte = pools.v_scales[from * per_row + g];
-            s = byte >= 0xf8 ? 0.0f : scale_of(byte);
-        } else {
-            s = scale_of(pools.k_scales[from * per_row + g]);
-            bool none = false;
-            for (int k = 0; k < per_row; ++k) none |= pools.v_scales[from * per_row + k] >= 0xf8;
-            if (none) s = __int_as_float(0x7fc00000);
-        }
-        store_values(out, w.x, s);
-        store_values(out + 8, w.y, s);
+        const float s = !none ? scale_of(byte) : is_v ? 0.0f : __int_as_float(0x7fc00000);
+        store_values(to, w.x, s);
+        store_values(to + 8, w.y, s);
     }
 }
 
@@ -428,13 +432,13 @@ extern "C" int citlali_cache4_expand(const void* k_codes, const void* k_scales, 
         set_last_error("cache4_expand: pages of %d (only of 64), %d heads, window %d", page_size, nkv, window);
         return kBadShape;
     }
-    if (!c4::aligned(k_codes, 8) || !c4::aligned(v_codes, 8) || !c4::aligned(keys, 16) || !c4::aligned(values, 16)) {
-        set_last_error("cache4_expand: codes must be 8-byte and pages 16-byte aligned");
+    if (!c4::aligned(k_codes, 8) || !c4::aligned(v_codes, 8) || !c4::aligned(v_scales, 4) || !c4::aligned(keys, 16) || !c4::aligned(values, 16)) {
+        set_last_error("cache4_expand: codes must be 8-byte, scales 4-byte and pages 16-byte aligned");
         return kBadAlignment;
     }
     const c4::Runs runs = {seq_start, seq_slot, seq_past, sequences, window};
     const c4::Pools pools = {(uint8_t*)k_codes, (uint8_t*)k_scales, (uint8_t*)v_codes, (uint8_t*)v_scales};
-    launch_kernel(c4::expand_kernel, dim3(pages, nkv), c4::kExpandThreads, 0, stream, runs, page_table, page_table_stride, pools,
+    launch_kernel(c4::expand_kernel, dim3(pages, nkv, 2), c4::kExpandThreads, 0, stream, runs, page_table, page_table_stride, pools,
                   (__nv_bfloat16*)keys, (__nv_bfloat16*)values, table_out, table_out_stride, slots_out, nkv, head_dim);
     return CITLALI_LAUNCH_CHECK();
 }

@@ -582,47 +582,78 @@ def _attention4_floats(nq: int, nkv: int, head_dim: int, page_size: int, max_new
     return l.citlali_attention4_scratch_floats(nq, nkv, head_dim, max_new)
 
 
-_EXPAND_FROM = 40                          # new tokens
 _EXPAND_BYTES = 1 << 30
 
 
-def _attention4_expands(q, q_stride, out, batch, nq, nkv, head_dim, page_size) -> bool:
-    """Whether runs go over pages that were made bfloat16 first, by the kernels of a cache of 16 bits."""
-    return (batch.max_new >= _EXPAND_FROM and q.dtype is torch.bfloat16 and page_size == 64 and nkv > 0 and nq % nkv == 0 and q_stride % 8 == 0
-            and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0 and lib().citlali_attention_run_form(q_stride, out.shape[1], head_dim, 64, batch.max_new) > 0)
+def _attention4_expands(batch, nq: int, nkv: int, head_dim: int, window: int, form: int, sms: int) -> bool:
+    """Whether runs of new tokens go over pages that are made bfloat16 first, by prompt attention (``form``: 2 on tcgen05, 1 on mma.sync).
+    Both ways' times, in microseconds: the kernel that reads codes does a tile of 16 columns (8 at head size 256) over 32 keys in so
+    many nanoseconds, divided over all SMs; prompt attention's blocks walk their keys one tile after another, whole blocks a SM.
+    Measured, codes / pages: one run over 2,048 keys, 16 heads over 8 of 128, 64 new tokens 25 / 49, 96: 28 / 50, 2,048: 277 / 54; four
+    over 2,048, 40 over 8: 48 tokens 71 / 89, 96: 123 / 92; four over 32,768: 64 tokens 1,015 / 1,270, 96: 1,466 / 1,273; heads of 64, 32 over
+    8, one over 8,192: 96 tokens 67 / 195, four over 32,768: 96 tokens 848 / 1,003."""
+    max_new = batch.max_new
+    if max_new < 48 or form == 0:
+        return False
+    group = nq // nkv
+    columns = 8 if head_dim == 256 else 16
+    head_tiles = -(-group // columns)
+    tokens = max(1, columns // -(-group // head_tiles))
+    unit = {64: 1.1e-3, 128: 1.4e-3}.get(head_dim, 2.8e-3)
+    if form == 2:                                    # a block: two heads over 128 new tokens, or one over 256
+        rows, heads, keys_of_tile, tile, resident = (128, nq // 2, 128, 2.2, 1) if group % 2 == 0 else (256, nq, 128, 2.2, 1)
+    else:
+        rows, heads, keys_of_tile, tile, resident = 64, nq, 64, 1.5 * head_dim / 64, max(1, 256 // head_dim)
+    codes = pages = longest = steps = 0
+    for past, n in zip(batch.past, batch.n_new):
+        keys = past + n if not window else min(past + n, window + n)
+        codes += -(-n // tokens) * head_tiles * nkv * (keys // 32 + 16)
+        pages += keys // 64 + 1
+        blocks = -(-n // rows)
+        first = keys - n if not window else min(keys - n, window)               # keys ahead of a block's own tokens
+        most = (first + (n if not window else min(n, window + rows))) // keys_of_tile + 1
+        longest = max(longest, most)
+        steps += heads * blocks * (first // keys_of_tile + 1 + (most - first // keys_of_tile) / 2)
+    walked = max(longest, -(-steps // (sms * resident * longest)) * longest if steps > sms * resident * longest else 0)
+    return 9 + codes * unit > 14 + walked * tile + pages * nkv * 64 * head_dim * 4 / 2.3e6
 
 
-def _attention4_expanded(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
+def _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, scale):
     """The pages that the rows see as bfloat16 (the values are exact there), then prompt attention over them: as many sequences at a
     time as a gigabyte holds, at least one."""
     require(not torch.cuda.is_current_stream_capturing(), "cache4_attention: runs of tokens are sized from the host's lists of lengths, "
             "which a captured step would freeze")
-    pools, l, page_bytes = _packed4(kv, nkv, head_dim, "cache4_attention"), lib(), 2 * nkv * 64 * head_dim * 2
     kc, ks, vc, vs, table, table_width = pools
-    tiles, ends = [], []                      # pages of each sequence, and where its last one lies in its row of the table
-    for p, n in zip(batch.past, batch.n_new):
-        ends.append((p + n - 1) // 64 + 1)
-        tiles.append(ends[-1] - (max(0, p - window + 1) // 64 if window else 0))
-    b0 = 0
-    while b0 < len(tiles):
+    l, stream, page_bytes = lib(), _stream(), nkv * 64 * head_dim * 2
+    past, n_new = batch.past, batch.n_new
+    ends = [(p + n + 63) // 64 for p, n in zip(past, n_new)]                     # where a sequence's last page lies in its row of the table
+    tiles = [e - (max(0, p - window + 1) // 64 & ~1) for e, p in zip(ends, past)] if window else ends        # (kernels read pairs of pages)
+    start, slot, seq_past = batch.seq_start.data_ptr(), batch.seq_slot.data_ptr(), batch.seq_past.data_ptr()
+    out_ptr, wide, b0, total = out.data_ptr(), out.shape[1], 0, len(tiles)
+    while b0 < total:
         b1, pages = b0 + 1, tiles[b0]
-        while b1 < len(tiles) and (pages + tiles[b1]) * page_bytes <= _EXPAND_BYTES:
+        while b1 < total and 2 * (pages + tiles[b1]) * page_bytes <= _EXPAND_BYTES:
             pages += tiles[b1]
             b1 += 1
-        count, width, max_new = b1 - b0, max(ends[b0:b1]), max(batch.n_new[b0:b1])
-        held = torch.empty((2, pages, nkv, 64, head_dim), dtype=torch.bfloat16, device=q.device)
-        found = torch.empty((count + 1, max(width, count)), dtype=torch.int32, device=q.device)        # the table's rows, then the slots
-        seq_start, seq_slot, seq_past = batch.seq_start[b0:b1 + 1], batch.seq_slot[b0:b1], batch.seq_past[b0:b1]
-        _check(l.citlali_cache4_expand(kc, ks, vc, vs, table, table_width, seq_start.data_ptr(), seq_slot.data_ptr(), seq_past.data_ptr(), count,
-                                       window, held[0].data_ptr(), held[1].data_ptr(), pages, found.data_ptr(), found.shape[1],
-                                       found[count].data_ptr(), 64, nkv, head_dim, _stream()), "cache4_expand")
-        run = _run_kernels[l.citlali_attention_run_form(q_stride, out.shape[1], head_dim, 64, max_new) == 2]
-        run(q, q_stride, held[0], held[1], found[:count], seq_start, found[count, :count], seq_past, out, count, max_new, nq, nkv, head_dim, 64,
-            window, scale)
+        count, width, max_new = b1 - b0, max(ends[b0:b1]), max(n_new[b0:b1])
+        # keys, values, the table's rows and the slots, in one piece that is given back in stream order
+        held = q.new_empty(2 * pages * page_bytes + 4 * count * (width + 1), dtype=torch.uint8)
+        keys = held.data_ptr()
+        values = keys + pages * page_bytes
+        rows = values + pages * page_bytes
+        slots = rows + 4 * count * width
+        where = (start + 4 * b0, slot + 4 * b0, seq_past + 4 * b0)
+        _check(l.citlali_cache4_expand(kc, ks, vc, vs, table, table_width, *where, count, window, keys, values, pages, rows, width, slots, 64, nkv,
+                                       head_dim, stream), "cache4_expand")
+        if l.citlali_attention_run_form(q_stride, wide, head_dim, 64, max_new) == 2:
+            _check(l.citlali_attention_prefill_tc(q.data_ptr(), q_stride, q.numel() // q_stride, keys, values, pages, rows, width, where[0], slots,
+                                                  where[2], out_ptr, wide, count, max_new, nq, nkv, head_dim, 64, window, scale, None, stream),
+                   "attention_prefill_tc")
+        else:
+            _check(l.citlali_attention_prefill(q.data_ptr(), q_stride, keys, values, rows, width, where[0], slots, where[2], out_ptr, wide, count,
+                                               max_new, nq, nkv, head_dim, head_dim, 64, window, 0, scale, 0.0, None, 0, None, None, 0, None, stream),
+                   "attention_prefill")
         b0 = b1
-
-
-_run_kernels = (attention_prefill, attention_prefill_tc)        # (as they are here: one who times the calls of this module times the whole)
 
 
 # Counters of the blocks that share a segment, zero between calls.  Calls on one stream follow one another and use the same ones; a call
@@ -656,8 +687,9 @@ def _arrivals_of(device, stream):
 def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
     """:func:`attention` over a cache in 4 bits: every row of the step over its slot's keys up to its own position (the last
     ``window`` of them; 0 or None: all).  bfloat16 with head size 64, 128 or 256 and pages of 64 runs on the tensor cores, anything
-    else in 32-bit arithmetic; longer runs of tokens go over pages that were made bfloat16 first.  A step of single tokens launches nothing that depends on the host's lists of lengths."""
-    kc, ks, vc, vs, table, table_width = _packed4(kv, nkv, head_dim, "cache4_attention")
+    else in 32-bit arithmetic; longer runs of tokens go over pages that were made bfloat16 first.  A step of single tokens launches
+    nothing that depends on the host's lists of lengths."""
+    pools = _packed4(kv, nkv, head_dim, "cache4_attention")
     row_slot, row_pos, seq_start = batch.row_slot, batch.row_pos, batch.seq_start
     rows, wide = row_slot.shape[0], nq * head_dim
     if not (q.dtype is out.dtype and out.dim() == 2 and out.shape[0] >= rows and out.shape[1] == wide and q_stride >= wide
@@ -668,12 +700,22 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
         require(False, "cache4_attention: the queries' rows do not fit")
     if rows == 0:
         return
-    q_ptr, window = q.data_ptr(), _i(window or 0)
-    if not batch.is_decode and _attention4_expands(q, q_stride, out, batch, nq, nkv, head_dim, kv.page_size):
-        _attention4_expanded(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale)
-        return
+    kc, ks, vc, vs, table, table_width = pools
+    q_ptr, window, single = q.data_ptr(), _i(window or 0), batch.is_decode
+    if not single and q.dtype is torch.bfloat16 and kv.page_size == 64 and nkv > 0 and nq % nkv == 0 and (q_ptr | out.data_ptr()) % 16 == 0:
+        key = (nq, nkv, head_dim, window, q_stride)
+        expands = batch.expands4.get(key)
+        if expands is None:
+            form = lib().citlali_attention_run_form(q_stride, wide, head_dim, 64, batch.max_new)
+            if _attention4_floats(nq, nkv, head_dim, 64, batch.max_new, _current_device()) < 0:
+                expands = form > 0 and batch.max_new >= 16           # (else the kernel in 32 bits)
+            else:
+                expands = _attention4_expands(batch, nq, nkv, head_dim, window, form, sm_count(q.device))
+            batch.expands4[key] = expands
+        if expands:
+            _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, float(scale))
+            return
     if q.dtype is torch.bfloat16 and q_stride % 8 == 0 and (q_ptr | kc | ks | vc | vs) % 16 == 0 and nkv > 0 and nq % nkv == 0:
-        single = batch.is_decode
         max_new = 1 if single else batch.max_new
         floats = _attention4_floats(nq, nkv, head_dim, kv.page_size, max_new, _current_device())
         if floats >= 0:

@@ -129,3 +129,15 @@ def test_command_line():
     assert a.cache_dtype == "int4" and a.logprobs == 3
     a = parse_args(["citlali_cli", "--model", "m", "--prompt-ids", "1"])
     assert a.cache_dtype is None and a.logprobs is None
+
+
+def test_which_way_runs_go():
+    """Few new tokens read the codes, prompts go over pages made bfloat16; and in between as measured (see ops._attention4_expands)."""
+    def expands(past, new, nq=16, nkv=8, d=128, window=0, form=2):
+        batch = cb.StepBatch(*[torch.zeros(1, dtype=torch.int32)] * 7, slots=list(range(len(new))), past=past, n_new=new)
+        return ops._attention4_expands(batch, nq, nkv, d, window, form, 148)
+    assert not expands([2000], [8]) and not expands([1952], [96]) and expands([0], [2048]) and not expands([0], [50])
+    assert not expands([2000] * 4, [48] * 4, 40) and expands([1952] * 4, [96] * 4, 40)
+    assert not expands([32704] * 4, [64] * 4, 40) and expands([32672] * 4, [96] * 4, 40)
+    assert not expands([8096], [96], 32, 8, 64, form=1) and not expands([100], [64], form=0)
+    assert not expands([40000], [60], window=128)

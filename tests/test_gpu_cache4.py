@@ -207,6 +207,7 @@ def test_large_and_tiny_numbers_are_held_at_the_ends_of_the_range():
 # ---- attention --------------------------------------------------------------------------------------------------------------
 
 def check_attention(st, nq, dtype, window, seed, out_rows=None, scale=None, expect_nan=None):
+    """By the kernels that read codes."""
     g = torch.Generator().manual_seed(seed)
     nkv, d, group = st.nkv, st.d, nq // st.nkv
     rows = len(st.row_slot)
@@ -214,7 +215,9 @@ def check_attention(st, nq, dtype, window, seed, out_rows=None, scale=None, expe
     pitch = (nq + 2 * nkv) * d
     q = (1.5 * torch.randn(rows, pitch, generator=g)).to(dtype)
     out = torch.full((out_rows or rows, nq * d), 5.0, dtype=dtype, device=DEV)
-    ops.cache4_attention(q.to(DEV), pitch, st.view(), st.batch(), out, nq, nkv, d, window, scale)
+    batch = st.batch()
+    batch.expands4[nq, nkv, d, window, pitch] = False
+    ops.cache4_attention(q.to(DEV), pitch, st.view(), batch, out, nq, nkv, d, window, scale)
     got = out.cpu().double()
     assert (got[rows:] == 5.0).all()
     row = 0
@@ -269,11 +272,11 @@ RUNS = [
     (16, 8, 128, [0], [1 + 16], 0),
     (16, 8, 128, [0, 5, 100], [7, 1, 39], 0),
     (40, 8, 128, [61, 200], [24, 5], 50),
-    (4, 4, 128, [0], [39], 0),
+    (4, 4, 128, [0], [150], 0),
     (8, 1, 64, [33, 0], [20, 3], 16),
     (6, 2, 256, [10], [9], 0),
     (40, 2, 128, [17], [4], 0),
-    (3, 1, 128, [1000, 3], [2, 37], 7),
+    (3, 1, 128, [1000, 3], [2, 70], 7),
 ]
 
 
@@ -512,7 +515,9 @@ def check_long_run(st, nq, window, seed, expect_nan=None):
     q = (1.5 * torch.randn(rows, pitch, generator=g)).bfloat16()
     out = torch.full((rows + 1, nq * d), 5.0, dtype=torch.bfloat16, device=DEV)
     before = ops.launch_count()
-    ops.cache4_attention(q.to(DEV), pitch, st.view(), st.batch(), out, nq, nkv, d, window, scale)
+    batch = st.batch()
+    batch.expands4[nq, nkv, d, window, pitch] = True         # whatever the times say
+    ops.cache4_attention(q.to(DEV), pitch, st.view(), batch, out, nq, nkv, d, window, scale)
     got = out.cpu().double()
     assert (got[rows:] == 5.0).all()
     row = 0
