@@ -409,6 +409,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     float factor[NT][2];                                 // of the columns 2t, 2t + 1
     // m: a running maximum less kWeightBits; the lowest number there is where there is none, which no sum with a score overflows to a NaN
     float m[NT][2], l[NT][4], o[NT][D / 16][4];
+    bool fresh = true;                                   // no unit of the piece has counted yet
     int u = 0, stop = 0, done = 0, pos0 = 0, last = 0, heads = 1, inverse = 256, used = 1;
     uint8_t *at = ring, *free_stage = ring;
 #pragma unroll 1
@@ -438,6 +439,7 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
             u = j.from;
             stop = j.to;
             if (u == stop) break;
+            fresh = true;
             used = j.part.used;
             heads = j.part.heads;
             inverse = j.inverse;
@@ -558,15 +560,18 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                         top = fmaxf(m[n][j], fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) - kWeightBits);
                         const float turn = fa::fast_exp2(m[n][j] - top);
                         m[n][j] = top;
-                        l[n][j] *= turn;
+                        if (!fresh) {                    // (else they are zeros)
+                            l[n][j] *= turn;
 #pragma unroll
-                        for (int i = 0; i < D / 16; ++i) { o[n][i][j] *= turn; o[n][i][j + 2] *= turn; }
+                            for (int i = 0; i < D / 16; ++i) { o[n][i][j] *= turn; o[n][i][j + 2] *= turn; }
+                        }
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
                             for (int i = j; i < 4; i += 2)
                                 if (w[h][n][i] != -INFINITY) w[h][n][i] = fmaf(e[h][n][i], factor[n][j], -top);
                     }
+                fresh = false;
             }
             uint32_t p[2][NT][2];
 #pragma unroll
