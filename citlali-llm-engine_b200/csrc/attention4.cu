@@ -41,7 +41,7 @@ constexpr int kWarps4 = 8, kThreads4 = 32 * kWarps4;
 constexpr float kWeightBits = 11.0f, kMostBits = 15.0f;         // of the largest weight when the maximum is looked for, and before it is again
 constexpr uint32_t kOnes = 0x3c003c00u;
 constexpr float kNoScore = -3.402823466e+38f;
-constexpr int kRoom = 2;                // what beginning a segment costs, in units
+constexpr int kRoom = 4;                // what beginning a segment costs, in units
 
 struct Attention4 {
     const __nv_bfloat16* q;
@@ -824,8 +824,10 @@ extern "C" int citlali_attention4(const void* q, size_t q_stride, const void* k_
                        "128 and 256, pages of 64)", nq, nkv, head_dim, page_size, window);
         return kBadShape;
     }
-    if (q_stride % 8 != 0 || ((uintptr_t)q & 15u) || (((uintptr_t)k_codes | (uintptr_t)k_scales | (uintptr_t)v_codes | (uintptr_t)v_scales) & 15u)) {
-        set_last_error("attention4: query rows, codes and scales must be 16-byte aligned (row pitch %zu elements)", q_stride);
+    if (q_stride % 8 != 0 || out_stride % 2 != 0 || ((uintptr_t)out & 3u) ||
+        (((uintptr_t)q | (uintptr_t)k_codes | (uintptr_t)k_scales | (uintptr_t)v_codes | (uintptr_t)v_scales | (uintptr_t)partial) & 15u)) {
+        set_last_error("attention4: query rows, codes, scales and scratch must be 16-byte aligned, rows of results 4-byte (pitches of %zu and "
+                       "%zu elements)", q_stride, out_stride);
         return kBadAlignment;
     }
     const c4::Tiling t = c4::tiling(nq / nkv, head_dim, max_new);
