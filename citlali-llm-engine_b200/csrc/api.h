@@ -185,9 +185,9 @@ int citlali_cache4_append(const void* qkv, int dtype, void* q_out, size_t q_out_
                           cudaStream_t stream);
 // keys[r], values[r] [nkv, head_dim] (out_dtype) = what the cache holds for position positions[r] of slot slots[r].
 int citlali_cache4_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
-                        const int32_t* page_table, int page_table_stride, int page_size, const int32_t* slots,
-                        const int32_t* positions, void* keys, void* values, int out_dtype, int rows, int nkv, int head_dim,
-                        cudaStream_t stream);
+                        const int32_t* page_table, int page_table_rows, int page_table_stride, int page_size, int pages,
+                        const int32_t* slots, const int32_t* positions, void* keys, void* values, int out_dtype, int rows, int nkv,
+                        int head_dim, cudaStream_t stream);
 // The pages of 64 that runs of new tokens see (from the pair with past - window + 1 on, if there is a window), as bfloat16: page after page of the
 // sequences [pages, nkv, 64, head_dim], zeros where no row sees anything; table_out [sequences, table_out_stride] and slots_out
 // [sequences] are the page table and slots under which the attention kernels of a cache of 16 bits find them.  pages: of all sequences.

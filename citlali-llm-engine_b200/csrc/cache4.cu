@@ -228,11 +228,12 @@ append_any_kernel(const T* __restrict__ qkv, T* q_out, size_t q_out_stride, cons
     }
 }
 
-// keys[r, h, :], values[r, h, :] = what the cache holds for position positions[r] of slot slots[r].  A thread a group.
+// keys[r, h, :], values[r, h, :] = what the cache holds for position positions[r] of slot slots[r]; NaN where there is no such slot,
+// position or page.  A thread a group.
 template <typename TO>
 __global__ void __launch_bounds__(kThreads)
 read_kernel(const __grid_constant__ Rows rows, const __grid_constant__ Pools pools, TO* __restrict__ keys, TO* __restrict__ values,
-            long long groups, int nkv, int d) {
+            long long groups, int slots, int pages, int nkv, int d) {
     dependents_may_launch();
     wait_for_predecessor();
     const int per_head = d / kGroup;
@@ -241,11 +242,16 @@ read_kernel(const __grid_constant__ Rows rows, const __grid_constant__ Pools poo
     const bool is_v = blockIdx.y != 0;
     const int g = (int)(i % per_head), head = (int)(i / per_head % nkv);
     const long long row = i / ((long long)per_head * nkv);
-    const int pos = rows.row_pos[row];
-    const int page = rows.page_table[(size_t)rows.row_slot[row] * rows.page_table_stride + pos / rows.page_size];
-    const size_t at = place(page, nkv, head, rows.page_size, pos % rows.page_size);
-    const uint2 w = *reinterpret_cast<const uint2*>((is_v ? pools.v_codes : pools.k_codes) + at * (d / 2) + g * 8);
-    const float s = scale_of((is_v ? pools.v_scales : pools.k_scales)[at * per_head + g]);
+    const int pos = rows.row_pos[row], slot = rows.row_slot[row], index = pos / rows.page_size;
+    const bool named = slot >= 0 && slot < slots && pos >= 0 && index < rows.page_table_stride;
+    const int page = named ? rows.page_table[(size_t)slot * rows.page_table_stride + index] : -1;
+    uint2 w = make_uint2(0, 0);
+    float s = __int_as_float(0x7fc00000);
+    if (page >= 0 && page < pages) {
+        const size_t at = place(page, nkv, head, rows.page_size, pos % rows.page_size);
+        w = *reinterpret_cast<const uint2*>((is_v ? pools.v_codes : pools.k_codes) + at * (d / 2) + g * 8);
+        s = scale_of((is_v ? pools.v_scales : pools.k_scales)[at * per_head + g]);
+    }
     TO* out = (is_v ? values : keys) + ((size_t)row * nkv + head) * d + g * kGroup;
     store_values(out, w.x, s);
     store_values(out + 8, w.y, s);
@@ -398,9 +404,9 @@ extern "C" int citlali_cache4_append(const void* qkv, int dtype, void* q_out, si
 }
 
 extern "C" int citlali_cache4_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
-                                   const int32_t* page_table, int page_table_stride, int page_size, const int32_t* slots,
-                                   const int32_t* positions, void* keys, void* values, int out_dtype, int rows, int nkv, int head_dim,
-                                   cudaStream_t stream) {
+                                   const int32_t* page_table, int page_table_rows, int page_table_stride, int page_size, int pages,
+                                   const int32_t* slots, const int32_t* positions, void* keys, void* values, int out_dtype, int rows,
+                                   int nkv, int head_dim, cudaStream_t stream) {
     if (rows <= 0) return 0;
     if (int bad = c4::check_sizes("cache4_read", nkv, head_dim, page_size)) return bad;
     if (!c4::aligned(k_codes, 8) || !c4::aligned(v_codes, 8) || !c4::aligned(keys, 16) || !c4::aligned(values, 16)) {
@@ -416,7 +422,7 @@ extern "C" int citlali_cache4_read(const void* k_codes, const void* k_scales, co
     const c4::Pools pools = {(uint8_t*)k_codes, (uint8_t*)k_scales, (uint8_t*)v_codes, (uint8_t*)v_scales};
     return CITLALI_DISPATCH_FLOAT(out_dtype, TO, [&]() {
         launch_kernel(c4::read_kernel<TO>, dim3((unsigned)blocks, 2), c4::kThreads, 0, stream, where, pools, (TO*)keys, (TO*)values, groups,
-                      nkv, head_dim);
+                      page_table_rows, pages, nkv, head_dim);
         return CITLALI_LAUNCH_CHECK();
     });
 }

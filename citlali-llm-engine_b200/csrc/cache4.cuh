@@ -75,8 +75,6 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
 __device__ __forceinline__ float scale_of(uint32_t byte) {
     return __half2float(__ushort_as_half((unsigned short)(byte << 7))) * kUnit;
 }
-// The value of nibble i of a word of eight codes.
-__device__ __forceinline__ float value_of(uint32_t word, int i, float s) { return (float)((int)((word >> (4 * i)) & 15u) - 8) * s; }
 
 // A word's eight values in bfloat16, two a word, in order.  (w & 0x000f000f) | 0x4300 is 136 + c there, and (136 + c) s - 136 s is
 // exact: s has four significant bits, 136 s eight at most.

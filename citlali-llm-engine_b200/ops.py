@@ -554,9 +554,9 @@ def cache4_append(qkv, kv, row_slot, row_pos, nq: int, nkv: int, head_dim: int, 
 
 def cache4_read(kv, slots, positions, dtype=torch.bfloat16):
     """What a cache in 4 bits holds: (keys, values) [rows, kv heads, head size] in ``dtype`` (bfloat16 holds the values exactly) for
-    ``positions[r]`` (int32) of slot ``slots[r]``."""
+    ``positions[r]`` (int32) of slot ``slots[r]``; NaN where the page table has no such slot or position, or names no page."""
     require(isinstance(kv.keys, Packed4), "cache4_read: the cache does not hold its keys and values in 4 bits")
-    _, nkv, _, width = kv.keys.codes.shape
+    pages, nkv, _, width = kv.keys.codes.shape
     pools = _packed4(kv, nkv, 2 * width, "cache4_read")
     rows = slots.numel()
     if not (slots.dtype is torch.int32 and positions.dtype is torch.int32 and positions.numel() == rows and _are_here(slots, positions)):
@@ -568,8 +568,9 @@ def cache4_read(kv, slots, positions, dtype=torch.bfloat16):
     keys, values = held.unbind(0)
     if rows:
         kc, ks, vc, vs, table, table_width = pools
-        _check(lib().citlali_cache4_read(kc, ks, vc, vs, table, table_width, _i(kv.page_size), slots.data_ptr(), positions.data_ptr(),
-                                         keys.data_ptr(), values.data_ptr(), _dtype_code(held), rows, nkv, 2 * width, _stream()), "cache4_read")
+        _check(lib().citlali_cache4_read(kc, ks, vc, vs, table, kv.page_table.shape[0], table_width, _i(kv.page_size), pages, slots.data_ptr(),
+                                         positions.data_ptr(), keys.data_ptr(), values.data_ptr(), _dtype_code(held), rows, nkv, 2 * width,
+                                         _stream()), "cache4_read")
     return keys, values
 
 

@@ -172,6 +172,22 @@ def test_append_without_storing_and_other_row_pitches():
     assert torch.equal(kv.keys.codes, before)
 
 
+def test_reading_what_is_not_there():
+    st = Step([70, 3], [1, 1], 2, 64, slots=4)
+    st.fill(3)
+    view = st.view()
+    view.page_table[st.slots[1], 1] = -1                 # names no page
+    view.page_table[st.slots[1], 0] = view.keys.codes.shape[0]
+    a, b, wide = st.slots[0], st.slots[1], view.page_table.shape[1] * 64
+    slots = [a, a, a, -1, 4, 2 ** 31 - 1, b, b, a, a]
+    positions = [0, -1, wide, 5, 5, 5, 64, 0, 2 ** 31 - 1, 70]
+    for dtype in (torch.bfloat16, torch.float32):
+        read = ops.cache4_read(view, *on_device(torch.tensor(slots, dtype=torch.int32), torch.tensor(positions, dtype=torch.int32)), dtype=dtype)
+        for part, have in zip((st.keys, st.values), read):
+            want = plain.gathered(part, st.table, a, 71, 64)
+            assert torch.equal(have[[0, 9]].cpu().double(), want[[0, 70]]) and have[1:9].isnan().all()
+
+
 def test_what_is_not_finite_stays_in_its_group():
     st = Step([0], [4], 1, 64)
     qkv = torch.zeros(4, 3 * 64)
