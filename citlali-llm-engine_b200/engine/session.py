@@ -285,11 +285,11 @@ class InferenceSession:
         stops = options.stop_ids if options.stop_ids is not None else self.model.spec.stop_token_ids
         batch = min(options.max_batch or self.max_batch, self.max_batch)
         self.stats = {}
-        self._alternatives = options.logprobs
+        before, self._alternatives = (self._alternatives, self.details), options.logprobs      # (on_token may generate something else)
         try:
             results = run_generation(self, prompts, opts, stops, batch, on_token)
         finally:
-            self._alternatives = self.details = None
+            self._alternatives, self.details = before
         self.check_device_errors()
         return results
 

@@ -510,8 +510,8 @@ def cache4_append(qkv, kv, row_slot, row_pos, nq: int, nkv: int, head_dim: int, 
     """:func:`qk_norm_rope_cache` for a cache in 4 bits (``kv``: its view, keys and values :class:`~.cache.Packed4`).  Of the rows
     ``qkv`` [rows, (nq + 2 nkv) head_dim] = [q | k | v], q and k heads get their norm (gains None: none) and the rotation of their
     first ``rotary_dim`` elements in pairs (i, i + rotary_dim / 2); queries go to ``q_out`` [rows, nq head_dim] (None: back into the
-    rows), keys and values into the page of each row's slot and position.  ``store`` False: the queries only.  The angles are the
-    products of position and frequency to more than 32 bits."""
+    rows), keys and values into the page of each row's slot and position (a place that two rows name holds a mixture of both).
+    ``store`` False: the queries only.  The angles are the products of position and frequency to more than 32 bits."""
     rows, width = qkv.shape
     wide = nq * head_dim
     if not (nq >= 0 and nkv >= 0 and width == wide + 2 * nkv * head_dim and rotary_dim % 2 == 0 and 0 <= rotary_dim <= head_dim
@@ -542,6 +542,10 @@ def cache4_append(qkv, kv, row_slot, row_pos, nq: int, nkv: int, head_dim: int, 
             require(False, "cache4_append: q_out is [rows, query heads * head size] of the rows' dtype and device, its rows apart")
         if rows <= 1:
             q_stride = wide
+        size, here = qkv.element_size(), qkv.data_ptr()
+        if (rows and q_ptr < here + rows * width * size and here < q_ptr + ((rows - 1) * q_stride + wide) * size
+                and not (q_ptr == here and (rows == 1 or q_stride == width))):
+            require(False, "cache4_append: q_out lies over the rows, but not over their queries")
     if rows == 0 or (nq == 0 and not store):
         return
     gain = q_gain if q_gain is not None else k_gain
@@ -647,7 +651,7 @@ def _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, 
         _check(l.citlali_cache4_expand(kc, ks, vc, vs, table, table_width, *where, count, window, keys, values, pages, rows, width, slots, 64, nkv,
                                        head_dim, stream), "cache4_expand")
         if l.citlali_attention_run_form(q_stride, wide, head_dim, 64, max_new) == 2:
-            _check(l.citlali_attention_prefill_tc(q.data_ptr(), q_stride, q.numel() // q_stride, keys, values, pages, rows, width, where[0], slots,
+            _check(l.citlali_attention_prefill_tc(q.data_ptr(), q_stride, batch.row_slot.shape[0], keys, values, pages, rows, width, where[0], slots,
                                                   where[2], out_ptr, wide, count, max_new, nq, nkv, head_dim, 64, window, scale, None, stream),
                    "attention_prefill_tc")
         else:
@@ -694,10 +698,12 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
     row_slot, row_pos, seq_start = batch.row_slot, batch.row_pos, batch.seq_start
     rows, wide = row_slot.shape[0], nq * head_dim
     if not (q.dtype is out.dtype and out.dim() == 2 and out.shape[0] >= rows and out.shape[1] == wide and q_stride >= wide
-            and q.numel() >= (rows - 1) * q_stride + wide and _are_here(q, out, row_slot, row_pos, seq_start, batch.seq_slot, batch.seq_past)):
+            and q.numel() >= (rows - 1) * q_stride + wide and not (batch.is_decode and len(batch.slots) > rows)
+            and _are_here(q, out, row_slot, row_pos, seq_start, batch.seq_slot, batch.seq_past)):
         _here("cache4_attention", q, out, row_slot, row_pos, seq_start, batch.seq_slot, batch.seq_past)
         require(q.dtype == out.dtype and out.dim() == 2 and out.shape[0] >= rows and out.shape[1] == wide,
                 "cache4_attention: the result is [rows, query heads * head size] of the queries' dtype")
+        require(not batch.is_decode or len(batch.slots) <= rows, "cache4_attention: a step of single tokens has a row for every sequence")
         require(False, "cache4_attention: the queries' rows do not fit")
     if rows == 0:
         return

@@ -504,6 +504,13 @@ def test_refusals():
         ops.cache4_append(q, kv, batch.row_slot[:1], batch.row_pos, 4, 2, 64, f, 64)
     with pytest.raises(cb.CitlaliError, match="q_out"):
         ops.cache4_append(q, kv, batch.row_slot, batch.row_pos, 4, 2, 64, f, 64, q_out=out[:1])
+    for over in (q[:, 64:320], torch.as_strided(q, (2, 256), (640, 1)), torch.as_strided(q, (2, 256), (256, 1))):
+        with pytest.raises(cb.CitlaliError, match="not over their queries"):
+            ops.cache4_append(q, kv, batch.row_slot, batch.row_pos, 4, 2, 64, f, 64, q_out=over)
+    with pytest.raises(cb.CitlaliError, match="a row for every sequence"):
+        many = Step([10, 3, 4], [1, 1, 1], 2, 64).batch()
+        many.row_slot, many.row_pos = batch.row_slot, batch.row_pos
+        ops.cache4_attention(q, 512, kv, many, out, 4, 2, 64, 0, 0.1)
     with pytest.raises(cb.CitlaliError, match="contiguous"):
         ops.cache4_append(q[:, ::2], kv, batch.row_slot, batch.row_pos, 2, 1, 64, f, 64)
     with pytest.raises(cb.CitlaliError, match="bfloat16 or float32"):
@@ -568,6 +575,35 @@ def test_a_token_that_is_not_finite_in_a_longer_run(d, which, window):
     part = getattr(st, which)
     part.scales[int(st.table[slot, at // 64]), :, at % 64] = 255
     check_long_run(st, 2, window, 2, expect_nan=lambda s, p: s == slot and p >= at and (not window or p < at + window))
+
+
+@pytest.mark.parametrize("expands", [False, True])
+def test_queries_that_end_with_their_last_row(expands):
+    """Rows of a wider projection, and nothing behind the last row's queries."""
+    st = Step([40, 0], [60, 30], 2, 128, seed=8)
+    st.fill(8)
+    rows, wide, pitch = 90, 4 * 128, 8 * 128
+    q = torch.randn(rows, pitch, generator=torch.Generator().manual_seed(2)).bfloat16().to(DEV)
+    made = []
+    for given in (q, q.flatten()[:(rows - 1) * pitch + wide].clone()):
+        batch, out = st.batch(), torch.full((rows, wide), 5.0, dtype=torch.bfloat16, device=DEV)
+        batch.expands4[4, 2, 128, 0, pitch] = expands
+        ops.cache4_attention(given, pitch, st.view(), batch, out, 4, 2, 128, 0, 0.1)
+        made.append(out)
+    assert torch.equal(made[0], made[1])
+
+
+def test_queries_over_the_rows_themselves():
+    st = Step([5, 0], [1, 1], 2, 64, seed=3)
+    s, p = on_device(torch.tensor(st.row_slot, dtype=torch.int32), torch.tensor(st.row_pos, dtype=torch.int32))
+    made = []
+    for how in (lambda x: None, lambda x: x[:, :256], lambda x: torch.empty(2, 256, dtype=x.dtype, device=DEV)):
+        qkv, view = torch.randn(2, 512, generator=torch.Generator().manual_seed(4)).bfloat16().to(DEV), st.view()
+        q_out = how(qkv)
+        ops.cache4_append(qkv, view, s, p, 4, 2, 64, freqs(64).to(DEV), 64, q_out=q_out)
+        made.append((qkv[:, :256] if q_out is None else q_out, view.keys.codes, view.values.codes))
+    for other in made[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(made[0], other))
 
 
 def test_longer_runs_a_few_sequences_at_a_time(monkeypatch):

@@ -10,7 +10,11 @@ import torch
 import citlali_b200 as cb
 import plain_cache4
 import plain_qwen3 as plain
+from citlali_b200 import ops
+from citlali_b200.engine.step import pack_step
+from citlali_b200.parts.base import part_class
 from helpers import random_tokens, tiny_config
+from test_gpu_parts import DEV, InterleavedRotary, close, handles, plain_interleaved_rotary, tol
 
 pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -126,6 +130,80 @@ def test_generation_says_what_scoring_says(model_dirs, dtype, cache_dtype, tempe
             assert s.alternatives[len(p) - 1:] == r.alternatives
     assert session.cache.slots.free_count == 3
     assert session.details is None
+
+
+def test_a_generation_within_a_generation(model_dirs):
+    session = cb.InferenceSession().load_model(model_dirs[("A", "float32")], max_context=64, dtype="float32", max_batch=2)
+    options = cb.GenerationOptions(max_new_tokens=4, max_context=64, stop_ids=[], logprobs=2)
+    prompt = random_tokens(512, 5, 1)
+    [alone] = session.generate([prompt], options)
+
+    def another(request, token):
+        session.generate([[3, 1]], cb.GenerationOptions(max_new_tokens=1, max_context=64, stop_ids=[]))
+        session.score([[3, 1, 2]])
+    [within] = session.generate([prompt], options, on_token=another)
+    assert (within.tokens, within.logprobs, within.alternatives) == (alone.tokens, alone.logprobs, alone.alternatives)
+    assert len(alone.logprobs) == 4 and session.details is None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [48, 64])
+@pytest.mark.parametrize("variant", ["plain", "window", "no_norm_no_rotation", "position_with_apply", "reader"])
+def test_a_layer_whatever_its_position_encoding(dtype, d, variant):
+    """The layer alone: what it caches lies within its groups' steps of the plain keys and values, and its rows are the plain
+    attention's over what it cached.  ``reader``: a second layer without keys reads the first one's."""
+    params = {"hidden_size": 40, "num_heads": 6, "num_kv_heads": 2, "head_dim": d, "qk_norm_eps": 1e-5, "window": None,
+              "position": {"kind": "rotary_half_split", "theta": 3e4, "rotary_dim": d}}
+    norms, rotate = True, True
+    if variant == "window":
+        params["window"] = 9
+    if variant == "no_norm_no_rotation":
+        params.update(qk_norm_eps=None, position={"kind": "none"})
+        norms = rotate = False
+    if variant == "position_with_apply":
+        cb.register_part("position", "interleaved_rotary", InterleavedRotary, replace=True)
+        params["position"] = {"kind": "interleaved_rotary", "theta": 3e4}
+        rotate = "interleaved"
+    ctx = cb.BuildContext(DEV, dtype, torch.zeros(4, dtype=torch.int32, device=DEV), packed4=True)
+    attn = part_class("mixer", "gqa_attention")(params, "a")
+    h, w = handles(attn, dtype, gain_spread=0.5)
+    attn.bind(h, ctx)
+    parts = [attn]
+    if variant == "reader":
+        parts.append(part_class("mixer", "gqa_attention")(dict(params, kv_projection=False), "a"))
+        parts[1].bind(h, ctx)
+    cache = cb.SequenceCache([attn.cache_requirement()], 2, 64 * 6, 64 * 3, dtype, DEV)
+    T, nq, nkv = 75, 6, 2
+    x = torch.randn(T, 40, generator=torch.Generator().manual_seed(d)).to(dtype)
+    project = lambda name, n: plain.linear(x.double(), w[f"a.{name}_proj.weight"]).view(T, n, d)
+    q, k, v = project("q", nq), project("k", nkv), project("v", nkv)
+    if norms:
+        q, k = (plain.head_rms_norm(y, w[f"a.{n}_norm.weight"], 1e-5) for y, n in ((q, "q"), (k, "k")))
+    if rotate:
+        turn = plain_interleaved_rotary if rotate == "interleaved" else plain.rotary_half_split
+        q, k = (turn(y, list(range(T)), 3e4) for y in (q, k))
+    other = cache.acquire()
+    for pieces in ([(0, T)], [(0, 40)] + [(t, t + 1) for t in range(40, T)]):
+        slot, made, held = cache.acquire(), [[] for _ in parts], []
+        for lo, hi in pieces:
+            batch = pack_step([cb.StepEntry(slot, [0] * (hi - lo), [])], [cache.length(slot)], 10, DEV)
+            cache.reserve(slot, hi)
+            for part, rows in zip(parts, made):
+                rows.append(part.forward(x[lo:hi].to(DEV).contiguous(), batch, cache.view(0), torch.zeros(hi - lo, 40, device=DEV)))
+            held.append([y.cpu().double() for y in ops.cache4_read(cache.view(0), batch.row_slot, batch.row_pos, dtype=torch.float32)])
+            cache.commit(slot, hi)
+        cache.release(slot)
+        keys, values = (torch.cat(y) for y in zip(*held))
+        for have, want in ((keys, k), (values, v)):
+            # half a step, at most (1 + 2^-4) most / 14, or what a scale rounded down cuts off the largest, 2^-4 of it: below 0.08 most;
+            # and the paths' own roundings, as for the other layers' tests
+            most = want.unflatten(-1, (-1, 16)).abs().amax(-1, keepdim=True).expand(T, nkv, d // 16, 16).flatten(-2)
+            assert ((have - want).abs() <= 0.08 * most + tol(dtype) * float(want.abs().max())).all()
+        rows = plain.causal_attention(q, keys, values, nq, nkv, window=params["window"]).reshape(T, nq * d)
+        want = plain.linear(rows, w["a.o_proj.weight"])
+        for part_rows in made:
+            close(torch.cat(part_rows), want, dtype)
+    cache.release(other)
 
 
 def test_scoring_follows_the_plain_model(model_dirs):
