@@ -297,19 +297,18 @@ def token_logprobs(logits, tokens=None, top: int = 0) -> dict:
         require(False, f"token_logprobs: {top} alternatives of {vocab} entries (at most 32)")
     if tokens is not None and not (tokens.dtype is torch.int32 and tokens.numel() == rows):
         require(False, "token_logprobs: tokens are int32, one a row")
-    floats = logits.new_empty((2 + top) * rows, dtype=torch.float32)
-    logprobs, entropy, top_logprobs = floats.split((rows, rows, top * rows))
-    found = {"entropy": entropy}
+    # (a tensor each: views of one piece of memory cost the host more than allocations do)
+    f32 = torch.float32
+    entropy = logits.new_empty(rows, dtype=f32)
+    found, logprobs, ids, beside = {"entropy": entropy}, None, None, None
     if tokens is not None:
-        found["logprobs"] = logprobs
-    ids = None
+        logprobs = found["logprobs"] = logits.new_empty(rows, dtype=f32)
     if top:
-        ids = found["top_ids"] = logits.new_empty((rows, top), dtype=torch.int32)
-        found["top_logprobs"] = top_logprobs.view(rows, top)
+        ids = found["top_ids"] = logits.new_empty(rows, top, dtype=torch.int32)
+        beside = found["top_logprobs"] = logits.new_empty(rows, top, dtype=f32)
     if rows:
-        at = floats.data_ptr()
-        _check(lib().citlali_token_logprobs(logits.data_ptr(), _dtype_code(logits), _ptr(tokens), at, at + 4 * rows, _ptr(ids), at + 8 * rows, rows,
-                                            vocab, top, _stream()), "token_logprobs")
+        _check(lib().citlali_token_logprobs(logits.data_ptr(), _dtype_code(logits), _ptr(tokens), _ptr(logprobs), entropy.data_ptr(), _ptr(ids),
+                                            _ptr(beside), rows, vocab, top, _stream()), "token_logprobs")
     return found
 
 
@@ -496,10 +495,12 @@ def _packed4(kv, nkv: int, head_dim: int, what: str):
     keys, values, table = kv.keys, kv.values, kv.page_table
     if type(keys) is Packed4 and type(values) is Packed4 and head_dim % 16 == 0 and 16 <= head_dim <= 256:
         kc, ks, vc, vs = keys.codes, keys.scales, values.codes, values.scales
-        codes, scales, row, u8 = kc.shape, ks.shape, table.shape, torch.uint8
-        if (len(row) == 2 and codes[1:] == (nkv, kv.page_size, head_dim // 2) and scales == (codes[0], nkv, kv.page_size, head_dim // 16)
-                and vc.shape == codes and vs.shape == scales and kc.dtype is u8 and ks.dtype is u8 and vc.dtype is u8 and vs.dtype is u8
-                and table.dtype is torch.int32 and _are_here(kc, ks, vc, vs, table)):
+        codes, row, u8, size = kc.shape, table.shape, torch.uint8, kv.page_size
+        pages = codes[0] if codes else 0
+        scales = (pages, nkv, size, head_dim // 16)
+        if (len(row) == 2 and codes == (pages, nkv, size, head_dim // 2) and vc.shape == codes and ks.shape == scales and vs.shape == scales
+                and kc.dtype is u8 and ks.dtype is u8 and vc.dtype is u8 and vs.dtype is u8 and table.dtype is torch.int32
+                and _are_here(kc, ks, vc, vs, table)):
             return kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), table.data_ptr(), row[1]
     _check_packed4(kv, nkv, head_dim, what)
     raise CitlaliError(f"{what}: the cache's view does not fit")
@@ -568,12 +569,12 @@ def cache4_read(kv, slots, positions, dtype=torch.bfloat16):
         require(False, "cache4_read: slots and positions are int32, one a row")
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         require(False, f"cache4_read: values come in bfloat16 or float32, not {dtype}")
-    held = slots.new_empty((2, rows, nkv, 2 * width), dtype=dtype)
-    keys, values = held.unbind(0)
+    keys = slots.new_empty(rows, nkv, 2 * width, dtype=dtype)
+    values = slots.new_empty(rows, nkv, 2 * width, dtype=dtype)
     if rows:
         kc, ks, vc, vs, table, table_width = pools
         _check(lib().citlali_cache4_read(kc, ks, vc, vs, table, kv.page_table.shape[0], table_width, _i(kv.page_size), pages, slots.data_ptr(),
-                                         positions.data_ptr(), keys.data_ptr(), values.data_ptr(), _dtype_code(held), rows, nkv, 2 * width,
+                                         positions.data_ptr(), keys.data_ptr(), values.data_ptr(), _dtype_code(keys), rows, nkv, 2 * width,
                                          _stream()), "cache4_read")
     return keys, values
 
@@ -695,20 +696,20 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
     else in 32-bit arithmetic; longer runs of tokens go over pages that were made bfloat16 first.  A step of single tokens launches
     nothing that depends on the host's lists of lengths."""
     pools = _packed4(kv, nkv, head_dim, "cache4_attention")
-    row_slot, row_pos, seq_start = batch.row_slot, batch.row_pos, batch.seq_start
+    row_slot, row_pos, seq_start, single = batch.row_slot, batch.row_pos, batch.seq_start, batch.is_decode
     rows, wide = row_slot.shape[0], nq * head_dim
     if not (q.dtype is out.dtype and out.dim() == 2 and out.shape[0] >= rows and out.shape[1] == wide and q_stride >= wide
-            and q.numel() >= (rows - 1) * q_stride + wide and not (batch.is_decode and len(batch.slots) > rows)
+            and q.numel() >= (rows - 1) * q_stride + wide and not (single and len(batch.slots) > rows)
             and _are_here(q, out, row_slot, row_pos, seq_start, batch.seq_slot, batch.seq_past)):
         _here("cache4_attention", q, out, row_slot, row_pos, seq_start, batch.seq_slot, batch.seq_past)
         require(q.dtype == out.dtype and out.dim() == 2 and out.shape[0] >= rows and out.shape[1] == wide,
                 "cache4_attention: the result is [rows, query heads * head size] of the queries' dtype")
-        require(not batch.is_decode or len(batch.slots) <= rows, "cache4_attention: a step of single tokens has a row for every sequence")
+        require(not single or len(batch.slots) <= rows, "cache4_attention: a step of single tokens has a row for every sequence")
         require(False, "cache4_attention: the queries' rows do not fit")
     if rows == 0:
         return
     kc, ks, vc, vs, table, table_width = pools
-    q_ptr, window, single = q.data_ptr(), _i(window or 0), batch.is_decode
+    q_ptr, window = q.data_ptr(), _i(window or 0)
     if not single and q.dtype is torch.bfloat16 and kv.page_size == 64 and nkv > 0 and nq % nkv == 0 and (q_ptr | out.data_ptr()) % 16 == 0:
         key = (nq, nkv, head_dim, window, q_stride)
         expands = batch.expands4.get(key)
