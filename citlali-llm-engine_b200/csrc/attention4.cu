@@ -159,36 +159,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
-__device__ __forceinline__ uint32_t as_word(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
-
-// A scale (or two keys' scales) as the conversion needs it.
-struct Scale {
-    __half2 s, low, high;                                // s, -1032 s, -72 s
-    __device__ __forceinline__ explicit Scale(uint32_t two_bytes) {      // bytes 0 and 2
-        s = as_half2(two_bytes << 7);
-        low = __hmul2(s, __float2half2_rn(-1032.0f));
-        high = __hmul2(s, __float2half2_rn(-72.0f));
-    }
-};
-// (w & mask) | bits in one instruction: written in C it becomes two, since only one of two constants fits an instruction.
-template <uint32_t kMask>
-__device__ __forceinline__ __half2 picked(uint32_t w, uint32_t bits) {
-    uint32_t x;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "n"(kMask), "r"(bits));
-    return as_half2(x);
-}
-// Nibbles 0 and 4 (first), 1 and 5 (second) of a word times the scale.  The two constants stay in registers.
-struct Words {
-    uint32_t low, high;
-    __device__ __forceinline__ Words() {
-        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(low));
-        asm volatile("mov.b32 %0, 0x54005400;" : "=r"(high));
-    }
-    __device__ __forceinline__ uint32_t first_of(uint32_t w, const Scale& k) const { return as_word(__hfma2(picked<0x000f000fu>(w, low), k.s, k.low)); }
-    __device__ __forceinline__ uint32_t second_of(uint32_t w, const Scale& k) const { return as_word(__hfma2(picked<0x00f000f0u>(w, high), k.s, k.high)); }
-};
-
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
     if constexpr (N == 1) {

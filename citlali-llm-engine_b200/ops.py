@@ -624,11 +624,41 @@ def _attention4_expands(batch, nq: int, nkv: int, head_dim: int, window: int, fo
     return 9 + codes * unit > 14 + walked * tile + pages * nkv * 64 * head_dim * 4 / 2.3e6
 
 
+def _attention4_tiles(batch, nkv: int, window: int, tokens: int, sms: int):
+    """The tiles of ``tokens`` new tokens of a step's runs, over all key/value heads, and how many blocks share the pages of one: twice as
+    many while a block of the longest has more to do than an even share of all on two blocks a multiprocessor, and eight pages."""
+    tiles = steps = longest = 0
+    for past, n in zip(batch.past, batch.n_new):
+        here = -(-n // tokens)
+        if here:
+            ends = [(past + first + min(tokens, n - first) - 1) // 64 - (max(0, past + first - window + 1) // 64 if window else 0) + 1
+                    for first in (0, (here - 1) * tokens)]           # pages of the first tile and of the last
+            tiles += here
+            longest = max(longest, *ends)
+            steps += here * sum(ends) / 2
+    cluster = 1
+    while cluster < 8 and -(-longest // cluster) > max(8, steps * nkv / (2 * sms)):
+        cluster *= 2
+    return tiles * nkv, cluster
+
+
+def _attention4_way(batch, nq: int, nkv: int, head_dim: int, window: int, q_stride: int, sms: int) -> tuple:
+    """How a step's runs of tokens are attended to: ("tiles", tiles, blocks of a tile) by the kernel on tcgen05, ("pages",) over pages
+    that are made bfloat16 first, or ("codes",) by the kernel for single tokens, or that in 32 bits."""
+    max_new, tokens = batch.max_new, lib().citlali_attention4_runs_tokens(nq, nkv, head_dim, 64)
+    if tokens and nq // nkv * max_new > 8:
+        return ("tiles",) + _attention4_tiles(batch, nkv, window, tokens, sms)
+    form = lib().citlali_attention_run_form(q_stride, nq * head_dim, head_dim, 64, max_new)
+    if _attention4_floats(nq, nkv, head_dim, 64, max_new, _current_device()) < 0:
+        expands = form > 0 and max_new >= 16                         # (else the kernel in 32 bits)
+    else:
+        expands = _attention4_expands(batch, nq, nkv, head_dim, window, form, sms)
+    return ("pages",) if expands else ("codes",)
+
+
 def _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, scale):
     """The pages that the rows see as bfloat16 (the values are exact there), then prompt attention over them: as many sequences at a
     time as a gigabyte holds, at least one."""
-    require(not torch.cuda.is_current_stream_capturing(), "cache4_attention: runs of tokens are sized from the host's lists of lengths, "
-            "which a captured step would freeze")
     kc, ks, vc, vs, table, table_width = pools
     l, stream, page_bytes = lib(), _stream(), nkv * 64 * head_dim * 2
     past, n_new = batch.past, batch.n_new
@@ -710,18 +740,20 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
         return
     kc, ks, vc, vs, table, table_width = pools
     q_ptr, window = q.data_ptr(), _i(window or 0)
-    if not single and q.dtype is torch.bfloat16 and kv.page_size == 64 and nkv > 0 and nq % nkv == 0 and (q_ptr | out.data_ptr()) % 16 == 0:
+    # (runs by the host's lists of lengths, which a captured step would freeze: there the kernel for single tokens reads the device's)
+    if (not single and not torch._C._cuda_isCurrentStreamCapturing() and q.dtype is torch.bfloat16 and kv.page_size == 64 and nkv > 0 and nq % nkv == 0
+            and (q_ptr | out.data_ptr() | kc | ks | vc | vs) % 16 == 0 and (q_stride | wide) % 8 == 0):
         key = (nq, nkv, head_dim, window, q_stride)
-        expands = batch.expands4.get(key)
-        if expands is None:
-            form = lib().citlali_attention_run_form(q_stride, wide, head_dim, 64, batch.max_new)
-            if _attention4_floats(nq, nkv, head_dim, 64, batch.max_new, _current_device()) < 0:
-                expands = form > 0 and batch.max_new >= 16           # (else the kernel in 32 bits)
-            else:
-                expands = _attention4_expands(batch, nq, nkv, head_dim, window, form, sm_count(q.device))
-            batch.expands4[key] = expands
-        if expands:
+        way = batch.runs4.get(key)
+        if way is None:
+            way = batch.runs4[key] = _attention4_way(batch, nq, nkv, head_dim, window, q_stride, sm_count(q.device))
+        if way[0] == "pages":
             _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, float(scale))
+            return
+        if way[0] == "tiles":
+            _check(lib().citlali_attention4_runs(
+                q_ptr, _sz(q_stride), kc, ks, vc, vs, table, table_width, seq_start.data_ptr(), batch.seq_slot.data_ptr(), batch.seq_past.data_ptr(),
+                out.data_ptr(), wide, len(batch.slots), way[1], way[2], nq, nkv, head_dim, 64, window, _f(scale), _stream()), "cache4_attention_runs")
             return
     if q.dtype is torch.bfloat16 and q_stride % 8 == 0 and (q_ptr | kc | ks | vc | vs) % 16 == 0 and nkv > 0 and nq % nkv == 0:
         max_new = 1 if single else batch.max_new

@@ -134,8 +134,8 @@ class StepBatch:
     layer_scratch: Optional[tuple] = None
     # by a delta rule's sizes: whether it runs in chunks in this step (``ops.delta_runs_in_chunks``; its layers ask one by one)
     delta_in_chunks: dict = field(default_factory=dict)
-    # by a layer's sizes: whether its runs over a cache in 4 bits go over pages made bfloat16 first (``ops.cache4_attention``; layers ask one by one)
-    expands4: dict = field(default_factory=dict)
+    # by a layer's sizes: which way its runs over a cache in 4 bits go (``ops.cache4_attention``; layers ask one by one)
+    runs4: dict = field(default_factory=dict)
     # A block on several residual streams may leave its last write-back undone, as (y, mix, out), for the next such
     # block to do together with its first read (one pass over the streams instead of two); the model does what is left
     # after the last layer.

@@ -222,8 +222,8 @@ def test_large_and_tiny_numbers_are_held_at_the_ends_of_the_range():
 
 # ---- attention --------------------------------------------------------------------------------------------------------------
 
-def check_attention(st, nq, dtype, window, seed, out_rows=None, scale=None, expect_nan=None):
-    """By the kernels that read codes."""
+def check_attention(st, nq, dtype, window, seed, out_rows=None, scale=None, expect_nan=None, way=("codes",)):
+    """By the kernels that read codes: those for single tokens, or with ``way`` ("tiles", tiles, cluster) the one for runs."""
     g = torch.Generator().manual_seed(seed)
     nkv, d, group = st.nkv, st.d, nq // st.nkv
     rows = len(st.row_slot)
@@ -232,7 +232,7 @@ def check_attention(st, nq, dtype, window, seed, out_rows=None, scale=None, expe
     q = (1.5 * torch.randn(rows, pitch, generator=g)).to(dtype)
     out = torch.full((out_rows or rows, nq * d), 5.0, dtype=dtype, device=DEV)
     batch = st.batch()
-    batch.expands4[nq, nkv, d, window, pitch] = False
+    batch.runs4[nq, nkv, d, window, pitch] = way
     ops.cache4_attention(q.to(DEV), pitch, st.view(), batch, out, nq, nkv, d, window, scale)
     got = out.cpu().double()
     assert (got[rows:] == 5.0).all()
@@ -249,6 +249,8 @@ def check_attention(st, nq, dtype, window, seed, out_rows=None, scale=None, expe
             # the weights' roundings (half a step of a half, subnormal below 2^-25 of the largest; none in 32 bits), the sums', the result's
             off = off + (2.0 ** -11 if dtype == torch.bfloat16 else 0.0) + (past + n + 64) / 32 * 2.0 ** -23
             tol = torch.finfo(dtype).eps / 2 * o.abs() + off * weight
+            if way[0] == "tiles":                        # (there a weight below 2^-20 of the largest is a subnormal half)
+                tol = tol + (past + n) * 2.0 ** -31 * v.nan_to_num(0.0).abs().max()
             if expect_nan is not None and expect_nan(s, past + i):
                 assert have.isnan().all()
             else:
@@ -301,6 +303,86 @@ def test_runs_of_tokens(nq, nkv, d, past, new, window):
     st = Step(past, new, nkv, d, seed=nq + d)
     st.fill(sum(new))
     check_attention(st, nq, torch.bfloat16, window, nq, out_rows=sum(new) + 1)
+
+
+TILES = [
+    # nq, nkv, d, past, new, window
+    (16, 8, 128, [0], [17], 0),
+    (16, 8, 128, [0, 5, 100], [7, 1, 39], 0),
+    (40, 8, 128, [61, 200], [24, 5], 50),
+    (4, 4, 128, [0], [150], 0),
+    (8, 1, 64, [33, 0], [20, 3], 16),
+    (40, 2, 128, [17], [4], 0),
+    (3, 1, 128, [1000, 3], [2, 70], 7),
+    (6, 2, 64, [700, 0, 64], [65, 128, 1], 0),
+    (128, 1, 64, [100], [3], 0),
+    (2, 1, 128, [640, 63], [129, 64], 64),
+]
+
+
+def tiles_of(nq, nkv, new):
+    tokens = 128 // (nq // nkv)
+    return nkv * sum(-(-n // tokens) for n in new)
+
+
+@pytest.mark.parametrize("nq,nkv,d,past,new,window", TILES)
+@pytest.mark.parametrize("cluster", [1, 2, 4, 8])
+def test_runs_of_tokens_in_tiles(nq, nkv, d, past, new, window, cluster):
+    st = Step(past, new, nkv, d, seed=nq + d)
+    st.fill(sum(new))
+    check_attention(st, nq, torch.bfloat16, window, nq, out_rows=sum(new) + 1, way=("tiles", tiles_of(nq, nkv, new), cluster))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("which", ["keys", "values"])
+@pytest.mark.parametrize("window", [0, 20])
+@pytest.mark.parametrize("cluster", [1, 2])
+def test_a_token_that_is_not_finite_in_tiles(d, which, window, cluster):
+    st = Step([30, 10], [90, 50], 1, d, seed=5)
+    st.fill(5)
+    slot, at = st.slots[0], 75
+    part = getattr(st, which)
+    part.scales[int(st.table[slot, at // 64]), 0, at % 64, d // 16 - 1] = 255
+    check_attention(st, 2, torch.bfloat16, window, 2, expect_nan=lambda s, p: s == slot and p >= at and (not window or p < at + window),
+                    way=("tiles", tiles_of(2, 1, st.new), cluster))
+
+
+def test_tiles_whose_scores_spread_and_odd_queries():
+    st = Step([500, 0, 63], [3, 70, 2], 2, 128, seed=9)
+    st.fill(9)
+    new = st.new
+    for cluster in (1, 4):
+        way = ("tiles", tiles_of(4, 2, new), cluster)
+        check_attention(st, 4, torch.bfloat16, 0, 3, scale=1.0, way=way)             # weights from 1 to 2^-200
+        check_attention(st, 4, torch.bfloat16, 0, 4, scale=0.0, way=way)             # all keys alike
+        q = torch.randn(75, 4 * 128, generator=torch.Generator().manual_seed(1)).bfloat16()
+        outs = []
+        stream = torch.cuda.Stream()
+        for up in (1.0, 2.0 ** 60, 2.0 ** -60, 1.0):
+            given, view, batch = (q * up).to(DEV), st.view(), st.batch()
+            batch.runs4[4, 2, 128, 0, 512] = way
+            out = torch.empty(75, 4 * 128, dtype=torch.bfloat16, device=DEV)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                ops.cache4_attention(given, 512, view, batch, out, 4, 2, 128, 0, 0.1 / up)
+            stream.synchronize()
+            outs.append(out)
+        assert all(torch.equal(outs[0], o) for o in outs[1:])
+        odd = q.clone()
+        odd[4] = 0.0
+        odd[5, 3] = float("nan")
+        odd[6, 130] = float("inf")
+        batch = st.batch()
+        batch.runs4[4, 2, 128, 0, 512] = way
+        out = torch.empty(75, 4 * 128, dtype=torch.bfloat16, device=DEV)
+        ops.cache4_attention(odd.to(DEV), 512, st.view(), batch, out, 4, 2, 128, 0, 0.1)
+        got, plainly = out.cpu().view(75, 4, 128), outs[0].cpu().view(75, 4, 128)
+        assert got[5, 0].isnan().all() and not got[6, 1].isfinite().any()
+        alike = torch.ones(75, 4, dtype=torch.bool)
+        alike[4] = alike[5, 0] = alike[6, 1] = False
+        assert torch.equal(got[alike], plainly[alike])
+        v = plain.gathered(st.values, st.table, st.slots[1], 2, 64).mean(0)          # row 4 is the second token of its sequence
+        assert ((got[4].double() - v.repeat_interleave(2, 0)).abs() <= 2.0 ** -8 * v.abs().max() + 2.0 ** -10).all()
 
 
 @pytest.mark.parametrize("nq,nkv,d,page,past,new,window,dtype", [
@@ -507,6 +589,11 @@ def test_refusals():
     for over in (q[:, 64:320], torch.as_strided(q, (2, 256), (640, 1)), torch.as_strided(q, (2, 256), (256, 1))):
         with pytest.raises(cb.CitlaliError, match="not over their queries"):
             ops.cache4_append(q, kv, batch.row_slot, batch.row_pos, 4, 2, 64, f, 64, q_out=over)
+    runs = Step([10], [2], 2, 64).batch()
+    for way, words in ((("tiles", 2, 3), "clusters"), (("tiles", 2, 16), "clusters"), (("tiles", 2, 0), "clusters")):
+        runs.runs4[4, 2, 64, 0, 512] = way
+        with pytest.raises(cb.CitlaliError, match=words):
+            ops.cache4_attention(q, 512, kv, runs, out, 4, 2, 64, 0, 0.1)
     with pytest.raises(cb.CitlaliError, match="a row for every sequence"):
         many = Step([10, 3, 4], [1, 1, 1], 2, 64).batch()
         many.row_slot, many.row_pos = batch.row_slot, batch.row_pos
@@ -539,7 +626,7 @@ def check_long_run(st, nq, window, seed, expect_nan=None):
     out = torch.full((rows + 1, nq * d), 5.0, dtype=torch.bfloat16, device=DEV)
     before = ops.launch_count()
     batch = st.batch()
-    batch.expands4[nq, nkv, d, window, pitch] = True         # whatever the times say
+    batch.runs4[nq, nkv, d, window, pitch] = ("pages",)      # whatever the times say
     ops.cache4_attention(q.to(DEV), pitch, st.view(), batch, out, nq, nkv, d, window, scale)
     got = out.cpu().double()
     assert (got[rows:] == 5.0).all()
@@ -577,8 +664,8 @@ def test_a_token_that_is_not_finite_in_a_longer_run(d, which, window):
     check_long_run(st, 2, window, 2, expect_nan=lambda s, p: s == slot and p >= at and (not window or p < at + window))
 
 
-@pytest.mark.parametrize("expands", [False, True])
-def test_queries_that_end_with_their_last_row(expands):
+@pytest.mark.parametrize("way", [("codes",), ("pages",), ("tiles", 4, 2)])
+def test_queries_that_end_with_their_last_row(way):
     """Rows of a wider projection, and nothing behind the last row's queries."""
     st = Step([40, 0], [60, 30], 2, 128, seed=8)
     st.fill(8)
@@ -587,7 +674,7 @@ def test_queries_that_end_with_their_last_row(expands):
     made = []
     for given in (q, q.flatten()[:(rows - 1) * pitch + wide].clone()):
         batch, out = st.batch(), torch.full((rows, wide), 5.0, dtype=torch.bfloat16, device=DEV)
-        batch.expands4[4, 2, 128, 0, pitch] = expands
+        batch.runs4[4, 2, 128, 0, pitch] = way
         ops.cache4_attention(given, pitch, st.view(), batch, out, 4, 2, 128, 0, 0.1)
         made.append(out)
     assert torch.equal(made[0], made[1])
