@@ -3,17 +3,16 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(f q . k_j - m),  f = scale log2(e),  over the keys lo..pos that a row sees
 //
-// A tile is 128 rows: pairs (token, query head) of one sequence and key/value head.  A block has a tile and the pages that its tokens see,
-// or, where that leaves multiprocessors idle or one block with much more to do than the others, a cluster of 2, 4 or 8 blocks shares the
-// pages.  A page is a step:
-//   warps 4-7   put its codes back, two threads a key: the codes come from memory into registers a page ahead, and go to shared memory as
-//               halves c s / 8 (exact, cache4.cuh) in rows of 128 bytes with the 128-byte swizzle, keys ahead of values; two pages deep.
-//   warps 8, 9  one lane each issues the products (tcgen05.mma, 128 rows, float sums): S = Q K^T, up to two pages ahead of the weights,
-//               and O += P V with P in tensor memory over the scores that it came from, and V as it was stored (its rows are the
-//               contraction).  An issuing thread spends 60 clocks on a product of 16 and 200 on telling a barrier of a page's: as much
-//               as a page's weights take if it had both.
-//   warps 0-3   a thread a row: 64 scores from tensor memory, the weights, their sum, and the weights back as halves.  A row's reference
-//               m only has to keep weights and sums in range: it is renewed, and O scaled, where 64 weights exceed 2^15.
+// A tile is 128 rows: pairs (token, query head) of one sequence and key/value head.  A block owns a multiprocessor and has a tile and the
+// pages that its tokens see, or a cluster of 2, 4 or 8 blocks shares the pages.  A page is a step, four are under way:
+//   warps 8-15  put its codes back, two threads a key, warps 8-11 the even pages and 12-15 the odd ones: the codes come from memory into
+//               registers a page ahead, and go to shared memory as halves c s / 8 (exact, cache4.cuh) in rows of 128 bytes with the 128-byte
+//               swizzle, keys ahead of values.
+//   warps 16, 17  one lane each issues the products (tcgen05.mma, 128 rows, float sums): S = Q K^T as far ahead as there is room, and
+//               O += P V with P in tensor memory over the scores that it came from, and V as it was stored (its rows are the contraction).
+//   warps 0-7   a thread a row, warps 0-3 the even pages and 4-7 the odd ones: the largest of 64 scores, read from tensor memory; the row's
+//               reference m, which goes from page to page between the two threads of a row and only has to keep weights in range (it is
+//               renewed, and O scaled, where a weight would exceed 2^15); then the weights, read again, as halves, and their sum.
 // The element order.  (w & 0x000f000f) | 0x6400 is a pair (i, i + 4) of a word's eight elements, so elements lie in the order 0 4 1 5 2 6
 // 3 7 in shared memory.  Queries have the same order, and results are put right on their way out.
 // Queries are made halves after they were multiplied by a power of two that puts the row's largest into [2^14, 2^15): exact for every
@@ -23,9 +22,12 @@
 // times a NaN would reach it; a row that does see it gets a NaN from the key.
 // A cluster's blocks leave O, m and the sum in their shared memory, and each merges an even share of the rows, always in the same order.
 //
-// Two blocks share a multiprocessor (256 columns of tensor memory each; shared memory is asked for so that a third does not fit, whose
-// wait for tensor memory could hold up its cluster): while one waits for its products, the other's threads have the issue slots, which
-// are what bounds it.  All waits are bounded; where one runs out, the block's results are NaN.
+// What bounds it: a page takes 1,400 clocks, of which the products take 512 and the exponentials 512 (16 a clock); the rest is the issue
+// of what puts codes back and of the softmax (issue slots half used) and the latencies between the roles.  A block spends about 4 us beside
+// its pages.  With the softmax on four warps and two blocks a multiprocessor a page took 2,300 clocks a block; with one issuing lane for both
+// products 2,700, since an MMA takes it 60 clocks and telling a barrier 200.  Measured (16 heads over 8 of 128): a prompt of 2,048 tokens 37 us
+// (over pages made bfloat16 first: 53), eight of 512 42 (48), 64 new tokens over 32,768 60 (by the kernel for single tokens: 116).
+// All waits are bounded; where one runs out, the block's results are NaN.
 #include "api.h"
 #include "cache4.cuh"
 #include "common.cuh"
@@ -37,20 +39,21 @@ namespace c4 {
 
 using namespace tc;
 
-constexpr int kRunRows = 128, kRunKeys = 64, kRunThreads = 320, kRunCluster = 8;
-constexpr int kSoftWarps = 4, kLoadWarps = 4, kScoreWarp = 8;             // (and one more for the values' products)
-constexpr float kRunBits = 6.0f, kRunMost = 32768.0f;                // log2 of the largest weight when m is renewed; a page's sum above which it is
+constexpr int kRunRows = 128, kRunKeys = 64, kRunThreads = 576, kRunCluster = 8;
+constexpr int kSoftWarps = 8, kLoadWarps = 8, kScoreWarp = 16;            // (and one more for the values' products)
+constexpr int kStages = 4;                                           // pages under way
+constexpr float kRunBits = 6.0f, kRunMost = 15.0f;                   // log2 of the largest weight when m is renewed, and above which it is
 constexpr float kNothingYet = -3.402823466e+38f;
-constexpr uint32_t kRunColumns = 256, kColScores = 0, kColOut = 128;         // of tensor memory; two pages' scores
+constexpr uint32_t kRunColumns = 512, kColScores = 0, kColOut = kStages * kRunKeys;         // of tensor memory; the scores of so many pages
 constexpr uint32_t kRegion = kRunKeys * 128;                         // bytes of 64 keys by 64 elements
 
 template <int D>
 struct RunLayout {
     static constexpr uint32_t part = D / 64 * kRegion, stage = 2 * part;         // keys (or values) of a page, and both
-    static constexpr uint32_t queries = 2 * part;                    // ahead of the two stages
-    static constexpr uint32_t bytes = D == 128 ? queries + 2 * stage + 1024 : 80 * 1024;       // at least what keeps a third block off the multiprocessor
-    static_assert(queries + 2 * stage + 1024 <= bytes && 2 * (bytes + 16384) <= 227 * 1024 && 3 * bytes > 227 * 1024, "two blocks fit");
-    static_assert(kRunRows * D * 4 <= 2 * stage, "a block's results take the stages' place");
+    static constexpr uint32_t queries = 2 * part;                    // ahead of the stages
+    static constexpr uint32_t needed = queries + kStages * stage + 1024, bytes = needed > 120 * 1024 ? needed : 120 * 1024;
+    static_assert(bytes + 8192 <= 227 * 1024 && 2 * bytes > 227 * 1024, "one block fits, and no second");
+    static_assert(kRunRows * D * 4 <= kStages * stage, "a block's results take the stages' place");
 };
 
 struct Runs4 {
@@ -67,9 +70,9 @@ struct Runs4 {
     float scale_log2;
 };
 
-// Four products over 16 elements of the contraction each, by the lane that has `go` (the whole warp comes here, so that descriptors
-// stay in registers that all lanes share: 15 % of a page's time), issued in one statement ( every value that
-// changes between them is an addition to a descriptor).  A in shared memory, 32 bytes further from one to the next as B is; or in tensor memory, with B's rows the contraction.
+// Four products over 16 elements of the contraction each, by the lane that has `go`.  The whole warp comes here, so that descriptors stay
+// in registers that all lanes share (a page took 15 % longer with one lane alone), and what changes between the four is an addition to
+// a descriptor.  A in shared memory, 32 bytes further from one to the next as B is; or in tensor memory, with B's rows the contraction.
 __device__ __forceinline__ void mma_four(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t go) {
     asm volatile(
         "{\n.reg .pred p, yes, go;\n.reg .b64 a, b;\n"
@@ -118,7 +121,7 @@ __device__ __forceinline__ uint64_t smem_desc_rows_are_k(uint32_t addr, uint32_t
     return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)((step >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
            (uint64_t)2 << 61;
 }
-// 32 columns of the thread's lane: loads (to be waited for), the wait (the registers go through it), and stores.
+// Columns of the thread's lane: loads (to be waited for), the waits (the registers go through them), and stores.
 #define CITLALI_R32(r) "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), \
     "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), \
     "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), \
@@ -179,16 +182,17 @@ struct HalfKey {
 };
 
 template <int D>
-__global__ void __launch_bounds__(kRunThreads, 2)
+__global__ void __launch_bounds__(kRunThreads, 1)
 attention4_runs_kernel(const __grid_constant__ Runs4 a) {
     using L = RunLayout<D>;
     extern __shared__ uint8_t raw[];
-    __shared__ __align__(8) uint64_t q_full, k_full[2], v_full[2], v_empty[2], s_full[2], p_full[2];
+    __shared__ __align__(8) uint64_t q_full, k_full[kStages], v_full[kStages], v_empty[kStages], s_full[kStages], p_full[kStages], m_known[2][4];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     __shared__ float row_factor[kRunRows];                           // what takes a row's scores to powers of two
+    __shared__ float row_m[kRunRows], row_l[2][kRunRows];            // the reference, and the sums of the even and the odd pages' weights
     __shared__ float2 row_sums[kRunRows];                            // (m, l)
-    __shared__ const __nv_bfloat16* row_q[kRunRows];
+    __shared__ float row_weights[kRunRows];                          // of the blocks' parts of this block's rows [row][block]
     __shared__ __nv_bfloat16* row_out[kRunRows];
     volatile int* abort_flag = &abort_word;
     const uint32_t queries = (smem_u32(raw) + 1023u) & ~1023u, base = queries + L::queries;
@@ -234,16 +238,21 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
 
     if (tid == 0) {
         abort_word = 0;
-        mbar_init(smem_u32(&q_full), kSoftWarps);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&k_full[i]), kLoadWarps);
-            mbar_init(smem_u32(&v_full[i]), kLoadWarps);
+        mbar_init(smem_u32(&q_full), kSoftWarps + kLoadWarps);
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(smem_u32(&k_full[i]), kLoadWarps / 2);
+            mbar_init(smem_u32(&v_full[i]), kLoadWarps / 2);
             mbar_init(smem_u32(&v_empty[i]), 1);
             mbar_init(smem_u32(&s_full[i]), 1);
-            mbar_init(smem_u32(&p_full[i]), kSoftWarps);
+            mbar_init(smem_u32(&p_full[i]), kSoftWarps / 2);
         }
+        for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&m_known[i >> 2][i & 3]), 1);
         fence_barrier_init();
         fence_async_proxy();
+    }
+    if (tid < kRunRows) {
+        const int token = tid / a.group;
+        row_out[tid] = a.out + (size_t)(row0 + token0 + token) * a.out_stride + (size_t)(kv * a.group + tid - token * a.group) * D;
     }
     if (warp == kScoreWarp) {
         tmem_alloc(smem_u32(&tmem_slot), kRunColumns);
@@ -256,153 +265,173 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
     dependents_may_launch();                                         // only now: this block holds its tensor memory
     wait_for_predecessor();
 
+    // ---- the first page's codes (a thread half a key and value), then the queries, by the warps of both kinds, eight rows each
+    // (a quarter of a warp: eight rows of shared memory, which meet no bank twice)
+    const int key = (warp & 3) * 16 + (lane & 15), half = lane >> 4, odd = warp >> 2 & 1;      // (odd: of a warp that takes the odd pages)
+    auto fetch = [&](HalfKey<D>& x, int page) {
+        const size_t at = place(page, a.nkv, kv, kRunKeys, key);
+        const uint4 *kc = reinterpret_cast<const uint4*>(a.k_codes + at * (D / 2) + half * (D / 4)),
+                    *vc = reinterpret_cast<const uint4*>(a.v_codes + at * (D / 2) + half * (D / 4));
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) { x.k[i] = __ldcg(kc + i); x.v[i] = __ldcg(vc + i); }
+        const size_t scales = at * (D / kGroup) + half * (D / 32);
+        if constexpr (D == 128) {
+            x.k_scales = __ldcg(reinterpret_cast<const uint32_t*>(a.k_scales + scales));
+            x.v_scales = __ldcg(reinterpret_cast<const uint32_t*>(a.v_scales + scales));
+        } else {
+            x.k_scales = __ldcg(reinterpret_cast<const uint16_t*>(a.k_scales + scales));
+            x.v_scales = __ldcg(reinterpret_cast<const uint16_t*>(a.v_scales + scales));
+        }
+    };
+    HalfKey<D> next = {};
+    int page_after = 0;
+    if (warp >= kSoftWarps && warp < kSoftWarps + kLoadWarps && pages > odd) {
+        if (pages > odd + 2) page_after = table[odd + 2];
+        fetch(next, table[odd]);
+    }
+    if (warp < kSoftWarps + kLoadWarps) {
+        // As they are, all on their way at once; then each lane makes its own pieces halves where they lie.  (Short loops: what runs once
+        // waits for its instructions more than for anything else.)
+        constexpr int lanes_of = D / 8, at_once = 32 / lanes_of;
+        constexpr int rows_of = kRunRows / (kSoftWarps + kLoadWarps);
+        const int piece = lane % lanes_of, first = warp * rows_of;
+        auto at = [&](int r) { return queries + (piece / 8) * (kRunRows * 128) + r * 128 + (((piece & 7) ^ (r & 7)) << 4); };
+        size_t from = 0;
+        {
+            const int r = min(first + lane % rows_of, used - 1), t = r / a.group;
+            from = (size_t)(row0 + token0 + t) * a.q_stride + (size_t)(kv * a.group + r - t * a.group) * D;
+        }
+#pragma unroll 2
+        for (int k = lane / lanes_of; k < rows_of; k += at_once) {
+            const __nv_bfloat16* src = a.q + __shfl_sync(0xffffffffu, from, k) + 8 * piece;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at(first + k)), "l"(src), "r"(first + k < used ? 16 : 0) : "memory");
+        }
+        fa::cp_async_commit();
+        fa::cp_async_wait<0>();
+#pragma unroll 1
+        for (int k = lane / lanes_of; k < rows_of; k += at_once) {
+            const uint4 in = ld_shared_v4(at(first + k));
+            uint32_t most = __vimax3_u16x2(in.x & 0x7fff7fffu, in.y & 0x7fff7fffu, __vmaxu2(in.z & 0x7fff7fffu, in.w & 0x7fff7fffu));
+            most = max(most << 16, most & 0x7fff0000u);
+#pragma unroll
+            for (int o = 1; o < lanes_of; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const int up = min(100, max(-113, 14 + 127 - (int)(most >> 23)));
+            const float by = copysignf(__int_as_float((127 + up) << 23), a.scale_log2);
+            auto two = [&](uint32_t low, uint32_t high) {            // the words' lower elements, and their upper ones
+                return make_uint2(packed(__uint_as_float(low << 16) * by, __uint_as_float(high << 16) * by),
+                                  packed(__uint_as_float(low & 0xffff0000u) * by, __uint_as_float(high & 0xffff0000u) * by));
+            };
+            const uint2 even = two(in.x, in.z), odd = two(in.y, in.w);           // elements (0, 4), (1, 5) and (2, 6), (3, 7)
+            st_shared_v4(at(first + k), even.x, even.y, odd.x, odd.y);
+            if (piece == 0) row_factor[first + k] = __int_as_float((127 - up) << 23) * (fabsf(a.scale_log2) * kUnit);
+        }
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&q_full));
+    }
+
     float m = kNothingYet, l = 0.0f;                                 // of the softmax threads' rows
     const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
     if (warp < kSoftWarps) {
-        // ---- queries: D / 8 lanes a row
-        const int row = tid, token = row / a.group;
+        // ---- a page's scores, weights and sum: the even pages' warps 0-3, the odd pages' warps 4-7, a thread a row
+        const int quarter = warp & 3, row = tid % kRunRows, token = row / a.group;
         const bool on = row < used;
-        row_out[row] = a.out + (size_t)(row0 + token0 + token) * a.out_stride + (size_t)(kv * a.group + row - token * a.group) * D;
-        {
-            // (as they are, all on their way at once; then each lane makes its own pieces halves where they lie: short loops, since
-            // what runs once waits for its instructions)
-            constexpr int lanes_of = D / 8, at_once = 32 / lanes_of;
-            const int piece = lane % lanes_of;
-            auto at = [&](int r) { return queries + (piece / 8) * (kRunRows * 128) + r * 128 + (((piece & 7) ^ (r & 7)) << 4); };
-            row_q[row] = on ? a.q + (size_t)(row0 + token0 + token) * a.q_stride + (size_t)(kv * a.group + row - token * a.group) * D : nullptr;
-            __syncwarp();
-#pragma unroll 4
-            for (int r = warp * 32 + lane / lanes_of; r < warp * 32 + 32; r += at_once) {
-                const __nv_bfloat16* from = row_q[r];
-                if (from) fa::cp_async16(at(r), from + 8 * piece);
-                else st_shared_v4(at(r), 0, 0, 0, 0);
-            }
-            fa::cp_async_commit();
-            fa::cp_async_wait<0>();
-#pragma unroll 4
-            for (int r = warp * 32 + lane / lanes_of; r < warp * 32 + 32; r += at_once) {
-                const uint4 in = ld_shared_v4(at(r));
-                const uint32_t p[4] = {in.x, in.y, in.z, in.w};
-                uint32_t most = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) most = max(most, max((p[k] & 0x7fffu) << 16, p[k] & 0x7fff0000u));
-#pragma unroll
-                for (int o = 1; o < lanes_of; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const int up = min(100, max(-113, 14 + 127 - (int)(most >> 23)));
-                const float by = __int_as_float((127 + up) << 23);
-                float y[8];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    y[2 * k] = __uint_as_float(p[k] << 16) * by;
-                    y[2 * k + 1] = __uint_as_float(p[k] & 0xffff0000u) * by;
-                }
-                st_shared_v4(at(r), packed(y[0], y[4]), packed(y[1], y[5]), packed(y[2], y[6]), packed(y[3], y[7]));
-                if (piece == 0) row_factor[r] = __int_as_float((127 - up) << 23) * (a.scale_log2 * kUnit);
-            }
-            fence_async_proxy();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&q_full));
-        }
-        // ---- a page's scores, weights and sum
+        mbar_wait(smem_u32(&q_full), 0, abort_flag, nullptr, 0);
+        __syncwarp();
         const float factor = row_factor[row];
         const int pos = on ? pos0 + token : -1, low = a.window > 0 ? pos - a.window + 1 : 0;
 #pragma unroll 1
-        for (int i = 0; i < pages; ++i) {
-            const uint32_t at_scores = tmem + lanes + kColScores + (i & 1) * kRunKeys;
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[i & 1]), (i >> 1) & 1u, abort_flag, nullptr, 0))) break;
+        for (int i = odd; i < pages; i += 2) {
+            const int stage = i % kStages;
+            const uint32_t at_scores = tmem + lanes + kColScores + stage * kRunKeys;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[stage]), i / kStages & 1u, abort_flag, nullptr, 0))) break;
             tc_fence_after();
             const int key0 = (page0 + i) * kRunKeys;
             // pages that some of the tile's tokens see in part (rows behind its last have queries of zeros, and are not stored)
             const bool border = key0 + kRunKeys - 1 > pos0 || (a.window > 0 && key0 <= last - a.window);
-            uint32_t s[64];
-            float by;
-            auto load = [&]() {
-                tmem_load32(at_scores, s);
-                tmem_load32(at_scores + 32, s + 32);
-                tmem_wait32(s);
-                tmem_wait32(s + 32);
-                by = factor;
+            const float by = border ? 1.0f : factor;
+            uint32_t x[32];
+            auto scores = [&](int c0) {
+                tmem_load32(at_scores + c0, x);
+                tmem_wait32(x);
                 if (border) {
-                    by = 1.0f;
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) {
-                        const int key = key0 + c;
-                        s[c] = __float_as_uint(key > pos || key < low ? -INFINITY : __uint_as_float(s[c]) * factor);
+                    for (int c = 0; c < 32; ++c) {
+                        const int at = key0 + c0 + c;
+                        x[c] = __float_as_uint(at > pos || at < low ? -INFINITY : __uint_as_float(x[c]) * factor);
                     }
                 }
             };
-            auto weigh = [&]() {                                     // the weights, in the first half of the registers, and their sum
-                float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < 32; ++c) {
-                    const float x = fa::fast_exp2(fmaf(__uint_as_float(s[2 * c]), by, -m)), y = fa::fast_exp2(fmaf(__uint_as_float(s[2 * c + 1]), by, -m));
-                    sums[c & 3] += x + y;
-                    s[c] = packed(x, y);
-                }
-                return (sums[0] + sums[1]) + (sums[2] + sums[3]);
-            };
-            float sum = 0.0f;
-            bool renew = i == 0;
-            if (!renew) {
-                load();
-                sum = weigh();
-                renew = __any_sync(0xffffffffu, sum > kRunMost);
-            }
-            if (renew) {
-                load();                                              // (the scores are still there)
-                float top = kNothingYet;
-#pragma unroll
-                for (int c = 0; c < 64; ++c) top = fmaxf(top, __uint_as_float(s[c]) * by);
-                top = fmaxf(m, top - kRunBits);
-                const float turn = fa::fast_exp2(m - top);
-                m = top;
-                l *= turn;
-                sum = weigh();
-                if (i > 0) {
-                    // (the product with the page before must have ended)
-                    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[(i - 1) & 1]), ((i - 1) >> 1) & 1u, abort_flag, nullptr, 0))) break;
-                    tc_fence_after();
+            float top = kNothingYet;
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(tmem + lanes + kColOut + c, o);
-                        tmem_wait16(o);
+            for (int c0 = 0; c0 < kRunKeys; c0 += 32) {
+                scores(c0);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * turn);
-                        tmem_store16(tmem + lanes + kColOut + c, o);
-                    }
+                for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(x[c]));
+            }
+            top *= by;                                               // (not negative: the queries have the scale's sign)
+            // the reference as the page before leaves it, and as this one does
+            float before = kNothingYet;
+            if (i > 0) {
+                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&m_known[odd ^ 1][quarter]), (i - 1) >> 1 & 1u, abort_flag, nullptr, 0))) break;
+                before = row_m[row];
+            }
+            const bool renew = __any_sync(0xffffffffu, top - before > kRunMost);
+            const float now = renew ? fmaxf(before, top - kRunBits) : before;
+            row_m[row] = now;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&m_known[odd][quarter]));
+            l *= fa::fast_exp2(m - now);
+            m = now;
+            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+            for (int c0 = 0; c0 < kRunKeys; c0 += 32) {
+                scores(c0);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    const float u = fa::fast_exp2(fmaf(__uint_as_float(x[2 * c]), by, -m)), v = fa::fast_exp2(fmaf(__uint_as_float(x[2 * c + 1]), by, -m));
+                    sums[c & 3] += u + v;
+                    x[c] = packed(u, v);
+                }
+                tmem_store16(at_scores + c0 / 2, x);        // (over scores that have been read)
+            }
+            l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            if (renew && i > 0) {
+                // (the product with the page before must have ended)
+                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[(i - 1) % kStages]), (i - 1) / kStages & 1u, abort_flag, nullptr, 0))) break;
+                tc_fence_after();
+                const float turn = fa::fast_exp2(before - now);
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    tmem_load32(tmem + lanes + kColOut + c, x);
+                    tmem_wait32(x);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * turn);
+                    tmem_store32(tmem + lanes + kColOut + c, x);
                 }
             }
-            l += sum;
-            tmem_store32(at_scores, s);
             tmem_store_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&p_full[i & 1]));
+            if (lane == 0) mbar_arrive(smem_u32(&p_full[stage]));
         }
-        if (pages > 0) mbar_wait(smem_u32(&v_empty[(pages - 1) & 1]), ((pages - 1) >> 1) & 1u, abort_flag, nullptr, 0);
+        if (pages > 0) {
+            const int end = pages - 1;
+            if ((end & 1) != odd) mbar_wait(smem_u32(&m_known[odd ^ 1][quarter]), end >> 1 & 1u, abort_flag, nullptr, 0);
+            const float now = row_m[row];                            // (of the last page)
+            l *= fa::fast_exp2(m - now);
+            if (!odd) row_sums[row].x = now;
+            mbar_wait(smem_u32(&v_empty[end % kStages]), end / kStages & 1u, abort_flag, nullptr, 0);
+        } else if (!odd) {
+            row_sums[row].x = kNothingYet;
+        }
+        row_l[odd][row] = l;
         __syncwarp();
         tc_fence_after();
     } else if (warp < kSoftWarps + kLoadWarps) {
         // ---- a page's keys and values
-        const int key = (warp - kSoftWarps) * 16 + (lane & 15), half = lane >> 4;       // (a quarter of a warp: eight rows, which meet no bank twice)
         constexpr int words = D / 16;                                // of a thread's half of a key
         const Words pairs;
-        auto fetch = [&](HalfKey<D>& x, int page) {
-            const size_t at = place(page, a.nkv, kv, kRunKeys, key);
-            const uint4 *kc = reinterpret_cast<const uint4*>(a.k_codes + at * (D / 2) + half * (D / 4)),
-                        *vc = reinterpret_cast<const uint4*>(a.v_codes + at * (D / 2) + half * (D / 4));
-#pragma unroll
-            for (int i = 0; i < D / 64; ++i) { x.k[i] = __ldcg(kc + i); x.v[i] = __ldcg(vc + i); }
-            const size_t scales = at * (D / kGroup) + half * (D / 32);
-            if constexpr (D == 128) {
-                x.k_scales = __ldcg(reinterpret_cast<const uint32_t*>(a.k_scales + scales));
-                x.v_scales = __ldcg(reinterpret_cast<const uint32_t*>(a.v_scales + scales));
-            } else {
-                x.k_scales = __ldcg(reinterpret_cast<const uint16_t*>(a.k_scales + scales));
-                x.v_scales = __ldcg(reinterpret_cast<const uint16_t*>(a.v_scales + scales));
-            }
-        };
         // chunk c (16 bytes) of row `key` lies at c ^ (key & 7)
         auto put = [&](uint32_t region, const uint4 (&codes)[D / 64], uint32_t scales) {
             const uint32_t to = region + (D == 128 ? half * kRegion : 64u * half) + key * 128;           // (a multiple of 64)
@@ -415,30 +444,28 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
                              pairs.second_of(w >> 8, scale));
             }
         };
-        HalfKey<D> next;
-        int page = pages > 0 ? table[0] : 0, page_after = pages > 1 ? table[1] : 0;
-        if (pages > 0) fetch(next, page);
 #pragma unroll 1
-        for (int i = 0; i < pages; ++i) {
+        for (int i = odd; i < pages; i += 2) {
             const HalfKey<D> x = next;
-            if (i + 1 < pages) {
+            if (i + 2 < pages) {
                 fetch(next, page_after);
-                if (i + 2 < pages) page_after = table[i + 2];
+                if (i + 4 < pages) page_after = table[i + 4];
             }
-            const uint32_t stage = base + (i & 1) * L::stage;
-            // the scores of the page before the last have come out: its keys' place is free
-            if (i > 1 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[i & 1]), ((i >> 1) & 1u) ^ 1u, abort_flag, nullptr, 0))) break;
+            const int place_of = i % kStages;
+            const uint32_t stage = base + place_of * L::stage, turn = i / kStages & 1u;
+            // the scores of the page that was here have come out: its keys' place is free
+            if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[place_of]), turn ^ 1u, abort_flag, nullptr, 0))) break;
             const uint32_t bad = __vcmpgeu4(x.v_scales, 0xf8f8f8f8u);
             const bool none = (bad | __shfl_xor_sync(0xffffffffu, bad, 16)) != 0;
             put(stage, x.k, none ? 0xffffffffu : x.k_scales);
             fence_async_proxy();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&k_full[i & 1]));
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[i & 1]), ((i >> 1) & 1u) ^ 1u, abort_flag, nullptr, 0))) break;
+            if (lane == 0) mbar_arrive(smem_u32(&k_full[place_of]));
+            if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[place_of]), turn ^ 1u, abort_flag, nullptr, 0))) break;
             put(stage + L::part, x.v, x.v_scales & ~bad);
             fence_async_proxy();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&v_full[i & 1]));
+            if (lane == 0) mbar_arrive(smem_u32(&v_full[place_of]));
         }
     } else if (warp == kScoreWarp) {
         // ---- the scores' products
@@ -448,15 +475,17 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
         if (pages > 0 && __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), 0, abort_flag, nullptr, 0))) {
 #pragma unroll 1
             for (int i = 0; i < pages; ++i) {
-                // (their place held the weights of the page before the last, which have been multiplied with its values)
-                if (i > 1 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[i & 1]), ((i >> 1) & 1u) ^ 1u, abort_flag, nullptr, 0))) break;
-                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[i & 1]), (i >> 1) & 1u, abort_flag, nullptr, 0))) break;
+                const int stage = i % kStages;
+                const uint32_t turn = i / kStages & 1u;
+                // (their place held the weights of a page before, which have been multiplied with its values)
+                if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[stage]), turn ^ 1u, abort_flag, nullptr, 0))) break;
+                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[stage]), turn, abort_flag, nullptr, 0))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < D / 64; ++k)
-                    mma_four(tmem + kColScores + (i & 1) * kRunKeys, asked + k * (kRunRows * 128 >> 4),
-                             keys + (i & 1) * (L::stage >> 4) + k * (kRegion >> 4), form, k > 0, go);
-                commit_if(smem_u32(&s_full[i & 1]), go);
+                    mma_four(tmem + kColScores + stage * kRunKeys, asked + k * (kRunRows * 128 >> 4), keys + stage * (L::stage >> 4) + k * (kRegion >> 4),
+                             form, k > 0, go);
+                commit_if(smem_u32(&s_full[stage]), go);
             }
         }
     } else {
@@ -466,23 +495,27 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
         const uint64_t vals = smem_desc_rows_are_k(base + L::part, kRegion);
 #pragma unroll 1
         for (int i = 0; i < pages; ++i) {
-            const uint32_t turn = (i >> 1) & 1u;
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_full[i & 1]), turn, abort_flag, nullptr, 0) && mbar_wait(smem_u32(&p_full[i & 1]), turn, abort_flag, nullptr, 0))) break;
+            const int stage = i % kStages;
+            const uint32_t turn = i / kStages & 1u;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_full[stage]), turn, abort_flag, nullptr, 0) &&
+                                             mbar_wait(smem_u32(&p_full[stage]), turn, abort_flag, nullptr, 0))) break;
             tc_fence_after();
-            mma_four_rows(tmem + kColOut, tmem + kColScores + (i & 1) * kRunKeys, vals + (i & 1) * (L::stage >> 4), form, i > 0, go);
-            commit_if(smem_u32(&v_empty[i & 1]), go);
+            mma_four_rows(tmem + kColOut, tmem + kColScores + stage * kRunKeys, vals + stage * (L::stage >> 4), form, i > 0, go);
+            commit_if(smem_u32(&v_empty[stage]), go);
         }
     }
     __syncwarp();
 
     // ---- the rows' parts, or their results: all pages have been read, so they take the stages' place, in 16-byte pieces that swap places so
     // that a quarter of a warp meets no bank twice
+    __syncthreads();
     if (warp < kSoftWarps) {
-        if (*abort_flag) l = __int_as_float(0x7fc00000);
-        row_sums[tid] = make_float2(m, l);
-        const float by = kUnit / l;
+        const int row = tid % kRunRows;
+        const float sum = *abort_flag ? __int_as_float(0x7fc00000) : row_l[0][row] + row_l[1][row], by = kUnit / sum;
+        if (!odd) row_sums[row].y = sum;
+        // (half of the elements each)
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        for (int c = odd * (D / 2); c < odd * (D / 2) + D / 2; c += 32) {
             uint32_t o[32];
             tmem_load32(tmem + lanes + kColOut + c, o);
             tmem_wait32(o);
@@ -492,13 +525,13 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
                     float y[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[8 * k + e]) * by;
-                    st_shared_v4(base + tid * (2 * D) + (((c / 8 + k) ^ (tid & 7)) << 4), fa::pack_bf16(y[0], y[2]), fa::pack_bf16(y[4], y[6]),
+                    st_shared_v4(base + row * (2 * D) + (((c / 8 + k) ^ (row & 7)) << 4), fa::pack_bf16(y[0], y[2]), fa::pack_bf16(y[4], y[6]),
                                  fa::pack_bf16(y[1], y[3]), fa::pack_bf16(y[5], y[7]));
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const uint32_t to = base + (tid * D << 2) + (((c / 4 + k) ^ (tid & 7)) << 4);
+                    const uint32_t to = base + (row * D << 2) + (((c / 4 + k) ^ (row & 7)) << 4);
                     if (pages > 0) st_shared_v4(to, o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                     else st_shared_v4(to, 0, 0, 0, 0);
                 }
@@ -522,24 +555,18 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
     }
     __syncwarp();
     cluster_sync_all();                                              // every block's parts are there
-    // the blocks' sums of this block's rows, then (weight, -), in the queries' place
-    float2(*row_sums_of)[kRunCluster + 1] = reinterpret_cast<float2(*)[kRunCluster + 1]>(raw + (queries - smem_u32(raw)));
     const int rows = kRunRows / cluster, mine = rank * rows, count = min(rows, used - mine);             // this block's of them
-    if (tid < count) {
-        const int row = mine + tid;
-        const uint32_t here = smem_u32(&row_sums[row]);
-        float M = kNothingYet, sum = 0.0f;
-#pragma unroll 4
-        for (int k = 0; k < cluster; ++k) {
-            const float2 ml = load2_cluster(cluster_addr(here, (rank + k) & (cluster - 1)));
-            row_sums_of[tid][k] = ml;
-            M = fmaxf(M, ml.x);
-        }
+    if (tid < kRunRows) {                                            // a thread a row and block
+        const int row = tid / cluster, k = tid % cluster;
+        const float2 ml = load2_cluster(cluster_addr(smem_u32(&row_sums[mine + row]), (rank + k) & (cluster - 1)));
+        float M = ml.x;
 #pragma unroll 1
-        for (int k = 0; k < cluster; ++k) sum = fmaf(row_sums_of[tid][k].y, fa::fast_exp2(row_sums_of[tid][k].x - M), sum);
-        const float by = kUnit / sum;
+        for (int o = 1; o < cluster; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float by = fa::fast_exp2(ml.x - M);
+        float sum = ml.y * by;
 #pragma unroll 1
-        for (int k = 0; k < cluster; ++k) row_sums_of[tid][k].x = fa::fast_exp2(row_sums_of[tid][k].x - M) * by;
+        for (int o = 1; o < cluster; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        row_weights[tid] = by * (kUnit / sum);
     }
     __syncthreads();
     // A thread a 16-byte piece of a row, from its own block's part on (all of them at one block's door would wait there): elements 0 4 1 5
@@ -560,7 +587,7 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
 #pragma unroll 4
         for (int k = 0; k < cluster; ++k) {
             const float4 v = load4_cluster(cluster_addr(here, (rank + k) & (cluster - 1)));
-            const float w = row_sums_of[known][k].x;
+            const float w = row_weights[known * cluster + k];
             y[0] = fmaf(v.x, w, y[0]); y[1] = fmaf(v.y, w, y[1]); y[2] = fmaf(v.z, w, y[2]); y[3] = fmaf(v.w, w, y[3]);
         }
         finish(row, y);

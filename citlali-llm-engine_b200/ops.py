@@ -591,29 +591,62 @@ def _attention4_floats(nq: int, nkv: int, head_dim: int, page_size: int, max_new
 _EXPAND_BYTES = 1 << 30
 
 
-def _attention4_expands(batch, nq: int, nkv: int, head_dim: int, window: int, form: int, sms: int) -> bool:
-    """Whether runs of new tokens go over pages that are made bfloat16 first, by prompt attention (``form``: 2 on tcgen05, 1 on mma.sync).
-    Both ways' times, in microseconds: the kernel that reads codes does a tile of 16 columns (8 at head size 256) over 32 keys in so
-    many nanoseconds, divided over all SMs; prompt attention's blocks walk their keys one tile after another, whole blocks a SM.
-    Measured, codes / pages: one run over 2,048 keys, 16 heads over 8 of 128, 64 new tokens 25 / 49, 96: 28 / 50, 2,048: 277 / 54; four
-    over 2,048, 40 over 8: 48 tokens 71 / 89, 96: 123 / 92; four over 32,768: 64 tokens 1,015 / 1,270, 96: 1,466 / 1,273; heads of 64, 32 over
-    8, one over 8,192: 96 tokens 67 / 195, four over 32,768: 96 tokens 848 / 1,003."""
-    max_new = batch.max_new
-    if max_new < 48 or form == 0:
-        return False
-    group = nq // nkv
-    columns = 8 if head_dim == 256 else 16
+def _attention4_way(batch, nq: int, nkv: int, head_dim: int, window: int, form: int, tokens: int, codes: bool, sms: int) -> tuple:
+    """How a step's runs of tokens are attended to: ("tiles", tiles, blocks that share one) by the kernel on tcgen05 (``tokens`` of a tile; 0:
+    it does not take the sizes), ("pages",) by prompt attention (``form``: 2 on tcgen05, 1 on mma.sync, 0 not at all) over pages that are
+    made bfloat16 first, or ("codes",) by the kernel for single tokens, if it takes the sizes, or that in 32 bits.  The one that takes least
+    time, in microseconds, by what each was measured to do:
+    codes: 10 and (more than 8 columns) 3 ahead, a tile of 16 columns (8 at head size 256) over 32 keys in `unit`, divided over all SMs;
+    pages: prompt attention's blocks walk their keys one tile after another, whole blocks a SM;
+    tiles: a block, alone on its SM, takes 0.73 a page and 4 beside; a tile's pages are shared by as many blocks as fit the SMs at once,
+    while that leaves a block more than six (of clusters of 8 no more than two thirds of the SMs).
+    Measured, codes / pages / tiles: one run over 2,048 keys, 16 heads over 8 of 128, 4 new tokens 12.6 / - / 13.0, 16: 16.9 / - / 13.1, 64: 25 / 52 /
+    14, 2,048: 220 / 53 / 37; four over 8,000, 6 tokens: 29.8 / - / 33.9, 16: 43.9 / - / 34.5; one over 32,768, 64: 116 / 619 / 60; 32 over 500, 8
+    tokens: 19.6 / - / 25.4; 4,096 new tokens: 761 / 96 / 113; heads of 64, 32 over 8, one over 8,192, 96 tokens: 68 / 195 / 31.  Tiles
+    shared by 1, 2, 4 and 8: four over 4,096, 40 over 8 heads, 5 to 24 tokens (32 tiles): 55, 35, 24, 50; one over 32,768 (8 tiles): 375, 194,
+    104, 60; 300 keys (32 tiles): 11.6, 12.4, 13.1, 34.6."""
+    n_new, group = batch.n_new, nq // nkv
+    max_new, columns = max(n_new), 8 if head_dim == 256 else 16
     head_tiles = -(-group // columns)
-    tokens = max(1, columns // -(-group // head_tiles))
-    unit = {64: 1.1e-3, 128: 1.4e-3}.get(head_dim, 2.8e-3)
+    at_once = columns // -(-group // head_tiles)
+    units = tiles = far = walked = 0
+    for past, n in zip(batch.past, n_new):           # (the host's time counts: one short step a sequence)
+        end = past + n
+        keys = end if not window or end < window + n else window + n
+        units += -(-n // at_once) * (keys // 32 + 16)
+        if tokens:
+            here = -(-n // tokens)
+            seen = keys // 64 + 1 if not window or n <= tokens or keys < window + tokens else (window + tokens) // 64 + 1          # pages of the last tile
+            tiles += here
+            if seen > far:
+                far = seen
+            walked += here * (seen if window else seen - (n >> 7))
+    unit, start = {64: 1.3e-3, 128: 1.6e-3}.get(head_dim, 2.8e-3), 13 if min(group, columns) * max_new > 8 else 10
+    best = start + units * head_tiles * nkv * unit if codes else 1e9 if max_new >= 16 else 0                 # (few rows in 32 bits: no worse)
+    way = ("codes",)
+    if tokens:
+        shared = 1
+        tiles *= nkv
+        while shared < 8 and far > 6 * shared and 2 * shared * tiles <= (sms if shared < 4 else 2 * sms // 3):
+            shared *= 2
+        time = 7 + max(far / shared * 0.73 + (3 if shared > 1 else 0), (walked * nkv * 0.73 + tiles * 4) / sms)
+        if time < best:
+            best, way = time, ("tiles", tiles, shared)
+    if form > 0 and best > 40 and max_new >= 48:
+        time = _attention4_pages_time(batch, nq, nkv, head_dim, window, form, sms)
+        if time < best:
+            way = ("pages",)
+    return way
+
+
+def _attention4_pages_time(batch, nq: int, nkv: int, head_dim: int, window: int, form: int, sms: int) -> float:
     if form == 2:                                    # a block: two heads over 128 new tokens, or one over 256
-        rows, heads, keys_of_tile, tile, resident = (128, nq // 2, 128, 2.2, 1) if group % 2 == 0 else (256, nq, 128, 2.2, 1)
+        rows, heads, keys_of_tile, tile, resident = (128, nq // 2, 128, 2.2, 1) if nq // nkv % 2 == 0 else (256, nq, 128, 2.2, 1)
     else:
         rows, heads, keys_of_tile, tile, resident = 64, nq, 64, 1.5 * head_dim / 64, max(1, 256 // head_dim)
-    codes = pages = longest = steps = 0
+    pages = longest = steps = 0
     for past, n in zip(batch.past, batch.n_new):
         keys = past + n if not window else min(past + n, window + n)
-        codes += -(-n // tokens) * head_tiles * nkv * (keys // 32 + 16)
         pages += keys // 64 + 1
         blocks = -(-n // rows)
         first = keys - n if not window else min(keys - n, window)               # keys ahead of a block's own tokens
@@ -621,39 +654,7 @@ def _attention4_expands(batch, nq: int, nkv: int, head_dim: int, window: int, fo
         longest = max(longest, most)
         steps += heads * blocks * (first // keys_of_tile + 1 + (most - first // keys_of_tile) / 2)
     walked = max(longest, -(-steps // (sms * resident * longest)) * longest if steps > sms * resident * longest else 0)
-    return 9 + codes * unit > 14 + walked * tile + pages * nkv * 64 * head_dim * 4 / 2.3e6
-
-
-def _attention4_tiles(batch, nkv: int, window: int, tokens: int, sms: int):
-    """The tiles of ``tokens`` new tokens of a step's runs, over all key/value heads, and how many blocks share the pages of one: twice as
-    many while a block of the longest has more to do than an even share of all on two blocks a multiprocessor, and eight pages."""
-    tiles = steps = longest = 0
-    for past, n in zip(batch.past, batch.n_new):
-        here = -(-n // tokens)
-        if here:
-            ends = [(past + first + min(tokens, n - first) - 1) // 64 - (max(0, past + first - window + 1) // 64 if window else 0) + 1
-                    for first in (0, (here - 1) * tokens)]           # pages of the first tile and of the last
-            tiles += here
-            longest = max(longest, *ends)
-            steps += here * sum(ends) / 2
-    cluster = 1
-    while cluster < 8 and -(-longest // cluster) > max(8, steps * nkv / (2 * sms)):
-        cluster *= 2
-    return tiles * nkv, cluster
-
-
-def _attention4_way(batch, nq: int, nkv: int, head_dim: int, window: int, q_stride: int, sms: int) -> tuple:
-    """How a step's runs of tokens are attended to: ("tiles", tiles, blocks of a tile) by the kernel on tcgen05, ("pages",) over pages
-    that are made bfloat16 first, or ("codes",) by the kernel for single tokens, or that in 32 bits."""
-    max_new, tokens = batch.max_new, lib().citlali_attention4_runs_tokens(nq, nkv, head_dim, 64)
-    if tokens and nq // nkv * max_new > 8:
-        return ("tiles",) + _attention4_tiles(batch, nkv, window, tokens, sms)
-    form = lib().citlali_attention_run_form(q_stride, nq * head_dim, head_dim, 64, max_new)
-    if _attention4_floats(nq, nkv, head_dim, 64, max_new, _current_device()) < 0:
-        expands = form > 0 and max_new >= 16                         # (else the kernel in 32 bits)
-    else:
-        expands = _attention4_expands(batch, nq, nkv, head_dim, window, form, sms)
-    return ("pages",) if expands else ("codes",)
+    return 14 + walked * tile + pages * nkv * 64 * head_dim * 4 / 2.3e6
 
 
 def _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, scale):
@@ -740,13 +741,19 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
         return
     kc, ks, vc, vs, table, table_width = pools
     q_ptr, window = q.data_ptr(), _i(window or 0)
+    if window < 0:
+        require(False, f"cache4_attention: the window is a number of keys (0 or None: all), not {window}")
     # (runs by the host's lists of lengths, which a captured step would freeze: there the kernel for single tokens reads the device's)
     if (not single and not torch._C._cuda_isCurrentStreamCapturing() and q.dtype is torch.bfloat16 and kv.page_size == 64 and nkv > 0 and nq % nkv == 0
             and (q_ptr | out.data_ptr() | kc | ks | vc | vs) % 16 == 0 and (q_stride | wide) % 8 == 0):
         key = (nq, nkv, head_dim, window, q_stride)
         way = batch.runs4.get(key)
         if way is None:
-            way = batch.runs4[key] = _attention4_way(batch, nq, nkv, head_dim, window, q_stride, sm_count(q.device))
+            l, max_new = lib(), batch.max_new
+            way = batch.runs4[key] = _attention4_way(
+                batch, nq, nkv, head_dim, window, l.citlali_attention_run_form(q_stride, wide, head_dim, 64, max_new),
+                l.citlali_attention4_runs_tokens(nq, nkv, head_dim, 64),
+                _attention4_floats(nq, nkv, head_dim, 64, max_new, _current_device()) >= 0, sm_count(q.device))
         if way[0] == "pages":
             _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, float(scale))
             return

@@ -132,12 +132,18 @@ def test_command_line():
 
 
 def test_which_way_runs_go():
-    """Few new tokens read the codes, prompts go over pages made bfloat16; and in between as measured (see ops._attention4_expands)."""
-    def expands(past, new, nq=16, nkv=8, d=128, window=0, form=2):
+    """By the times that ops._attention4_way works out."""
+    def way(past, new, nq=16, nkv=8, d=128, window=0, form=2, tokens=None, codes=True):
         batch = cb.StepBatch(*[torch.zeros(1, dtype=torch.int32)] * 7, slots=list(range(len(new))), past=past, n_new=new)
-        return ops._attention4_expands(batch, nq, nkv, d, window, form, 148)
-    assert not expands([2000], [8]) and not expands([1952], [96]) and expands([0], [2048]) and not expands([0], [50])
-    assert not expands([2000] * 4, [48] * 4, 40) and expands([1952] * 4, [96] * 4, 40)
-    assert not expands([32704] * 4, [64] * 4, 40) and expands([32672] * 4, [96] * 4, 40)
-    assert not expands([8096], [96], 32, 8, 64, form=1) and not expands([100], [64], form=0)
-    assert not expands([40000], [60], window=128)
+        return ops._attention4_way(batch, nq, nkv, d, window, form, 128 // (nq // nkv) if tokens is None else tokens, codes, 148)
+    # few columns read the codes, more of them go in tiles that as many blocks share as fit at once, the longest prompts over pages
+    assert way([2000], [4]) == ("codes",) and way([2000], [64]) == ("tiles", 8, 8) and way([0], [2048]) == ("tiles", 256, 1)
+    assert way([8000] * 4, [6] * 4) == ("codes",) and way([8000] * 4, [16] * 4) == ("tiles", 32, 4) and way([500] * 32, [4] * 32) == ("codes",)
+    assert way([5000, 5600, 6300, 7000], [5, 24, 11, 18], 40, window=4096) == ("tiles", 32, 4)
+    assert way([300] * 4, [24] * 4, 40) == ("tiles", 32, 1) and way([0], [4096])[0] == "pages"
+    assert way([2000, 10, 300], [100, 1, 0])[0] == "tiles"
+    # sizes that the kernel for tiles does not take
+    assert way([2000], [8], tokens=0) == ("codes",) and way([1952], [96], tokens=0) == ("codes",) and way([0], [2048], tokens=0) == ("pages",)
+    assert way([2000] * 4, [40] * 4, 40, tokens=0) == ("codes",) and way([1952] * 4, [96] * 4, 40, tokens=0) == ("pages",)
+    assert way([100], [64], form=0, tokens=0) == ("codes",) and way([40000], [60], window=128, tokens=0) == ("codes",)
+    assert way([0], [100], d=80, form=1, tokens=0, codes=False) == ("pages",) and way([0], [5], d=80, form=1, tokens=0, codes=False) == ("codes",)
