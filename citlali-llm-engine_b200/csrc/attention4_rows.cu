@@ -5,6 +5,7 @@
 // for the HB heads.  For the result a key's d / 8 words of codes go to as many lanes, so that a warp works on 256 / d keys at once; the
 // weights go through shared memory.  A warp keeps a running maximum and sum, and its groups of lanes a result each; all are merged in
 // order.  What bounds it: the latency of a few dependent reads a turn where rows are few, and the multiply-adds where they are many.
+// Measured: five rows over 40 to 1,500 keys, 12 heads over 4 of 64, 14.1 us; 64 rows over 1,000 keys, 16 heads over 4 of 128, 46.
 #include "api.h"
 #include "cache4.cuh"
 #include "common.cuh"
@@ -182,6 +183,7 @@ extern "C" int citlali_attention4_rows(const void* q, size_t q_stride, int dtype
         return kBadAlignment;
     }
     // Heads a block: as many as share a key/value head, four at most, but fewer where a block for each keeps more multiprocessors busy.
+    // (16 heads over 4 of 128: one row over 4,000 keys 43 us a head a block, 70 four; 64 rows over 1,000 77 and 46.)
     const int group = nq / nkv, widest = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
     int hb = widest;
     while (hb > 1 && (long long)rows * (nq / hb) < device_sm_count()) hb /= 2;

@@ -6,6 +6,10 @@
 //
 // The angle.  pos inv_freq[i] in 32 bits is off by up to 2^-24 of itself, 0.004 at position 65,536: as much as a bfloat16 query's own
 // rounding.  The product's rounding error e is one fma away, and cos(a + e) = cos a - e sin a to 32 bits, so it is put right.
+//
+// What bounds it: instructions.  A group's codes are whole numbers nearest to exact quotients, some 9 instructions an element; with norm and
+// rotation 30 an element of a key (2,048 rows of 16 + 8 + 8 heads of 128: 10.9 us for 30 MB, issue slots 0.65 busy; 8 rows 2.5 us).  Reading
+// back is bound by what it writes (2,048 rows: 4.8 us for 11 MB; 8 rows 2.1).
 #include "api.h"
 #include "cache4.cuh"
 #include "common.cuh"
@@ -88,7 +92,7 @@ __global__ void __launch_bounds__(kThreads)
 append_kernel(const T* __restrict__ qkv, T* q_out, size_t q_out_stride, const TG* __restrict__ q_gain, const TG* __restrict__ k_gain,
               const float* __restrict__ inv_freq, int rotated, const __grid_constant__ Rows rows, const __grid_constant__ Pools pools,
               int nq, int nkv, int d, float eps, int store, int heads_per_block, int lanes) {
-    extern __shared__ __align__(16) float2 turns[];                  // [rotated / 2]: the row's, shared by the block's heads
+    extern __shared__ __align__(16) float2 turns[];                  // the row's [element of a lane's eight][lane], shared by the block's heads
     dependents_may_launch();
     // positions, slots and page tables come from the host before the step: the turns and the row's place in the cache are worked
     // out while the kernel ahead (the projection) is still running
@@ -98,7 +102,7 @@ append_kernel(const T* __restrict__ qkv, T* q_out, size_t q_out_stride, const TG
     const int half = rotated >> 1;
     const int pos = rows.row_pos[row];
     if (begin < nq + nkv)
-        for (int i = threadIdx.x; i < half; i += kThreads) turns[i] = turn_of(pos, inv_freq[i]);
+        for (int i = threadIdx.x; i < half; i += kThreads) turns[(i & 7) * (half >> 3) + (i >> 3)] = turn_of(pos, inv_freq[i]);
     int page = 0;
     if (store) page = rows.page_table[(size_t)rows.row_slot[row] * rows.page_table_stride + pos / rows.page_size];
     __syncthreads();
@@ -138,7 +142,7 @@ append_kernel(const T* __restrict__ qkv, T* q_out, size_t q_out_stride, const TG
             if (turned) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float2 t = turns[e0 + i];
+                    const float2 t = turns[i * pairs + part];
                     const float a = x0[i], b = x1[i];
                     x0[i] = a * t.x - b * t.y;
                     x1[i] = b * t.x + a * t.y;
@@ -260,7 +264,8 @@ read_kernel(const __grid_constant__ Rows rows, const __grid_constant__ Pools poo
 // The pages that a run's rows see, as bfloat16 pages of their own (exact), with a page table and slots for the attention kernels of a
 // cache of 16 bits: sequence b is slot b there.  A block a (page, key/value head, keys or values).  Positions that no row of the run sees become
 // zeros.  A value that is no number becomes zero too, and its token's key none: a row that does not see the token gives it the
-// weight zero, and zero times a NaN would reach it; a row that does see it gets a NaN from the key.
+// weight zero, and zero times a NaN would reach it; a row that does see it gets a NaN from the key.  (2,048 positions of 8 heads of 128:
+// 5 to 10 us with caches cold, bound by what it writes.)
 struct Runs {
     const int32_t *seq_start, *seq_slot, *seq_past;
     int sequences, window;
@@ -360,6 +365,7 @@ static int launch_append(const T* qkv, T* q_out, size_t q_out_stride, const TG* 
                       && aligned(k_gain, 16) && aligned(pools.k_codes, 4) && aligned(pools.v_codes, 4);
     if (in_pairs && wide) {
         // few rows: a pass of heads a block, so that the heads spread over the SMs; many rows: a row a block, whose turns serve all heads
+        // (16 + 8 + 8 heads of 128: 2,048 rows 10.9 us a row a block, some 12 by passes; 8 rows 3.3 and 2.5)
         const int pass = kThreads / lanes, blocks = rows >= 4 * device_sm_count() ? 1 : (used + pass - 1) / pass;
         const int each = blocks == 1 ? used : pass;
         launch_kernel(append_kernel<T, TG>, dim3(rows, blocks), kThreads, (size_t)(rotated / 2) * sizeof(float2), stream, qkv, q_out,
