@@ -189,12 +189,12 @@ int citlali_cache4_read(const void* k_codes, const void* k_scales, const void* v
                         const int32_t* slots, const int32_t* positions, void* keys, void* values, int out_dtype, int rows, int nkv,
                         int head_dim, cudaStream_t stream);
 // Attention of runs of new tokens over the cache in 4 bits on tcgen05 (bfloat16; head sizes 64 and 128, pages of 64).  A tile is
-// citlali_attention4_runs_tokens() tokens of a sequence (0: other sizes) for one key/value head; tiles: of all sequences and key/value
-// heads; cluster: the blocks (1, 2, 4 or 8) that share a tile's pages.
+// citlali_attention4_runs_tokens() tokens of a sequence (0: other sizes) for one key/value head; sequences with fewer than least_new new
+// tokens are left out; tiles: of all others and key/value heads; cluster: the blocks (1, 2, 4 or 8) that share a tile's pages.
 int citlali_attention4_runs_tokens(int nq, int nkv, int head_dim, int page_size);
 int citlali_attention4_runs(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes,
                             const void* v_scales, const int32_t* page_table, int page_table_stride, const int32_t* seq_start,
-                            const int32_t* seq_slot, const int32_t* seq_past, void* out, size_t out_stride, int sequences, int tiles,
+                            const int32_t* seq_slot, const int32_t* seq_past, void* out, size_t out_stride, int sequences, int least_new, int tiles,
                             int cluster, int nq, int nkv, int head_dim, int page_size, int window, float scale, cudaStream_t stream);
 // The pages of 64 that runs of new tokens see (from the pair with past - window + 1 on, if there is a window), as bfloat16: page after page of the
 // sequences [pages, nkv, 64, head_dim], zeros where no row sees anything; table_out [sequences, table_out_stride] and slots_out
@@ -210,7 +210,7 @@ int citlali_attention4_rows(const void* q, size_t q_stride, int dtype, const voi
                             const int32_t* row_slot, const int32_t* row_pos, void* out, size_t out_stride, int rows, int nq,
                             int nkv, int head_dim, int page_size, int window, float scale, cudaStream_t stream);
 // The same on the tensor cores, bfloat16, for single tokens (seq_start null: a row a sequence, seq_slot and seq_past the rows' slots and
-// positions) and for runs of at most max_new tokens.  Lengths are read on the device only.  partial: as many floats as
+// positions) and for runs of at most max_new tokens (sequences with more are left out).  Lengths are read on the device only.  partial: as many floats as
 // citlali_attention4_scratch_floats says, of this call alone.  arrived (may be null: a second kernel merges what blocks share): counters,
 // two a multiprocessor, zero before the call and zero again behind it, that no other call on its way uses.
 int citlali_attention4_supports(int head_dim, int page_size);

@@ -30,8 +30,8 @@
 // that merges them in the same order, or, where the caller gives counters, for the block that comes last (one sequence of 900 keys: 8.8 us,
 // with the second kernel 10.0).  So every sum has an order that the step's lengths fix.
 //
-// Measured (16 heads over 8 of 128, single tokens): 64 sequences of mixed lengths, 170 MB, 50.7 us; 8 of 4,096 18.0; two of 40,960 30.5; one
-// of 900 7.6.  A unit takes a warp some 4,000 clocks, sixteen warps an SM, which is 5.2 TB/s of the 6.5 there are: the integer
+// Measured (single tokens, heads of 128): 64 sequences of 128 to 8,192 keys, 40 heads over 8, 170 MB, 50.7 us; 16 heads over 8: 8 of 4,096
+// keys, 38 MB, 18.0, two of 40,960 30.5, one of 900 7.6.  A unit takes a warp some 4,000 clocks, sixteen warps an SM, which is 5.2 TB/s of the 6.5 there are: the integer
 // pipe that picks codes apart is busy half of the time, latencies are the rest.  Some 10 us go by beside that: the launch, the first
 // reads (lengths, page numbers, codes, one after another: 3), and merging what warps and blocks share (3 to 4).
 #include "api.h"
@@ -47,7 +47,7 @@ constexpr int kWarps4 = 8, kThreads4 = 32 * kWarps4;
 constexpr float kWeightBits = 11.0f, kMostBits = 15.0f;         // of the largest weight when the maximum is looked for, and before it is again
 constexpr uint32_t kOnes = 0x3c003c00u;
 constexpr float kNoScore = -3.402823466e+38f;
-// What beginning a segment costs, in units (one of 900 keys, 64 of mixed lengths: 1 unit 9.4, 52.9 us; 2 8.7, 52.1; 4 7.8, 51.0).
+// What beginning a segment costs, in units (one of 900 keys, 64 of 128 to 8,192: 1 unit 9.4, 52.9 us; 2 8.7, 52.1; 4 7.8, 51.0).
 constexpr int kRoom = 4;
 
 struct Attention4 {
@@ -62,6 +62,7 @@ struct Attention4 {
     int sequences, nq, nkv, group;
     int tokens, heads, head_tiles;                       // of a tile; the tiles a group's heads are cut into
     int window;
+    int most;                                            // sequences with more new tokens than this are left out
     float scale_log2;
     float* partial;                                      // [blocks][2][columns][m, l, two unused, D values]
     int32_t* arrived;                                    // [blocks], zero before and after: parts in memory of the segment that begins in a block
@@ -77,6 +78,7 @@ __device__ __forceinline__ Sequence sequence_of(const Attention4& a, int b) {
     s.past = a.seq_past[b];
     s.row = a.seq_start ? a.seq_start[b] : b;
     s.fresh = a.seq_start ? a.seq_start[b + 1] - s.row : 1;
+    if (s.fresh > a.most) s.fresh = 0;
     const int lo = a.window > 0 ? max(0, s.past - a.window + 1) : 0;
     s.first_unit = lo / kUnitKeys;
     s.units = s.fresh > 0 ? (s.past + s.fresh - 1) / kUnitKeys - s.first_unit + 1 : 0;
@@ -741,7 +743,7 @@ attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
 }
 
 // How a step's columns are tiled: 8 at a time where a segment has no more (two blocks an SM), else 16 (one).  16 for 8 columns: one
-// sequence of 900 keys 7.7 -> 8.3 us, 8 of 4,096 18.0 -> 22.8, 64 of mixed lengths 50.7 -> 70.0.
+// sequence of 900 keys 7.7 -> 8.3 us, 8 of 4,096 18.0 -> 22.8, 64 of 128 to 8,192 50.7 -> 70.0.
 struct Tiling {
     int wide;            // columns / 8
     int tokens, heads, head_tiles;
@@ -834,7 +836,7 @@ extern "C" int citlali_attention4(const void* q, size_t q_stride, const void* k_
     a.out = (__nv_bfloat16*)out; a.out_stride = out_stride;
     a.sequences = sequences; a.nq = nq; a.nkv = nkv; a.group = nq / nkv;
     a.tokens = t.tokens; a.heads = t.heads; a.head_tiles = t.head_tiles;
-    a.window = window; a.scale_log2 = scale * 1.4426950408889634f; a.partial = partial; a.arrived = arrived;
+    a.window = window; a.most = max_new; a.scale_log2 = scale * 1.4426950408889634f; a.partial = partial; a.arrived = arrived;
     if (head_dim == 64) return t.wide == 1 ? c4::launch<64, 1>(a, blocks, stream) : c4::launch<64, 2>(a, blocks, stream);
     if (head_dim == 128) return t.wide == 1 ? c4::launch<128, 1>(a, blocks, stream) : c4::launch<128, 2>(a, blocks, stream);
     return c4::launch<256, 1>(a, blocks, stream);

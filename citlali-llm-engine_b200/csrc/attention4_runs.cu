@@ -66,6 +66,7 @@ struct Runs4 {
     __nv_bfloat16* out;
     size_t out_stride;
     int sequences, nq, nkv, group, tokens;                           // tokens: of a tile
+    int least;                                                       // sequences with fewer new tokens are left out
     int window, cluster;
     float scale_log2;
 };
@@ -207,7 +208,8 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
 #pragma unroll 1
         for (int b0 = 0; b0 < a.sequences && b < 0; b0 += 32) {
             int mine = 0;
-            if (b0 + lane < a.sequences) mine = (a.seq_start[b0 + lane + 1] - a.seq_start[b0 + lane] + a.tokens - 1) / a.tokens * a.nkv;
+            if (b0 + lane < a.sequences) mine = a.seq_start[b0 + lane + 1] - a.seq_start[b0 + lane];
+            mine = mine < a.least ? 0 : (mine + a.tokens - 1) / a.tokens * a.nkv;
             int sum = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -619,7 +621,7 @@ extern "C" int citlali_attention4_runs_tokens(int nq, int nkv, int head_dim, int
 extern "C" int citlali_attention4_runs(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes,
                                        const void* v_scales, const int32_t* page_table, int page_table_stride, const int32_t* seq_start,
                                        const int32_t* seq_slot, const int32_t* seq_past, void* out, size_t out_stride, int sequences,
-                                       int tiles, int cluster, int nq, int nkv, int head_dim, int page_size, int window, float scale,
+                                       int least_new, int tiles, int cluster, int nq, int nkv, int head_dim, int page_size, int window, float scale,
                                        cudaStream_t stream) {
     if (sequences <= 0 || tiles <= 0) return 0;
     const int tokens = citlali_attention4_runs_tokens(nq, nkv, head_dim, page_size);
@@ -646,6 +648,7 @@ extern "C" int citlali_attention4_runs(const void* q, size_t q_stride, const voi
     a.seq_start = seq_start; a.seq_slot = seq_slot; a.seq_past = seq_past;
     a.out = (__nv_bfloat16*)out; a.out_stride = out_stride;
     a.sequences = sequences; a.nq = nq; a.nkv = nkv; a.group = nq / nkv; a.tokens = tokens;
+    a.least = least_new > 1 ? least_new : 1;
     a.window = window; a.cluster = cluster; a.scale_log2 = scale * 1.4426950408889634f;
     return head_dim == 64 ? c4::launch_runs<64>(a, tiles, stream) : c4::launch_runs<128>(a, tiles, stream);
 }

@@ -592,8 +592,8 @@ _EXPAND_BYTES = 1 << 30
 
 
 def _attention4_way(batch, nq: int, nkv: int, head_dim: int, window: int, form: int, tokens: int, codes: bool, sms: int) -> tuple:
-    """How a step's runs of tokens are attended to: ("tiles", tiles, blocks that share one) by the kernel on tcgen05 (``tokens`` of a tile; 0:
-    it does not take the sizes), ("pages",) by prompt attention (``form``: 2 on tcgen05, 1 on mma.sync, 0 not at all) over pages that are
+    """How a step's runs of tokens are attended to: ("tiles", n, tiles, blocks that share one) by the kernel on tcgen05 (``tokens`` of a tile; 0:
+    it does not take the sizes), but sequences of up to n new tokens, if n is not 0, by the kernel for single tokens, ("pages",) by prompt attention (``form``: 2 on tcgen05, 1 on mma.sync, 0 not at all) over pages that are
     made bfloat16 first, or ("codes",) by the kernel for single tokens, if it takes the sizes, or that in 32 bits.  The one that takes least
     time, in microseconds, by what each was measured to do:
     codes: 10 and (more than 8 columns) 3 ahead, a tile of 16 columns (8 at head size 256) over 32 keys in `unit`, divided over all SMs;
@@ -602,36 +602,53 @@ def _attention4_way(batch, nq: int, nkv: int, head_dim: int, window: int, form: 
     while that leaves a block more than six (of clusters of 8 no more than two thirds of the SMs).
     Measured, codes / pages / tiles: one run over 2,048 keys, 16 heads over 8 of 128, 4 new tokens 12.6 / - / 13.0, 16: 16.9 / - / 13.1, 64: 25 / 52 /
     14, 2,048: 220 / 53 / 37; four over 8,000, 6 tokens: 29.8 / - / 33.9, 16: 43.9 / - / 34.5; one over 32,768, 64: 116 / 619 / 60; 32 over 500, 8
-    tokens: 19.6 / - / 25.4; 4,096 new tokens: 761 / 96 / 113; heads of 64, 32 over 8, one over 8,192, 96 tokens: 68 / 195 / 31.  Tiles
+    tokens: 19.6 / - / 25.4; one of 512 among 63 of one over 4,000 keys: 119 / 935 / 210, the short ones by codes 86; 4,096 new tokens: 761 / 96 / 113; heads of 64, 32 over 8, one over 8,192, 96 tokens: 68 / 195 / 31.  Tiles
     shared by 1, 2, 4 and 8: four over 4,096, 40 over 8 heads, 5 to 24 tokens (32 tiles): 55, 35, 24, 50; one over 32,768 (8 tiles): 375, 194,
     104, 60; 300 keys (32 tiles): 11.6, 12.4, 13.1, 34.6."""
     n_new, group = batch.n_new, nq // nkv
     max_new, columns = max(n_new), 8 if head_dim == 256 else 16
     head_tiles = -(-group // columns)
     at_once = columns // -(-group // head_tiles)
-    units = tiles = far = walked = 0
+    few = max(1, 8 // group)                         # as many new tokens make at most 8 columns, or are one
+    units = units_few = tiles = far = walked = tiles_few = far_few = walked_few = 0
     for past, n in zip(batch.past, n_new):           # (the host's time counts: one short step a sequence)
         end = past + n
         keys = end if not window or end < window + n else window + n
-        units += -(-n // at_once) * (keys // 32 + 16)
-        if tokens:
-            here = -(-n // tokens)
-            seen = keys // 64 + 1 if not window or n <= tokens or keys < window + tokens else (window + tokens) // 64 + 1          # pages of the last tile
+        work = -(-n // at_once) * (keys // 32 + 16)
+        here = -(-n // tokens) if tokens else 0
+        seen = keys // 64 + 1 if not window or n <= tokens or keys < window + tokens else (window + tokens) // 64 + 1          # pages of the last tile
+        if n <= few:
+            units_few += work
+            tiles_few += here
+            walked_few += here * seen
+            if seen > far_few:
+                far_few = seen
+        else:
+            units += work
             tiles += here
+            walked += here * (seen if window else seen - (n >> 7))
             if seen > far:
                 far = seen
-            walked += here * (seen if window else seen - (n >> 7))
-    unit, start = {64: 1.3e-3, 128: 1.6e-3}.get(head_dim, 2.8e-3), 13 if min(group, columns) * max_new > 8 else 10
-    best = start + units * head_tiles * nkv * unit if codes else 1e9 if max_new >= 16 else 0                 # (few rows in 32 bits: no worse)
-    way = ("codes",)
-    if tokens:
+
+    def in_tiles(tiles, far, walked):
         shared = 1
-        tiles *= nkv
         while shared < 8 and far > 6 * shared and 2 * shared * tiles <= (sms if shared < 4 else 2 * sms // 3):
             shared *= 2
-        time = 7 + max(far / shared * 0.73 + (3 if shared > 1 else 0), (walked * nkv * 0.73 + tiles * 4) / sms)
+        return 7 + max(far / shared * 0.73 + (3 if shared > 1 else 0), (walked * nkv * 0.73 + tiles * 4) / sms), shared
+    unit, start = {64: 1.3e-3, 128: 1.6e-3}.get(head_dim, 2.8e-3), 13 if min(group, columns) * max_new > 8 else 10
+    unit *= head_tiles * nkv
+    best = start + (units + units_few) * unit if codes else 1e9 if max_new >= 16 else 0                 # (few rows in 32 bits: no worse)
+    way = ("codes",)
+    if tiles:
+        all_tiles = (tiles + tiles_few) * nkv
+        time, shared = in_tiles(all_tiles, max(far, far_few), walked + walked_few)
         if time < best:
-            best, way = time, ("tiles", tiles, shared)
+            best, way = time, ("tiles", 0, all_tiles, shared)
+        if tiles_few and codes:
+            time, shared = in_tiles(tiles * nkv, far, walked)
+            time += 8 + units_few * unit
+            if time < best:
+                best, way = time, ("tiles", few, tiles * nkv, shared)
     if form > 0 and best > 40 and max_new >= 48:
         time = _attention4_pages_time(batch, nq, nkv, head_dim, window, form, sms)
         if time < best:
@@ -740,7 +757,7 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
     if rows == 0:
         return
     kc, ks, vc, vs, table, table_width = pools
-    q_ptr, window = q.data_ptr(), _i(window or 0)
+    q_ptr, window, most = q.data_ptr(), _i(window or 0), 0
     if window < 0:
         require(False, f"cache4_attention: the window is a number of keys (0 or None: all), not {window}")
     # (runs by the host's lists of lengths, which a captured step would freeze: there the kernel for single tokens reads the device's)
@@ -758,12 +775,15 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
             _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, float(scale))
             return
         if way[0] == "tiles":
+            most = way[1]                                            # new tokens of the sequences that the kernel for single tokens takes
             _check(lib().citlali_attention4_runs(
                 q_ptr, _sz(q_stride), kc, ks, vc, vs, table, table_width, seq_start.data_ptr(), batch.seq_slot.data_ptr(), batch.seq_past.data_ptr(),
-                out.data_ptr(), wide, len(batch.slots), way[1], way[2], nq, nkv, head_dim, 64, window, _f(scale), _stream()), "cache4_attention_runs")
-            return
+                out.data_ptr(), wide, len(batch.slots), most + 1, way[2], way[3], nq, nkv, head_dim, 64, window, _f(scale), _stream()),
+                "cache4_attention_runs")
+            if most == 0:
+                return
     if q.dtype is torch.bfloat16 and q_stride % 8 == 0 and (q_ptr | kc | ks | vc | vs) % 16 == 0 and nkv > 0 and nq % nkv == 0:
-        max_new = 1 if single else batch.max_new
+        max_new = 1 if single else most or batch.max_new
         floats = _attention4_floats(nq, nkv, head_dim, kv.page_size, max_new, _current_device())
         if floats >= 0:
             # of this call alone, and given back in stream order: two graphs, or two streams, share nothing

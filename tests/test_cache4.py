@@ -137,11 +137,11 @@ def test_which_way_runs_go():
         batch = cb.StepBatch(*[torch.zeros(1, dtype=torch.int32)] * 7, slots=list(range(len(new))), past=past, n_new=new)
         return ops._attention4_way(batch, nq, nkv, d, window, form, 128 // (nq // nkv) if tokens is None else tokens, codes, 148)
     # few columns read the codes, more of them go in tiles that as many blocks share as fit at once, the longest prompts over pages
-    assert way([2000], [4]) == ("codes",) and way([2000], [64]) == ("tiles", 8, 8) and way([0], [2048]) == ("tiles", 256, 1)
-    assert way([8000] * 4, [6] * 4) == ("codes",) and way([8000] * 4, [16] * 4) == ("tiles", 32, 4) and way([500] * 32, [4] * 32) == ("codes",)
-    assert way([5000, 5600, 6300, 7000], [5, 24, 11, 18], 40, window=4096) == ("tiles", 32, 4)
-    assert way([300] * 4, [24] * 4, 40) == ("tiles", 32, 1) and way([0], [4096])[0] == "pages"
-    assert way([2000, 10, 300], [100, 1, 0])[0] == "tiles"
+    assert way([2000], [4]) == ("codes",) and way([2000], [64]) == ("tiles", 0, 8, 8) and way([0], [2048]) == ("tiles", 0, 256, 1)
+    assert way([8000] * 4, [6] * 4) == ("codes",) and way([8000] * 4, [16] * 4) == ("tiles", 0, 32, 4) and way([500] * 32, [4] * 32) == ("codes",)
+    assert way([5000, 5600, 6300, 7000], [5, 24, 11, 18], 40, window=4096) == ("tiles", 0, 32, 4)
+    assert way([300] * 4, [24] * 4, 40) == ("tiles", 0, 32, 1) and way([0], [4096])[0] == "pages"
+    assert way([2000, 10, 300], [100, 1, 0])[:2] == ("tiles", 0) and way([0] + [4000] * 63, [512] + [1] * 63)[:3] == ("tiles", 4, 64)
     # sizes that the kernel for tiles does not take
     assert way([2000], [8], tokens=0) == ("codes",) and way([1952], [96], tokens=0) == ("codes",) and way([0], [2048], tokens=0) == ("pages",)
     assert way([2000] * 4, [40] * 4, 40, tokens=0) == ("codes",) and way([1952] * 4, [96] * 4, 40, tokens=0) == ("pages",)

@@ -223,7 +223,7 @@ def test_large_and_tiny_numbers_are_held_at_the_ends_of_the_range():
 # ---- attention --------------------------------------------------------------------------------------------------------------
 
 def check_attention(st, nq, dtype, window, seed, out_rows=None, scale=None, expect_nan=None, way=("codes",)):
-    """By the kernels that read codes: those for single tokens, or with ``way`` ("tiles", tiles, cluster) the one for runs."""
+    """By the kernels that read codes: those for single tokens, or with ``way`` ("tiles", 0, tiles, cluster) the one for runs."""
     g = torch.Generator().manual_seed(seed)
     nkv, d, group = st.nkv, st.d, nq // st.nkv
     rows = len(st.row_slot)
@@ -330,7 +330,22 @@ def tiles_of(nq, nkv, new):
 def test_runs_of_tokens_in_tiles(nq, nkv, d, past, new, window, cluster):
     st = Step(past, new, nkv, d, seed=nq + d)
     st.fill(sum(new))
-    check_attention(st, nq, torch.bfloat16, window, nq, out_rows=sum(new) + 1, way=("tiles", tiles_of(nq, nkv, new), cluster))
+    check_attention(st, nq, torch.bfloat16, window, nq, out_rows=sum(new) + 1, way=("tiles", 0, tiles_of(nq, nkv, new), cluster))
+
+
+@pytest.mark.parametrize("nq,nkv,d,past,new,window,few", [
+    (4, 2, 128, [300, 0, 77, 1000, 5, 64], [1, 90, 4, 1, 0, 5], 0, 4),
+    (8, 1, 64, [10, 700, 0], [1, 1, 33], 50, 1),
+    (5, 1, 128, [10, 70], [40, 1], 0, 1),
+])
+def test_short_and_long_runs_in_one_step(nq, nkv, d, past, new, window, few):
+    """Sequences of up to ``few`` new tokens by the kernel for single tokens, the others in tiles: each row by one of them."""
+    st = Step(past, new, nkv, d, seed=nq + d)
+    st.fill(sum(new))
+    before = ops.launch_count()
+    check_attention(st, nq, torch.bfloat16, window, nq, out_rows=sum(new) + 1,
+                    way=("tiles", few, tiles_of(nq, nkv, [n for n in new if n > few]), 2))
+    assert ops.launch_count() - before == 2
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -344,7 +359,7 @@ def test_a_token_that_is_not_finite_in_tiles(d, which, window, cluster):
     part = getattr(st, which)
     part.scales[int(st.table[slot, at // 64]), 0, at % 64, d // 16 - 1] = 255
     check_attention(st, 2, torch.bfloat16, window, 2, expect_nan=lambda s, p: s == slot and p >= at and (not window or p < at + window),
-                    way=("tiles", tiles_of(2, 1, st.new), cluster))
+                    way=("tiles", 0, tiles_of(2, 1, st.new), cluster))
 
 
 def test_tiles_whose_scores_spread_and_odd_queries():
@@ -352,7 +367,7 @@ def test_tiles_whose_scores_spread_and_odd_queries():
     st.fill(9)
     new = st.new
     for cluster in (1, 4):
-        way = ("tiles", tiles_of(4, 2, new), cluster)
+        way = ("tiles", 0, tiles_of(4, 2, new), cluster)
         check_attention(st, 4, torch.bfloat16, 0, 3, scale=1.0, way=way)             # weights from 1 to 2^-200
         check_attention(st, 4, torch.bfloat16, 0, 4, scale=0.0, way=way)             # all keys alike
         q = torch.randn(75, 4 * 128, generator=torch.Generator().manual_seed(1)).bfloat16()
@@ -590,7 +605,7 @@ def test_refusals():
         with pytest.raises(cb.CitlaliError, match="not over their queries"):
             ops.cache4_append(q, kv, batch.row_slot, batch.row_pos, 4, 2, 64, f, 64, q_out=over)
     runs = Step([10], [2], 2, 64).batch()
-    for way, words in ((("tiles", 2, 3), "clusters"), (("tiles", 2, 16), "clusters"), (("tiles", 2, 0), "clusters")):
+    for way, words in ((("tiles", 0, 2, 3), "clusters"), (("tiles", 0, 2, 16), "clusters"), (("tiles", 0, 2, 0), "clusters")):
         runs.runs4[4, 2, 64, 0, 512] = way
         with pytest.raises(cb.CitlaliError, match=words):
             ops.cache4_attention(q, 512, kv, runs, out, 4, 2, 64, 0, 0.1)
@@ -664,7 +679,7 @@ def test_a_token_that_is_not_finite_in_a_longer_run(d, which, window):
     check_long_run(st, 2, window, 2, expect_nan=lambda s, p: s == slot and p >= at and (not window or p < at + window))
 
 
-@pytest.mark.parametrize("way", [("codes",), ("pages",), ("tiles", 4, 2)])
+@pytest.mark.parametrize("way", [("codes",), ("pages",), ("tiles", 0, 4, 2)])
 def test_queries_that_end_with_their_last_row(way):
     """Rows of a wider projection, and nothing behind the last row's queries."""
     st = Step([40, 0], [60, 30], 2, 128, seed=8)
