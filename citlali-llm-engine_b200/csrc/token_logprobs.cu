@@ -203,10 +203,13 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
     const int tiles = (stop - first) / kTile;            // whole ones
     const int tail = lead + vectors * kVec;
     const T* base = x + lead + ((long long)first + tid) * kVec;
+    // A share of less than a tile goes to the threads an entry at a time, so that all have some and the warps' largest make a bound
+    // (1,000 rows of 700 bfloat16 entries, five likeliest: 55 us in vectors, 15 so; longer ones lose a microsecond by it).
+    const bool spread = TOP && tiles == 0;
     auto index_of = [&](int tile, int thread, int e) {   // the entry's, or -1: there is none
         if (tile <= tiles) {
-            const int vector = first + tile * kTile + e / kVec * kThreads + thread;
-            return vector < stop ? lead + vector * kVec + e % kVec : -1;
+            const int i = spread ? first * kVec + e * kThreads + thread : (first + tile * kTile + e / kVec * kThreads + thread) * kVec + e % kVec;
+            return i < stop * kVec ? lead + i : -1;
         }
         if (e == 0 && rank == 0 && thread < lead) return thread;
         return e == 0 && rank == cluster - 1 && thread >= 32 && tail + thread - 32 < vocab ? tail + thread - 32 : -1;
@@ -224,14 +227,22 @@ token_logprobs_kernel(const T* __restrict__ logits, const int32_t* __restrict__ 
         }
         const int rest = first + tiles * kTile;
         if (to > tiles && rest < stop) {
+            if (spread) {
 #pragma unroll
-            for (int k = 0; k < kEach / kVec; ++k) {
-                const int vector = rest + k * kThreads + tid;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (vector < stop) v = *reinterpret_cast<const uint4*>(x + lead + (long long)vector * kVec);
-                const T* in = reinterpret_cast<const T*>(&v);
+                for (int e = 0; e < kEach; ++e) {
+                    const int index = index_of(tiles, tid, e);
+                    y[e] = index >= 0 ? ldf(x, index) : -INFINITY;
+                }
+            } else {
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) y[k * kVec + e] = vector < stop ? ldf(in, e) : -INFINITY;
+                for (int k = 0; k < kEach / kVec; ++k) {
+                    const int vector = rest + k * kThreads + tid;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (vector < stop) v = *reinterpret_cast<const uint4*>(x + lead + (long long)vector * kVec);
+                    const T* in = reinterpret_cast<const T*>(&v);
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) y[k * kVec + e] = vector < stop ? ldf(in, e) : -INFINITY;
+                }
             }
             use(y, tiles);
         }

@@ -56,7 +56,8 @@ def check(x, tokens, top):
 
 
 @pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (1, 1, 0), (3, 5, 5), (2, 31, 31), (5, 33, 32), (1, 4096, 20), (7, 4097, 3), (2, 50257, 5),
-                                            (9, 8191, 32), (3, 151936, 20), (700, 1001, 7), (1, 300001, 32), (4, 12289, 1)])
+                                            (9, 8191, 32), (3, 151936, 20), (700, 1001, 7), (1, 300001, 32), (4, 12289, 1),
+                                            (3, 520, 32), (2, 700, 5), (3, 1500, 32), (4, 2047, 20), (2, 4100, 32)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_against_64_bits(rows, vocab, top, dtype):
     g = torch.Generator().manual_seed(rows * 31 + vocab)
