@@ -212,7 +212,7 @@ int citlali_attention4_rows(const void* q, size_t q_stride, int dtype, const voi
 // The same on the tensor cores, bfloat16, for single tokens (seq_start null: a row a sequence, seq_slot and seq_past the rows' slots and
 // positions) and for runs of at most max_new tokens (sequences with more are left out).  Lengths are read on the device only.  partial: as many floats as
 // citlali_attention4_scratch_floats says, of this call alone.  arrived (may be null: a second kernel merges what blocks share): counters,
-// two a multiprocessor, zero before the call and zero again behind it, that no other call on its way uses.
+// four a multiprocessor, zero before the call and zero again behind it, that no other call on its way uses.
 int citlali_attention4_supports(int head_dim, int page_size);
 size_t citlali_attention4_scratch_floats(int nq, int nkv, int head_dim, int max_new);
 int citlali_attention4(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes,

@@ -65,7 +65,7 @@ struct Attention4 {
     int most;                                            // sequences with more new tokens than this are left out
     float scale_log2;
     float* partial;                                      // [blocks][2][columns][m, l, two unused, D values]
-    int32_t* arrived;                                    // [blocks], zero before and after: parts in memory of the segment that begins in a block
+    int32_t* arrived;                                    // [2][blocks], zero before and after: parts in memory of the segment that begins in a block, and of a group of them
 };
 
 // What a sequence of the step asks for: `units` of 32 keys for each of `segments` (head tile of a key/value head, token tile).
@@ -214,62 +214,69 @@ struct Layout {
     static constexpr int jobs = 8;                       // at most one a stage, one that ends, one that was looked up, and the end
     static_assert(stages + 3 <= jobs && (jobs & (jobs - 1)) == 0, "a piece's description is read before it is written over");
     static constexpr int ring = stages * stage;
-    static_assert(ring >= parked && ring % 16 == 0 && parked % 16 == 0, "a warp parks its last part in its ring");
+    static_assert(ring >= parked && ring % 64 == 0 && (codes + scales) % 64 == 0 && parked % 16 == 0, "a warp parks its last part in its ring");
     static constexpr int bytes = kWarps4 * (ring + parked + 2 * (int)sizeof(Part) + jobs * (int)sizeof(Job));
     static constexpr int per_sm = D == 256 ? 1 : (NT == 1 ? 2 : 1);
 };
 
-// The result of a segment from its parts in memory, part 0 in slot 1 of block `first`, part p in slot 0 of block first + p, in the order
-// of the keys.  All parts are brought to shared memory at once (`room` bytes there), as many columns at a time as fit.  This runs once
-// in a block, when its instructions have yet to be fetched: short loops are worth more here than unrolled ones.
+// The result of a segment from its parts in memory (`to` null), or one part from several: part 0 is in slot 1 of block `first`, part p in
+// slot 0 of block first + p; `count` of them, from `from` on, `step` apart, in the order of the keys.  They are brought to shared memory (`room`
+// bytes there), at most kParts at once and as many columns at a time as fit (more parts: as many as the threads have one element each
+// of).  This runs once in a block, when its instructions have yet to be fetched: short loops are worth more here than unrolled ones.
+constexpr int kParts = 32;
 template <int D>
-__device__ __forceinline__ void merge_parts(const Attention4& a, int columns, int first, int parts, int row, int used, int head0, int heads,
-                                            uint8_t* shared, int room, int threads) {
+__device__ __forceinline__ void merge_parts(const Attention4& a, int columns, int first, int from, int step, int count, const Part& part,
+                                            float* to, uint8_t* shared, int room, int threads) {
     constexpr int kRow = (D + 4) * 4;                    // bytes of a part's column
-    const int inverse = inverse_of(heads), slot = columns * kRow, fit = parts * used * kRow <= room ? used : min(used, room / (parts * kRow));
-    const uint8_t* part0 = reinterpret_cast<const uint8_t*>(a.partial) + (size_t)(first * 2 + 1) * slot;
-    auto its = [&](int p) { return part0 + (size_t)p * (2 * slot) - (p ? slot : 0); };
+    const int inverse = inverse_of(part.heads), slot = columns * kRow, at_once = min(count, kParts);
+    const int fit = min(min(part.used, room / (at_once * kRow)), count > at_once ? threads / D : part.used);
+    auto its = [&](int q) {
+        const int p = from + q * step;
+        return reinterpret_cast<const uint8_t*>(a.partial) + (size_t)((first + p) * 2 + (p == 0)) * slot;
+    };
     const uint32_t dst = (uint32_t)__cvta_generic_to_shared(shared);
 #pragma unroll 1
-    for (int column0 = 0; column0 < used; column0 += max(fit, 1)) {
-        const int here = min(max(fit, 1), used - column0), pieces = here * (kRow / 16);
-        __syncthreads();                                 // the room is free
-        if (fit > 0) {
+    for (int column0 = 0; column0 < part.used; column0 += fit) {
+        const int here = min(fit, part.used - column0), pieces = here * (kRow / 16);
+        float M = kNoScore, sum = 0.0f, value = 0.0f;
 #pragma unroll 1
-            for (int p = threadIdx.x >> 5; p < parts; p += threads >> 5)
+        for (int q0 = 0; q0 < count; q0 += kParts) {
+            const int n = min(kParts, count - q0);
+            __syncthreads();                             // the room is free
 #pragma unroll 1
-                for (int k = threadIdx.x & 31; k < pieces; k += 32) fa::cp_async16(dst + (p * pieces + k) * 16, its(p) + column0 * kRow + k * 16);
+            for (int p = threadIdx.x >> 5; p < n; p += threads >> 5)
+#pragma unroll 1
+                for (int k = threadIdx.x & 31; k < pieces; k += 32) fa::cp_async16(dst + (p * pieces + k) * 16, its(q0 + p) + column0 * kRow + k * 16);
             fa::cp_async_commit();
             fa::cp_async_wait<0>();
             __syncthreads();
-        }
 #pragma unroll 1
-        for (int i = threadIdx.x; i < here * D; i += threads) {
-            const int column = i / D, e = i % D;
-            float M = kNoScore, sum = 0.0f, value = 0.0f;
-            if (fit > 0) {
+            for (int i = threadIdx.x; i < here * D; i += threads) {
+                const int column = i / D, e = i % D;
+                if (q0 == 0) { M = kNoScore; sum = value = 0.0f; }
                 const float* one = reinterpret_cast<const float*>(shared) + column * (D + 4);
+                const float before = M;
 #pragma unroll 4
-                for (int p = 0; p < parts; ++p) M = fmaxf(M, one[p * here * (D + 4)]);
+                for (int p = 0; p < n; ++p) M = fmaxf(M, one[p * here * (D + 4)]);
+                const float turn = fa::fast_exp2(before - M);
+                sum *= turn;
+                value *= turn;
 #pragma unroll 4
-                for (int p = 0; p < parts; ++p) {
+                for (int p = 0; p < n; ++p) {
                     const float by = fa::fast_exp2(one[p * here * (D + 4)] - M);
                     sum = fmaf(one[p * here * (D + 4) + 1], by, sum);
                     value = fmaf(one[p * here * (D + 4) + 4 + e], by, value);
                 }
-            } else {                                     // more parts than the room holds of one column
-#pragma unroll 1
-                for (int p = 0; p < parts; ++p) M = fmaxf(M, __ldcg(reinterpret_cast<const float*>(its(p) + (column0 + column) * kRow)));
-#pragma unroll 1
-                for (int p = 0; p < parts; ++p) {
-                    const float* one = reinterpret_cast<const float*>(its(p) + (column0 + column) * kRow);
-                    const float by = fa::fast_exp2(__ldcg(one) - M);
-                    sum = fmaf(__ldcg(one + 1), by, sum);
-                    value = fmaf(__ldcg(one + 4 + e), by, value);
+                if (q0 + n < count) continue;
+                if (to) {
+                    float* mine = to + (column0 + column) * (D + 4);
+                    mine[4 + e] = value;
+                    if (e == 0) *reinterpret_cast<float2*>(mine) = make_float2(M, sum);
+                } else {
+                    const int token = token_of(column0 + column, part.heads, inverse), head = column0 + column - token * part.heads;
+                    a.out[(size_t)(part.row + token) * a.out_stride + (size_t)(part.head0 + head) * D + e] = __float2bfloat16_rn(value * (kUnit / sum));
                 }
             }
-            const int token = token_of(column0 + column, heads, inverse), head = column0 + column - token * heads;
-            a.out[(size_t)(row + token) * a.out_stride + (size_t)(head0 + head) * D + e] = __float2bfloat16_rn(value * (kUnit / sum));
         }
     }
 }
@@ -282,9 +289,9 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     constexpr int C = L::columns, S = L::stages;
     constexpr int KW = D / 32, VW = D / 64;              // words of a key and of a value that a lane holds
     constexpr int KSC = 2 * L::codes, VSC = KSC + L::scales;              // in a stage: keys' codes, values' codes, keys' scales, values' scales
-    extern __shared__ __align__(16) uint8_t shared[];
+    extern __shared__ __align__(128) uint8_t shared[];    // (values' codes swap halves of 64 bytes by an address bit)
     __shared__ Part pending[2];                          // what goes to memory: of a segment that began earlier, and of one that goes on
-    __shared__ int2 merged[2];                           // of those: the first block and the number of parts, where this block merges them
+    __shared__ int4 merged[2];                           // of those: what this block merges
     dependents_may_launch();
     // (positions and page tables come from the host before the step; what other kernels write is read behind the wait)
     // (the warp's number by way of a shuffle: so the compiler knows that all lanes go the same way wherever it decides)
@@ -698,25 +705,51 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
         if (!all && tid == 0) pending[begins ? 1 : 0] = part;
     }
     if (a.arrived == nullptr) return;
-    // The block whose part of a segment comes to memory last merges them all; nobody waits for anybody.
+    // The block whose part of a segment comes to memory last merges them all; nobody waits for anybody.  Parts of more than kParts blocks
+    // are merged so by kParts neighbours first, into the first one's place (one sequence of 64,000 keys, 8 heads over one: 960 us by one block
+    // alone when its room held no column of all 250 parts, XX so).
     const uint32_t share = kWarps4 * each;
-    __syncthreads();
-    if (lane == 0 && warp < 2 && pending[warp].used) {
-        const uint32_t begins = pending[warp].first;
-        const int first = (int)(begins / share), count = (int)((begins + pending[warp].units - 1) / share) - first + 1;
-        int before;                                      // (ordered behind the block's writes, which the barrier has put ahead, and ahead of what is read)
-        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.arrived + first) : "memory");
-        const bool last_one = before == count - 1;
-        if (last_one) a.arrived[first] = 0;              // as the next call wants it
-        merged[warp] = last_one ? make_int2(first, count) : make_int2(0, 0);
-    }
-    __syncthreads();
+    auto blocks_of = [&](const Part& part) { return (int)((part.first + part.units - 1) / share) - (int)(part.first / share) + 1; };
 #pragma unroll 1
-    for (int k = 0; k < 2; ++k) {
-        const Part part = pending[k];
-        if (part.used && merged[k].y)
-            merge_parts<D>(a, C, merged[k].x, merged[k].y, part.row, part.used, part.head0, part.heads, shared,
-                           kWarps4 * (L::ring + L::parked), kThreads4);
+    for (int level = 0;; ++level) {
+        __syncthreads();
+        if (lane == 0 && warp < 2) {
+            const Part part = pending[warp];
+            int4 what = make_int4(0, 0, 0, 0);           // the segment's first block, and the parts to merge: from, step, count
+            if (part.used && (level == 0 || (merged[warp].w && blocks_of(part) > kParts))) {
+                const int first = (int)(part.first / share), all = blocks_of(part), own = (int)blockIdx.x - first;
+                what = make_int4(first, 0, 1, all);
+                int32_t* arrived = a.arrived + first;
+                if (all > kParts && level == 0) {        // (counted apart: the segment's last block may be another one's first)
+                    what.y = own / kParts * kParts;
+                    what.w = min(kParts, all - what.y);
+                    arrived += gridDim.x + what.y;
+                } else if (level == 1) {
+                    what.z = kParts;
+                    what.w = (all + kParts - 1) / kParts;
+                }
+                int before;                              // (ordered behind the block's writes, which the barrier has put ahead, and ahead of what is read)
+                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(arrived) : "memory");
+                if (before == what.w - 1) *arrived = 0;  // as the next call wants it
+                else what.w = 0;
+            }
+            merged[warp] = what;
+        }
+        __syncthreads();
+        bool more = false;                               // (for all threads alike)
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+            const Part part = pending[k];
+            const int4 what = merged[k];
+            if (!part.used || !what.w) continue;
+            float* to = nullptr;
+            if (level == 0 && blocks_of(part) > kParts) {
+                to = a.partial + (size_t)((what.x + what.y) * 2 + (what.y == 0)) * C * (D + 4);
+                more = true;
+            }
+            merge_parts<D>(a, C, what.x, what.y, what.z, what.w, part, to, shared, kWarps4 * (L::ring + L::parked), kThreads4);
+        }
+        if (!more) return;
     }
 }
 
@@ -738,8 +771,9 @@ attention4_merge_kernel(const __grid_constant__ Attention4 a, int columns) {
     const Piece piece = piece_of(s, here.base, end, end + 1);
     if (piece.first < begin || piece.first >= end) return;               // it began earlier, or only its room is here
     const Tile tile = tile_of(a, s, piece.segment);
-    merge_parts<D>(a, columns, blockIdx.x, (int)((piece.first + s.units - 1) / share - blockIdx.x) + 1, s.row + tile.token0, tile.used(),
-                   tile.head0, tile.heads, shared, kMergeRoom, kMergeThreads);
+    const Part part = {piece.first, s.units, s.row + tile.token0, tile.head0, tile.heads, tile.used()};
+    merge_parts<D>(a, columns, blockIdx.x, 0, 1, (int)((piece.first + s.units - 1) / share - blockIdx.x) + 1, part, nullptr, shared, kMergeRoom,
+                   kMergeThreads);
 }
 
 // How a step's columns are tiled: 8 at a time where a segment has no more (two blocks an SM), else 16 (one).  16 for 8 columns: one
@@ -816,8 +850,8 @@ extern "C" int citlali_attention4(const void* q, size_t q_stride, const void* k_
         set_last_error("attention4: the scratch holds %zu floats, too few", partial_floats);
         return kTooLarge;
     }
-    if (arrived != nullptr && arrived_ints < (size_t)blocks) {
-        set_last_error("attention4: room for %zu counters, %d blocks", arrived_ints, blocks);
+    if (arrived != nullptr && arrived_ints < 2 * (size_t)blocks) {
+        set_last_error("attention4: room for %zu counters, two for each of %d blocks", arrived_ints, blocks);
         return kTooLarge;
     }
     const long long units = ((long long)page_table_stride * page_size + max_new) / c4::kUnitKeys + 2 + c4::kRoom;

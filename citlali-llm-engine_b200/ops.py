@@ -717,12 +717,12 @@ _arrivals = {}                              # (device, stream) -> counters
 _arrivals_spare = {}                        # device -> (zeroed counters, how many are given away)
 _arrivals_kept = []
 _arrivals_lock = threading.Lock()
-_ARRIVALS_SPARE = 1 << 18
+_ARRIVALS_SPARE = 1 << 19
 
 
 def _arrivals_of(device, stream):
     """Counters for one call of ``citlali_attention4`` on this device and stream, or None."""
-    each = -(-2 * sm_count(device) // 64) * 64
+    each = -(-4 * sm_count(device) // 64) * 64
     with _arrivals_lock:
         spare, used = _arrivals_spare.get(device.index, (None, 0))
         if torch._C._cuda_isCurrentStreamCapturing():

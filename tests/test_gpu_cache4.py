@@ -574,6 +574,32 @@ def test_merging_by_the_last_block_or_by_a_second_kernel(monkeypatch, lengths):
     assert all(int(c.abs().sum()) == 0 for c in ops._arrivals.values())
 
 
+@pytest.mark.parametrize("nq,nkv,d,lengths", [(4, 1, 64, [9000, 40, 300]), (8, 1, 128, [20000]), (32, 1, 128, [9999, 700]), (8, 1, 256, [10000])])
+def test_a_segment_of_many_blocks(monkeypatch, nq, nkv, d, lengths):
+    """More parts than are merged at once: 32 neighbours first, then what they made; or by the second kernel in pieces of 32.  The order of
+    additions differs between the two, so they may be a step of bfloat16 apart."""
+    st = Step([n - 1 for n in lengths], [1] * len(lengths), nkv, d, seed=4)
+    st.fill(4)
+    got = check_attention(st, nq, torch.bfloat16, 0, 9)
+    q = (1.5 * torch.randn(len(lengths), (nq + 2 * nkv) * d, generator=torch.Generator().manual_seed(9))).bfloat16().to(DEV)         # the same
+    view, batch, outs = st.view(), st.batch(), []
+    monkeypatch.setattr(ops, "_arrivals_spare", {})
+    for _ in range(2):
+        out = torch.empty(len(lengths), nq * d, dtype=torch.bfloat16, device=DEV)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        before = ops.launch_count()
+        with torch.cuda.graph(graph):
+            ops.cache4_attention(q, (nq + 2 * nkv) * d, view, batch, out, nq, nkv, d, 0, 1.0 / math.sqrt(d))
+        assert ops.launch_count() - before == 2
+        graph.replay()
+        torch.cuda.synchronize()
+        outs.append(out.cpu().double())
+    assert torch.equal(outs[0], outs[1])
+    assert ((outs[0] - got).abs() <= 2.0 ** -7 * got.abs() + 2.0 ** -15 * got.abs().max()).all()
+    assert all(int(c.abs().sum()) == 0 for c in ops._arrivals.values())
+
+
 def test_refusals():
     st = Step([10], [2], 2, 64)
     kv, batch = st.view(), st.batch()
