@@ -706,8 +706,8 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
     }
     if (a.arrived == nullptr) return;
     // The block whose part of a segment comes to memory last merges them all; nobody waits for anybody.  Parts of more than kParts blocks
-    // are merged so by kParts neighbours first, into the first one's place (one sequence of 64,000 keys, 8 heads over one: 960 us by one block
-    // alone when its room held no column of all 250 parts, XX so).
+    // are merged so by kParts neighbours first, into the first one's place (one sequence of 64,000 keys, 8 heads over one of 128: 24 us;
+    // by one block alone, whose room held no column of all 250 parts, 960).
     const uint32_t share = kWarps4 * each;
     auto blocks_of = [&](const Part& part) { return (int)((part.first + part.units - 1) / share) - (int)(part.first / share) + 1; };
 #pragma unroll 1
