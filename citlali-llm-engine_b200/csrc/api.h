@@ -210,7 +210,7 @@ int citlali_attention4_rows(const void* q, size_t q_stride, int dtype, const voi
                             const int32_t* row_slot, const int32_t* row_pos, void* out, size_t out_stride, int rows, int nq,
                             int nkv, int head_dim, int page_size, int window, float scale, cudaStream_t stream);
 // The same on the tensor cores, bfloat16, for single tokens (seq_start null: a row a sequence, seq_slot and seq_past the rows' slots and
-// positions) and for runs of at most max_new tokens (sequences with more are left out).  Lengths are read on the device only.  partial: as many floats as
+// positions) and for runs of some max_new tokens; sequences with more than most_new are left out (0: none).  Lengths are read on the device only.  partial: as many floats as
 // citlali_attention4_scratch_floats says, of this call alone.  arrived (may be null: a second kernel merges what blocks share): counters,
 // four a multiprocessor, zero before the call and zero again behind it, that no other call on its way uses.
 int citlali_attention4_supports(int head_dim, int page_size);
@@ -218,7 +218,7 @@ size_t citlali_attention4_scratch_floats(int nq, int nkv, int head_dim, int max_
 int citlali_attention4(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes,
                        const void* v_scales, const int32_t* page_table, int page_table_stride, const int32_t* seq_start,
                        const int32_t* seq_slot, const int32_t* seq_past, void* out, size_t out_stride, float* partial,
-                       size_t partial_floats, int32_t* arrived, size_t arrived_ints, int sequences, int max_new, int nq, int nkv, int head_dim, int page_size,
+                       size_t partial_floats, int32_t* arrived, size_t arrived_ints, int sequences, int max_new, int most_new, int nq, int nkv, int head_dim, int page_size,
                        int window, float scale, cudaStream_t stream);
 
 // tokens[r] = argmax of logits[r, :] over finite values, lowest index on ties.

@@ -728,10 +728,13 @@ attention4_kernel(const __grid_constant__ Attention4 a) {
                     what.z = kParts;
                     what.w = (all + kParts - 1) / kParts;
                 }
-                int before;                              // (ordered behind the block's writes, which the barrier has put ahead, and ahead of what is read)
-                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(arrived) : "memory");
-                if (before == what.w - 1) *arrived = 0;  // as the next call wants it
-                else what.w = 0;
+                // (a group of one block, a segment's last, is complete; its counter may be the next segment's first group's)
+                if (what.w > 1) {
+                    int before;                          // (ordered behind the block's writes, which the barrier has put ahead, and ahead of what is read)
+                    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(arrived) : "memory");
+                    if (before == what.w - 1) *arrived = 0;      // as the next call wants it
+                    else what.w = 0;
+                }
             }
             merged[warp] = what;
         }
@@ -830,8 +833,8 @@ extern "C" size_t citlali_attention4_scratch_floats(int nq, int nkv, int head_di
 extern "C" int citlali_attention4(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes,
                                   const void* v_scales, const int32_t* page_table, int page_table_stride, const int32_t* seq_start,
                                   const int32_t* seq_slot, const int32_t* seq_past, void* out, size_t out_stride, float* partial,
-                                  size_t partial_floats, int32_t* arrived, size_t arrived_ints, int sequences, int max_new, int nq, int nkv, int head_dim, int page_size,
-                                  int window, float scale, cudaStream_t stream) {
+                                  size_t partial_floats, int32_t* arrived, size_t arrived_ints, int sequences, int max_new, int most_new, int nq, int nkv, int head_dim,
+                                  int page_size, int window, float scale, cudaStream_t stream) {
     if (sequences <= 0 || max_new <= 0) return 0;
     if (!citlali_attention4_supports(head_dim, page_size) || nq <= 0 || nkv <= 0 || nq % nkv != 0 || window < 0) {
         set_last_error("attention4: no kernel for %d query heads over %d key/value heads of %d with pages of %d, window %d (head sizes 64, "
@@ -870,7 +873,7 @@ extern "C" int citlali_attention4(const void* q, size_t q_stride, const void* k_
     a.out = (__nv_bfloat16*)out; a.out_stride = out_stride;
     a.sequences = sequences; a.nq = nq; a.nkv = nkv; a.group = nq / nkv;
     a.tokens = t.tokens; a.heads = t.heads; a.head_tiles = t.head_tiles;
-    a.window = window; a.most = max_new; a.scale_log2 = scale * 1.4426950408889634f; a.partial = partial; a.arrived = arrived;
+    a.window = window; a.most = most_new > 0 ? most_new : 0x7fffffff; a.scale_log2 = scale * 1.4426950408889634f; a.partial = partial; a.arrived = arrived;
     if (head_dim == 64) return t.wide == 1 ? c4::launch<64, 1>(a, blocks, stream) : c4::launch<64, 2>(a, blocks, stream);
     if (head_dim == 128) return t.wide == 1 ? c4::launch<128, 1>(a, blocks, stream) : c4::launch<128, 2>(a, blocks, stream);
     return c4::launch<256, 1>(a, blocks, stream);

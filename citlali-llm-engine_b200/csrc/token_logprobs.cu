@@ -6,7 +6,7 @@
 // Entries that are not finite have no probability, as in sampling.cu; a row without a finite entry has none at all (log
 // probabilities of minus infinity, entropy 0, ids -1).  Logits are float32 or bfloat16; all sums are float32.
 //
-// What bounds it: reading the logits once (1,000 rows of 151,936 float32: 109.5 us, 5.5 TB/s); with few rows the passes over the
+// What bounds it: reading the logits once (1,000 rows of 151,936 float32: 107 us, 5.7 TB/s); with few rows the passes over the
 // likeliest that follow (8 rows, 20 likeliest: 10.4 us, of which reading takes 2).  A cluster of 1 to 8 blocks takes a row, a block an even share of it; a thread has 16
 // entries in registers and the next 16 on their way.  m, S and T are the thread's own until the end (the running maximum is looked
 // at once for 16 entries).
@@ -32,7 +32,7 @@ constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNone = 0x7fffffff;                        // no entry: behind every index
 
-// Tiles ahead of the first bound (1,000 rows of 151,936: 4 and 8 109.5 us, 16 113.6), and what the first block has room to sort.
+// Tiles ahead of the first bound (1,000 rows of 151,936: 4 and 8 alike, 16 4 us longer), and what the first block has room to sort.
 constexpr int kWindow = 8, kFound = 512;
 
 struct Summary { float m, s, t; };

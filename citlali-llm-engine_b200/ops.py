@@ -741,8 +741,8 @@ def _arrivals_of(device, stream):
 def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
     """:func:`attention` over a cache in 4 bits: every row of the step over its slot's keys up to its own position (the last
     ``window`` of them; 0 or None: all).  bfloat16 with head size 64, 128 or 256 and pages of 64 runs on the tensor cores, anything
-    else in 32-bit arithmetic; longer runs of tokens go over pages that were made bfloat16 first.  A step of single tokens launches
-    nothing that depends on the host's lists of lengths."""
+    else in 32-bit arithmetic.  Runs of tokens go the way that takes least (:func:`_attention4_way`); a step of single tokens, and
+    a captured one, launches nothing that depends on the host's lists of lengths."""
     pools = _packed4(kv, nkv, head_dim, "cache4_attention")
     row_slot, row_pos, seq_start, single = batch.row_slot, batch.row_pos, batch.seq_start, batch.is_decode
     rows, wide = row_slot.shape[0], nq * head_dim
@@ -795,8 +795,8 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
             start, slot, past = (None, row_slot, row_pos) if single else (seq_start.data_ptr(), batch.seq_slot, batch.seq_past)
             _check(lib().citlali_attention4(
                 q_ptr, _sz(q_stride), kc, ks, vc, vs, table, table_width, start, slot.data_ptr(), past.data_ptr(), out.data_ptr(), wide,
-                partial.data_ptr(), floats, _ptr(arrived), 0 if arrived is None else arrived.numel(), len(batch.slots), max_new, nq, nkv, head_dim,
-                kv.page_size, window, _f(scale), stream), "cache4_attention" if arrived is not None else "cache4_attention_merged")
+                partial.data_ptr(), floats, _ptr(arrived), 0 if arrived is None else arrived.numel(), len(batch.slots), max_new, most, nq, nkv,
+                head_dim, kv.page_size, window, _f(scale), stream), "cache4_attention" if arrived is not None else "cache4_attention_merged")
             return
     _check(lib().citlali_attention4_rows(
         q_ptr, _sz(q_stride), _dtype_code(q), kc, ks, vc, vs, table, table_width, row_slot.data_ptr(), row_pos.data_ptr(), out.data_ptr(), wide, rows,

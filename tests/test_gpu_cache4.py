@@ -574,10 +574,12 @@ def test_merging_by_the_last_block_or_by_a_second_kernel(monkeypatch, lengths):
     assert all(int(c.abs().sum()) == 0 for c in ops._arrivals.values())
 
 
-@pytest.mark.parametrize("nq,nkv,d,lengths", [(4, 1, 64, [9000, 40, 300]), (8, 1, 128, [20000]), (32, 1, 128, [9999, 700]), (8, 1, 256, [10000])])
+@pytest.mark.parametrize("nq,nkv,d,lengths", [(4, 1, 64, [9000, 40, 300]), (8, 1, 128, [20000]), (32, 1, 128, [9999, 700]), (8, 1, 256, [10000]),
+                                                (4, 2, 128, [8090]), (3, 3, 128, [8090]), (2, 2, 128, [8100, 8090])])
 def test_a_segment_of_many_blocks(monkeypatch, nq, nkv, d, lengths):
     """More parts than are merged at once: 32 neighbours first, then what they made; or by the second kernel in pieces of 32.  The order of
-    additions differs between the two, so they may be a step of bfloat16 apart."""
+    additions differs between the two, so they may be a step of bfloat16 apart.  (8,090 keys are 253 units: 33 blocks, and the next
+    segment begins in the last of them.)"""
     st = Step([n - 1 for n in lengths], [1] * len(lengths), nkv, d, seed=4)
     st.fill(4)
     got = check_attention(st, nq, torch.bfloat16, 0, 9)
@@ -598,6 +600,40 @@ def test_a_segment_of_many_blocks(monkeypatch, nq, nkv, d, lengths):
     assert torch.equal(outs[0], outs[1])
     assert ((outs[0] - got).abs() <= 2.0 ** -7 * got.abs() + 2.0 ** -15 * got.abs().max()).all()
     assert all(int(c.abs().sum()) == 0 for c in ops._arrivals.values())
+
+
+def test_a_captured_step_of_runs_follows_the_device():
+    """A captured step of two runs, replayed with the same rows dealt out otherwise: by the lengths on the device."""
+    q = torch.randn(8, 4 * 128, generator=torch.Generator().manual_seed(1)).bfloat16().to(DEV)
+    outs = []
+    for new in ([3, 5], [7, 1]):
+        st = Step([100, 40], new, 1, 128, seed=6, slots=4)
+        st.fill(6)
+        batch, out = st.batch(), torch.empty(8, 256, dtype=torch.bfloat16, device=DEV)
+        batch.runs4[2, 1, 128, 0, 512] = ("codes",)
+        ops.cache4_attention(q, 512, st.view(), batch, out, 2, 1, 128, 0, 0.1)
+        outs.append((st, st.batch(), out))
+    (st, batch, want), (other, other_batch, other_want) = outs
+    view, out = st.view(), torch.empty(8, 256, dtype=torch.bfloat16, device=DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.cache4_attention(q, 512, view, batch, out, 2, 1, 128, 0, 0.1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    for name in ("row_slot", "row_pos", "seq_start", "seq_slot", "seq_past"):
+        getattr(batch, name).copy_(getattr(other_batch, name))
+    for mine, its in ((view.keys, other.view().keys), (view.values, other.view().values)):
+        mine.codes.copy_(its.codes)
+        mine.scales.copy_(its.scales)
+    view.page_table.copy_(other.view().page_table)
+    graph.replay()
+    torch.cuda.synchronize()
+    # (other tiles: either is off by half a step of bfloat16 and by 2^-11 of the weighted values, at most the largest)
+    most = plain.values(other.values.codes, other.values.scales).nan_to_num(0.0).abs().max()
+    got, wanted = out.cpu().double(), other_want.cpu().double()
+    assert ((got - wanted).abs() <= 2.0 ** -7 * wanted.abs() + 2.0 ** -10 * most).all()
 
 
 def test_refusals():
