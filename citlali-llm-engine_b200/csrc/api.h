@@ -195,7 +195,7 @@ int citlali_attention4_runs_tokens(int nq, int nkv, int head_dim, int page_size)
 int citlali_attention4_runs(const void* q, size_t q_stride, const void* k_codes, const void* k_scales, const void* v_codes,
                             const void* v_scales, const int32_t* page_table, int page_table_stride, const int32_t* seq_start,
                             const int32_t* seq_slot, const int32_t* seq_past, void* out, size_t out_stride, int sequences, int least_new, int tiles,
-                            int cluster, int nq, int nkv, int head_dim, int page_size, int window, float scale, cudaStream_t stream);
+                            int cluster, int nq, int nkv, int head_dim, int page_size, int window, float scale, int32_t* error_flag, cudaStream_t stream);
 // The pages of 64 that runs of new tokens see (from the pair with past - window + 1 on, if there is a window), as bfloat16: page after page of the
 // sequences [pages, nkv, 64, head_dim], zeros where no row sees anything; table_out [sequences, table_out_stride] and slots_out
 // [sequences] are the page table and slots under which the attention kernels of a cache of 16 bits find them.  pages: of all sequences.

@@ -27,7 +27,7 @@
 // its pages.  With the softmax on four warps and two blocks a multiprocessor a page took 2,300 clocks a block; with one issuing lane for both
 // products 2,700, since an MMA takes it 60 clocks and telling a barrier 200.  Measured (16 heads over 8 of 128): a prompt of 2,048 tokens 37 us
 // (over pages made bfloat16 first: 53), eight of 512 42 (48), 64 new tokens over 32,768 60 (by the kernel for single tokens: 116).
-// All waits are bounded; where one runs out, the block's results are NaN.
+// All waits are bounded; one that runs out reports through the error word, and the block's results are NaN.
 #include "api.h"
 #include "cache4.cuh"
 #include "common.cuh"
@@ -69,6 +69,7 @@ struct Runs4 {
     int least;                                                       // sequences with fewer new tokens are left out
     int window, cluster;
     float scale_log2;
+    int32_t* error_flag;
 };
 
 // Four products over 16 elements of the contraction each, by the lane that has `go`.  The whole warp comes here, so that descriptors stay
@@ -338,7 +339,7 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
         // ---- a page's scores, weights and sum: the even pages' warps 0-3, the odd pages' warps 4-7, a thread a row
         const int quarter = warp & 3, row = tid % kRunRows, token = row / a.group;
         const bool on = row < used;
-        mbar_wait(smem_u32(&q_full), 0, abort_flag, nullptr, 0);
+        mbar_wait(smem_u32(&q_full), 0, abort_flag, a.error_flag, 401);
         __syncwarp();
         const float factor = row_factor[row];
         const int pos = on ? pos0 + token : -1, low = a.window > 0 ? pos - a.window + 1 : 0;
@@ -346,7 +347,7 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
         for (int i = odd; i < pages; i += 2) {
             const int stage = i % kStages;
             const uint32_t at_scores = tmem + lanes + kColScores + stage * kRunKeys;
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[stage]), i / kStages & 1u, abort_flag, nullptr, 0))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[stage]), i / kStages & 1u, abort_flag, a.error_flag, 402))) break;
             tc_fence_after();
             const int key0 = (page0 + i) * kRunKeys;
             // pages that some of the tile's tokens see in part (rows behind its last have queries of zeros, and are not stored)
@@ -375,7 +376,7 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
             // the reference as the page before leaves it, and as this one does
             float before = kNothingYet;
             if (i > 0) {
-                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&m_known[odd ^ 1][quarter]), (i - 1) >> 1 & 1u, abort_flag, nullptr, 0))) break;
+                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&m_known[odd ^ 1][quarter]), (i - 1) >> 1 & 1u, abort_flag, a.error_flag, 403))) break;
                 before = row_m[row];
             }
             const bool renew = __any_sync(0xffffffffu, top - before > kRunMost);
@@ -400,7 +401,7 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
             l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
             if (renew && i > 0) {
                 // (the product with the page before must have ended)
-                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[(i - 1) % kStages]), (i - 1) / kStages & 1u, abort_flag, nullptr, 0))) break;
+                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[(i - 1) % kStages]), (i - 1) / kStages & 1u, abort_flag, a.error_flag, 404))) break;
                 tc_fence_after();
                 const float turn = fa::fast_exp2(before - now);
 #pragma unroll 1
@@ -419,11 +420,11 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
         }
         if (pages > 0) {
             const int end = pages - 1;
-            if ((end & 1) != odd) mbar_wait(smem_u32(&m_known[odd ^ 1][quarter]), end >> 1 & 1u, abort_flag, nullptr, 0);
+            if ((end & 1) != odd) mbar_wait(smem_u32(&m_known[odd ^ 1][quarter]), end >> 1 & 1u, abort_flag, a.error_flag, 405);
             const float now = row_m[row];                            // (of the last page)
             l *= fa::fast_exp2(m - now);
             if (!odd) row_sums[row].x = now;
-            mbar_wait(smem_u32(&v_empty[end % kStages]), end / kStages & 1u, abort_flag, nullptr, 0);
+            mbar_wait(smem_u32(&v_empty[end % kStages]), end / kStages & 1u, abort_flag, a.error_flag, 406);
         } else if (!odd) {
             row_sums[row].x = kNothingYet;
         }
@@ -456,14 +457,14 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
             const int place_of = i % kStages;
             const uint32_t stage = base + place_of * L::stage, turn = i / kStages & 1u;
             // the scores of the page that was here have come out: its keys' place is free
-            if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[place_of]), turn ^ 1u, abort_flag, nullptr, 0))) break;
+            if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[place_of]), turn ^ 1u, abort_flag, a.error_flag, 407))) break;
             const uint32_t bad = __vcmpgeu4(x.v_scales, 0xf8f8f8f8u);
             const bool none = (bad | __shfl_xor_sync(0xffffffffu, bad, 16)) != 0;
             put(stage, x.k, none ? 0xffffffffu : x.k_scales);
             fence_async_proxy();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&k_full[place_of]));
-            if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[place_of]), turn ^ 1u, abort_flag, nullptr, 0))) break;
+            if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[place_of]), turn ^ 1u, abort_flag, a.error_flag, 408))) break;
             put(stage + L::part, x.v, x.v_scales & ~bad);
             fence_async_proxy();
             __syncwarp();
@@ -474,14 +475,14 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
         constexpr uint32_t form = instr_desc_half(kRunRows, kRunKeys, false);
         const uint64_t asked = smem_desc_sw128(queries, 0), keys = smem_desc_sw128(base, 0);
         const uint32_t go = elected();
-        if (pages > 0 && __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), 0, abort_flag, nullptr, 0))) {
+        if (pages > 0 && __all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), 0, abort_flag, a.error_flag, 409))) {
 #pragma unroll 1
             for (int i = 0; i < pages; ++i) {
                 const int stage = i % kStages;
                 const uint32_t turn = i / kStages & 1u;
                 // (their place held the weights of a page before, which have been multiplied with its values)
-                if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[stage]), turn ^ 1u, abort_flag, nullptr, 0))) break;
-                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[stage]), turn, abort_flag, nullptr, 0))) break;
+                if (i >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_empty[stage]), turn ^ 1u, abort_flag, a.error_flag, 410))) break;
+                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[stage]), turn, abort_flag, a.error_flag, 411))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < D / 64; ++k)
@@ -499,8 +500,8 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
         for (int i = 0; i < pages; ++i) {
             const int stage = i % kStages;
             const uint32_t turn = i / kStages & 1u;
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_full[stage]), turn, abort_flag, nullptr, 0) &&
-                                             mbar_wait(smem_u32(&p_full[stage]), turn, abort_flag, nullptr, 0))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_full[stage]), turn, abort_flag, a.error_flag, 412) &&
+                                             mbar_wait(smem_u32(&p_full[stage]), turn, abort_flag, a.error_flag, 413))) break;
             tc_fence_after();
             mma_four_rows(tmem + kColOut, tmem + kColScores + stage * kRunKeys, vals + stage * (L::stage >> 4), form, i > 0, go);
             commit_if(smem_u32(&v_empty[stage]), go);
@@ -622,7 +623,7 @@ extern "C" int citlali_attention4_runs(const void* q, size_t q_stride, const voi
                                        const void* v_scales, const int32_t* page_table, int page_table_stride, const int32_t* seq_start,
                                        const int32_t* seq_slot, const int32_t* seq_past, void* out, size_t out_stride, int sequences,
                                        int least_new, int tiles, int cluster, int nq, int nkv, int head_dim, int page_size, int window, float scale,
-                                       cudaStream_t stream) {
+                                       int32_t* error_flag, cudaStream_t stream) {
     if (sequences <= 0 || tiles <= 0) return 0;
     const int tokens = citlali_attention4_runs_tokens(nq, nkv, head_dim, page_size);
     if (tokens == 0 || window < 0) {
@@ -650,5 +651,6 @@ extern "C" int citlali_attention4_runs(const void* q, size_t q_stride, const voi
     a.sequences = sequences; a.nq = nq; a.nkv = nkv; a.group = nq / nkv; a.tokens = tokens;
     a.least = least_new > 1 ? least_new : 1;
     a.window = window; a.cluster = cluster; a.scale_log2 = scale * 1.4426950408889634f;
+    a.error_flag = error_flag;
     return head_dim == 64 ? c4::launch_runs<64>(a, tiles, stream) : c4::launch_runs<128>(a, tiles, stream);
 }

@@ -674,7 +674,7 @@ def _attention4_pages_time(batch, nq: int, nkv: int, head_dim: int, window: int,
     return 14 + walked * tile + pages * nkv * 64 * head_dim * 4 / 2.3e6
 
 
-def _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, scale):
+def _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, scale, error_flag):
     """The pages that the rows see as bfloat16 (the values are exact there), then prompt attention over them: as many sequences at a
     time as a gigabyte holds, at least one."""
     kc, ks, vc, vs, table, table_width = pools
@@ -701,7 +701,7 @@ def _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, 
                                        head_dim, stream), "cache4_expand")
         if l.citlali_attention_run_form(q_stride, wide, head_dim, 64, max_new) == 2:
             _check(l.citlali_attention_prefill_tc(q.data_ptr(), q_stride, batch.row_slot.shape[0], keys, values, pages, rows, width, where[0], slots,
-                                                  where[2], out_ptr, wide, count, max_new, nq, nkv, head_dim, 64, window, scale, None, stream),
+                                                  where[2], out_ptr, wide, count, max_new, nq, nkv, head_dim, 64, window, scale, _ptr(error_flag), stream),
                    "attention_prefill_tc")
         else:
             _check(l.citlali_attention_prefill(q.data_ptr(), q_stride, keys, values, rows, width, where[0], slots, where[2], out_ptr, wide, count,
@@ -738,11 +738,12 @@ def _arrivals_of(device, stream):
     return counters
 
 
-def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale):
+def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, scale, error_flag=None):
     """:func:`attention` over a cache in 4 bits: every row of the step over its slot's keys up to its own position (the last
     ``window`` of them; 0 or None: all).  bfloat16 with head size 64, 128 or 256 and pages of 64 runs on the tensor cores, anything
     else in 32-bit arithmetic.  Runs of tokens go the way that takes least (:func:`_attention4_way`); a step of single tokens, and
-    a captured one, launches nothing that depends on the host's lists of lengths."""
+    a captured one, launches nothing that depends on the host's lists of lengths.  ``error_flag``: the word that a wait which runs
+    out is reported by."""
     pools = _packed4(kv, nkv, head_dim, "cache4_attention")
     row_slot, row_pos, seq_start, single = batch.row_slot, batch.row_pos, batch.seq_start, batch.is_decode
     rows, wide = row_slot.shape[0], nq * head_dim
@@ -772,14 +773,14 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
                 l.citlali_attention4_runs_tokens(nq, nkv, head_dim, 64),
                 _attention4_floats(nq, nkv, head_dim, 64, max_new, _current_device()) >= 0, sm_count(q.device))
         if way[0] == "pages":
-            _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, float(scale))
+            _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, float(scale), error_flag)
             return
         if way[0] == "tiles":
             most = way[1]                                            # new tokens of the sequences that the kernel for single tokens takes
             _check(lib().citlali_attention4_runs(
                 q_ptr, _sz(q_stride), kc, ks, vc, vs, table, table_width, seq_start.data_ptr(), batch.seq_slot.data_ptr(), batch.seq_past.data_ptr(),
-                out.data_ptr(), wide, len(batch.slots), most + 1, way[2], way[3], nq, nkv, head_dim, 64, window, _f(scale), _stream()),
-                "cache4_attention_runs")
+                out.data_ptr(), wide, len(batch.slots), most + 1, way[2], way[3], nq, nkv, head_dim, 64, window, _f(scale),
+                _ptr(error_flag), _stream()), "cache4_attention_runs")
             if most == 0:
                 return
     if q.dtype is torch.bfloat16 and q_stride % 8 == 0 and (q_ptr | kc | ks | vc | vs) % 16 == 0 and nkv > 0 and nq % nkv == 0:

@@ -106,7 +106,7 @@ class GQAttention:
             self.rotary_dim = self.d
             self.inv_freq = torch.zeros(self.d // 2, dtype=torch.float32, device=ctx.device)   # no rotation by the kernel
         self.dtype = ctx.dtype
-        self.packed4 = ctx.packed4
+        self.packed4, self.error_flag = ctx.packed4, ctx.error_flag
         require(not self.packed4 or self.d % 16 == 0 and self.d <= 256,
                 f"{self.prefix}: a cache in 4 bits takes head sizes that are multiples of 16 up to 256, not {self.d}")
 
@@ -167,7 +167,8 @@ class GQAttention:
             if store:
                 ops.cache4_append(qkv, *rows, self.inv_freq[:0], 0)
         out = torch.empty((batch.rows, self.nq * self.d), dtype=self.dtype, device=qkv.device)
-        ops.cache4_attention(qkv, qkv.shape[1], cache_view, batch, out, self.nq, self.nkv, self.d, int(self.window or 0), self.scale)
+        ops.cache4_attention(qkv, qkv.shape[1], cache_view, batch, out, self.nq, self.nkv, self.d, int(self.window or 0), self.scale,
+                             self.error_flag)
         self.o.forward(out, accumulate_into=residual, emit=emit)
         return residual
 

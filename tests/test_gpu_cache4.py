@@ -752,8 +752,10 @@ def test_queries_that_end_with_their_last_row(way):
     for given in (q, q.flatten()[:(rows - 1) * pitch + wide].clone()):
         batch, out = st.batch(), torch.full((rows, wide), 5.0, dtype=torch.bfloat16, device=DEV)
         batch.runs4[4, 2, 128, 0, pitch] = way
-        ops.cache4_attention(given, pitch, st.view(), batch, out, 4, 2, 128, 0, 0.1)
+        flag = torch.zeros(4, dtype=torch.int32, device=DEV)
+        ops.cache4_attention(given, pitch, st.view(), batch, out, 4, 2, 128, 0, 0.1, error_flag=flag)
         made.append(out)
+        assert not flag.any()                            # (no wait ran out)
     assert torch.equal(made[0], made[1])
 
 
