@@ -142,7 +142,9 @@ class DecoderModel:
         if self.spec.residual_streams is not None:
             out.add("hyper_connection")
         if self.ctx.packed4:
-            out.update(("cache4", "attention4_rows") if dtype == torch.float32 else ("cache4", "attention4"))
+            out.update(("cache4", "attention4_rows") if dtype == torch.float32 else ("cache4", "attention4", "attention4_runs"))
+            if any(getattr(p, "takes_packed4", False) and p.d not in (64, 128, 256) for b in self.layers for p in b.parts()):
+                out.add("attention4_rows")
         for owner in [self.final_norm, self.embedding_norm, self.embedding_addition] + [p for b in self.layers for p in [b] + list(b.parts())]:
             if owner is not None:
                 out.update(named_sources(owner, dtype))

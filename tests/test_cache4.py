@@ -62,7 +62,7 @@ def test_cache_dtype_argument():
 def test_models_whose_mixers_cannot_are_refused():
     ctx = cb.BuildContext(torch.device("cpu"), torch.bfloat16, packed4=True)
     model = cb.DecoderModel(tiny_config("A").to_model_spec(), ctx)
-    assert {"cache4", "attention4"} <= set(model.kernel_sources())
+    assert {"cache4", "attention4", "attention4_runs"} <= set(model.kernel_sources())
     from citlali_b200.measure import gidirax_config
     spec = gidirax_config(256, 4, 512).to_model_spec()
     cb.DecoderModel(spec, cb.BuildContext(torch.device("cpu"), torch.bfloat16))
