@@ -22,11 +22,11 @@
 // times a NaN would reach it; a row that does see it gets a NaN from the key.
 // A cluster's blocks leave O, m and the sum in their shared memory, and each merges an even share of the rows, always in the same order.
 //
-// What bounds it: a page takes 1,400 clocks, of which the products take 512 and the exponentials 512 (16 a clock); the rest is the issue
+// What bounds it: a page takes 1,280 clocks, of which the products take 512 and the exponentials 512 (16 a clock); the rest is the issue
 // of what puts codes back and of the softmax (issue slots half used) and the latencies between the roles.  A block spends about 4 us beside
 // its pages.  With the softmax on four warps and two blocks a multiprocessor a page took 2,300 clocks a block; with one issuing lane for both
-// products 2,700, since an MMA takes it 60 clocks and telling a barrier 200.  Measured (16 heads over 8 of 128): a prompt of 2,048 tokens 37 us
-// (over pages made bfloat16 first: 53), eight of 512 42 (48), 64 new tokens over 32,768 60 (by the kernel for single tokens: 116).
+// products 2,700, since an MMA takes it 60 clocks and telling a barrier 200.  Measured (16 heads over 8 of 128): a prompt of 2,048 tokens 34 us
+// (over pages made bfloat16 first: 53), eight of 512 40 (48), 64 new tokens over 32,768 56 (by the kernel for single tokens: 116).
 // All waits are bounded; one that runs out reports through the error word, and the block's results are NaN.
 #include "api.h"
 #include "cache4.cuh"
@@ -293,8 +293,7 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
         fetch(next, table[odd]);
     }
     if (warp < kSoftWarps + kLoadWarps) {
-        // As they are, all on their way at once; then each lane makes its own pieces halves where they lie.  (Short loops: what runs once
-        // waits for its instructions more than for anything else.)
+        // D / 8 lanes a row: a lane's pieces all on their way at once, then made halves
         constexpr int lanes_of = D / 8, at_once = 32 / lanes_of;
         constexpr int rows_of = kRunRows / (kSoftWarps + kLoadWarps);
         const int piece = lane % lanes_of, first = warp * rows_of;
@@ -304,16 +303,17 @@ attention4_runs_kernel(const __grid_constant__ Runs4 a) {
             const int r = min(first + lane % rows_of, used - 1), t = r / a.group;
             from = (size_t)(row0 + token0 + t) * a.q_stride + (size_t)(kv * a.group + r - t * a.group) * D;
         }
-#pragma unroll 2
-        for (int k = lane / lanes_of; k < rows_of; k += at_once) {
-            const __nv_bfloat16* src = a.q + __shfl_sync(0xffffffffu, from, k) + 8 * piece;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at(first + k)), "l"(src), "r"(first + k < used ? 16 : 0) : "memory");
+        uint4 its[rows_of / at_once];
+#pragma unroll
+        for (int i = 0; i < rows_of / at_once; ++i) {
+            const int k = lane / lanes_of + i * at_once;
+            const uint4* src = reinterpret_cast<const uint4*>(a.q + __shfl_sync(0xffffffffu, from, k) + 8 * piece);
+            its[i] = first + k < used ? *src : make_uint4(0, 0, 0, 0);
         }
-        fa::cp_async_commit();
-        fa::cp_async_wait<0>();
-#pragma unroll 1
-        for (int k = lane / lanes_of; k < rows_of; k += at_once) {
-            const uint4 in = ld_shared_v4(at(first + k));
+#pragma unroll
+        for (int i = 0; i < rows_of / at_once; ++i) {
+            const int k = lane / lanes_of + i * at_once;
+            const uint4 in = its[i];
             uint32_t most = __vimax3_u16x2(in.x & 0x7fff7fffu, in.y & 0x7fff7fffu, __vmaxu2(in.z & 0x7fff7fffu, in.w & 0x7fff7fffu));
             most = max(most << 16, most & 0x7fff0000u);
 #pragma unroll

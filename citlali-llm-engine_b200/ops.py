@@ -592,19 +592,20 @@ _EXPAND_BYTES = 1 << 30
 
 
 def _attention4_way(batch, nq: int, nkv: int, head_dim: int, window: int, form: int, tokens: int, codes: bool, sms: int) -> tuple:
-    """How a step's runs of tokens are attended to: ("tiles", n, tiles, blocks that share one) by the kernel on tcgen05 (``tokens`` of a tile; 0:
-    it does not take the sizes), but sequences of up to n new tokens, if n is not 0, by the kernel for single tokens, ("pages",) by prompt attention (``form``: 2 on tcgen05, 1 on mma.sync, 0 not at all) over pages that are
-    made bfloat16 first, or ("codes",) by the kernel for single tokens, if it takes the sizes, or that in 32 bits.  The one that takes least
-    time, in microseconds, by what each was measured to do:
+    """How a step's runs of tokens are attended to: ("tiles", n, tiles, blocks that share one) by the kernel on tcgen05 (``tokens`` of a
+    tile; 0: it does not take the sizes), but sequences of up to n new tokens, if n is not 0, by the kernel for single tokens; ("pages",) by
+    prompt attention (``form``: 2 on tcgen05, 1 on mma.sync, 0 not at all) over pages that are made bfloat16 first; or ("codes",) by the
+    kernel for single tokens, if it takes the sizes, or that in 32 bits.  The one that takes least time, in microseconds, by what each was
+    measured to do:
     codes: 10 and (more than 8 columns) 3 ahead, a tile of 16 columns (8 at head size 256) over 32 keys in `unit`, divided over all SMs;
     pages: prompt attention's blocks walk their keys one tile after another, whole blocks a SM;
-    tiles: a block, alone on its SM, takes 0.73 a page and 4 beside; a tile's pages are shared by as many blocks as fit the SMs at once,
+    tiles: a block, alone on its SM, takes 0.68 a page and 4 beside; a tile's pages are shared by as many blocks as fit the SMs at once,
     while that leaves a block more than six (of clusters of 8 no more than two thirds of the SMs).
-    Measured, codes / pages / tiles: one run over 2,048 keys, 16 heads over 8 of 128, 4 new tokens 12.6 / - / 13.0, 16: 16.9 / - / 13.1, 64: 25 / 52 /
-    14, 2,048: 220 / 53 / 37; four over 8,000, 6 tokens: 29.8 / - / 33.9, 16: 43.9 / - / 34.5; one over 32,768, 64: 116 / 619 / 60; 32 over 500, 8
-    tokens: 19.6 / - / 25.4; one of 512 among 63 of one over 4,000 keys: 119 / 935 / 210, the short ones by codes 86; 4,096 new tokens: 761 / 96 / 113; heads of 64, 32 over 8, one over 8,192, 96 tokens: 68 / 195 / 31.  Tiles
-    shared by 1, 2, 4 and 8: four over 4,096, 40 over 8 heads, 5 to 24 tokens (32 tiles): 55, 35, 24, 50; one over 32,768 (8 tiles): 375, 194,
-    104, 60; 300 keys (32 tiles): 11.6, 12.4, 13.1, 34.6."""
+    Measured, codes / pages / tiles: one run over 2,048 keys, 16 heads over 8 of 128, 4 new tokens 12.3 / - / 12.3, 16: 16.2 / - / 12.4, 64:
+    24 / 52 / 14, 2,048: 217 / 53 / 34; four over 8,000, 6 tokens: 29.8 / - / 33.9, 16: 43.9 / - / 34.5; one over 32,768, 64: 115 / 620 / 56; 32 over
+    500, 8 tokens: 19.6 / - / 25.4; one of 512 among 63 of one over 4,000 keys: 119 / 935 / 210, the short ones by codes 85; 4,096 new tokens:
+    761 / 96 / 113; heads of 64, 32 over 8, one over 8,192, 96 tokens: 66 / 195 / 29.  Tiles shared by 1, 2, 4 and 8: four over 4,096, 40 over 8
+    heads, 5 to 24 tokens (32 tiles): 51, 33, 23, 47; one over 32,768 (8 tiles): 346, 179, 96, 56; 300 keys (32 tiles): 11.6, 12.4, 13.1, 34.6."""
     n_new, group = batch.n_new, nq // nkv
     max_new, columns = max(n_new), 8 if head_dim == 256 else 16
     head_tiles = -(-group // columns)
@@ -634,7 +635,7 @@ def _attention4_way(batch, nq: int, nkv: int, head_dim: int, window: int, form: 
         shared = 1
         while shared < 8 and far > 6 * shared and 2 * shared * tiles <= (sms if shared < 4 else 2 * sms // 3):
             shared *= 2
-        return 7 + max(far / shared * 0.73 + (3 if shared > 1 else 0), (walked * nkv * 0.73 + tiles * 4) / sms), shared
+        return 7 + max(far / shared * 0.68 + (3 if shared > 1 else 0), (walked * nkv * 0.68 + tiles * 4) / sms), shared
     unit, start = {64: 1.3e-3, 128: 1.6e-3}.get(head_dim, 2.8e-3), 13 if min(group, columns) * max_new > 8 else 10
     unit *= head_tiles * nkv
     best = start + (units + units_few) * unit if codes else 1e9 if max_new >= 16 else 0                 # (few rows in 32 bits: no worse)
