@@ -588,13 +588,20 @@ def _attention4_floats(nq: int, nkv: int, head_dim: int, page_size: int, max_new
     return l.citlali_attention4_scratch_floats(nq, nkv, head_dim, max_new)
 
 
+@functools.lru_cache(maxsize=None)
+def _attention4_takes(nq: int, nkv: int, head_dim: int) -> tuple:
+    """The tokens of a tile of the kernel for runs (0: it does not take the sizes), and whether the one for single tokens takes them."""
+    l = lib()
+    return l.citlali_attention4_runs_tokens(nq, nkv, head_dim, 64), bool(l.citlali_attention4_supports(head_dim, 64))
+
+
 _EXPAND_BYTES = 1 << 30
 
 
-def _attention4_way(batch, nq: int, nkv: int, head_dim: int, window: int, form: int, tokens: int, codes: bool, sms: int) -> tuple:
+def _attention4_way(batch, nq: int, nkv: int, head_dim: int, window: int, form, tokens: int, codes: bool, sms: int) -> tuple:
     """How a step's runs of tokens are attended to: ("tiles", n, tiles, blocks that share one) by the kernel on tcgen05 (``tokens`` of a
     tile; 0: it does not take the sizes), but sequences of up to n new tokens, if n is not 0, by the kernel for single tokens; ("pages",) by
-    prompt attention (``form``: 2 on tcgen05, 1 on mma.sync, 0 not at all) over pages that are made bfloat16 first; or ("codes",) by the
+    prompt attention (``form()``: 2 on tcgen05, 1 on mma.sync, 0 not at all) over pages that are made bfloat16 first; or ("codes",) by the
     kernel for single tokens, if it takes the sizes, or that in 32 bits.  The one that takes least time, in microseconds, by what each was
     measured to do:
     codes: 10 and (more than 8 columns) 3 ahead, a tile of 16 columns (8 at head size 256) over 32 keys in `unit`, divided over all SMs;
@@ -650,9 +657,9 @@ def _attention4_way(batch, nq: int, nkv: int, head_dim: int, window: int, form: 
             time += 8 + units_few * unit
             if time < best:
                 best, way = time, ("tiles", few, tiles * nkv, shared)
-    if form > 0 and best > 40 and max_new >= 48:
-        time = _attention4_pages_time(batch, nq, nkv, head_dim, window, form, sms)
-        if time < best:
+    if best > 40 and max_new >= 16:
+        form = form()                                # (asked for only where it can matter)
+        if form > 0 and _attention4_pages_time(batch, nq, nkv, head_dim, window, form, sms) < best:
             way = ("pages",)
     return way
 
@@ -768,11 +775,10 @@ def cache4_attention(q, q_stride, kv, batch, out, nq, nkv, head_dim, window, sca
         key = (nq, nkv, head_dim, window, q_stride)
         way = batch.runs4.get(key)
         if way is None:
-            l, max_new = lib(), batch.max_new
+            max_new, (tokens, codes) = batch.max_new, _attention4_takes(nq, nkv, head_dim)
             way = batch.runs4[key] = _attention4_way(
-                batch, nq, nkv, head_dim, window, l.citlali_attention_run_form(q_stride, wide, head_dim, 64, max_new),
-                l.citlali_attention4_runs_tokens(nq, nkv, head_dim, 64),
-                _attention4_floats(nq, nkv, head_dim, 64, max_new, _current_device()) >= 0, sm_count(q.device))
+                batch, nq, nkv, head_dim, window, lambda: lib().citlali_attention_run_form(q_stride, wide, head_dim, 64, max_new), tokens, codes,
+                sm_count(q.device))
         if way[0] == "pages":
             _attention4_expanded(q, q_stride, kv, pools, batch, out, nq, nkv, head_dim, window, float(scale), error_flag)
             return

@@ -135,7 +135,7 @@ def test_which_way_runs_go():
     """By the times that ops._attention4_way works out."""
     def way(past, new, nq=16, nkv=8, d=128, window=0, form=2, tokens=None, codes=True):
         batch = cb.StepBatch(*[torch.zeros(1, dtype=torch.int32)] * 7, slots=list(range(len(new))), past=past, n_new=new)
-        return ops._attention4_way(batch, nq, nkv, d, window, form, 128 // (nq // nkv) if tokens is None else tokens, codes, 148)
+        return ops._attention4_way(batch, nq, nkv, d, window, lambda: form, 128 // (nq // nkv) if tokens is None else tokens, codes, 148)
     # few columns read the codes, more of them go in tiles that as many blocks share as fit at once, the longest prompts over pages
     assert way([2000], [4]) == ("codes",) and way([2000], [64]) == ("tiles", 0, 8, 8) and way([0], [2048]) == ("tiles", 0, 256, 1)
     assert way([8000] * 4, [6] * 4) == ("codes",) and way([8000] * 4, [16] * 4) == ("tiles", 0, 32, 4) and way([500] * 32, [4] * 32) == ("codes",)
@@ -146,4 +146,4 @@ def test_which_way_runs_go():
     assert way([2000], [8], tokens=0) == ("codes",) and way([1952], [96], tokens=0) == ("codes",) and way([0], [2048], tokens=0) == ("pages",)
     assert way([2000] * 4, [40] * 4, 40, tokens=0) == ("codes",) and way([1952] * 4, [96] * 4, 40, tokens=0) == ("pages",)
     assert way([100], [64], form=0, tokens=0) == ("codes",) and way([40000], [60], window=128, tokens=0) == ("codes",)
-    assert way([0], [100], d=80, form=1, tokens=0, codes=False) == ("pages",) and way([0], [5], d=80, form=1, tokens=0, codes=False) == ("codes",)
+    assert way([0], [100], d=80, form=1, tokens=0, codes=False) == way([0], [20], d=80, form=1, tokens=0, codes=False) == ("pages",) and way([0], [5], d=80, form=1, tokens=0, codes=False) == ("codes",)
